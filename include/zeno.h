@@ -310,6 +310,79 @@ void* zeno_model_create_from_string_ex(const char* mjcf_string, uint32_t semanti
 void zeno_model_destroy(void* model);
 const void* zeno_model_table(void* model, const char* name, uint64_t* nbytes);
 
+/* ---------------------------------------------------------------- policy operators
+ *
+ * Operators of the policies that act in and train on the worlds' observations (no
+ * counterpart in the reference).  All pointers are device memory of the current device;
+ * every call queues its kernels on `cuda_stream` (NULL: the default stream) and returns
+ * without waiting; nothing is allocated.  Return values: 0, ZENO_INVALID_ARGUMENT (the
+ * reason is in zeno_last_error) or ZENO_METAL_ERROR (a CUDA error).  A workspace may be
+ * reused as soon as the stream has passed the call. */
+
+#define ZENO_DTYPE_F32 0u
+#define ZENO_DTYPE_BF16 1u
+
+/* A tensor [batch, tokens, heads, width]: strides in elements of the first three axes;
+ * the last one is contiguous (g and beta have no width, reset has no heads). */
+typedef struct {
+  void* data;
+  int64_t stride[3];
+} ZenoTensor;
+
+/* Gated delta rule, per environment and value head, with a state S [key_dim, value_dim]:
+ *   S <- exp(g) S, or 0 where an episode begins (reset != 0, or exp(g) == 0)
+ *   u  = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
+ * normalize: q and k are divided by sqrt(|x|^2 + 1e-6) first.  Value head h reads key head
+ * h / (value_heads / key_heads).  A reset clears the state whatever it held, infinities
+ * and NaN included.  Widths are 1..128, any strides. */
+typedef struct {
+  uint32_t batch, tokens, key_heads, value_heads, key_dim, value_dim;
+  uint32_t dtype;     /* of q, k, v, out and their gradients: ZENO_DTYPE_* */
+  uint32_t normalize; /* 0 or 1 */
+  float scale;
+  uint32_t _pad;
+  ZenoTensor q, k;     /* [batch, tokens, key_heads, key_dim] */
+  ZenoTensor v;        /* [batch, tokens, value_heads, value_dim] */
+  ZenoTensor g, beta;  /* float [batch, tokens, value_heads] */
+  ZenoTensor reset;    /* uint8 [batch, tokens]; data NULL: no episode begins */
+  const float* initial_state; /* [batch, value_heads, key_dim, value_dim], contiguous; NULL: zero */
+  float* final_state;         /* same shape; may be initial_state; NULL: not written */
+  ZenoTensor out;             /* [batch, tokens, value_heads, value_dim] */
+  float* saved; /* written by forward for backward: zeno_delta_rule_saved_bytes; NULL: no gradients wanted */
+} ZenoDeltaRule;
+
+/* What backward reads and writes besides the ZenoDeltaRule of its forward call (whose
+ * inputs and saved are unchanged; out is not read).  d_final and d_initial may be NULL. */
+typedef struct {
+  ZenoTensor d_out;     /* read, as out */
+  const float* d_final; /* read, as final_state */
+  ZenoTensor d_q, d_k, d_v;  /* written, as q, k, v */
+  ZenoTensor d_g, d_beta;    /* written, as g, beta */
+  float* d_initial;     /* written, as initial_state */
+} ZenoDeltaRuleGrads;
+
+#define ZENO_DELTA_FORWARD 0u
+#define ZENO_DELTA_BACKWARD 1u
+uint64_t zeno_delta_rule_workspace_bytes(const ZenoDeltaRule* p, uint32_t pass);
+uint64_t zeno_delta_rule_saved_bytes(const ZenoDeltaRule* p);
+int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d, void* workspace,
+                             uint64_t workspace_bytes, void* cuda_stream);
+/* The recurrent form, for acting: tokens is usually 1, final_state usually initial_state
+ * (updated in place).  Same results as forward up to rounding. */
+int zeno_delta_rule_step(const ZenoDeltaRule* p, void* cuda_stream);
+
+/* Newton-Schulz orthogonalisation of `count` matrices [rows, cols], as the Muon optimiser
+ * applies it to an update M: X = M / (|M|_F + 1e-7), then `steps` times
+ *   X <- a X + (b A + c A A) X,  A = X X^T,  (a, b, c) = (3.4445, -4.7750, 2.0315)
+ * (on the transposed matrix where rows > cols).  Strides in elements: of a matrix, a row
+ * and a column of `update`; `out` is contiguous [count, rows, cols] of the same type.
+ * Sums are held in 32 bits. */
+uint64_t zeno_orthogonalize_workspace_bytes(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype);
+int zeno_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows,
+                       uint32_t cols, uint32_t dtype, uint32_t steps, void* workspace, uint64_t workspace_bytes,
+                       void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,6 +112,31 @@ ffi.cdef("""
     const void* zeno_model_table(void* model, const char* name, uint64_t* nbytes);
 """)
 
+# policy operators (zeno_b200/operators.py)
+ffi.cdef("""
+    typedef struct { void* data; int64_t stride[3]; } ZenoTensor;
+    typedef struct {
+        uint32_t batch; uint32_t tokens; uint32_t key_heads; uint32_t value_heads; uint32_t key_dim; uint32_t value_dim;
+        uint32_t dtype; uint32_t normalize; float scale; uint32_t _pad;
+        ZenoTensor q; ZenoTensor k; ZenoTensor v; ZenoTensor g; ZenoTensor beta; ZenoTensor reset;
+        const float* initial_state; float* final_state; ZenoTensor out; float* saved;
+    } ZenoDeltaRule;
+    typedef struct {
+        ZenoTensor d_out; const float* d_final; ZenoTensor d_q; ZenoTensor d_k; ZenoTensor d_v;
+        ZenoTensor d_g; ZenoTensor d_beta; float* d_initial;
+    } ZenoDeltaRuleGrads;
+    uint64_t zeno_delta_rule_workspace_bytes(const ZenoDeltaRule* p, uint32_t pass);
+    uint64_t zeno_delta_rule_saved_bytes(const ZenoDeltaRule* p);
+    int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+    int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d, void* workspace,
+                                 uint64_t workspace_bytes, void* cuda_stream);
+    int zeno_delta_rule_step(const ZenoDeltaRule* p, void* cuda_stream);
+    uint64_t zeno_orthogonalize_workspace_bytes(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype);
+    int zeno_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows,
+                           uint32_t cols, uint32_t dtype, uint32_t steps, void* workspace, uint64_t workspace_bytes,
+                           void* cuda_stream);
+""")
+
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libzeno.so"
 CONTACT_DTYPE = np.dtype([("position_pen", "4f4"), ("normal_friction", "4f4"), ("indices", "4u4"),
                           ("impulses", "4f4")])

@@ -1,6 +1,6 @@
 """Build libzeno.so in-tree (zeno_b200/lib/libzeno.so) with nvcc for sm_100a.
 
-The kernel is compiled with -fmad=false and IEEE division / square root so that every
+The step kernel is compiled with -fmad=false and IEEE division / square root so that every
 floating-point operation is the one written in the source (explicit __fmaf_rn calls
 are the only fused operations); host model-building code is compiled with
 -ffp-contract=off for the same reason.
@@ -37,8 +37,12 @@ NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-fmad=false", "-prec-div
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-Wall",
              f"-I{CUDA_HOME / 'include'}", f"-I{INCLUDE}"]
 CU_SOURCES = ["step_kernel.cu", "fast_step.cu", "noalloc.cu", "math_eval.cu"]
-CXX_SOURCES = ["mjcf.cpp", "model.cpp", "fast_model.cpp", "world.cpp", "capi.cpp"]
-HEADERS = ["zeno_types.h", "devmath.cuh", "physics.cuh", "model_access.cuh", "stage_clock.cuh", "fast_model.h", "step_kernel.h", "scene.h", "model.h", "world.h"]
+# the policy operators are ordinary floating-point code: fused multiply-adds are welcome
+OP_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
+OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_backward.cu", "delta_backward_f32.cu", "newton_schulz.cu"]
+CXX_SOURCES = ["mjcf.cpp", "model.cpp", "fast_model.cpp", "world.cpp", "capi.cpp", "policy_ops.cpp"]
+HEADERS = ["zeno_types.h", "devmath.cuh", "physics.cuh", "model_access.cuh", "stage_clock.cuh", "fast_model.h", "step_kernel.h", "scene.h", "model.h", "world.h",
+           "policy_ops.h", "delta_mma.cuh", "delta_backward.cuh"]
 
 
 def _newer(target: Path, deps) -> bool:
@@ -50,7 +54,7 @@ def _newer(target: Path, deps) -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every CUDA/C++ source and link libzeno.so; returns the library path."""
-    deps = [CSRC / s for s in CU_SOURCES + CXX_SOURCES + HEADERS] + [INCLUDE / "zeno.h", Path(__file__)]
+    deps = [CSRC / s for s in CU_SOURCES + OP_SOURCES + CXX_SOURCES + HEADERS] + [INCLUDE / "zeno.h", Path(__file__)]
     if not force and _newer(LIB, deps):
         return LIB
     OBJ_DIR.mkdir(exist_ok=True)
@@ -68,6 +72,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
     jobs = [[NVCC, *NVCC_FLAGS, f"-I{INCLUDE}", "-c", str(CSRC / src), "-o", str(OBJ_DIR / (src + ".o"))]
             for src in CU_SOURCES]
+    jobs += [[NVCC, *OP_FLAGS, f"-I{INCLUDE}", "-c", str(CSRC / src), "-o", str(OBJ_DIR / (src + ".o"))]
+             for src in OP_SOURCES]
     jobs += [[cxx, *CXX_FLAGS, "-c", str(CSRC / src), "-o", str(OBJ_DIR / (src + ".o"))] for src in CXX_SOURCES]
     objs = [cmd[-1] for cmd in jobs]
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as pool:

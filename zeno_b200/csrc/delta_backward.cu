@@ -1,0 +1,18 @@
+// The bfloat16 instances of the gated delta rule's backward pass, and its workspace.
+#include "delta_backward.cuh"
+
+namespace zb {
+
+cudaError_t launch_delta_backward_f32(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream);
+
+// Shared key heads: 32-bit rows of dq and dk for each value head.
+uint64_t delta_backward_workspace(const ZenoDeltaRule& p) {
+  return p.key_heads == p.value_heads ? 0 : 2 * uint64_t(p.batch) * p.tokens * p.value_heads * p.key_dim * 4;
+}
+
+cudaError_t launch_delta_backward(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream) {
+  return p.dtype == ZENO_DTYPE_BF16 ? delta::by_heads<__nv_bfloat16>(p, d, workspace, stream)
+                                    : launch_delta_backward_f32(p, d, workspace, stream);
+}
+
+}  // namespace zb

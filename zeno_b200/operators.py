@@ -1,0 +1,248 @@
+"""Operators of policies that act in batched worlds, on PyTorch CUDA tensors.
+
+``delta_rule_step`` acts: one token for every environment, the memory of each updated in
+place, cleared where the world reports the end of an episode.  ``delta_rule`` runs the
+same recurrence over a stored rollout in chunks, with gradients, for learning.
+``orthogonalize`` is the Newton-Schulz step of the Muon optimiser for the matrices around
+them.  The kernels are in libzeno.so and run on the current stream of the tensors' device;
+there is no fallback.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from ._ffi import _lib, ffi
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_MAX_DIM = 128
+
+Tensor = torch.Tensor
+
+
+def _check(code: int, what: str) -> None:
+    if code != 0:
+        raise RuntimeError(f"{what} failed with error code {code}: {ffi.string(_lib.zeno_last_error()).decode()}")
+
+
+def _stream(device: torch.device):
+    return ffi.cast("void*", torch.cuda.current_stream(device).cuda_stream)
+
+
+def _expect(name: str, x: Tensor, shape: Tuple[int, ...], dtypes, device: torch.device) -> None:
+    if x.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    if x.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {x.dtype}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, q on {device}")
+
+
+def _check_inputs(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: Optional[Tensor], lead: int) -> None:
+    """``lead``: the axes in front of the heads (2: batch and tokens, 1: batch)."""
+    if q.dim() != lead + 2 or v.dim() != lead + 2:
+        axes = "[batch, tokens, heads, width]" if lead == 2 else "[batch, heads, width]"
+        raise ValueError(f"q, k and v must be {axes}, got {tuple(q.shape)} and {tuple(v.shape)}")
+    if q.device.type != "cuda":
+        raise ValueError(f"expected CUDA tensors, got q on {q.device}")
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"q must be float32 or bfloat16, got {q.dtype}")
+    heads, width = v.shape[lead], v.shape[lead + 1]
+    if not (1 <= q.shape[lead + 1] <= _MAX_DIM and 1 <= width <= _MAX_DIM):
+        raise ValueError(f"head widths must be 1 to {_MAX_DIM}, got {q.shape[lead + 1]} and {width}")
+    if q.shape[lead] < 1 or heads < 1 or heads % q.shape[lead]:
+        raise ValueError(f"the {heads} value heads must be a multiple of the {q.shape[lead]} key heads")
+    front = q.shape[:lead]
+    _expect("k", k, q.shape, (q.dtype,), q.device)
+    _expect("v", v, (*front, heads, width), (q.dtype,), q.device)
+    _expect("g", g, (*front, heads), (torch.float32,), q.device)
+    _expect("beta", beta, (*front, heads), (torch.float32,), q.device)
+    if reset is not None:
+        _expect("reset", reset, front, (torch.uint8, torch.bool), q.device)
+
+
+def _rows(x: Tensor) -> Tensor:
+    """x, or a copy of it where its last axis is not contiguous."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _put(field, x: Tensor, token_axis: bool = True) -> None:
+    field.data = ffi.cast("void*", x.data_ptr())
+    s = x.stride()
+    if token_axis:
+        field.stride = (s[0], s[1], s[2] if len(s) > 2 else 0)
+    else:
+        field.stride = (s[0], 0, s[1] if len(s) > 1 else 0)
+
+
+def _arguments(q, k, v, g, beta, reset, initial, final, out, scale, normalize, token_axis=True):
+    p = ffi.new("ZenoDeltaRule*")
+    p.batch, p.tokens = q.shape[0], q.shape[1] if token_axis else 1
+    p.key_heads, p.key_dim = q.shape[-2], q.shape[-1]
+    p.value_heads, p.value_dim = v.shape[-2], v.shape[-1]
+    p.dtype, p.normalize, p.scale = _DTYPES[q.dtype], bool(normalize), scale
+    _put(p.q, q, token_axis)
+    _put(p.k, k, token_axis)
+    _put(p.v, v, token_axis)
+    _put(p.g, g, token_axis)
+    _put(p.beta, beta, token_axis)
+    _put(p.out, out, token_axis)
+    if reset is not None:
+        _put(p.reset, reset, token_axis)
+    if initial is not None:
+        p.initial_state = ffi.cast("float*", initial.data_ptr())
+    if final is not None:
+        p.final_state = ffi.cast("float*", final.data_ptr())
+    return p
+
+
+def _workspace(p, which: int, device: torch.device) -> Tuple[object, int, Optional[Tensor]]:
+    n = _lib.zeno_delta_rule_workspace_bytes(p, which)
+    if not n:
+        return ffi.NULL, 0, None
+    w = torch.empty(n, dtype=torch.uint8, device=device)
+    return ffi.cast("void*", w.data_ptr()), n, w
+
+
+def _forward(q, k, v, g, beta, reset, initial, scale, normalize, save):
+    out = torch.empty_like(v)
+    if out.stride(-1) != 1:
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    final = torch.empty((v.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+    p = _arguments(q, k, v, g, beta, reset, initial, final, out, scale, normalize)
+    saved = None
+    with torch.cuda.device(q.device):
+        if save:
+            saved = torch.empty(_lib.zeno_delta_rule_saved_bytes(p) // 4, dtype=torch.float32, device=q.device)
+            p.saved = ffi.cast("float*", saved.data_ptr())
+        at, n, _keep = _workspace(p, 0, q.device)
+        _check(_lib.zeno_delta_rule_forward(p, at, n, _stream(q.device)), "delta_rule")
+    return out, final, saved
+
+
+class _DeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, reset, initial, scale, normalize):
+        out, final, saved = _forward(q, k, v, g, beta, reset, initial, scale, normalize, True)
+        ctx.save_for_backward(q, k, v, g, beta, reset, initial, saved)
+        ctx.scale, ctx.normalize = scale, normalize
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, d_final):
+        q, k, v, g, beta, reset, initial, saved = ctx.saved_tensors
+        if d_out is None:
+            d_out = torch.zeros((1,) * v.dim(), dtype=v.dtype, device=v.device).expand(v.shape)
+            d_out = d_out if v.shape[-1] == 1 else d_out.contiguous()
+        d_out = _rows(d_out)
+        if d_final is not None:
+            d_final = d_final.contiguous()
+        p = _arguments(q, k, v, g, beta, reset, initial, None, d_out, ctx.scale, ctx.normalize)
+        p.saved = ffi.cast("float*", saved.data_ptr())
+        d = ffi.new("ZenoDeltaRuleGrads*")
+        grads = [torch.empty_like(x) for x in (q, k, v, g, beta)]
+        grads = [y if i > 2 or y.stride(-1) == 1 else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+                 for i, y in enumerate(grads)]
+        for field, x in zip((d.d_q, d.d_k, d.d_v, d.d_g, d.d_beta, d.d_out), (*grads, d_out)):
+            _put(field, x)
+        if d_final is not None:
+            d.d_final = ffi.cast("float*", d_final.data_ptr())
+        d_initial = None
+        if initial is not None and ctx.needs_input_grad[6]:
+            d_initial = torch.empty_like(initial)
+            d.d_initial = ffi.cast("float*", d_initial.data_ptr())
+        with torch.cuda.device(q.device):
+            at, n, _keep = _workspace(p, 1, q.device)
+            _check(_lib.zeno_delta_rule_backward(p, d, at, n, _stream(q.device)), "delta_rule backward")
+        return (*grads, None, d_initial, None, None)
+
+
+def delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: Optional[Tensor] = None,
+               initial_state: Optional[Tensor] = None, *, scale: Optional[float] = None,
+               normalize: bool = True) -> Tuple[Tensor, Tensor]:
+    """Gated delta rule over a rollout: ``(out [B, T, H, dv], final_state [B, H, dk, dv])``.
+
+    For each environment and value head a state S [dk, dv] walks over the tokens::
+
+        S = exp(g) * S          # zero where an episode begins
+        u = beta * (v - S^T k)
+        S = S + k u^T
+        out = scale * S^T q
+
+    ``q``, ``k`` [B, T, Hk, dk] and ``v`` [B, T, H, dv] are float32 or bfloat16 (one type),
+    H a multiple of Hk (value head h reads key head h // (H // Hk)), widths up to 128.
+    ``g`` (log decay) and ``beta`` [B, T, H] are float32.  ``reset`` [B, T] (uint8 or bool)
+    marks the first token of an episode: the state in front of it is dropped, whatever it
+    held.  ``initial_state`` [B, H, dk, dv] float32 is the state in front of the rollout
+    (None: zero).  ``normalize`` divides q and k by sqrt(|x|^2 + 1e-6).  ``scale``
+    defaults to dk ** -0.5.
+
+    Any strides are taken (a time-major buffer's transposed view needs no copy) as long as
+    the last axis is contiguous.  The state is held in 32 bits.  Gradients flow to q, k, v,
+    g, beta and initial_state; they are sums in a fixed order, so they repeat bit for bit.
+    """
+    _check_inputs(q, k, v, g, beta, reset, 2)
+    if initial_state is not None:
+        _expect("initial_state", initial_state, (v.shape[0], v.shape[2], q.shape[3], v.shape[3]), (torch.float32,), q.device)
+        initial_state = initial_state.contiguous()
+    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, initial_state)):
+        return _DeltaRule.apply(q, k, v, g, beta, reset, initial_state, scale, normalize)
+    out, final, _ = _forward(q, k, v, g, beta, reset, initial_state, scale, normalize, False)
+    return out, final
+
+
+def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tensor, reset: Optional[Tensor] = None,
+                    *, scale: Optional[float] = None, normalize: bool = True) -> Tensor:
+    """One token of ``delta_rule`` for every environment, without gradients: returns out [B, H, dv].
+
+    ``q``, ``k`` [B, Hk, dk], ``v`` [B, H, dv], ``g``, ``beta`` [B, H], ``reset`` [B] (a
+    world's ``dones`` buffer can be passed as it is).  ``state`` [B, H, dk, dv] float32,
+    contiguous, is updated in place."""
+    _check_inputs(q, k, v, g, beta, reset, 1)
+    _expect("state", state, (v.shape[0], v.shape[1], q.shape[2], v.shape[2]), (torch.float32,), q.device)
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is updated in place")
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, g, beta, state)):
+        raise RuntimeError("delta_rule_step has no gradients: call it under torch.no_grad(), and delta_rule to learn")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    p = _arguments(q, k, v, g, beta, reset, state, state, out, scale, normalize, token_axis=False)
+    with torch.cuda.device(q.device):
+        _check(_lib.zeno_delta_rule_step(p, _stream(q.device)), "delta_rule_step")
+    return out
+
+
+def orthogonalize(update: Tensor, steps: int = 5) -> Tensor:
+    """Newton-Schulz orthogonalisation of a matrix [..., m, n] (or a stack of them), as the
+    Muon optimiser applies it to its momentum: ``X = M / |M|``, then ``steps`` times
+    ``X = a X + (b A + c A A) X`` with ``A = X X^T`` and (a, b, c) = (3.4445, -4.7750,
+    2.0315), on the transposed matrix where m > n.  float32 or bfloat16, any strides; the
+    result is contiguous and of the same type, without a gradient."""
+    if update.dim() < 2:
+        raise ValueError(f"expected a matrix or a stack of matrices, got shape {tuple(update.shape)}")
+    if update.device.type != "cuda":
+        raise ValueError(f"expected a CUDA tensor, got one on {update.device}")
+    if update.dtype not in _DTYPES:
+        raise TypeError(f"update must be float32 or bfloat16, got {update.dtype}")
+    if not 0 <= steps <= 100:
+        raise ValueError(f"steps must be 0 to 100, got {steps}")
+    m, n = update.shape[-2:]
+    x = update.detach()
+    x = x.unsqueeze(0) if x.dim() == 2 else x if x.dim() == 3 else x.reshape(-1, m, n)
+    out = torch.empty(update.shape, dtype=update.dtype, device=update.device)
+    if not update.numel():
+        return out
+    with torch.cuda.device(update.device):
+        dtype = _DTYPES[update.dtype]
+        need = _lib.zeno_orthogonalize_workspace_bytes(x.shape[0], m, n, dtype)
+        work = torch.empty(need, dtype=torch.uint8, device=update.device)
+        strides = ffi.new("int64_t[3]", x.stride())
+        _check(_lib.zeno_orthogonalize(ffi.cast("void*", x.data_ptr()), strides, ffi.cast("void*", out.data_ptr()), x.shape[0], m, n,
+                                       dtype, steps, ffi.cast("void*", work.data_ptr()), need, _stream(update.device)), "orthogonalize")
+    return out
