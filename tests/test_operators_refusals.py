@@ -78,8 +78,8 @@ def test_sizes_are_known_without_a_gpu():
     assert _lib.zeno_delta_rule_saved_bytes(p) == 3 * 4 * 3 * 64 * 64 * 4
     assert _lib.zeno_delta_rule_saved_bytes(arguments(tokens=32)) == 0
     assert _lib.zeno_delta_rule_saved_bytes(arguments(key_dim=0)) == 0
-    assert _lib.zeno_orthogonalize_workspace_bytes(1, 64, 29, 0) > 0
-    assert _lib.zeno_orthogonalize_workspace_bytes(1, 64, 29, 9) == 0
+    assert _lib.zeno_orthogonalize_workspace_bytes(1, 100, 290, 0) > 0
+    assert _lib.zeno_orthogonalize_workspace_bytes(1, 100, 290, 9) == 0
 
 
 def test_no_rows_is_not_an_error():
@@ -96,7 +96,7 @@ def test_orthogonalize_entry_refuses():
     assert call(at, s, at, 1, 8, 8, 0, 101, at, big, ffi.NULL) == INVALID and "steps" in message()
     assert call(at, s, at, 70000, 8, 8, 0, 5, at, big, ffi.NULL) == INVALID and "matrices" in message()
     assert call(ffi.NULL, s, at, 1, 8, 8, 0, 5, at, big, ffi.NULL) == INVALID
-    assert call(at, s, at, 1, 8, 8, 0, 5, at, 16, ffi.NULL) == INVALID and "workspace" in message()
+    assert call(at, s, at, 1, 100, 100, 0, 5, at, 16, ffi.NULL) == INVALID and "workspace" in message()
     assert call(at, s, ffi.cast("void*", 4097), 1, 8, 8, 0, 5, at, big, ffi.NULL) == INVALID and "aligned" in message()
     assert call(ffi.NULL, ffi.NULL, ffi.NULL, 0, 8, 8, 0, 5, ffi.NULL, 0, ffi.NULL) == 0
 

@@ -138,10 +138,11 @@ int zeno_orthogonalize(const void* update, const int64_t* strides, void* out, ui
   if (!why.empty()) return zb::refuse(what, why);
   if (steps > 100) return zb::refuse(what, "more than 100 steps");
   if (!count || !rows || !cols) return ZENO_SUCCESS;
-  if (!update || !strides || !out || !workspace) return zb::refuse(what, "NULL arguments");
+  const uint64_t need = zeno_orthogonalize_workspace_bytes(count, rows, cols, dtype);
+  if (!update || !strides || !out || (need && !workspace)) return zb::refuse(what, "NULL arguments");
   if (!zb::aligned(update, zb::item(dtype)) || !zb::aligned(out, zb::item(dtype))) return zb::refuse(what, "update or out is not aligned to its elements");
   if (!zb::aligned(workspace, 256)) return zb::refuse(what, "workspace must be aligned to 256 bytes");
-  if (workspace_bytes < zeno_orthogonalize_workspace_bytes(count, rows, cols, dtype)) return zb::refuse(what, "workspace is too small");
+  if (workspace_bytes < need) return zb::refuse(what, "workspace is too small");
   return zb::status(what, zb::launch_orthogonalize(update, strides, out, count, rows, cols, dtype, steps, workspace,
                                                    static_cast<cudaStream_t>(cuda_stream)));
 }

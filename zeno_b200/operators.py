@@ -241,8 +241,8 @@ def orthogonalize(update: Tensor, steps: int = 5) -> Tensor:
     with torch.cuda.device(update.device):
         dtype = _DTYPES[update.dtype]
         need = _lib.zeno_orthogonalize_workspace_bytes(x.shape[0], m, n, dtype)
-        work = torch.empty(need, dtype=torch.uint8, device=update.device)
+        work = torch.empty(need, dtype=torch.uint8, device=update.device) if need else None
         strides = ffi.new("int64_t[3]", x.stride())
         _check(_lib.zeno_orthogonalize(ffi.cast("void*", x.data_ptr()), strides, ffi.cast("void*", out.data_ptr()), x.shape[0], m, n,
-                                       dtype, steps, ffi.cast("void*", work.data_ptr()), need, _stream(update.device)), "orthogonalize")
+                                       dtype, steps, ffi.cast("void*", work.data_ptr() if need else 0), need, _stream(update.device)), "orthogonalize")
     return out
