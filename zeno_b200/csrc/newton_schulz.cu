@@ -31,7 +31,7 @@ namespace zb {
 namespace ns {
 namespace {
 
-constexpr int kNormBlocks = 64;
+constexpr uint32_t kNormBlocks = 256;  // of a matrix, at most
 constexpr int kTile = 128;     // rows and columns of a product's tile, and the padding of every matrix
 constexpr int kDeep = 64;      // contracted values of a stage: 128 bytes, the swizzle's width
 constexpr int kPlane = kTile * kDeep * 2;  // bytes of one operand's stage, one limb
@@ -41,70 +41,92 @@ __host__ __device__ constexpr uint64_t padded(uint64_t x) { return (x + kTile - 
 
 // ---------------------------------------------------------------- norm and first planes
 
-// Sum of squares, in 64 bits (no overflow, no underflow): block y's part of matrix x.
-template <class T>
-__global__ void __launch_bounds__(256) norm_kernel(const T* from, Matrix s, double* part) {
+// Sums over a block of 256 threads, in every thread.
+__device__ __forceinline__ double block_sum(double x) {
   __shared__ double sum[8];
-  const T* at = from + int64_t(blockIdx.x) * s.matrix;
-  const uint64_t n = uint64_t(s.m) * s.n;
-  double x = 0.0;
-  for (uint64_t i = blockIdx.y * 256ull + threadIdx.x; i < n; i += 256ull * gridDim.y) {
-    // neighbouring threads along the axis that is dense in memory
-    const uint64_t r = s.col <= s.row ? i / s.n : i % s.m, c = s.col <= s.row ? i % s.n : i / s.m;
-    const double y = up(at[int64_t(r) * s.row + int64_t(c) * s.col]);
-    x = fma(y, y, x);
-  }
   for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
   if ((threadIdx.x & 31) == 0) sum[threadIdx.x >> 5] = x;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) x += sum[i];
-    part[blockIdx.x * gridDim.y + blockIdx.y] = x;
-  }
+  x = 0.0;
+  for (int i = 0; i < 8; ++i) x += sum[i];
+  return x;
 }
 
+// The next kernel's blocks may start (they wait for this kernel's end before they read) ...
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// ... and this one's for the kernel in front of it.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Sum of squares, in 64 bits (no overflow, no underflow): block y's rows of matrix x, a warp a row
+// along the axis that is dense in memory.
+template <class T>
+__global__ void __launch_bounds__(256) norm_kernel(const T* from, Matrix s, double* part) {
+  wait_for_previous();
+  let_next_start();
+  const T* at = from + int64_t(blockIdx.x) * s.matrix;
+  const bool by_row = s.col <= s.row;
+  const uint32_t rows = by_row ? s.m : s.n, cols = by_row ? s.n : s.m;
+  const int64_t row = by_row ? s.row : s.col, col = by_row ? s.col : s.row;
+  double x = 0.0;
+  for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    const T* line = at + int64_t(r) * row;
+#pragma unroll 4
+    for (uint32_t c = threadIdx.x & 31; c < cols; c += 32) {
+      const double y = up(line[int64_t(c) * col]);
+      x = fma(y, y, x);
+    }
+  }
+  x = block_sum(x);
+  if (threadIdx.x == 0) part[blockIdx.x * gridDim.y + blockIdx.y] = x;
+}
+
+// By a whole block of 256 threads; parts <= 256.
 __device__ __forceinline__ double inverse_norm(const double* part, uint32_t parts) {
-  double sum = 0.0;
-  for (uint32_t i = 0; i < parts; ++i) sum += part[i];
-  return 1.0 / (sqrt(sum) + kEps);
+  return 1.0 / (sqrt(block_sum(threadIdx.x < parts ? part[threadIdx.x] : 0.0)) + kEps);
 }
 
 // X's planes in both orientations, zero in the padding: [count][2 limbs][mp][np] and [count][2 limbs][np][mp],
-// and the first extra exponent of each matrix.
+// and the first extra exponent of each matrix.  A block has 64 x 64 elements.
 template <class T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* from, Matrix s, const double* part, uint32_t parts, __half* x, __half* xt,
                                                      int* extra) {
-  __shared__ float tile[32][33];
+  __shared__ float tile[64][65];
+  wait_for_previous();
+  let_next_start();
   const uint32_t mp = uint32_t(padded(s.m)), np = uint32_t(padded(s.n));
   const double inverse = inverse_norm(part + uint64_t(blockIdx.z) * parts, parts);
   const int more = first_extra(inverse);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) extra[blockIdx.z] = more;
   const double f = inverse * scalbn(double(kScale), more);
   const T* at = from + int64_t(blockIdx.z) * s.matrix;
-  const uint32_t i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
-  const int a = threadIdx.x & 31, b = threadIdx.x >> 5;
+  const uint32_t i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
   const bool by_row = s.col <= s.row;
-  for (int k = b; k < 32; k += 8) {
-    const int ti = by_row ? k : a, tj = by_row ? a : k;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < 4096; e += 256) {
+    const int ti = by_row ? e >> 6 : e & 63, tj = by_row ? e & 63 : e >> 6;
     const uint32_t i = i0 + ti, j = j0 + tj;
     tile[ti][tj] = i < s.m && j < s.n ? float(f * up(at[int64_t(i) * s.row + int64_t(j) * s.col])) : 0.0f;
   }
   __syncthreads();
   const uint64_t plane = uint64_t(mp) * np;
   x += uint64_t(blockIdx.z) * 2 * plane, xt += uint64_t(blockIdx.z) * 2 * plane;
-  for (int k = b; k < 32; k += 8) {
-    const float y = tile[k][a], z = tile[a][k];
-    const __half yh = __float2half_rn(y), zh = __float2half_rn(z);
+  const int a = (threadIdx.x & 31) * 2;
+#pragma unroll 4
+  for (int k = threadIdx.x >> 5; k < 64; k += 8) {
     const uint64_t p = uint64_t(i0 + k) * np + j0 + a, q = uint64_t(j0 + k) * mp + i0 + a;
-    x[p] = yh, xt[q] = zh;
-    x[plane + p] = __float2half_rn(y - __half2float(yh));
-    xt[plane + q] = __float2half_rn(z - __half2float(zh));
+    const __half2 y = __floats2half2_rn(tile[k][a], tile[k][a + 1]), z = __floats2half2_rn(tile[a][k], tile[a + 1][k]);
+    const float2 fy = __half22float2(y), fz = __half22float2(z);
+    *reinterpret_cast<__half2*>(x + p) = y;
+    *reinterpret_cast<__half2*>(xt + q) = z;
+    *reinterpret_cast<__half2*>(x + plane + p) = __floats2half2_rn(tile[k][a] - fy.x, tile[k][a + 1] - fy.y);
+    *reinterpret_cast<__half2*>(xt + plane + q) = __floats2half2_rn(tile[a][k] - fz.x, tile[a + 1][k] - fz.y);
   }
 }
 
 // No steps: the normalised matrix itself, in the caller's orientation.
 template <class T>
 __global__ void __launch_bounds__(256) normalise_kernel(const T* from, Matrix s, const double* part, uint32_t parts, T* out, bool transposed) {
+  wait_for_previous();
   const double f = inverse_norm(part + uint64_t(blockIdx.x) * parts, parts);
   const T* at = from + int64_t(blockIdx.x) * s.matrix;
   const uint64_t n = uint64_t(s.m) * s.n;
@@ -165,10 +187,12 @@ __device__ __forceinline__ void tensor_mma(uint32_t d, uint64_t a, uint64_t b, b
 __device__ __forceinline__ void tensor_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// 16 rows and 64 columns of accumulators: v[4 c + x] is column 8 c + 2 (lane % 4) + (x & 1) of row
+// lane / 4 + 8 (x >> 1), as the tiles of mma.sync have it.
 __device__ __forceinline__ void tensor_load(float (&r)[32], uint32_t at) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
       "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
         "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
@@ -178,45 +202,66 @@ __device__ __forceinline__ void tensor_load(float (&r)[32], uint32_t at) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// Four 8 x 8 tiles of 16-bit values to shared memory, lane l giving the address of row l % 8 of tile l / 8.
+__device__ __forceinline__ void store_tiles(uint32_t at, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void store_tiles_transposed(uint32_t at, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t from, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(from), "r"(x),
+               "r"(y), "r"(z)
+               : "memory");
+}
+
 enum Kind { kGram, kSquare, kApply, kLast };  // A; B; X in both orientations; X to the caller
 
 struct Product {
   uint32_t depth;         // contracted length, a multiple of kDeep
-  uint32_t rows, cols;    // padded sizes of the result
-  const __half* add;      // planes that the epilogue adds (A for B, X for X)
-  __half* out;            // result planes
-  __half* out_t;          // kApply: the transposed planes
-  void* last;             // kLast: the caller's array
+  uint32_t cols;          // padded columns of the result
   int add_limbs, out_limbs, out_t_limbs;
   uint32_t step;
   const int* extra;       // first extra exponents
+  void* last;             // kLast: the caller's array
   uint32_t m, n;          // kLast: X's sizes
   uint32_t transposed;    // kLast: the caller's matrices are X^T
   uint32_t* failed;       // set where a barrier was waited for in vain
 };
 
-template <int LIMBS>
-constexpr int kStages = LIMBS == 2 ? 3 : 6;
+// Shared memory: a ring of 6 units of 32 KB; a stage is one unit (both operands' hi limbs) or two (hi
+// and lo).  Behind the last stage come two units with the tile that the epilogue adds, and the
+// other four, once the products are done, hold the result's limb planes in both orientations.
+constexpr int kUnits = 6, kUnit = 2 * kPlane;
+constexpr int kSmem = kUnits * kUnit + 1024 + 256;
 template <int LIMBS>
 constexpr int kColumns = LIMBS == 2 ? 4 * kTile : kTile;  // of TMEM
-template <int LIMBS>
-constexpr int kSmem = kStages<LIMBS> * 2 * LIMBS * kPlane + 1024 + 256;
+
+// Byte of element (row, col) in a unit that holds a 128 x 128 tile as two swizzled boxes of 64 columns.
+__device__ __forceinline__ uint32_t in_unit(uint32_t row, uint32_t col) {
+  return (col >> 6) * kPlane + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
 
 // One block: one 128 x 128 tile of L R^T (rows of both along the contracted index), then the
-// step's epilogue.  Warp 0 loads, warp 1 issues the matrix instructions, warps 4 to 7 read
-// the accumulators, 32 rows each.
+// step's epilogue.  Warp 0 loads, warp 1 issues the matrix instructions, warps 4 to 11 read
+// the accumulators, 32 rows and 64 columns each.
 template <int LIMBS, Kind KIND, class T>
-__global__ void __launch_bounds__(256, 1)
-product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__ CUtensorMap right, const __grid_constant__ Product p) {
-  constexpr int S = kStages<LIMBS>;
+__global__ void __launch_bounds__(384, 1)
+product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__ CUtensorMap right, const __grid_constant__ CUtensorMap add,
+               const __grid_constant__ CUtensorMap out, const __grid_constant__ CUtensorMap out_t, const __grid_constant__ Product p) {
+  constexpr int S = kUnits / LIMBS;
   extern __shared__ unsigned char raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + S * 2 * LIMBS * kPlane);  // full[S], empty[S], done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 1);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kUnits * kUnit);  // full[S], empty[S], done, added
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr bool kSymmetric = KIND == kGram || KIND == kSquare;
 
   uint32_t ti, tj;
-  if (KIND == kGram || KIND == kSquare) {  // lower triangle, row by row
+  if (kSymmetric) {  // lower triangle, row by row
     const uint32_t t = blockIdx.x;
     ti = uint32_t((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);
     while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
@@ -228,8 +273,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   const uint32_t z = blockIdx.y;
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < S; ++s) barrier_init(smem_at(bars + s), 1), barrier_init(smem_at(bars + S + s), 1);
-    barrier_init(smem_at(bars + 2 * S), 1);
+    for (int s = 0; s < 2 * S + 2; ++s) barrier_init(smem_at(bars + s), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -241,20 +285,37 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const int stages = int(p.depth / kDeep);
+  const uint32_t unit0 = smem_at(base);
+  const int first_add = stages * LIMBS % kUnits;
+  const uint32_t done = smem_at(bars + 2 * S), added = smem_at(bars + 2 * S + 1);
+  wait_for_previous();
+  let_next_start();
+  asm volatile("fence.proxy.async;" ::: "memory");  // the planes may come from ordinary stores
 
   if (warp == 0 && lane == 0) {
     int k = 0;
     bool ok = true;
-    for (; k < stages && ok; ++k) {
+    for (; k < stages; ++k) {
       const int s = k % S;
       if (k >= S) ok = barrier_wait(smem_at(bars + S + s), (k / S - 1) & 1);
       if (!ok) break;
-      const uint32_t bar = smem_at(bars + s), at = smem_at(base + s * 2 * LIMBS * kPlane);
-      barrier_expect(bar, 2 * LIMBS * kPlane);
+      const uint32_t bar = smem_at(bars + s), at = unit0 + s * LIMBS * kUnit;
+      barrier_expect(bar, LIMBS * kUnit);
 #pragma unroll
       for (int l = 0; l < LIMBS; ++l) {
         tma_load(at + l * kPlane, &left, bar, k * kDeep, int(ti * kTile), int(z * 2 + l));
         tma_load(at + (LIMBS + l) * kPlane, &right, bar, k * kDeep, int(tj * kTile), int(z * 2 + l));
+      }
+    }
+    if (KIND != kGram && ok) {
+      for (int j = stages; j < stages + 2 / LIMBS && ok; ++j)
+        if (j >= S) ok = barrier_wait(smem_at(bars + S + j % S), (j / S - 1) & 1);
+      if (ok) {
+        barrier_expect(added, p.add_limbs * kUnit);
+        for (int l = 0; l < p.add_limbs; ++l)
+          for (int half = 0; half < 2; ++half)
+            tma_load(unit0 + (first_add + l) % kUnits * kUnit + half * kPlane, &add, added, int(tj * kTile) + half * kDeep, int(ti * kTile),
+                     int(z * 2 + l));
       }
     }
     if (!ok) {  // let the copies in flight land before the block ends
@@ -263,12 +324,12 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
     }
   } else if (warp == 1 && lane == 0) {
     bool ok = true;
-    for (int k = 0; k < stages && ok; ++k) {
+    for (int k = 0; k < stages; ++k) {
       const int s = k % S;
       ok = barrier_wait(smem_at(bars + s), (k / S) & 1);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t at = smem_at(base + s * 2 * LIMBS * kPlane);
+      const uint32_t at = unit0 + s * LIMBS * kUnit;
 #pragma unroll
       for (int kk = 0; kk < kDeep; kk += 16) {
         const uint64_t a = operand(at + kk * 2), b = operand(at + LIMBS * kPlane + kk * 2);
@@ -277,7 +338,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
         } else {
           // The tensor cores' sums drop what is below 2^-24 of the running sum, always towards zero;
           // three sums for hi hi in turn and one for the small products keep that below the operands' 2^-23
-          // (one sum of 3 x 2048 products: 1.4e-5 of the result, against 1.6e-6).
+          // (2048 x 2048: one sum of 3 x 2048 products leaves 1.4e-5 of the result, these 4.5e-6, 32-bit torch 3.7e-6).
           const uint64_t al = operand(at + kPlane + kk * 2), bl = operand(at + (LIMBS + 1) * kPlane + kk * 2);
           tensor_mma(tmem + (k % 3) * kTile, a, b, k >= 3 || kk > 0);
           tensor_mma(tmem + 3 * kTile, a, bl, k > 0 || kk > 0);
@@ -286,93 +347,86 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       }
       tensor_commit(smem_at(bars + S + s));
     }
-    if (ok) tensor_commit(smem_at(bars + 2 * S));
+    if (ok) tensor_commit(done);
     else atomicExch(p.failed, 1u);
   } else if (warp >= 4) {
-    bool ok = barrier_wait(smem_at(bars + 2 * S), 0);
+    // Scales: X 2^(12 + E), A and B 2^(12 + 2 E), their products the sums of the two.
+    const int first = p.extra[z], now = extra_at(first, p.step), next = extra_at(first, p.step + 1);
+    const float f = KIND == kGram     ? kUnscale
+                    : KIND == kSquare ? kC * exp2f(float(-12 - 2 * now))
+                    : KIND == kApply  ? exp2f(float(-12 - 3 * now + next))
+                                      : exp2f(float(-24 - 3 * now));
+    const float g = KIND == kSquare ? kB : KIND == kApply ? kA * exp2f(float(next - now)) : kA * exp2f(float(-12 - now));
+    bool ok = barrier_wait(done, 0);
+    if (KIND != kGram && ok) ok = barrier_wait(added, 0);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int quarter = warp & 3;
-      const uint32_t i = ti * kTile + quarter * 32 + lane;
-      const uint64_t plane = uint64_t(p.rows) * p.cols;
-      const __half* add = p.add + uint64_t(z) * 2 * plane + uint64_t(i) * p.cols;
-      __half* out = p.out + uint64_t(z) * 2 * plane + uint64_t(i) * p.cols;
-      // Scales: X 2^(12 + E), A and B 2^(12 + 2 E), their products the sums of the two.
-      const int now = extra_at(p.extra[z], p.step), next = extra_at(p.extra[z], p.step + 1);
-      const float f = KIND == kGram     ? kUnscale
-                      : KIND == kSquare ? kC * exp2f(float(-12 - 2 * now))
-                      : KIND == kApply  ? exp2f(float(-12 - 3 * now + next))
-                                        : exp2f(float(-24 - 3 * now));
-      const float g = KIND == kSquare ? kB : KIND == kApply ? kA * exp2f(float(next - now)) : kA * exp2f(float(-12 - now));
+      const int quarter = warp & 3, gi = lane >> 2, qj = (lane & 3) * 2;
+      const bool mirror = KIND == kApply || (kSymmetric && ti != tj);
+      const int limbs_t = KIND == kApply ? p.out_t_limbs : p.out_limbs;
+      const unsigned char* add0 = base + first_add * kUnit;
+      const unsigned char* add1 = base + (first_add + 1) % kUnits * kUnit;
 #pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
-        const uint32_t j0 = tj * kTile + c;
+      for (int part = 0; part < 2; ++part) {
+        const uint32_t r0 = quarter * 32 + part * 16, c0 = ((warp >> 2) - 1) * 64;
         float v[32];
-        tensor_load(v, tmem + (uint32_t(quarter * 32) << 16) + c);
+        const uint32_t at = tmem + (r0 << 16) + c0;
+        tensor_load(v, at);
         if (LIMBS == 2) {
           float w[32];
 #pragma unroll 1
           for (int u = 1; u < 4; ++u) {
             if (u < 3 && u >= stages) continue;
-            tensor_load(w, tmem + (uint32_t(quarter * 32) << 16) + u * kTile + c);
+            tensor_load(w, at + u * kTile);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] += w[e];
           }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float y[8] = {};
-          if (KIND != kGram) {
-            for (int l = 0; l < p.add_limbs; ++l) {
-              const uint4 w = *reinterpret_cast<const uint4*>(add + l * plane + j0 + q * 8);
-              const __half2* h = reinterpret_cast<const __half2*>(&w);
+        for (int e = 0; e < 32; e += 2) {
+          const uint32_t row = r0 + gi + ((e >> 1) & 1) * 8, col = c0 + (e >> 2) * 8 + qj;
+          if (KIND == kGram) {
+            v[e] *= f, v[e + 1] *= f;
+          } else {
+            float2 y = __half22float2(*reinterpret_cast<const __half2*>(add0 + in_unit(row, col)));
+            if (p.add_limbs == 2) {
+              const float2 w = __half22float2(*reinterpret_cast<const __half2*>(add1 + in_unit(row, col)));
+              y.x += w.x, y.y += w.y;
+            }
+            v[e] = fmaf(v[e], f, g * y.x), v[e + 1] = fmaf(v[e + 1], f, g * y.y);
+          }
+          if constexpr (KIND == kLast) {
+            const uint32_t i = ti * kTile + row, j = tj * kTile + col;
+            T* to = static_cast<T*>(p.last) + uint64_t(z) * p.m * p.n;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 t = __half22float2(h[e]);
-                y[2 * e] += t.x, y[2 * e + 1] += t.y;
+            for (int q = 0; q < 2; ++q)
+              if (i < p.m && j + q < p.n) {
+                T* at_out = to + (p.transposed ? uint64_t(j + q) * p.m + i : uint64_t(i) * p.n + j + q);
+                if constexpr (sizeof(T) == 2) *at_out = __float2bfloat16_rn(v[e + q]);
+                else *at_out = v[e + q];
               }
-            }
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[q * 8 + e] = KIND == kGram ? v[q * 8 + e] * f : fmaf(v[q * 8 + e], f, g * y[e]);
         }
-        if constexpr (KIND == kLast) {
-          T* to = static_cast<T*>(p.last) + uint64_t(z) * p.m * p.n;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const uint32_t j = j0 + e;
-            if (i < p.m && j < p.n) {
-              T* at = to + (p.transposed ? uint64_t(j) * p.m + i : uint64_t(i) * p.n + j);
-              const float y = v[e];
-              if constexpr (sizeof(T) == 2) *at = __float2bfloat16_rn(y);
-              else *at = y;
-            }
-          }
-        } else {
-          const bool mirror = (KIND == kGram || KIND == kSquare) && ti != tj;
-          __half* out_t = KIND == kApply ? p.out_t : p.out;
-          const uint64_t pitch = KIND == kApply ? p.rows : p.cols;
-          const int limbs_t = KIND == kApply ? p.out_t_limbs : p.out_limbs;
-          out_t += uint64_t(z) * 2 * plane + i;
+        if constexpr (KIND != kLast) {
+          const uint32_t tile_row = lane & 7, right_tile = (lane >> 4) * 8, low_tile = ((lane >> 3) & 1) * 8;
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
             if (l >= p.out_limbs) break;
-            __half2 h[16];
+            const uint32_t u_row = unit0 + (first_add + 2 + l) % kUnits * kUnit, u_col = unit0 + (first_add + 4 + l) % kUnits * kUnit;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              h[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-              const float2 t = __half22float2(h[e]);
-              v[2 * e] -= t.x, v[2 * e + 1] -= t.y;
-            }
+            for (int c = 0; c < 64; c += 16) {
+              uint32_t h[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(out + l * plane + j0 + q * 8) = *reinterpret_cast<const uint4*>(&h[4 * q]);
-            if ((KIND == kApply || mirror) && l < limbs_t) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                out_t[l * plane + uint64_t(j0 + 2 * e) * pitch] = __low2half(h[e]);
-                out_t[l * plane + uint64_t(j0 + 2 * e + 1) * pitch] = __high2half(h[e]);
+              for (int e = 0; e < 4; ++e) {
+                float* x = &v[c / 2 + e * 2];
+                const __half2 y = __floats2half2_rn(x[0], x[1]);
+                const float2 b = __half22float2(y);
+                x[0] -= b.x, x[1] -= b.y;
+                h[e] = *reinterpret_cast<const uint32_t*>(&y);
               }
+              store_tiles(u_row + in_unit(r0 + low_tile + tile_row, c0 + c + right_tile), h);
+              if (mirror && l < limbs_t) store_tiles_transposed(u_col + in_unit(c0 + c + right_tile + tile_row, r0 + low_tile), h);
             }
           }
         }
@@ -380,6 +434,24 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     } else if (lane == 0) {
       atomicExch(p.failed, 1u);
+    }
+    if (KIND != kLast) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (warp == 4 && lane == 0 && ok) {
+        const bool mirror = KIND == kApply || ti != tj;
+        const int limbs_t = KIND == kApply ? p.out_t_limbs : p.out_limbs;
+        for (int l = 0; l < p.out_limbs; ++l)
+          for (int half = 0; half < 2; ++half) {
+            tma_store(&out, unit0 + (first_add + 2 + l) % kUnits * kUnit + half * kPlane, int(tj * kTile) + half * kDeep, int(ti * kTile),
+                      int(z * 2 + l));
+            if (mirror && l < limbs_t)
+              tma_store(&out_t, unit0 + (first_add + 4 + l) % kUnits * kUnit + half * kPlane, int(ti * kTile) + half * kDeep,
+                        int(tj * kTile), int(z * 2 + l));
+          }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
     }
   }
   __syncthreads();
@@ -427,19 +499,33 @@ struct Layout {
   }
 };
 
+// A launch whose blocks may start while the kernel in front of it ends.
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = size_t(smem), c.stream = stream;
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &a, c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+struct Maps {
+  CUtensorMap left, right, add, out, out_t;
+};
+
 template <int LIMBS, Kind KIND, class T>
-cudaError_t launch(const CUtensorMap& l, const CUtensorMap& r, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
+cudaError_t launch(const Maps& m, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
   const auto kernel = product_kernel<LIMBS, KIND, T>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<LIMBS>);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(tiles, count), 256, kSmem<LIMBS>, stream>>>(l, r, p);
-  return cudaGetLastError();
+  return launch_after(kernel, dim3(tiles, count), 384, kSmem, stream, m.left, m.right, m.add, m.out, m.out_t, p);
 }
 
 template <Kind KIND, class T>
-cudaError_t launch(int limbs, const CUtensorMap& l, const CUtensorMap& r, const Product& p, uint32_t tiles, uint32_t count,
-                   cudaStream_t stream) {
-  return limbs == 2 ? launch<2, KIND, T>(l, r, p, tiles, count, stream) : launch<1, KIND, T>(l, r, p, tiles, count, stream);
+cudaError_t launch(int limbs, const Maps& m, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
+  return limbs == 2 ? launch<2, KIND, T>(m, p, tiles, count, stream) : launch<1, KIND, T>(m, p, tiles, count, stream);
 }
 
 template <class T>
@@ -456,14 +542,16 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
   const T* from = static_cast<const T*>(update);
   const uint32_t mp = uint32_t(padded(s.m)), np = uint32_t(padded(s.n));
 
-  norm_kernel<T><<<dim3(s.count, kNormBlocks), 256, 0, stream>>>(from, s, part);
-  if (steps == 0) {
-    normalise_kernel<T><<<dim3(s.count, kNormBlocks), 256, 0, stream>>>(from, s, part, kNormBlocks, static_cast<T*>(out), transposed);
-    return cudaGetLastError();
-  }
-  planes_kernel<T><<<dim3(np / 32, mp / 32, s.count), 256, 0, stream>>>(from, s, part, kNormBlocks, x[0], xt[0], extra);
+  const uint32_t dense_rows = s.col <= s.row ? s.m : s.n;
+  const uint32_t parts = dense_rows >= 8 * kNormBlocks ? kNormBlocks : (dense_rows + 7) / 8;
+  cudaError_t e = launch_after(norm_kernel<T>, dim3(s.count, parts), 256, 0, stream, from, s, part);
+  if (e != cudaSuccess) return e;
+  if (steps == 0)
+    return launch_after(normalise_kernel<T>, dim3(s.count, 64), 256, 0, stream, from, s, static_cast<const double*>(part), parts,
+                        static_cast<T*>(out), transposed);
+  e = launch_after(planes_kernel<T>, dim3(np / 64, mp / 64, s.count), 256, 0, stream, from, s, static_cast<const double*>(part), parts, x[0],
+                   xt[0], extra);
   CUtensorMap mx[2], mxt[2], ma, mb;
-  cudaError_t e = cudaGetLastError();
   const uint64_t layers = uint64_t(s.count) * 2;
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
     e = make_map(&mx[i], x[i], np, mp, layers);
@@ -471,23 +559,21 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
   }
   if (e == cudaSuccess) e = make_map(&ma, a, mp, mp, layers);
   if (e == cudaSuccess) e = make_map(&mb, b, mp, mp, layers);
-  const uint32_t mt = mp / kTile, nt = np / kTile;
+  const uint32_t mt = mp / kTile, nt = np / kTile, lower = mt * (mt + 1) / 2;
   // limbs of a step's products
   const auto limbs_of = [&](uint32_t i) { return sizeof(T) == 4 || mt == 1 || i + 1 >= steps ? 2 : 1; };
   for (uint32_t i = 0; i < steps && e == cudaSuccess; ++i) {
     const int now = i & 1, next = now ^ 1, limbs = limbs_of(i);
     Product p{};
-    p.m = s.m, p.n = s.n, p.transposed = transposed, p.failed = failed, p.extra = extra, p.step = i;
-    p.depth = np, p.rows = mp, p.cols = mp, p.add = a, p.out = a;
-    p.add_limbs = p.out_limbs = limbs;
-    e = launch<kGram, T>(limbs, mx[now], mx[now], p, mt * (mt + 1) / 2, s.count, stream);
-    p.depth = mp, p.out = b;
-    if (e == cudaSuccess) e = launch<kSquare, T>(limbs, ma, ma, p, mt * (mt + 1) / 2, s.count, stream);
-    p.cols = np, p.add = x[now], p.out = x[next], p.out_t = xt[next], p.last = out;
-    p.add_limbs = p.out_limbs = 2, p.out_t_limbs = limbs_of(i + 1);
+    p.m = s.m, p.n = s.n, p.transposed = transposed, p.failed = failed, p.extra = extra, p.step = i, p.last = out;
+    p.depth = np, p.cols = mp, p.add_limbs = p.out_limbs = limbs;
+    e = launch<kGram, T>(limbs, Maps{mx[now], mx[now], ma, ma, ma}, p, lower, s.count, stream);
+    p.depth = mp;
+    if (e == cudaSuccess) e = launch<kSquare, T>(limbs, Maps{ma, ma, ma, mb, mb}, p, lower, s.count, stream);
+    p.cols = np, p.add_limbs = p.out_limbs = 2, p.out_t_limbs = limbs_of(i + 1);
+    const Maps m{mb, mxt[now], mx[now], mx[next], mxt[next]};
     if (e == cudaSuccess)
-      e = i + 1 < steps ? launch<kApply, T>(limbs, mb, mxt[now], p, mt * nt, s.count, stream)
-                        : launch<kLast, T>(limbs, mb, mxt[now], p, mt * nt, s.count, stream);
+      e = i + 1 < steps ? launch<kApply, T>(limbs, m, p, mt * nt, s.count, stream) : launch<kLast, T>(limbs, m, p, mt * nt, s.count, stream);
   }
   return e;
 }
