@@ -40,7 +40,7 @@ struct BackwardSmem {
   __align__(16) __half state[2][VC * (DK + 8)];  // S0^T, then R^T [channel][key channel]
   // M and X with k's factors, rows of the later token; M^T and X^T with q's and k's, rows of the earlier one
   __align__(16) __half mk[2][C * CP], xk[2][C * CP], mq[2][C * CP], xt[2][C * CP];
-  float fmk[C], fxk[C], fmq[C], fxt[C];
+  float fmk[C], fxk[C], fmq[C], fxt[C], fk[C];
   float beta_part[8][C], beta_pairs[C];
   float dot_q[8][C], dot_row[8][C], dot_col[8][C];
   float end_part[8];
@@ -303,7 +303,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           const int j = tid + u * NW * 32, row = j / (VC / 8), at = (j % (VC / 8)) * 8;
           const int64_t t = t0 + row;
           if (t >= from && t < to && at < dv) {
-            load8(go[u], d_out + t * d.d_out.stride[1] + at, dv - at, vec_do);
+            unpack8<T>(go[u], fetch8(d_out + t * d.d_out.stride[1] + at, dv - at, vec_do));
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) go[u][i] = 0.0f;
@@ -356,6 +356,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         }
       }
       store_planes<DK / 8>(sm.state[0], sm.state[1], SP, st, pow2_scale(e_state), warp, lane);
+      if (tid < C) sm.fk[tid] = sm.gates.token[tid].fk;
       pair_matrices<DK, NW, L, true>(sm.gates, sm.pairs, &sm.gram, sm.q[0], sm.k[0], warp, lane);
       __syncthreads();
 
@@ -389,10 +390,10 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int i = n * 8 + qj + (x & 1);
-            const float a = sm.gates.carried[i], z = sm.gates.to_end[i];
+            const float a = sm.gates.ak[i], z = sm.gates.zk[i];
             const float v = In<T>::up(sm.v[i * VP + c0 + gi + (x >> 1) * 8]);
-            w[n][x] = a == 0.0f ? v : v - w[n][x] * ((x < 2 ? f0 : f1) * a * sm.gates.fk[i]);
-            e[n][x] = z == 0.0f ? 0.0f : e[n][x] * ((x < 2 ? f2 : f3) * z * sm.gates.fk[i]);
+            w[n][x] = a == 0.0f ? v : v - w[n][x] * ((x < 2 ? f0 : f1) * a);
+            e[n][x] = z == 0.0f ? 0.0f : e[n][x] * ((x < 2 ? f2 : f3) * z);
           }
         solve_forward(w, sm.pairs, lane);
 #pragma unroll
@@ -495,7 +496,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
             const bool on = kind & 1 ? j < i : j <= i;
             float y = on ? acc[n >> 1][half * 2 + (n & 1)] * unit : 0.0f;
             if (kind == 3 && on) db = fmaf(y, sm.gram.at[i][j], db);
-            if (on) y *= sm.gates.beta[j] * decay(sm.gates, i, j) * (kind == 2 ? sm.gates.fq[i] : later ? sm.gates.fk[j] : sm.gates.fk[i]);
+            if (on) y *= sm.gates.beta[j] * decay(sm.gates.token[i], sm.gates.token[j]) * (kind == 2 ? sm.gates.fq[i] : later ? sm.gates.token[j].fk : sm.gates.token[i].fk);
             x[n] = y;
             most = fmaxf(most, fabsf(y));
           }
@@ -565,9 +566,9 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         float x0, x1;
         row_dots<DK, N, L>(gq, sm.q[0], sm.gates.fq, r, k0, lane, x0, x1);
         if ((lane & 3) == 0) sm.dot_q[group][i0] = x0, sm.dot_q[group][i0 + 8] = x1;
-        row_dots<DK, N, L>(g_row, sm.k[0], sm.gates.fk, r, k0, lane, x0, x1);
+        row_dots<DK, N, L>(g_row, sm.k[0], sm.fk, r, k0, lane, x0, x1);
         if ((lane & 3) == 0) sm.dot_row[group][i0] = x0, sm.dot_row[group][i0 + 8] = x1;
-        row_dots<DK, N, L>(g_col, sm.k[0], sm.gates.fk, r, k0, lane, x0, x1);
+        row_dots<DK, N, L>(g_col, sm.k[0], sm.fk, r, k0, lane, x0, x1);
         if ((lane & 3) == 0) sm.dot_col[group][i0] = x0, sm.dot_col[group][i0 + 8] = x1;
       }
       __syncthreads();
@@ -578,14 +579,14 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           for (int x = 0; x < 4; ++x) g_row[n][x] += g_col[n][x];
         write_rows<DK, N, L, OUT>(gq, sm.q[0], sm.gates.fq, sm.gates.nq, p.normalize, sm.dot_q, GROUPS, nullptr, d_q, d.d_q.stride[1],
                                   t0, lo, hi, r, k0, dk, dq_pairs, lane);
-        write_rows<DK, N, L, OUT>(g_row, sm.k[0], sm.gates.fk, sm.gates.nk, p.normalize, sm.dot_row, GROUPS, sm.dot_col, d_k,
+        write_rows<DK, N, L, OUT>(g_row, sm.k[0], sm.fk, sm.gates.nk, p.normalize, sm.dot_row, GROUPS, sm.dot_col, d_k,
                                   d.d_k.stride[1], t0, lo, hi, r, k0, dk, dk_pairs, lane);
       }
       if (warp == 0) {  // gates
         float dg = 0.0f, db = sm.beta_pairs[lane];
         for (int g = 0; g < GROUPS; ++g) dg += sm.dot_q[g][lane] + sm.dot_row[g][lane] - sm.dot_col[g][lane];
         for (int v = 0; v < NW; ++v) db += sm.beta_part[v][lane];
-        const int mine = sm.gates.episode[lane];
+        const int mine = sm.gates.token[lane].episode;
         if (lane == 31)
           for (int v = 0; v < NW; ++v) dg += sm.end_part[v];
         // sum over the later tokens of the same episode
@@ -609,12 +610,12 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int i = n * 8 + qj + (c & 1);
-            const float a = sm.gates.carried[i];
+            const float ak = sm.gates.ak[i], aq = sm.gates.aq[i];
             const int at = i * DP + c0 + gi + (c >> 1) * 8;
             float y = __half2float(sm.d_out[0][at]);
             if (L == 2) y += __half2float(sm.d_out[L - 1][at]);
-            x[n][c] = a == 0.0f ? 0.0f : y * (a * u_out * sm.gates.fq[i]);
-            e[n][c] = a == 0.0f ? 0.0f : e[n][c] * (-a * sm.gates.fk[i]);
+            x[n][c] = aq == 0.0f ? 0.0f : y * (aq * u_out);
+            e[n][c] = ak == 0.0f ? 0.0f : e[n][c] * -ak;
           }
         state_update<DK, L>(rt, keep, x, sm.q[0], lane);
         state_update<DK, L>(rt, 1.0f, e, sm.k[0], lane);

@@ -29,13 +29,15 @@ struct ForwardSmem {
 };
 
 template <int DK, int NW, class T>
-__global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_constant__ ZenoDeltaRule p) {
+// Threads of an SM: 512 where the state is 32 registers a thread (4096 x 32 tokens, 64 x 64: 461 us against 544 with
+// 384 and 714 with 256), 384 where it is 64 (2 x 4096 tokens, 128 x 128: 1250 us against 1405 with 512).
+__global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) delta_forward_kernel(const __grid_constant__ ZenoDeltaRule p) {
   extern __shared__ __align__(16) unsigned char raw[];
   using Smem = ForwardSmem<DK, NW, T>;
   constexpr int L = In<T>::limbs;
   Smem& sm = *reinterpret_cast<Smem*>(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int gi = lane >> 2, qj = (lane & 3) * 2;
+  const int qj = (lane & 3) * 2;
   const uint32_t h = blockIdx.x % p.value_heads, b = blockIdx.x / p.value_heads;
   const int dk = int(p.key_dim), dv = int(p.value_dim);
   const int v0 = int(blockIdx.y) * 16 * NW;
@@ -46,14 +48,9 @@ __global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_con
                         ((p.out.stride[0] | p.out.stride[1] | p.out.stride[2]) & 1) == 0;
   const int64_t state_at = int64_t(blockIdx.x) * dk * dv;
 
-  float st[DK / 8][4];
-#pragma unroll
-  for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int c = c0 + gi + (x >> 1) * 8, r = n * 8 + qj + (x & 1);
-      st[n][x] = p.initial_state && c < dv && r < dk ? p.initial_state[state_at + int64_t(r) * dv + c] : 0.0f;
-    }
+  float st[DK / 8][4] = {};
+  if (p.initial_state)
+    for_state<DK, 16 * NW>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
   if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
   __syncthreads();
 
@@ -71,16 +68,12 @@ __global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_con
       int64_t hi = t1;
       if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
       load_rows<DK, NW, T>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, t0, lo, hi, tid);
-      bool finite = true;
-#pragma unroll
-      for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) finite &= fabsf(st[n][x]) < INFINITY;
-      if (!finite) sm.gates.state_bad = 1;
+      int e0, e1;
+      if (!row_exps_finite<DK / 8>(st, e0, e1)) sm.gates.state_bad = 1;
       __syncthreads();
       // A value that is not finite must not reach another episode, nor an earlier token,
       // through a product with zero: such a chunk is taken token by token.
-      if ((sm.gates.bad || (sm.gates.state_bad && sm.gates.episode[C - 1] > 0)) && hi - lo > 1) {
+      if ((sm.gates.bad || (sm.gates.state_bad && sm.gates.marks != 0)) && hi - lo > 1) {
         hi = lo + 1;
         __syncthreads();
         if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
@@ -93,8 +86,6 @@ __global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_con
 
       // E^T = V^T - a (S0^T K^T), O^T = a (S0^T Q^T)
       float e[4][4] = {}, o[4][4] = {};
-      int e0, e1;
-      row_exps<DK / 8>(st, e0, e1);
       {
         const float s0 = pow2_scale(e0), s1 = pow2_scale(e1);
 #pragma unroll
@@ -106,22 +97,27 @@ __global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_con
         }
       }
       const float f0 = pow2_unscale(e0), f1 = pow2_unscale(e1);
-      constexpr int VP = 16 * NW + 16 / int(sizeof(T));
+      float v[4][4];
+      load_values(v, sm.v + warp * 16, 16 * NW + 16 / int(sizeof(T)), lane);
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n) {
+        const float2 ak = *reinterpret_cast<const float2*>(&sm.gates.ak[n * 8 + qj]);
+        const float2 aq = *reinterpret_cast<const float2*>(&sm.gates.aq[n * 8 + qj]);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int i = n * 8 + qj + (x & 1);
-          const float a = sm.gates.carried[i], f = x < 2 ? f0 : f1;
-          const float v = In<T>::up(sm.v[i * VP + warp * 16 + gi + (x >> 1) * 8]);
-          e[n][x] = a == 0.0f ? v : v - e[n][x] * (f * a * sm.gates.fk[i]);
-          o[n][x] = a == 0.0f ? 0.0f : o[n][x] * (f * a * sm.gates.fq[i] * p.scale);
+          const float a = x & 1 ? ak.y : ak.x, b = (x & 1 ? aq.y : aq.x) * p.scale, f = x < 2 ? f0 : f1;
+          // a dropped state contributes nothing, whatever it held
+          e[n][x] = a == 0.0f ? v[n][x] : fmaf(-e[n][x], f * a, v[n][x]);
+          o[n][x] = a == 0.0f ? 0.0f : o[n][x] * (f * b);
         }
+      }
       solve_forward(e, sm.pairs, lane);  // now W^T
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n) {
+        const float2 be = *reinterpret_cast<const float2*>(&sm.gates.beta[n * 8 + qj]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) e[n][x] *= sm.gates.beta[n * 8 + qj + (x & 1)];  // U^T
+        for (int x = 0; x < 4; ++x) e[n][x] *= x & 1 ? be.y : be.x;  // U^T
+      }
       {  // O^T += U^T P^T
         row_exps<4>(e, e0, e1);
         const float s0 = pow2_scale(e0), s1 = pow2_scale(e1), g0 = pow2_unscale(e0), g1 = pow2_unscale(e1);
@@ -144,21 +140,22 @@ __global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_con
             }
           }
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2; ++n) {
+            const float2 fp = *reinterpret_cast<const float2*>(&sm.pairs.fp[i * 16 + n * 8 + qj]);
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              o[2 * i + n][x] = fmaf(acc[n][x], (x < 2 ? g0 : g1) * p.scale * sm.pairs.fp[i * 16 + n * 8 + qj + (x & 1)], o[2 * i + n][x]);
+              o[2 * i + n][x] = fmaf(acc[n][x], (x < 2 ? g0 : g1) * p.scale * (x & 1 ? fp.y : fp.x), o[2 * i + n][x]);
+          }
         }
       }
       store_out(o, out, p.out.stride[1], t0, lo, hi, c0, dv, pairs_ok, lane);
       // S^T <- a_C S^T + (D_C U)^T K
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n) {
+        const float2 zk = *reinterpret_cast<const float2*>(&sm.gates.zk[n * 8 + qj]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int i = n * 8 + qj + (x & 1);
-          e[n][x] *= sm.gates.to_end[i] * sm.gates.fk[i];
-        }
+        for (int x = 0; x < 4; ++x) e[n][x] *= x & 1 ? zk.y : zk.x;
+      }
       state_update<DK, L>(st, sm.gates.keep, e, sm.k[0], lane);
       __syncthreads();
       if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
@@ -166,15 +163,8 @@ __global__ void __launch_bounds__(NW * 32) delta_forward_kernel(const __grid_con
       lo = hi;
     }
   }
-  if (p.final_state) {
-#pragma unroll
-    for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int c = c0 + gi + (x >> 1) * 8, r = n * 8 + qj + (x & 1);
-        if (c < dv && r < dk) p.final_state[state_at + int64_t(r) * dv + c] = st[n][x];
-      }
-  }
+  if (p.final_state)
+    for_state<DK, 16 * NW>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { p.final_state[state_at + at] = x; });
 }
 
 template <int DK, int NW, class T>

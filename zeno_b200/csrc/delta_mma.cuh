@@ -104,48 +104,43 @@ struct In<float> {
   static __device__ __forceinline__ float up(float x) { return x; }
 };
 
-// 8 values of a row from `at` on; those at or past `n` are zero.  vec: 16-byte loads allowed.
-__device__ __forceinline__ void load8(float (&x)[8], const __nv_bfloat16* at, int n, bool vec) {
-  if (vec && n >= 8) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(at));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < n ? __bfloat162float(at[i]) : 0.0f;
-  }
-}
-__device__ __forceinline__ void load8(float (&x)[8], const float* at, int n, bool vec) {
-  if (vec && n >= 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(at)), b = __ldg(reinterpret_cast<const float4*>(at) + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < n ? at[i] : 0.0f;
-  }
-}
+// One token of a chunk, as the token-by-token matrices read it.
+struct __align__(16) Token {
+  float hi, lo;  // running sum of the log decays, base 2, in two parts (differences of long sums are exact enough)
+  float fk;      // what takes the scaled row of K to the normalised one
+  int episode;   // resets up to and including this token
+};
 
 // Gates of one chunk.
 struct Gates {
-  double total[C];    // running sum of the log decays (64 bits: differences of long sums are exact enough)
-  float carried[C];   // a_i: decay from the state in front of the chunk; 0 behind a reset, and for absent tokens
+  Token token[C];
+  __align__(16) float carried[C];  // a_i: decay from the state in front of the chunk; 0 behind a reset, and for absent tokens
   float to_end[C];    // D_Ci: decay from token i to the chunk's end, 0 for absent tokens
   float beta[C];
-  int episode[C];     // resets up to and including token i
-  float fk[C], fq[C]; // what takes the scaled rows of K and Q to the normalised ones
+  float fq[C];        // what takes the scaled row of Q to the normalised one
   float nk[C], nq[C]; // 1 / norm of the rows (1 where they are not normalised)
+  float ak[C], aq[C], zk[C];  // a_i fk_i, a_i fq_i, D_Ci fk_i
   unsigned marks;     // the tokens that clear the state
   float keep;         // a_C: what is left of the state in front of the chunk
   int bad;            // some input of this chunk is not finite
   int state_bad;      // some element of the state in front of this chunk is not finite
 };
 
-__device__ __forceinline__ float decay(const Gates& s, int i, int j) {  // from token j to token i, j <= i
-  return s.episode[i] == s.episode[j] ? expf(float(s.total[i] - s.total[j])) : 0.0f;
+__device__ __forceinline__ float decay(const Token& i, const Token& j) {  // from token j to token i, j <= i
+  return i.episode == j.episode ? exp2f((i.hi - j.hi) + (i.lo - j.lo)) : 0.0f;
+}
+
+// max.NaN: not a number where one of the two is none
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
+// 1 / sqrt(x): the approximation and one Newton step
+__device__ __forceinline__ float inverse_sqrt(float x) {
+  const float y = rsqrtf(x);
+  return fmaf(0.5f * y, fmaf(-x * y, y, 1.0f), y);
 }
 
 // Where one block's tokens are.
@@ -198,84 +193,143 @@ __device__ __forceinline__ void scan_gates(Gates& s, const ZenoDeltaRule& p, con
   }
   const unsigned marks = __ballot_sync(kAll, clear);
   const int episode = __popc(marks & (kAll >> (31 - lane)));
+  sum *= 1.4426950408889634;
   const double last = __shfl_sync(kAll, sum, 31);
-  s.total[lane] = sum;
-  s.episode[lane] = episode;
+  s.token[lane].hi = float(sum);
+  s.token[lane].lo = float(sum - float(sum));
+  s.token[lane].episode = episode;
   s.beta[lane] = be;
-  s.carried[lane] = here && episode == 0 ? expf(float(sum)) : 0.0f;
+  s.carried[lane] = here && episode == 0 ? exp2f(float(sum)) : 0.0f;
   if (lane == 0) s.marks = marks;
-  if (lane == 0) s.keep = marks == 0 ? expf(float(last)) : 0.0f;
-  s.to_end[lane] = here && episode == __popc(marks) ? expf(float(last - sum)) : 0.0f;
+  if (lane == 0) s.keep = marks == 0 ? exp2f(float(last)) : 0.0f;
+  s.to_end[lane] = here && episode == __popc(marks) ? exp2f(float(last - sum)) : 0.0f;
   if (!(fabsf(x) < INFINITY) || !(fabsf(be) < INFINITY)) s.bad = 1;
 }
 
+// One warp, once the gates and the rows' factors are there.
+__device__ __forceinline__ void join_factors(Gates& s, int lane) {
+  const float fk = s.token[lane].fk, a = s.carried[lane];
+  s.ak[lane] = a * fk, s.aq[lane] = a * s.fq[lane], s.zk[lane] = s.to_end[lane] * fk;
+}
+
+// 8 values of a row as they are in memory.
+struct Eight {
+  uint4 a, b;  // b: the second half of 32-bit values
+};
+template <class T>
+__device__ __forceinline__ Eight fetch8(const T* at, int n, bool vec) {
+  Eight r;
+  if (vec && n >= 8) {
+    r.a = __ldg(reinterpret_cast<const uint4*>(at));
+    if (sizeof(T) == 4) r.b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+  } else {
+    uint32_t w[8] = {};
+    if constexpr (sizeof(T) == 2) {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) w[i >> 1] |= uint32_t(u[i]) << (16 * (i & 1));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) w[i] = __float_as_uint(at[i]);
+    }
+    r.a = make_uint4(w[0], w[1], w[2], w[3]), r.b = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void unpack8(float (&x)[8], const Eight& r) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+  }
+}
+
 // All warps: rows of Q and K as scaled limb planes [C][DK + 8], their factors, and V as it is
-// [C][16 NW + 16 / sizeof(T)], zero for absent tokens and past the widths.
+// [C][16 NW + 16 / sizeof(T)], zero for absent tokens and past the widths.  All loads of a batch are
+// under way before the first is used.
 template <int DK, int NW, class T>
 __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, const Rows<T>& r, __half* qp, __half* kp, T* vp,
                                           int v0, int64_t t0, int64_t lo, int64_t hi, int tid) {
-  constexpr int LR = DK / 8, PITCH = DK + 8, PLANE = C * PITCH;
+  constexpr int LR = DK / 8, PITCH = DK + 8, PLANE = C * PITCH, THREADS = NW * 32;
   constexpr int VC = 16 * NW, VP = VC + 16 / int(sizeof(T));
+  constexpr int JOBS = 2 * C * LR / THREADS < 1 ? 1 : 2 * C * LR / THREADS, VJOBS = C * VC / 8 / THREADS;
+  constexpr int BATCH = sizeof(T) == 2 ? (JOBS < 4 ? JOBS : 4) : (JOBS < 2 ? JOBS : 2);
   const int dk = int(p.key_dim), dv = int(p.value_dim);
   bool bad = false;
-#pragma unroll 2
-  for (int j = tid; j < 2 * C * LR; j += NW * 32) {
-    const int row = (j / LR) % C, at = (j % LR) * 8;
-    const bool is_k = j >= C * LR;
+  Eight v[VJOBS];
+#pragma unroll
+  for (int u = 0; u < VJOBS; ++u) {
+    const int j = tid + u * THREADS, row = j / (VC / 8), at = (j % (VC / 8)) * 8;
     const int64_t t = t0 + row;
-    const bool here = t >= lo && t < hi;
-    float x[8];
-    const T* from = is_k ? r.k + t * p.k.stride[1] : r.q + t * p.q.stride[1];
-    if (here) {
-      load8(x, from + at, dk - at, r.vec_qk);
-    } else {
+    v[u] = Eight{};
+    if (t >= lo && t < hi && v0 + at < dv) v[u] = fetch8(r.v + t * p.v.stride[1] + v0 + at, dv - v0 - at, r.vec_v);
+  }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+  for (int first = 0; first < JOBS; first += BATCH) {
+    Eight raw[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int j = tid + (first + u) * THREADS, row = (j / LR) % C, at = (j % LR) * 8;
+      const int64_t t = t0 + row;
+      raw[u] = Eight{};
+      if (t >= lo && t < hi && at < dk && j < 2 * C * LR)
+        raw[u] = fetch8(j >= C * LR ? r.k + t * p.k.stride[1] + at : r.q + t * p.q.stride[1] + at, dk - at, r.vec_qk);
     }
-    float sum = 0.0f, most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum), most = fmaxf(most, fabsf(x[i]));
+    for (int u = 0; u < BATCH; ++u) {
+      const int j = tid + (first + u) * THREADS, row = (j / LR) % C, at = (j % LR) * 8;
+      const bool is_k = j >= C * LR;
+      float x[8];
+      unpack8<T>(x, raw[u]);
+      float sum = 0.0f, most = 0.0f;
 #pragma unroll
-    for (int d = 1; d < LR; d <<= 1) {
-      sum += __shfl_xor_sync(kAll, sum, d);
-      most = fmaxf(most, __shfl_xor_sync(kAll, most, d));
-    }
-    bad |= !(sum < INFINITY);
-    const int e = pow2_exp(most);
-    const float sc = pow2_scale(e);
-    uint4 hi4, lo4;
-    split(x[0] * sc, x[1] * sc, hi4.x, lo4.x);
-    split(x[2] * sc, x[3] * sc, hi4.y, lo4.y);
-    split(x[4] * sc, x[5] * sc, hi4.z, lo4.z);
-    split(x[6] * sc, x[7] * sc, hi4.w, lo4.w);
-    __half* to = (is_k ? kp : qp) + row * PITCH + at;
-    *reinterpret_cast<uint4*>(to) = hi4;
-    if (In<T>::limbs == 2) *reinterpret_cast<uint4*>(to + PLANE) = lo4;
-    if (at == 0) {
-      const float n = p.normalize ? 1.0f / sqrtf(sum + kNormEps) : 1.0f;
-      if (is_k) s.fk[row] = n * pow2_unscale(e), s.nk[row] = n;
-      else s.fq[row] = n * pow2_unscale(e), s.nq[row] = n;
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum), most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+      for (int d = 1; d < LR; d <<= 1) {
+        sum += __shfl_xor_sync(kAll, sum, d);
+        most = fmaxf(most, __shfl_xor_sync(kAll, most, d));
+      }
+      bad |= !(sum < INFINITY);
+      const int e = pow2_exp(most);
+      const float sc = pow2_scale(e);
+      uint4 hi4, lo4;
+      split(x[0] * sc, x[1] * sc, hi4.x, lo4.x);
+      split(x[2] * sc, x[3] * sc, hi4.y, lo4.y);
+      split(x[4] * sc, x[5] * sc, hi4.z, lo4.z);
+      split(x[6] * sc, x[7] * sc, hi4.w, lo4.w);
+      const float n = p.normalize ? inverse_sqrt(sum + kNormEps) : 1.0f, f = n * pow2_unscale(e);
+      if (2 * C * LR % THREADS == 0 || j < 2 * C * LR) {
+        __half* to = (is_k ? kp : qp) + row * PITCH + at;
+        *reinterpret_cast<uint4*>(to) = hi4;
+        if (In<T>::limbs == 2) *reinterpret_cast<uint4*>(to + PLANE) = lo4;
+        if (at == 0) {
+          if (is_k) s.token[row].fk = f, s.nk[row] = n;
+          else s.fq[row] = f, s.nq[row] = n;
+        }
+      }
     }
   }
-#pragma unroll 2
-  for (int j = tid; j < C * VC / 8; j += NW * 32) {
-    const int row = j / (VC / 8), at = (j % (VC / 8)) * 8;
-    const int64_t t = t0 + row;
-    const bool here = t >= lo && t < hi;
-    float x[8];
-    if (here && v0 + at < dv) {
-      load8(x, r.v + t * p.v.stride[1] + v0 + at, dv - v0 - at, r.vec_v);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    }
+  for (int u = 0; u < VJOBS; ++u) {
+    const int j = tid + u * THREADS, row = j / (VC / 8), at = (j % (VC / 8)) * 8;
+    float x[8], most = 0.0f;
+    unpack8<T>(x, v[u]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(x[i]));
+    bad |= !(most < INFINITY);
     T* to = vp + row * VP + at;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bad |= !(fabsf(x[i]) < INFINITY);
-      if constexpr (sizeof(T) == 2) to[i] = __float2bfloat16_rn(x[i]);  // exact: it was bfloat16
-      else to[i] = x[i];
-    }
+    *reinterpret_cast<uint4*>(to) = v[u].a;
+    if (sizeof(T) == 4) *(reinterpret_cast<uint4*>(to) + 1) = v[u].b;
   }
   if (bad) s.bad = 1;
 }
@@ -308,12 +362,14 @@ __device__ __forceinline__ void rows_times_rows(float (&acc)[2][4], const __half
 //   t: (I + N_rr)^-1 of the two diagonal blocks, a scale each [C][TP]
 //   p: P_ij = D q_i.k_j (j <= i) with a scale for each row; backward: its transpose [C][CP]
 // gram (backward): D k_i.k_j, j < i.
+constexpr int kSquarePitch = 20;
 struct Pairs {
   __align__(16) __half n[2][16 * TP];
   __align__(16) __half t[2][C * TP];
   __align__(16) __half p[2][C * CP];
-  float fn, ft[2], fp[C];
-  float square[2][16 * 17];  // a diagonal block on its way to its inverse
+  __align__(16) float fp[C];
+  float fn, ft[2];
+  __align__(16) float square[2][16 * kSquarePitch];  // diagonal blocks of N, transposed, on their way to the inverses
 };
 struct Gram {
   float at[C][C + 1];
@@ -326,34 +382,47 @@ __device__ __forceinline__ void store_split(__half* hi, __half* lo, int at, floa
   *reinterpret_cast<uint32_t*>(lo + at) = l;
 }
 
-// One warp: N of diagonal block r and the inverse of I + N.  Lane j < 16 solves column j by
-// forward substitution, right-looking: a step's updates do not wait for one another.
+// One warp: N of both diagonal blocks and the inverses of I + N.  Lane c + 16 r solves column c of
+// block r by forward substitution, right-looking: a step's updates do not wait for one another.
 template <int DK, int LIMBS>
-__device__ __forceinline__ void diagonal_inverse(const Gates& s, Pairs& m, Gram* gram, const __half* kp, int r, int lane) {
+__device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Gram* gram, const __half* kp, int lane) {
   constexpr int PITCH = DK + 8;
-  float acc[2][4] = {};
-  rows_times_rows<DK, LIMBS>(acc, kp + r * 16 * PITCH, kp + r * 16 * PITCH, lane);
-  float* sq = m.square[r];
   const int gi = lane >> 2, qj = (lane & 3) * 2;
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+  for (int r = 0; r < 2; ++r) {
+    float acc[2][4] = {};
+    rows_times_rows<DK, LIMBS>(acc, kp + r * 16 * PITCH, kp + r * 16 * PITCH, lane);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = gi + (x >> 1) * 8, j = n * 8 + qj + (x & 1);
-      const int ti = r * 16 + i, tj = r * 16 + j;
-      const float y = j < i ? acc[n][x] * s.fk[ti] * s.fk[tj] * decay(s, ti, tj) : 0.0f;
-      sq[j * 17 + i] = y * s.beta[tj];
-      if (gram) gram->at[ti][tj] = y;
+    for (int half = 0; half < 2; ++half) {
+      const int i = gi + half * 8;
+      const Token ti = s.token[r * 16 + i];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = (x >> 1) * 8 + qj + (x & 1);
+        const Token tj = s.token[r * 16 + j];
+        const float y = j < i ? acc[x >> 1][half * 2 + (x & 1)] * (ti.fk * tj.fk) * decay(ti, tj) : 0.0f;
+        m.square[r][j * kSquarePitch + i] = y * s.beta[r * 16 + j];
+        if (gram) gram->at[r * 16 + i][r * 16 + j] = y;
+      }
     }
+  }
   __syncwarp();
   float t[16];
-  const int c = lane & 15;
+  const int c = lane & 15, r = lane >> 4;
+  const float* sq = m.square[r];
 #pragma unroll
   for (int i = 0; i < 16; ++i) t[i] = i == c ? 1.0f : 0.0f;
 #pragma unroll
-  for (int j = 0; j < 15; ++j)
+  for (int j = 0; j < 15; ++j) {
 #pragma unroll
-    for (int i = j + 1; i < 16; ++i) t[i] = fmaf(-sq[j * 17 + i], t[j], t[i]);
+    for (int q = (j + 1) & ~3; q < 16; q += 4) {
+      const float4 n = *reinterpret_cast<const float4*>(sq + j * kSquarePitch + q);
+      const float w[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (q + x > j) t[q + x] = fmaf(-w[x], t[j], t[q + x]);
+    }
+  }
   float most = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(t[i]));
@@ -361,16 +430,14 @@ __device__ __forceinline__ void diagonal_inverse(const Gates& s, Pairs& m, Gram*
   for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(kAll, most, d));
   const int e = pow2_exp(most);
   const float sc = pow2_scale(e);
-  if (lane < 16) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float x = t[i] * sc;
-      const __half hi = __float2half_rn(x);
-      m.t[0][(r * 16 + i) * TP + c] = hi;
-      m.t[1][(r * 16 + i) * TP + c] = __float2half_rn(x - __half2float(hi));
-    }
+  for (int i = 0; i < 16; ++i) {
+    const float x = t[i] * sc;
+    const __half hi = __float2half_rn(x);
+    m.t[0][(r * 16 + i) * TP + c] = hi;
+    m.t[1][(r * 16 + i) * TP + c] = __float2half_rn(x - __half2float(hi));
   }
-  if (lane == 0) m.ft[r] = pow2_unscale(e);
+  if (c == 0) m.ft[r] = pow2_unscale(e);
 }
 
 // One warp: N_10.
@@ -386,7 +453,8 @@ __device__ __forceinline__ void lower_block(const Gates& s, Pairs& m, Gram* gram
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int i = gi + (x >> 1) * 8, j = n * 8 + qj + (x & 1);
-      const float y = acc[n][x] * s.fk[16 + i] * s.fk[j] * decay(s, 16 + i, j);
+      const Token ti = s.token[16 + i], tj = s.token[j];
+      const float y = acc[n][x] * (ti.fk * tj.fk) * decay(ti, tj);
       if (gram) gram->at[16 + i][j] = y;
       acc[n][x] = y * s.beta[j];
       most = fmaxf(most, fabsf(acc[n][x]));
@@ -414,11 +482,16 @@ __device__ __forceinline__ void score_rows(const Gates& s, Pairs& m, const __hal
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int i = r * 16 + gi + half * 8;
+    const Token ti = s.token[i];
+    const float fq = s.fq[i];
     float x[8], most = 0.0f;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const int j = (n >> 1) * 8 + qj + (n & 1);
-      x[n] = j <= i ? acc[n >> 1][half * 2 + (n & 1)] * s.fq[i] * s.fk[j] * decay(s, i, j) : 0.0f;
+      x[n] = 0.0f;
+      if (n >= 4 && r == 0) continue;
+      const Token tj = s.token[j];
+      if (j <= i) x[n] = acc[n >> 1][half * 2 + (n & 1)] * (fq * tj.fk) * decay(ti, tj);
       most = fmaxf(most, fabsf(x[n]));
     }
     most = quad_max(most);
@@ -441,11 +514,15 @@ __device__ __forceinline__ void score_columns(const Gates& s, Pairs& m, const __
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int j = r * 16 + gi + half * 8;
+    const Token tj = s.token[j];
     float x[8], most = 0.0f;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const int i = (n >> 1) * 8 + qi + (n & 1);
-      x[n] = j <= i ? acc[n >> 1][half * 2 + (n & 1)] * s.fq[i] * s.fk[j] * decay(s, i, j) : 0.0f;
+      x[n] = 0.0f;
+      if (n < 4 && r == 1) continue;
+      const Token ti = s.token[i];
+      if (j <= i) x[n] = acc[n >> 1][half * 2 + (n & 1)] * (s.fq[i] * tj.fk) * decay(ti, tj);
       most = fmaxf(most, fabsf(x[n]));
     }
     most = quad_max(most);
@@ -459,13 +536,18 @@ __device__ __forceinline__ void score_columns(const Gates& s, Pairs& m, const __
 
 // All warps: the three kinds of matrices, spread over the warps.
 template <int DK, int NW, int LIMBS, bool BACKWARD>
-__device__ __forceinline__ void pair_matrices(const Gates& s, Pairs& m, Gram* gram, const __half* qp, const __half* kp, int warp,
-                                              int lane) {
-  for (int job = warp; job < 5; job += NW) {
-    if (job < 2) diagonal_inverse<DK, LIMBS>(s, m, gram, kp, job, lane);
-    else if (job < 4 && BACKWARD) score_columns<DK, LIMBS>(s, m, qp, kp, job - 2, lane);
-    else if (job < 4) score_rows<DK, LIMBS>(s, m, qp, kp, 3 - job, lane);
-    else lower_block<DK, LIMBS>(s, m, gram, kp, lane);
+__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Gram* gram, const __half* qp, const __half* kp, int warp, int lane) {
+#pragma unroll 1
+  for (int job = warp; job < 4; job += NW) {
+    if (job == 0) {
+      diagonal_inverses<DK, LIMBS>(s, m, gram, kp, lane);
+    } else if (job < 3) {
+      if (BACKWARD) score_columns<DK, LIMBS>(s, m, qp, kp, job - 1, lane);
+      else score_rows<DK, LIMBS>(s, m, qp, kp, 2 - job, lane);
+    } else {
+      lower_block<DK, LIMBS>(s, m, gram, kp, lane);
+      join_factors(s, lane);
+    }
   }
 }
 
@@ -539,6 +621,58 @@ __device__ __forceinline__ void row_exps(const float (&t)[N][4], int& e0, int& e
     m1 = fmaxf(m1, fmaxf(fabsf(t[n][2]), fabsf(t[n][3])));
   }
   e0 = pow2_exp(quad_max(m0)), e1 = pow2_exp(quad_max(m1));
+}
+// ... and whether all of the thread's values are finite.
+template <int N>
+__device__ __forceinline__ bool row_exps_finite(const float (&t)[N][4], int& e0, int& e1) {
+  float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    m0 = max_nan(m0, max_nan(fabsf(t[n][0]), fabsf(t[n][1])));
+    m1 = max_nan(m1, max_nan(fabsf(t[n][2]), fabsf(t[n][3])));
+  }
+  const bool finite = max_nan(m0, m1) < INFINITY;
+  e0 = pow2_exp(quad_max(m0)), e1 = pow2_exp(quad_max(m1));
+  return finite;
+}
+// V^T[channel][token] of a warp's 16 channels from the rows [C][pitch].
+__device__ __forceinline__ void load_values(float (&t)[4][4], const __nv_bfloat16* v, int pitch, int lane) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // 16 tokens: tiles 2 h, 2 h + 1
+    uint32_t r[4];
+    ldsm4t(r, smem_at(v + (h * 16 + (lane >> 4) * 8 + (lane & 7)) * pitch + ((lane >> 3) & 1) * 8));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      t[2 * h + (x >> 1)][(x & 1) * 2] = __uint_as_float(r[x] << 16);
+      t[2 * h + (x >> 1)][(x & 1) * 2 + 1] = __uint_as_float(r[x] & 0xffff0000u);
+    }
+  }
+}
+__device__ __forceinline__ void load_values(float (&t)[4][4], const float* v, int pitch, int lane) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) t[n][x] = v[(n * 8 + (lane & 3) * 2 + (x & 1)) * pitch + (lane >> 2) + (x >> 1) * 8];
+}
+// A state [dk][dv] to and from a warp's transposed accumulators.  FULL: the widths are the kernel's own.
+template <int DK, int VC, class F>
+__device__ __forceinline__ void for_state(float (&st)[DK / 8][4], int dk, int dv, int c0, int lane, F f) {
+  const int gi = lane >> 2, qj = (lane & 3) * 2;
+  if (dk == DK && dv == VC) {  // offsets known when compiled
+    const int64_t at = int64_t(qj) * VC + c0 + gi;
+#pragma unroll
+    for (int n = 0; n < DK / 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) f(st[n][x], at + (n * 8 + (x & 1)) * VC + (x >> 1) * 8);
+  } else {
+#pragma unroll
+    for (int n = 0; n < DK / 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int c = c0 + gi + (x >> 1) * 8, r = n * 8 + qj + (x & 1);
+        if (c < dv && r < dk) f(st[n][x], int64_t(r) * dv + c);
+      }
+  }
 }
 
 // out[4][4] += S^T X^T for the chunk's rows X (limb planes [C][DK + 8]), S scaled by s0, s1: [16 channels][C tokens].
