@@ -662,7 +662,8 @@ cudaError_t launch(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, cudaStre
   const auto kernel = delta_backward_kernel<DK, NW, T, OUT>;
   constexpr int smem = int(sizeof(BackwardSmem<DK, NW, T>));
   static_assert(smem <= 227 * 1024, "shared memory of a block");
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, smem, allowed);
   if (e != cudaSuccess) return e;
   kernel<<<p.batch * p.value_heads, NW * 32, smem, stream>>>(p, d);
   return cudaGetLastError();

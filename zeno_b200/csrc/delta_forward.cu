@@ -171,7 +171,8 @@ template <int DK, int NW, class T>
 cudaError_t launch(const ZenoDeltaRule& p, cudaStream_t stream) {
   const auto kernel = delta_forward_kernel<DK, NW, T>;
   constexpr int smem = int(sizeof(ForwardSmem<DK, NW, T>));
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, smem, allowed);
   if (e != cudaSuccess) return e;
   const dim3 grid(p.batch * p.value_heads, (p.value_dim + 16 * NW - 1) / (16 * NW));
   kernel<<<grid, NW * 32, smem, stream>>>(p);

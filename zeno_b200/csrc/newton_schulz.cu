@@ -518,7 +518,8 @@ struct Maps {
 template <int LIMBS, Kind KIND, class T>
 cudaError_t launch(const Maps& m, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
   const auto kernel = product_kernel<LIMBS, KIND, T>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, kSmem, allowed);
   if (e != cudaSuccess) return e;
   return launch_after(kernel, dim3(tiles, count), 384, kSmem, stream, m.left, m.right, m.add, m.out, m.out_t, p);
 }

@@ -187,7 +187,8 @@ cudaError_t launch(const void* update, const Matrix& s, bool transposed, void* o
   const int mp = int(s.m + 15) / 16 * 16, np = int(s.n + 15) / 16 * 16;
   const int smem = 4 * mp * (np + 8 + 2 * kPitch);
   const auto kernel = small_kernel<WARPS, T>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kernel, 4 * int(kSmallRows) * int(kSmallCols + 8 + 2 * kPitch), allowed);
   if (e != cudaSuccess) return e;
   kernel<<<s.count, WARPS * 32, smem, stream>>>(static_cast<const T*>(update), s, static_cast<T*>(out), steps, transposed);
   return cudaGetLastError();

@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/zeno.h"
@@ -12,6 +13,20 @@ namespace zb {
 constexpr int kDeltaMaxDim = 128;  // largest key or value width of a head
 constexpr int kDeltaChunk = 32;    // tokens of one chunk (one lane each in the gate scan)
 constexpr float kNormEps = 1e-6f;  // under the root of the norms of q and k
+
+// Lets a kernel use `bytes` of dynamic shared memory, once for each device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& devices) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (devices.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) devices.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 uint64_t delta_saved_bytes(const ZenoDeltaRule& p);
 uint64_t delta_backward_workspace(const ZenoDeltaRule& p);

@@ -9,6 +9,8 @@ there is no fallback.
 """
 from __future__ import annotations
 
+import struct
+from contextlib import nullcontext
 from typing import Optional, Tuple
 
 import torch
@@ -16,9 +18,18 @@ import torch
 from ._ffi import _lib, ffi
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_FLAGS = (torch.uint8, torch.bool)
 _MAX_DIM = 128
 
 Tensor = torch.Tensor
+
+# The C structs as flat records: a call writes one in a single pack, a third of the time of
+# filling it field by field.  ZenoTensor is a pointer and three strides.
+_RULE = struct.Struct("@8IfI" + "P3q" * 6 + "2P" + "P3q" + "P")
+_GRADS = struct.Struct("@P3qP" + "P3q" * 5 + "P")
+assert _RULE.size == ffi.sizeof("ZenoDeltaRule") and _GRADS.size == ffi.sizeof("ZenoDeltaRuleGrads")
+_RULE_PTR, _GRADS_PTR = ffi.typeof("ZenoDeltaRule*"), ffi.typeof("ZenoDeltaRuleGrads*")
+_ADDRESS, _NO_TENSOR = ffi.typeof("void*"), (0, 0, 0, 0)
 
 
 def _check(code: int, what: str) -> None:
@@ -26,8 +37,14 @@ def _check(code: int, what: str) -> None:
         raise RuntimeError(f"{what} failed with error code {code}: {ffi.string(_lib.zeno_last_error()).decode()}")
 
 
-def _stream(device: torch.device):
-    return ffi.cast("void*", torch.cuda.current_stream(device).cuda_stream)
+def _stream(index: int):
+    """The current stream of a device, as the C entries take it."""
+    return ffi.cast(_ADDRESS, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _on(index: int):
+    """A context in which the device is the current one."""
+    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _expect(name: str, x: Tensor, shape: Tuple[int, ...], dtypes, device: torch.device) -> None:
@@ -39,27 +56,32 @@ def _expect(name: str, x: Tensor, shape: Tuple[int, ...], dtypes, device: torch.
         raise ValueError(f"{name} is on {x.device}, q on {device}")
 
 
-def _check_inputs(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: Optional[Tensor], lead: int) -> None:
-    """``lead``: the axes in front of the heads (2: batch and tokens, 1: batch)."""
-    if q.dim() != lead + 2 or v.dim() != lead + 2:
+def _check_inputs(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: Optional[Tensor], lead: int):
+    """``lead``: the axes in front of the heads (2: batch and tokens, 1: batch).  Returns the
+    state's shape."""
+    qs, vs, dtype, device = q.shape, v.shape, q.dtype, q.device
+    if len(qs) != lead + 2 or len(vs) != lead + 2:
         axes = "[batch, tokens, heads, width]" if lead == 2 else "[batch, heads, width]"
-        raise ValueError(f"q, k and v must be {axes}, got {tuple(q.shape)} and {tuple(v.shape)}")
-    if q.device.type != "cuda":
-        raise ValueError(f"expected CUDA tensors, got q on {q.device}")
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"q must be float32 or bfloat16, got {q.dtype}")
-    heads, width = v.shape[lead], v.shape[lead + 1]
-    if not (1 <= q.shape[lead + 1] <= _MAX_DIM and 1 <= width <= _MAX_DIM):
-        raise ValueError(f"head widths must be 1 to {_MAX_DIM}, got {q.shape[lead + 1]} and {width}")
-    if q.shape[lead] < 1 or heads < 1 or heads % q.shape[lead]:
-        raise ValueError(f"the {heads} value heads must be a multiple of the {q.shape[lead]} key heads")
-    front = q.shape[:lead]
-    _expect("k", k, q.shape, (q.dtype,), q.device)
-    _expect("v", v, (*front, heads, width), (q.dtype,), q.device)
-    _expect("g", g, (*front, heads), (torch.float32,), q.device)
-    _expect("beta", beta, (*front, heads), (torch.float32,), q.device)
+        raise ValueError(f"q, k and v must be {axes}, got {tuple(qs)} and {tuple(vs)}")
+    if device.type != "cuda":
+        raise ValueError(f"expected CUDA tensors, got q on {device}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"q must be float32 or bfloat16, got {dtype}")
+    key_heads, dk = qs[lead:]
+    heads, dv = vs[lead:]
+    if not (1 <= dk <= _MAX_DIM and 1 <= dv <= _MAX_DIM):
+        raise ValueError(f"head widths must be 1 to {_MAX_DIM}, got {dk} and {dv}")
+    if key_heads < 1 or heads < 1 or heads % key_heads:
+        raise ValueError(f"the {heads} value heads must be a multiple of the {key_heads} key heads")
+    front = qs[:lead]
+    gates = vs[:-1]
+    _expect("k", k, qs, (dtype,), device)
+    _expect("v", v, front + vs[lead:], (dtype,), device)
+    _expect("g", g, gates, (torch.float32,), device)
+    _expect("beta", beta, gates, (torch.float32,), device)
     if reset is not None:
-        _expect("reset", reset, front, (torch.uint8, torch.bool), q.device)
+        _expect("reset", reset, front, _FLAGS, device)
+    return (qs[0], heads, dk, dv)
 
 
 def _rows(x: Tensor) -> Tensor:
@@ -67,34 +89,32 @@ def _rows(x: Tensor) -> Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _put(field, x: Tensor, token_axis: bool = True) -> None:
-    field.data = ffi.cast("void*", x.data_ptr())
+def _tokens(x: Optional[Tensor]):
+    """A ZenoTensor of [batch, tokens, ...]."""
+    if x is None:
+        return _NO_TENSOR
     s = x.stride()
-    if token_axis:
-        field.stride = (s[0], s[1], s[2] if len(s) > 2 else 0)
-    else:
-        field.stride = (s[0], 0, s[1] if len(s) > 1 else 0)
+    return x.data_ptr(), s[0], s[1], s[2] if len(s) > 2 else 0
 
 
-def _arguments(q, k, v, g, beta, reset, initial, final, out, scale, normalize, token_axis=True):
-    p = ffi.new("ZenoDeltaRule*")
-    p.batch, p.tokens = q.shape[0], q.shape[1] if token_axis else 1
-    p.key_heads, p.key_dim = q.shape[-2], q.shape[-1]
-    p.value_heads, p.value_dim = v.shape[-2], v.shape[-1]
-    p.dtype, p.normalize, p.scale = _DTYPES[q.dtype], bool(normalize), scale
-    _put(p.q, q, token_axis)
-    _put(p.k, k, token_axis)
-    _put(p.v, v, token_axis)
-    _put(p.g, g, token_axis)
-    _put(p.beta, beta, token_axis)
-    _put(p.out, out, token_axis)
-    if reset is not None:
-        _put(p.reset, reset, token_axis)
-    if initial is not None:
-        p.initial_state = ffi.cast("float*", initial.data_ptr())
-    if final is not None:
-        p.final_state = ffi.cast("float*", final.data_ptr())
-    return p
+def _one_token(x: Optional[Tensor]):
+    """A ZenoTensor of [batch, ...], a single token."""
+    if x is None:
+        return _NO_TENSOR
+    s = x.stride()
+    return x.data_ptr(), s[0], 0, s[1] if len(s) > 1 else 0
+
+
+def _address(x: Optional[Tensor]) -> int:
+    return 0 if x is None else x.data_ptr()
+
+
+def _rule(tensor, q, k, v, g, beta, reset, initial, final, out, scale, normalize, saved=None):
+    qs, vs = q.shape, v.shape
+    return ffi.from_buffer(_RULE_PTR, _RULE.pack(
+        qs[0], qs[1] if tensor is _tokens else 1, qs[-2], vs[-2], qs[-1], vs[-1], _DTYPES[q.dtype], bool(normalize), scale, 0,
+        *tensor(q), *tensor(k), *tensor(v), *tensor(g), *tensor(beta), *tensor(reset), _address(initial), _address(final),
+        *tensor(out), _address(saved)))
 
 
 def _workspace(p, which: int, device: torch.device) -> Tuple[object, int, Optional[Tensor]]:
@@ -102,22 +122,23 @@ def _workspace(p, which: int, device: torch.device) -> Tuple[object, int, Option
     if not n:
         return ffi.NULL, 0, None
     w = torch.empty(n, dtype=torch.uint8, device=device)
-    return ffi.cast("void*", w.data_ptr()), n, w
+    return ffi.cast(_ADDRESS, w.data_ptr()), n, w
 
 
 def _forward(q, k, v, g, beta, reset, initial, scale, normalize, save):
     out = torch.empty_like(v)
     if out.stride(-1) != 1:
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    final = torch.empty((v.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
-    p = _arguments(q, k, v, g, beta, reset, initial, final, out, scale, normalize)
+    device = q.device
+    final = torch.empty((v.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device)
+    p = _rule(_tokens, q, k, v, g, beta, reset, initial, final, out, scale, normalize)
     saved = None
-    with torch.cuda.device(q.device):
+    with _on(device.index):
         if save:
-            saved = torch.empty(_lib.zeno_delta_rule_saved_bytes(p) // 4, dtype=torch.float32, device=q.device)
-            p.saved = ffi.cast("float*", saved.data_ptr())
-        at, n, _keep = _workspace(p, 0, q.device)
-        _check(_lib.zeno_delta_rule_forward(p, at, n, _stream(q.device)), "delta_rule")
+            saved = torch.empty(_lib.zeno_delta_rule_saved_bytes(p) // 4, dtype=torch.float32, device=device)
+            p = _rule(_tokens, q, k, v, g, beta, reset, initial, final, out, scale, normalize, saved)
+        at, n, _keep = _workspace(p, 0, device)
+        _check(_lib.zeno_delta_rule_forward(p, at, n, _stream(device.index)), "delta_rule")
     return out, final, saved
 
 
@@ -140,23 +161,17 @@ class _DeltaRule(torch.autograd.Function):
         d_out = _rows(d_out)
         if d_final is not None:
             d_final = d_final.contiguous()
-        p = _arguments(q, k, v, g, beta, reset, initial, None, d_out, ctx.scale, ctx.normalize)
-        p.saved = ffi.cast("float*", saved.data_ptr())
-        d = ffi.new("ZenoDeltaRuleGrads*")
+        p = _rule(_tokens, q, k, v, g, beta, reset, initial, None, d_out, ctx.scale, ctx.normalize, saved)
         grads = [torch.empty_like(x) for x in (q, k, v, g, beta)]
         grads = [y if i > 2 or y.stride(-1) == 1 else torch.empty(y.shape, dtype=y.dtype, device=y.device)
                  for i, y in enumerate(grads)]
-        for field, x in zip((d.d_q, d.d_k, d.d_v, d.d_g, d.d_beta, d.d_out), (*grads, d_out)):
-            _put(field, x)
-        if d_final is not None:
-            d.d_final = ffi.cast("float*", d_final.data_ptr())
-        d_initial = None
-        if initial is not None and ctx.needs_input_grad[6]:
-            d_initial = torch.empty_like(initial)
-            d.d_initial = ffi.cast("float*", d_initial.data_ptr())
-        with torch.cuda.device(q.device):
+        d_initial = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[6] else None
+        d = ffi.from_buffer(_GRADS_PTR, _GRADS.pack(*_tokens(d_out), _address(d_final), *(x for y in grads for x in _tokens(y)),
+                                                    _address(d_initial)))
+        index = q.device.index
+        with _on(index):
             at, n, _keep = _workspace(p, 1, q.device)
-            _check(_lib.zeno_delta_rule_backward(p, d, at, n, _stream(q.device)), "delta_rule backward")
+            _check(_lib.zeno_delta_rule_backward(p, d, at, n, _stream(index)), "delta_rule backward")
         return (*grads, None, d_initial, None, None)
 
 
@@ -184,9 +199,9 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: 
     the last axis is contiguous.  The state is held in 32 bits.  Gradients flow to q, k, v,
     g, beta and initial_state; they are sums in a fixed order, so they repeat bit for bit.
     """
-    _check_inputs(q, k, v, g, beta, reset, 2)
+    state = _check_inputs(q, k, v, g, beta, reset, 2)
     if initial_state is not None:
-        _expect("initial_state", initial_state, (v.shape[0], v.shape[2], q.shape[3], v.shape[3]), (torch.float32,), q.device)
+        _expect("initial_state", initial_state, state, (torch.float32,), q.device)
         initial_state = initial_state.contiguous()
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     q, k, v = _rows(q), _rows(k), _rows(v)
@@ -203,8 +218,7 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, st
     ``q``, ``k`` [B, Hk, dk], ``v`` [B, H, dv], ``g``, ``beta`` [B, H], ``reset`` [B] (a
     world's ``dones`` buffer can be passed as it is).  ``state`` [B, H, dk, dv] float32,
     contiguous, is updated in place."""
-    _check_inputs(q, k, v, g, beta, reset, 1)
-    _expect("state", state, (v.shape[0], v.shape[1], q.shape[2], v.shape[2]), (torch.float32,), q.device)
+    _expect("state", state, _check_inputs(q, k, v, g, beta, reset, 1), (torch.float32,), q.device)
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is updated in place")
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, g, beta, state)):
@@ -212,9 +226,10 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, st
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    p = _arguments(q, k, v, g, beta, reset, state, state, out, scale, normalize, token_axis=False)
-    with torch.cuda.device(q.device):
-        _check(_lib.zeno_delta_rule_step(p, _stream(q.device)), "delta_rule_step")
+    p = _rule(_one_token, q, k, v, g, beta, reset, state, state, out, scale, normalize)
+    index = q.device.index
+    with _on(index):
+        _check(_lib.zeno_delta_rule_step(p, _stream(index)), "delta_rule_step")
     return out
 
 
@@ -238,11 +253,11 @@ def orthogonalize(update: Tensor, steps: int = 5) -> Tensor:
     out = torch.empty(update.shape, dtype=update.dtype, device=update.device)
     if not update.numel():
         return out
-    with torch.cuda.device(update.device):
+    index = update.device.index
+    with _on(index):
         dtype = _DTYPES[update.dtype]
         need = _lib.zeno_orthogonalize_workspace_bytes(x.shape[0], m, n, dtype)
         work = torch.empty(need, dtype=torch.uint8, device=update.device) if need else None
-        strides = ffi.new("int64_t[3]", x.stride())
-        _check(_lib.zeno_orthogonalize(ffi.cast("void*", x.data_ptr()), strides, ffi.cast("void*", out.data_ptr()), x.shape[0], m, n,
-                                       dtype, steps, ffi.cast("void*", work.data_ptr() if need else 0), need, _stream(update.device)), "orthogonalize")
+        _check(_lib.zeno_orthogonalize(ffi.cast(_ADDRESS, x.data_ptr()), x.stride(), ffi.cast(_ADDRESS, out.data_ptr()), x.shape[0], m, n,
+                                       dtype, steps, ffi.cast(_ADDRESS, _address(work)), need, _stream(index)), "orthogonalize")
     return out
