@@ -176,6 +176,21 @@ def test_extreme_gates_and_zero_rows():
     check_gradients(x, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("norm", [False, True])
+def test_tiny_and_empty_rows(norm, dtype):
+    x = list(inputs(2, 70, 2, 2, 64, 64, dtype, norm=norm))
+    for t, f in [(3, 0.0), (20, 1e-4), (21, 1e-9), (40, 1e-12), (50, 0.0), (66, 1e-6)]:
+        x[0][:, t] *= f
+        x[1][:, t + 2] *= f
+    check_forward(x, dtype, normalize=norm)
+    check_gradients(x, dtype, normalize=norm)
+    x[0][:] = 0
+    check_gradients(x, dtype, normalize=norm)
+    x[1][:] = 0
+    check_gradients(x, dtype, normalize=norm)
+
+
 @pytest.mark.parametrize("size", [1e-15, 1e-3, 1e6, 1e15])
 def test_magnitudes(size):
     x = list(inputs(2, 50, 1, 2, 64, 64, torch.float32))

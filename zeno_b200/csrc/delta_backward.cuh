@@ -28,50 +28,51 @@ template <int DK, int NW, class T>
 struct BackwardSmem {
   static constexpr int L = In<T>::limbs;
   static constexpr int VC = 16 * NW;
+  static constexpr int GROUPS = DK / (2 * DK / NW < 16 ? 16 : 2 * DK / NW);
   Gates gates;
-  Pairs pairs;
   Gram gram;
+  struct Early {  // up to phase A
+    Pairs pairs;
+    __align__(16) T v[C * (VC + 16 / int(sizeof(T)))];
+  };
+  struct Late {  // from the token-by-token gradients on: M and X with the rows' factors, later token by earlier one
+    __align__(16) __half m[2][C * CP];
+    __align__(16) __half x[2][C * CP];
+  };
+  __align__(16) unsigned char pair_space[sizeof(Early) > sizeof(Late) ? sizeof(Early) : sizeof(Late)];
   __align__(16) __half q[L][C * (DK + 8)];
   __align__(16) __half k[L][C * (DK + 8)];
   __align__(16) __half d_out[L][C * (VC + 8)];
-  __align__(16) T v[C * (VC + 16 / int(sizeof(T)))];
-  __align__(16) __half w[2][VC * CP];         // W^T [channel][token]
-  __align__(16) __half d_e[2][VC * CP];       // dE^T
+  __align__(16) __half w[2][VC * CP];            // W^T [channel][token]; before, the squares on their way to the inverses
+  __align__(16) __half d_e[2][VC * CP];          // dE^T
   __align__(16) __half state[2][VC * (DK + 8)];  // S0^T, then R^T [channel][key channel]
-  // M and X with k's factors, rows of the later token; M^T and X^T with q's and k's, rows of the earlier one
-  __align__(16) __half mk[2][C * CP], xk[2][C * CP], mq[2][C * CP], xt[2][C * CP];
-  float fmk[C], fxk[C], fmq[C], fxt[C], fk[C];
-  float beta_part[8][C], beta_pairs[C];
-  float dot_q[8][C], dot_row[8][C], dot_col[8][C];
-  float end_part[8];
+  float fm[3], fx[3];                            // scales of the blocks (0,0), (1,0), (1,1) of M and X
+  float fk[C], inv_fk[C], inv_fq[C];
+  float beta_part[NW][C], beta_pairs[2][C];
+  float dot_q[GROUPS][C], dot_row[GROUPS][C], dot_col[GROUPS][C];
+  float end_part[NW];
   unsigned most_out, most_state, most_r, most_w, most_e;  // largest finite magnitudes (float bits)
   int r_bad;
 };
 
-__device__ __forceinline__ void raise(unsigned* at, float x) {
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(kAll, x, d));
-  if ((threadIdx.x & 31) == 0 && x < INFINITY) atomicMax(at, __float_as_uint(x));
+// Takes a warp's largest magnitude to `at` (float bits), and notes in `bad` if one is not finite.
+__device__ __forceinline__ void raise(unsigned* at, int& bad, float x) {
+  unsigned u = __reduce_max_sync(kAll, __float_as_uint(x));  // NaN and infinity above all others
+  if (u >= 0x7f800000u) {
+    bad = 1;
+    u = __reduce_max_sync(kAll, fabsf(x) < INFINITY ? __float_as_uint(x) : 0u);
+  }
+  if ((threadIdx.x & 31) == 0) atomicMax(at, u);
 }
 
 template <int N>
-__device__ __forceinline__ float most_of(const float (&t)[N][4]) {
+__device__ __forceinline__ float most_of(const float (&t)[N][4]) {  // NaN where one is
   float m = 0.0f;
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) m = fmaxf(m, fabsf(t[n][x]));
+    for (int x = 0; x < 4; ++x) m = max_nan(m, fabsf(t[n][x]));
   return m;
-}
-
-template <int N>
-__device__ __forceinline__ bool finite(const float (&t)[N][4]) {
-  bool ok = true;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) ok &= fabsf(t[n][x]) < INFINITY;
-  return ok;
 }
 
 // A warp's transposed tiles (channel rows) to limb planes of the given pitch.
@@ -95,30 +96,38 @@ __device__ __forceinline__ void mma2(float (&acc0)[4], float (&acc1)[4], const u
   if (LB == 2) mma(acc0, ah, bl[0], bl[1]), mma(acc1, ah, bl[2], bl[3]);
 }
 
-// Rows of a token-by-token plane (pitch CP, two limbs) times rows of K or Q (limb planes), blocks
-// [from, to) of 16, into 16 x 8 N tiles from column c0 on; the result times the row's factor.
-template <int DK, int N, int L>
-__device__ __forceinline__ void pairs_times_rows(float (&out)[N][4], const __half* plane, const float* factor, const __half* x,
-                                                 int r, int from, int to, int c0, int lane) {
+// The blocks of M or X that rows [16 r, 16 r + 16) meet, times rows of K or Q (limb planes), into
+// 16 x 8 N tiles from column c0 on.  TRANSPOSED: the rows are the earlier tokens.  Each block has a scale
+// of its own, each row of the result a factor.
+template <int DK, int N, int L, bool TRANSPOSED>
+__device__ __forceinline__ void pairs_times_rows(float (&out)[N][4], const __half* plane, const float* scales, const float* row_factor,
+                                                 const __half* x, int r, int c0, int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
-  float acc[N][4] = {};
-  for (int j = from; j < to; ++j) {
+  const float r0 = row_factor[r * 16 + (lane >> 2)], r1 = row_factor[r * 16 + (lane >> 2) + 8];
+#pragma unroll 1
+  for (int j = TRANSPOSED ? r : 0; j < (TRANSPOSED ? 2 : r + 1); ++j) {
     uint32_t ah[4], al[4];
-    a_rows(ah, plane + r * 16 * CP + j * 16, CP, lane);
-    a_rows(al, plane + C * CP + r * 16 * CP + j * 16, CP, lane);
+    if (TRANSPOSED) {
+      a_cols(ah, plane + j * 16 * CP + r * 16, CP, lane);
+      a_cols(al, plane + C * CP + j * 16 * CP + r * 16, CP, lane);
+    } else {
+      a_rows(ah, plane + r * 16 * CP + j * 16, CP, lane);
+      a_rows(al, plane + C * CP + r * 16 * CP + j * 16, CP, lane);
+    }
+    const float f = scales[r + j], f0 = f * r0, f1 = f * r1;
 #pragma unroll
     for (int n = 0; n < N; n += 2) {
+      float acc[2][4] = {};
       uint32_t bh[4], bl[4] = {};
       b_cols(bh, x + j * 16 * PITCH + c0 + n * 8, PITCH, lane);
       if (L == 2) b_cols(bl, x + PLANE + j * 16 * PITCH + c0 + n * 8, PITCH, lane);
-      mma2<2, L>(acc[n], acc[n + 1], ah, al, bh, bl);
+      mma2<2, L>(acc[0], acc[1], ah, al, bh, bl);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) out[n + u][c] = fmaf(acc[u][c], c < 2 ? f0 : f1, out[n + u][c]);
     }
   }
-  const float f0 = factor[r * 16 + (lane >> 2)], f1 = factor[r * 16 + (lane >> 2) + 8];
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) out[n][c] = fmaf(acc[n][c], c < 2 ? f0 : f1, out[n][c]);
 }
 
 // Rows of a [tokens] x [channels] operand times the state planes.  LA limbs; COLS: stored [channel][token].
@@ -231,14 +240,22 @@ __device__ __forceinline__ bool even(const ZenoTensor& t, int width) {
          ((t.stride[0] | t.stride[1] | t.stride[2]) & 1) == 0;
 }
 
+// Blocks of an SM.
+template <int DK, int NW>
+constexpr int kBlocks = (DK == 32 || (DK == 64 && NW > 2) ? 384 : 256) / (NW * 32);
+
 // OUT: type of the dq and dk rows (float: the workspace of shared heads, reduced afterwards).
 template <int DK, int NW, class T, class OUT>
-__global__ void __launch_bounds__(NW * 32)
+__global__ void __launch_bounds__(NW * 32, kBlocks<DK, NW>)
 delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_constant__ ZenoDeltaRuleGrads d) {
   extern __shared__ __align__(16) unsigned char raw[];
   using Smem = BackwardSmem<DK, NW, T>;
   constexpr int L = In<T>::limbs, VC = 16 * NW, VP = VC + 16 / int(sizeof(T)), DP = VC + 8, SP = DK + 8;
   Smem& sm = *reinterpret_cast<Smem*>(raw);
+  typename Smem::Early& early = *reinterpret_cast<typename Smem::Early*>(sm.pair_space);
+  typename Smem::Late& late = *reinterpret_cast<typename Smem::Late*>(sm.pair_space);
+  Squares& squares = *reinterpret_cast<Squares*>(sm.w[0]);
+  static_assert(sizeof(Squares) <= sizeof(sm.w), "the squares fit in W's place");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int gi = lane >> 2, qj = (lane & 3) * 2;
   const uint32_t h = blockIdx.x % p.value_heads, b = blockIdx.x / p.value_heads;
@@ -257,18 +274,12 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
   float* d_beta = static_cast<float*>(d.d_beta.data) + int64_t(b) * d.d_beta.stride[0] + int64_t(h) * d.d_beta.stride[2];
   const int64_t state_at = int64_t(blockIdx.x) * dk * dv;
 
-  float rt[DK / 8][4];  // R^T
-#pragma unroll
-  for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int c = c0 + gi + (x >> 1) * 8, r = n * 8 + qj + (x & 1);
-      rt[n][x] = d.d_final && c < dv && r < dk ? d.d_final[state_at + int64_t(r) * dv + c] : 0.0f;
-    }
+  float rt[DK / 8][4] = {};  // R^T
+  if (d.d_final) for_state<DK, VC>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { x = d.d_final[state_at + at]; });
+  bool has_r = d.d_final != nullptr;  // R is not zero
   if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0, sm.r_bad = 0, sm.most_out = sm.most_state = sm.most_r = sm.most_w = sm.most_e = 0;
   __syncthreads();
-  raise(&sm.most_r, most_of<DK / 8>(rt));
-  if (!finite<DK / 8>(rt)) sm.r_bad = 1;
+  if (has_r) raise(&sm.most_r, sm.r_bad, most_of<DK / 8>(rt));
 
   const int64_t T_ = p.tokens;
   const int64_t chunks = (T_ + C - 1) / C;
@@ -277,7 +288,8 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
     for (int64_t hi = t1; hi > t0;) {
       int64_t lo = t0;
       // ---- loads
-      float st[DK / 8][4];  // S0^T
+      bool has_state = chunk > 0 || p.initial_state != nullptr;
+      float st[DK / 8][4] = {};  // S0^T
       if (chunk > 0) {
         const float4* from = reinterpret_cast<const float4*>(p.saved + ((int64_t(blockIdx.x) * (chunks - 1) + chunk - 1) * VC + c0) * DK);
 #pragma unroll
@@ -285,124 +297,132 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           const float4 x = __ldcs(from + n * 32 + lane);
           st[n][0] = x.x, st[n][1] = x.y, st[n][2] = x.z, st[n][3] = x.w;
         }
-      } else {
-#pragma unroll
-        for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int c = c0 + gi + (x >> 1) * 8, r = n * 8 + qj + (x & 1);
-            st[n][x] = p.initial_state && c < dv && r < dk ? p.initial_state[state_at + int64_t(r) * dv + c] : 0.0f;
-          }
+      } else if (has_state) {
+        for_state<DK, VC>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
       }
-      float go[2][8];
-      const auto load_out = [&](int64_t from, int64_t to) {
-        bool bad = false;
-        float most = 0.0f;
+      if (has_state) raise(&sm.most_state, sm.gates.state_bad, most_of<DK / 8>(st));
+      Eight raw_out[2];
+#pragma unroll 1
+      for (;;) {
+        if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int j = tid + u * NW * 32, row = j / (VC / 8), at = (j % (VC / 8)) * 8;
           const int64_t t = t0 + row;
-          if (t >= from && t < to && at < dv) {
-            unpack8<T>(go[u], fetch8(d_out + t * d.d_out.stride[1] + at, dv - at, vec_do));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) go[u][i] = 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            bad |= !(fabsf(go[u][i]) < INFINITY);
-            most = fmaxf(most, fabsf(go[u][i]));
-          }
+          raw_out[u] = Eight{};
+          if (t >= lo && t < hi && at < dv) raw_out[u] = fetch8(d_out + t * d.d_out.stride[1] + at, dv - at, vec_do);
         }
-        raise(&sm.most_out, most);
-        if (bad) sm.gates.bad = 1;
-      };
-      if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
-      load_rows<DK, NW, T>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, 0, t0, lo, hi, tid);
-      load_out(lo, hi);
-      if (!finite<DK / 8>(st)) sm.gates.state_bad = 1;
-      raise(&sm.most_state, most_of<DK / 8>(st));
-      __syncthreads();
-      // A value that is not finite must not reach another episode through a product with
-      // zero: such a chunk is taken episode by episode.
-      if ((sm.gates.bad || sm.gates.state_bad || sm.r_bad) && (sm.gates.marks >> 1) != 0) {
+        load_rows<DK, NW, T, true>(sm.gates, p, rows, sm.q[0], sm.k[0], early.v, 0, t0, lo, hi, tid);
+        float most = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float x[8];
+          unpack8<T>(x, raw_out[u]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(x[i]));
+        }
+        raise(&sm.most_out, sm.gates.bad, most);
+        __syncthreads();
+        // A value that is not finite must not reach another episode through a product with
+        // zero: such a chunk is taken episode by episode.
+        if (lo > t0 || !(sm.gates.bad || sm.gates.state_bad || sm.r_bad) || (sm.gates.marks >> 1) == 0) break;
         lo = t0 + 31 - __clz(int(sm.gates.marks));
+        has_state = false;  // the episode's first token drops it
         __syncthreads();
-        if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0, sm.most_out = sm.most_state = 0;
-        __syncthreads();
-        if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
-        load_rows<DK, NW, T>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, 0, t0, lo, hi, tid);
-        load_out(lo, hi);
-#pragma unroll
-        for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) st[n][x] = 0.0f;  // the episode's first token drops the state
+        if (tid == 0) sm.most_out = 0;
         __syncthreads();
       }
-      const int e_out = pow2_exp(__uint_as_float(sm.most_out)), e_state = pow2_exp(__uint_as_float(sm.most_state));
-      const float u_out = pow2_unscale(e_out) * p.scale, u_state = pow2_unscale(e_state);
+      const int e_out = pow2_exp(__uint_as_float(sm.most_out));
+      const float u_out = pow2_unscale(e_out) * p.scale;
       {
         const float sc = pow2_scale(e_out);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int j = tid + u * NW * 32, row = j / (VC / 8), at = (j % (VC / 8)) * 8;
+          float x[8];
+          unpack8<T>(x, raw_out[u]);
           uint4 h4, l4;
-          split(go[u][0] * sc, go[u][1] * sc, h4.x, l4.x);
-          split(go[u][2] * sc, go[u][3] * sc, h4.y, l4.y);
-          split(go[u][4] * sc, go[u][5] * sc, h4.z, l4.z);
-          split(go[u][6] * sc, go[u][7] * sc, h4.w, l4.w);
+          split(x[0] * sc, x[1] * sc, h4.x, l4.x);
+          split(x[2] * sc, x[3] * sc, h4.y, l4.y);
+          split(x[4] * sc, x[5] * sc, h4.z, l4.z);
+          split(x[6] * sc, x[7] * sc, h4.w, l4.w);
           *reinterpret_cast<uint4*>(&sm.d_out[0][row * DP + at]) = h4;
           if (L == 2) *reinterpret_cast<uint4*>(&sm.d_out[L - 1][row * DP + at]) = l4;
         }
       }
-      store_planes<DK / 8>(sm.state[0], sm.state[1], SP, st, pow2_scale(e_state), warp, lane);
-      if (tid < C) sm.fk[tid] = sm.gates.token[tid].fk;
-      pair_matrices<DK, NW, L, true>(sm.gates, sm.pairs, &sm.gram, sm.q[0], sm.k[0], warp, lane);
-      __syncthreads();
+      if (tid < C) {
+        const float fk = sm.gates.token[tid].fk;
+        sm.fk[tid] = fk, sm.inv_fk[tid] = 1.0f / fk, sm.inv_fq[tid] = 1.0f / sm.gates.fq[tid];
+      }
+      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], warp, lane);
 
-      // ---- phase A: this warp's value channels
+      // S0^T times K^T as the limbs are made; they also go to shared memory, for phase B
       float w[4][4] = {}, e[4][4] = {};
       const float keep = sm.gates.keep;
-      {
-        float end = 0.0f;  // of <S_C, R>
-        if (keep != 0.0f) {
+      float end = 0.0f, u_state = 0.0f;  // end: this warp's part of <S_C, R>
+      if (has_state) {
+        if (has_r && keep != 0.0f) {
 #pragma unroll
           for (int n = 0; n < DK / 8; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x) end = fmaf(st[n][x], rt[n][x], end);
           end *= keep;
         }
-        int e0, e1, e2, e3;
-        row_exps<DK / 8>(st, e0, e1);
-        row_exps<DK / 8>(rt, e2, e3);
-        const float s0 = pow2_scale(e0), s1 = pow2_scale(e1), s2 = pow2_scale(e2), s3 = pow2_scale(e3);
+        const int ex = pow2_exp(__uint_as_float(sm.most_state));
+        const float sc = pow2_scale(ex);
+        u_state = pow2_unscale(ex);
 #pragma unroll
         for (int kk = 0; kk < DK; kk += 16) {
           uint32_t ah[4], al[4];
-          split_a(ah, al, st[kk / 8], st[kk / 8 + 1], s0, s1);
+          split_a(ah, al, st[kk / 8], st[kk / 8 + 1], sc, sc);
           state_times_rows<DK, L>(w, ah, al, sm.k[0], kk, lane);
-          split_a(ah, al, rt[kk / 8], rt[kk / 8 + 1], s2, s3);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int at = (c0 + gi + (h & 1) * 8) * SP + kk + (h >> 1) * 8 + qj;
+            *reinterpret_cast<uint32_t*>(&sm.state[0][at]) = ah[h];
+            *reinterpret_cast<uint32_t*>(&sm.state[1][at]) = al[h];
+          }
+        }
+      }
+      const int e_r = pow2_exp(__uint_as_float(sm.most_r));
+      const float u_r = pow2_unscale(e_r);
+      if (has_r) {
+        const float sc = pow2_scale(e_r);
+#pragma unroll
+        for (int kk = 0; kk < DK; kk += 16) {
+          uint32_t ah[4], al[4];
+          split_a(ah, al, rt[kk / 8], rt[kk / 8 + 1], sc, sc);
           state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, lane);
         }
-        const float f0 = pow2_unscale(e0), f1 = pow2_unscale(e1), f2 = pow2_unscale(e2), f3 = pow2_unscale(e3);
+      }
+      __syncthreads();
+
+      // ---- phase A: this warp's value channels
+      {
+        float v[4][4];
+        load_values(v, early.v + c0, VP, lane);
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 4; ++n) {
+          const float2 ak = *reinterpret_cast<const float2*>(&sm.gates.ak[n * 8 + qj]);
+          const float2 zk = *reinterpret_cast<const float2*>(&sm.gates.zk[n * 8 + qj]);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const int i = n * 8 + qj + (x & 1);
-            const float a = sm.gates.ak[i], z = sm.gates.zk[i];
-            const float v = In<T>::up(sm.v[i * VP + c0 + gi + (x >> 1) * 8]);
-            w[n][x] = a == 0.0f ? v : v - w[n][x] * ((x < 2 ? f0 : f1) * a);
-            e[n][x] = z == 0.0f ? 0.0f : e[n][x] * ((x < 2 ? f2 : f3) * z);
+            const float a = x & 1 ? ak.y : ak.x, z = x & 1 ? zk.y : zk.x;
+            w[n][x] = a == 0.0f ? v[n][x] : fmaf(-w[n][x], u_state * a, v[n][x]);
+            e[n][x] = z == 0.0f ? 0.0f : e[n][x] * (u_r * z);
           }
-        solve_forward(w, sm.pairs, lane);
+        }
+        solve_forward(w, early.pairs, lane);
+        if (has_r) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < 4; ++n) {
+            const float2 be = *reinterpret_cast<const float2*>(&sm.gates.beta[n * 8 + qj]);
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            end = fmaf(e[n][x], w[n][x] * sm.gates.beta[n * 8 + qj + (x & 1)], end);
+            for (int x = 0; x < 4; ++x) end = fmaf(e[n][x], w[n][x] * (x & 1 ? be.y : be.x), end);
+          }
 #pragma unroll
-        for (int m = 1; m < 32; m <<= 1) end += __shfl_xor_sync(kAll, end, m);
+          for (int m = 1; m < 32; m <<= 1) end += __shfl_xor_sync(kAll, end, m);
+        }
         if (lane == 0) sm.end_part[warp] = end;
       }
       // dU^T += dO^T P
@@ -414,15 +434,15 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           uint32_t ah[4], al[4] = {}, bh[4], bl[4];
           a_cols(ah, sm.d_out[0] + i * 16 * DP + c0, DP, lane);
           if (L == 2) a_cols(al, sm.d_out[L - 1] + i * 16 * DP + c0, DP, lane);
-          b_rows(bh, sm.pairs.p[0] + r * 16 * CP + i * 16, CP, lane);
-          b_rows(bl, sm.pairs.p[1] + r * 16 * CP + i * 16, CP, lane);
+          b_rows(bh, early.pairs.p[0] + r * 16 * CP + i * 16, CP, lane);
+          b_rows(bl, early.pairs.p[1] + r * 16 * CP + i * 16, CP, lane);
           mma2<L, 2>(acc[0], acc[1], ah, al, bh, bl);
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            e[2 * r + n][x] = fmaf(acc[n][x], u_out * sm.pairs.fp[r * 16 + n * 8 + qj + (x & 1)], e[2 * r + n][x]);
+            e[2 * r + n][x] = fmaf(acc[n][x], u_out * early.pairs.fp[r * 16 + n * 8 + qj + (x & 1)], e[2 * r + n][x]);
       }
       // dbeta: dU . w over this warp's channels; then dW = beta dU
 #pragma unroll
@@ -437,10 +457,11 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           const float be = sm.gates.beta[n * 8 + qj + x];
           e[n][x] *= be, e[n][x + 2] *= be;
         }
-      solve_backward(e, sm.pairs, lane);  // now dE^T
+      solve_backward(e, early.pairs, lane);  // now dE^T
       store_out(e, d_v, d.d_v.stride[1], t0, lo, hi, c0, dv, dv_pairs, lane);
-      raise(&sm.most_w, most_of<4>(w));
-      raise(&sm.most_e, most_of<4>(e));
+      int unused;
+      raise(&sm.most_w, unused, most_of<4>(w));
+      raise(&sm.most_e, unused, most_of<4>(e));
       __syncthreads();
       const int e_w = pow2_exp(__uint_as_float(sm.most_w)), e_e = pow2_exp(__uint_as_float(sm.most_e));
       const float u_w = pow2_unscale(e_w), u_e = pow2_unscale(e_e);
@@ -448,71 +469,67 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       store_planes<4>(sm.d_e[0], sm.d_e[1], CP, e, pow2_scale(e_e), warp, lane);
       __syncthreads();
 
-      // ---- token-by-token matrices of the gradients: jobs of 16 rows
-      for (int job = warp; job < 8; job += NW) {
-        const int kind = job >> 1, r = (job & 1) ^ (kind & 1);  // 0: M, 1: X, 2: M^T, 3: X^T; a warp gets long and short rows
-        const bool later = kind < 2;                             // rows are the later token
-        float acc[4][4] = {};
-        const int from = later ? 0 : r, to = later ? r + 1 : 2;
+      // ---- M and X, one 16 x 16 block a job: rows later tokens i, columns earlier tokens j
 #pragma unroll 1
+      for (int job = warp; job < 3; job += NW) {
+        const int r = (job + 1) >> 1, c = job >> 1;  // (0,0), (1,0), (1,1)
+        float am[2][4] = {}, ax[2][4] = {};
+#pragma unroll 2
         for (int kk = 0; kk < VC; kk += 16) {
-          uint32_t ah[4], al[4] = {};
-          if (kind == 0) {
-            a_rows(ah, sm.d_out[0] + r * 16 * DP + kk, DP, lane);
-            if (L == 2) a_rows(al, sm.d_out[L - 1] + r * 16 * DP + kk, DP, lane);
-          } else {
-            const __half* a = kind == 1 ? sm.d_e[0] : sm.w[0];
-            a_cols(ah, a + kk * CP + r * 16, CP, lane);
-            a_cols(al, a + VC * CP + kk * CP + r * 16, CP, lane);
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c < from || c >= to) continue;
-            uint32_t bh[4], bl[4] = {};
-            if (kind == 2) {
-              b_rows(bh, sm.d_out[0] + c * 16 * DP + kk, DP, lane);
-              if (L == 2) b_rows(bl, sm.d_out[L - 1] + c * 16 * DP + kk, DP, lane);
-            } else {
-              const __half* y = kind == 3 ? sm.d_e[0] : sm.w[0];
-              b_cols(bh, y + kk * CP + c * 16, CP, lane);
-              b_cols(bl, y + VC * CP + kk * CP + c * 16, CP, lane);
-            }
-            if (kind == 0 && L == 1) mma2<1, 2>(acc[2 * c], acc[2 * c + 1], ah, al, bh, bl);
-            else if (kind == 2 && L == 1) mma2<2, 1>(acc[2 * c], acc[2 * c + 1], ah, al, bh, bl);
-            else mma2<2, 2>(acc[2 * c], acc[2 * c + 1], ah, al, bh, bl);
-          }
+          uint32_t ah[4], al[4] = {}, bh[4], bl[4];
+          b_cols(bh, sm.w[0] + kk * CP + c * 16, CP, lane);
+          b_cols(bl, sm.w[1] + kk * CP + c * 16, CP, lane);
+          a_rows(ah, sm.d_out[0] + r * 16 * DP + kk, DP, lane);
+          if (L == 2) a_rows(al, sm.d_out[L - 1] + r * 16 * DP + kk, DP, lane);
+          mma2<L, 2>(am[0], am[1], ah, al, bh, bl);
+          a_cols(ah, sm.d_e[0] + kk * CP + r * 16, CP, lane);
+          a_cols(al, sm.d_e[1] + kk * CP + r * 16, CP, lane);
+          mma2<2, 2>(ax[0], ax[1], ah, al, bh, bl);
         }
-        const float unit = (kind & 1) ? -u_e * u_w : u_out * u_w;
-        __half* plane = kind == 0 ? sm.mk[0] : kind == 1 ? sm.xk[0] : kind == 2 ? sm.mq[0] : sm.xt[0];
-        float* factor = kind == 0 ? sm.fmk : kind == 1 ? sm.fxk : kind == 2 ? sm.fmq : sm.fxt;
+        const float um = u_out * u_w, ux = -u_e * u_w;
+        float mm = 0.0f, mx = 0.0f, db[4] = {};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int row = r * 16 + gi + half * 8;
-          float x[8], most = 0.0f, db = 0.0f;
+          const int i = r * 16 + gi + half * 8;
+          const Token ti = sm.gates.token[i];
+          const float fq = sm.gates.fq[i];
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
-            const int col = (n >> 1) * 8 + qj + (n & 1);
-            const int i = later ? row : col, j = later ? col : row;
-            const bool on = kind & 1 ? j < i : j <= i;
-            float y = on ? acc[n >> 1][half * 2 + (n & 1)] * unit : 0.0f;
-            if (kind == 3 && on) db = fmaf(y, sm.gram.at[i][j], db);
-            if (on) y *= sm.gates.beta[j] * decay(sm.gates.token[i], sm.gates.token[j]) * (kind == 2 ? sm.gates.fq[i] : later ? sm.gates.token[j].fk : sm.gates.token[i].fk);
-            x[n] = y;
-            most = fmaxf(most, fabsf(y));
-          }
-          most = quad_max(most);
-          const int ex = pow2_exp(most);
-          const float sc = pow2_scale(ex);
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            store_split(plane, plane + C * CP, row * CP + n * 8 + qj, x[2 * n] * sc, x[2 * n + 1] * sc);
-          if ((lane & 3) == 0) factor[row] = pow2_unscale(ex);
-          if (kind == 3) {
-            db += __shfl_xor_sync(kAll, db, 1);
-            db += __shfl_xor_sync(kAll, db, 2);
-            if ((lane & 3) == 0) sm.beta_pairs[row] = db;
+          for (int n = 0; n < 4; ++n) {
+            const int j = c * 16 + (n >> 1) * 8 + qj + (n & 1);
+            const Token tj = sm.gates.token[j];
+            float& ym = am[n >> 1][half * 2 + (n & 1)];
+            float& yx = ax[n >> 1][half * 2 + (n & 1)];
+            const float f = j <= i ? sm.gates.beta[j] * decay(ti, tj) * tj.fk : 0.0f;
+            const float x = yx * ux;  // -dE_i . w_j
+            if (j < i) db[n] = fmaf(x, sm.gram.at[i][j], db[n]);
+            ym = j <= i ? ym * um * (f * fq) : 0.0f;
+            yx = j < i ? x * (f * ti.fk) : 0.0f;
+            mm = fmaxf(mm, fabsf(ym)), mx = fmaxf(mx, fabsf(yx));
           }
         }
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+          mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, m)), mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, m));
+          if (m >= 4) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) db[n] += __shfl_xor_sync(kAll, db[n], m);
+          }
+        }
+        if (gi == 0) {  // of the earlier tokens: block column 0 has two blocks
+#pragma unroll
+          for (int n = 0; n < 4; ++n) sm.beta_pairs[r][c * 16 + (n >> 1) * 8 + qj + (n & 1)] = db[n];
+        }
+        const int em = pow2_exp(mm), ex = pow2_exp(mx);
+        const float sm_m = pow2_scale(em), sm_x = pow2_scale(ex);
+        if (lane == 0) sm.fm[job] = pow2_unscale(em), sm.fx[job] = pow2_unscale(ex);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int at = (r * 16 + gi + half * 8) * CP + c * 16 + n * 8 + qj;
+            store_split(late.m[0], late.m[1], at, am[n][2 * half] * sm_m, am[n][2 * half + 1] * sm_m);
+            store_split(late.x[0], late.x[1], at, ax[n][2 * half] * sm_x, ax[n][2 * half + 1] * sm_x);
+          }
       }
       __syncthreads();
 
@@ -522,47 +539,52 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       const bool works = group < GROUPS;
       float gq[N][4] = {}, g_row[N][4] = {}, g_col[N][4] = {};
       if (works) {
-        const float a0 = sm.gates.carried[r * 16 + gi], a1 = sm.gates.carried[r * 16 + gi + 8];
-        float acc[N][4] = {};
-        rows_times_state<DK, NW, N, L, false>(acc, sm.d_out[0], DP, C * DP, sm.state[0], r, k0, lane);
+        if (has_state) {
+          const float a0 = sm.gates.carried[r * 16 + gi], a1 = sm.gates.carried[r * 16 + gi + 8];
+          float acc[N][4] = {};
+          rows_times_state<DK, NW, N, L, false>(acc, sm.d_out[0], DP, C * DP, sm.state[0], r, k0, lane);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float a = x < 2 ? a0 : a1;
-            gq[n][x] = a == 0.0f ? 0.0f : acc[n][x] * (a * u_out * u_state);
-            acc[n][x] = 0.0f;
-          }
-        rows_times_state<DK, NW, N, 2, true>(acc, sm.d_e[0], CP, VC * CP, sm.state[0], r, k0, lane);
+            for (int x = 0; x < 4; ++x) {
+              const float a = x < 2 ? a0 : a1;
+              gq[n][x] = a == 0.0f ? 0.0f : acc[n][x] * (a * u_out * u_state);
+              acc[n][x] = 0.0f;
+            }
+          rows_times_state<DK, NW, N, 2, true>(acc, sm.d_e[0], CP, VC * CP, sm.state[0], r, k0, lane);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float a = x < 2 ? a0 : a1;
-            g_row[n][x] = a == 0.0f ? 0.0f : acc[n][x] * (-a * u_e * u_state);
-          }
-        pairs_times_rows<DK, N, L>(gq, sm.mk[0], sm.fmk, sm.k[0], r, 0, r + 1, k0, lane);
-        pairs_times_rows<DK, N, L>(g_row, sm.xk[0], sm.fxk, sm.k[0], r, 0, r + 1, k0, lane);
-        pairs_times_rows<DK, N, L>(g_col, sm.mq[0], sm.fmq, sm.q[0], r, r, 2, k0, lane);
-        pairs_times_rows<DK, N, L>(g_col, sm.xt[0], sm.fxt, sm.k[0], r, r, 2, k0, lane);
+            for (int x = 0; x < 4; ++x) {
+              const float a = x < 2 ? a0 : a1;
+              g_row[n][x] = a == 0.0f ? 0.0f : acc[n][x] * (-a * u_e * u_state);
+            }
+        }
+        pairs_times_rows<DK, N, L, false>(gq, late.m[0], sm.fm, sm.inv_fq, sm.k[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, false>(g_row, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, true>(g_col, late.m[0], sm.fm, sm.inv_fk, sm.q[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, true>(g_col, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, k0, lane);
       }
-      __syncthreads();
-      const int e_r = pow2_exp(__uint_as_float(sm.most_r));
-      store_planes<DK / 8>(sm.state[0], sm.state[1], SP, rt, pow2_scale(e_r), warp, lane);
-      __syncthreads();
+      if (has_r) {
+        if (has_state) __syncthreads();
+        store_planes<DK / 8>(sm.state[0], sm.state[1], SP, rt, pow2_scale(e_r), warp, lane);
+        __syncthreads();
+      }
       if (works) {
-        float acc[N][4] = {};
-        rows_times_state<DK, NW, N, 2, true>(acc, sm.w[0], CP, VC * CP, sm.state[0], r, k0, lane);
-        const float u = u_w * pow2_unscale(e_r);
         const int i0 = r * 16 + gi;
-        const float z0 = sm.gates.to_end[i0] * sm.gates.beta[i0] * u, z1 = sm.gates.to_end[i0 + 8] * sm.gates.beta[i0 + 8] * u;
+        if (has_r) {
+          float acc[N][4] = {};
+          rows_times_state<DK, NW, N, 2, true>(acc, sm.w[0], CP, VC * CP, sm.state[0], r, k0, lane);
+          const float u = u_w * u_r;
+          const float z0 = sm.gates.to_end[i0] * sm.gates.beta[i0] * u, z1 = sm.gates.to_end[i0 + 8] * sm.gates.beta[i0 + 8] * u;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float z = x < 2 ? z0 : z1;
-            if (z != 0.0f) g_col[n][x] = fmaf(acc[n][x], z, g_col[n][x]);
-          }
+            for (int x = 0; x < 4; ++x) {
+              const float z = x < 2 ? z0 : z1;
+              if (z != 0.0f) g_col[n][x] = fmaf(acc[n][x], z, g_col[n][x]);
+            }
+        }
         float x0, x1;
         row_dots<DK, N, L>(gq, sm.q[0], sm.gates.fq, r, k0, lane, x0, x1);
         if ((lane & 3) == 0) sm.dot_q[group][i0] = x0, sm.dot_q[group][i0 + 8] = x1;
@@ -583,7 +605,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
                                   d.d_k.stride[1], t0, lo, hi, r, k0, dk, dk_pairs, lane);
       }
       if (warp == 0) {  // gates
-        float dg = 0.0f, db = sm.beta_pairs[lane];
+        float dg = 0.0f, db = sm.beta_pairs[1][lane] + (lane < 16 ? sm.beta_pairs[0][lane] : 0.0f);
         for (int g = 0; g < GROUPS; ++g) dg += sm.dot_q[g][lane] + sm.dot_row[g][lane] - sm.dot_col[g][lane];
         for (int v = 0; v < NW; ++v) db += sm.beta_part[v][lane];
         const int mine = sm.gates.token[lane].episode;
@@ -602,41 +624,36 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           d_beta[t * d.d_beta.stride[1]] = db;
         }
       }
-      // ---- R^T <- a_C R^T + (a dO)^T Q - (a dE)^T K
-      {
+      // ---- R^T <- a_C R^T + (a dO)^T Q - (a dE)^T K, where something still asks for it
+      const bool more = chunk > 0 || lo > t0 || d.d_initial != nullptr;
+      if (more) {
         float x[4][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 4; ++n) {
+          const float2 ak = *reinterpret_cast<const float2*>(&sm.gates.ak[n * 8 + qj]);
+          const float2 aq = *reinterpret_cast<const float2*>(&sm.gates.aq[n * 8 + qj]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int i = n * 8 + qj + (c & 1);
-            const float ak = sm.gates.ak[i], aq = sm.gates.aq[i];
-            const int at = i * DP + c0 + gi + (c >> 1) * 8;
+            const float fk = c & 1 ? ak.y : ak.x, fq = c & 1 ? aq.y : aq.x;
+            const int at = (n * 8 + qj + (c & 1)) * DP + c0 + gi + (c >> 1) * 8;
             float y = __half2float(sm.d_out[0][at]);
             if (L == 2) y += __half2float(sm.d_out[L - 1][at]);
-            x[n][c] = aq == 0.0f ? 0.0f : y * (aq * u_out);
-            e[n][c] = ak == 0.0f ? 0.0f : e[n][c] * -ak;
+            x[n][c] = fq == 0.0f ? 0.0f : y * (fq * u_out);
+            e[n][c] = fk == 0.0f ? 0.0f : e[n][c] * -fk;
           }
+        }
         state_update<DK, L>(rt, keep, x, sm.q[0], lane);
         state_update<DK, L>(rt, 1.0f, e, sm.k[0], lane);
+        has_r = true;
       }
       __syncthreads();
       if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0, sm.r_bad = 0, sm.most_out = sm.most_state = sm.most_r = sm.most_w = sm.most_e = 0;
       __syncthreads();
-      raise(&sm.most_r, most_of<DK / 8>(rt));
-      if (!finite<DK / 8>(rt)) sm.r_bad = 1;
+      if (more) raise(&sm.most_r, sm.r_bad, most_of<DK / 8>(rt));
       hi = lo;
     }
   }
-  if (d.d_initial) {
-#pragma unroll
-    for (int n = 0; n < DK / 8; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int c = c0 + gi + (x >> 1) * 8, r = n * 8 + qj + (x & 1);
-        if (c < dv && r < dk) d.d_initial[state_at + int64_t(r) * dv + c] = rt[n][x];
-      }
-  }
+  if (d.d_initial) for_state<DK, VC>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { d.d_initial[state_at + at] = x; });
 }
 
 // dq and dk of a key head: the sum over its value heads, in their order.

@@ -23,6 +23,7 @@ struct ForwardSmem {
   static constexpr int L = In<T>::limbs;
   Gates gates;
   Pairs pairs;
+  Squares squares;
   __align__(16) __half q[L][C * (DK + 8)];
   __align__(16) __half k[L][C * (DK + 8)];
   __align__(16) T v[C * (16 * NW + 16 / int(sizeof(T)))];
@@ -51,6 +52,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
   float st[DK / 8][4] = {};
   if (p.initial_state)
     for_state<DK, 16 * NW>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
+  bool has_state = p.initial_state != nullptr;  // there is a state in front of the chunk
   if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
   __syncthreads();
 
@@ -66,27 +68,25 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
     }
     for (int64_t lo = t0; lo < t1;) {
       int64_t hi = t1;
-      if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
-      load_rows<DK, NW, T>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, t0, lo, hi, tid);
       int e0, e1;
       if (!row_exps_finite<DK / 8>(st, e0, e1)) sm.gates.state_bad = 1;
-      __syncthreads();
-      // A value that is not finite must not reach another episode, nor an earlier token,
-      // through a product with zero: such a chunk is taken token by token.
-      if ((sm.gates.bad || (sm.gates.state_bad && sm.gates.marks != 0)) && hi - lo > 1) {
+#pragma unroll 1
+      for (;;) {
+        if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
+        load_rows<DK, NW, T, false>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, t0, lo, hi, tid);
+        __syncthreads();
+        // A value that is not finite must not reach another episode, nor an earlier token,
+        // through a product with zero: such a chunk is taken token by token.
+        if (hi - lo == 1 || !(sm.gates.bad || (sm.gates.state_bad && sm.gates.marks != 0))) break;
         hi = lo + 1;
         __syncthreads();
-        if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
-        if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
-        load_rows<DK, NW, T>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, t0, lo, hi, tid);
-        __syncthreads();
       }
-      pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, nullptr, sm.q[0], sm.k[0], warp, lane);
+      pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, sm.squares, nullptr, sm.q[0], sm.k[0], warp, lane);
       __syncthreads();
 
       // E^T = V^T - a (S0^T K^T), O^T = a (S0^T Q^T)
       float e[4][4] = {}, o[4][4] = {};
-      {
+      if (has_state) {
         const float s0 = pow2_scale(e0), s1 = pow2_scale(e1);
 #pragma unroll
         for (int kk = 0; kk < DK; kk += 16) {
@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         for (int x = 0; x < 4; ++x) e[n][x] *= x & 1 ? zk.y : zk.x;
       }
       state_update<DK, L>(st, sm.gates.keep, e, sm.k[0], lane);
+      has_state = true;
       __syncthreads();
       if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
       __syncthreads();

@@ -120,6 +120,7 @@ struct Gates {
   float fq[C];        // what takes the scaled row of Q to the normalised one
   float nk[C], nq[C]; // 1 / norm of the rows (1 where they are not normalised)
   float ak[C], aq[C], zk[C];  // a_i fk_i, a_i fq_i, D_Ci fk_i
+  unsigned most[2];   // largest magnitudes of Q and K, as float bits (backward)
   unsigned marks;     // the tokens that clear the state
   float keep;         // a_C: what is left of the state in front of the chunk
   int bad;            // some input of this chunk is not finite
@@ -257,7 +258,13 @@ __device__ __forceinline__ void unpack8(float (&x)[8], const Eight& r) {
 // All warps: rows of Q and K as scaled limb planes [C][DK + 8], their factors, and V as it is
 // [C][16 NW + 16 / sizeof(T)], zero for absent tokens and past the widths.  All loads of a batch are
 // under way before the first is used.
-template <int DK, int NW, class T>
+//
+// A row is scaled by its own largest value.  With normalised rows that leaves factors of nearly
+// one size (a row far below the norms' 1e-3 is not scaled up further, and an empty one neither).
+// UNIFORM (backward, which multiplies two rows' factors into one matrix and divides them out again):
+// rows that are not normalised share the largest value of the chunk's Q or K instead, found in a
+// pass of its own.
+template <int DK, int NW, class T, bool UNIFORM>
 __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, const Rows<T>& r, __half* qp, __half* kp, T* vp,
                                           int v0, int64_t t0, int64_t lo, int64_t hi, int tid) {
   constexpr int LR = DK / 8, PITCH = DK + 8, PLANE = C * PITCH, THREADS = NW * 32;
@@ -266,6 +273,23 @@ __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, cons
   constexpr int BATCH = sizeof(T) == 2 ? (JOBS < 4 ? JOBS : 4) : (JOBS < 2 ? JOBS : 2);
   const int dk = int(p.key_dim), dv = int(p.value_dim);
   bool bad = false;
+  if (UNIFORM && !p.normalize) {
+    if (tid < 2) s.most[tid] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int j = tid; j < 2 * C * LR; j += THREADS) {
+      const int row = (j / LR) % C, at = (j % LR) * 8;
+      const int64_t t = t0 + row;
+      if (t >= lo && t < hi && at < dk) {
+        float x[8], most = 0.0f;
+        unpack8<T>(x, fetch8(j >= C * LR ? r.k + t * p.k.stride[1] + at : r.q + t * p.q.stride[1] + at, dk - at, r.vec_qk));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+        if (most < INFINITY) atomicMax(&s.most[j >= C * LR], __float_as_uint(most));
+      }
+    }
+    __syncthreads();
+  }
   Eight v[VJOBS];
 #pragma unroll
   for (int u = 0; u < VJOBS; ++u) {
@@ -300,6 +324,8 @@ __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, cons
         most = fmaxf(most, __shfl_xor_sync(kAll, most, d));
       }
       bad |= !(sum < INFINITY);
+      if (p.normalize) most = fmaxf(most, 0x1p-12f);
+      else if (UNIFORM) most = fmaxf(__uint_as_float(s.most[is_k]), 0x1p-40f);
       const int e = pow2_exp(most);
       const float sc = pow2_scale(e);
       uint4 hi4, lo4;
@@ -338,7 +364,7 @@ __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, cons
 template <int DK, int LIMBS>
 __device__ __forceinline__ void rows_times_rows(float (&acc)[2][4], const __half* x, const __half* y, int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
-#pragma unroll
+#pragma unroll 2
   for (int kk = 0; kk < DK; kk += 16) {
     uint32_t a[4], b[4];
     a_rows(a, x + kk, PITCH, lane);
@@ -363,13 +389,15 @@ __device__ __forceinline__ void rows_times_rows(float (&acc)[2][4], const __half
 //   p: P_ij = D q_i.k_j (j <= i) with a scale for each row; backward: its transpose [C][CP]
 // gram (backward): D k_i.k_j, j < i.
 constexpr int kSquarePitch = 20;
+struct Squares {  // diagonal blocks of N, transposed, on their way to the inverses
+  __align__(16) float at[2][16 * kSquarePitch];
+};
 struct Pairs {
   __align__(16) __half n[2][16 * TP];
   __align__(16) __half t[2][C * TP];
   __align__(16) __half p[2][C * CP];
   __align__(16) float fp[C];
   float fn, ft[2];
-  __align__(16) float square[2][16 * kSquarePitch];  // diagonal blocks of N, transposed, on their way to the inverses
 };
 struct Gram {
   float at[C][C + 1];
@@ -385,7 +413,7 @@ __device__ __forceinline__ void store_split(__half* hi, __half* lo, int at, floa
 // One warp: N of both diagonal blocks and the inverses of I + N.  Lane c + 16 r solves column c of
 // block r by forward substitution, right-looking: a step's updates do not wait for one another.
 template <int DK, int LIMBS>
-__device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Gram* gram, const __half* kp, int lane) {
+__device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* kp, int lane) {
   constexpr int PITCH = DK + 8;
   const int gi = lane >> 2, qj = (lane & 3) * 2;
 #pragma unroll
@@ -401,7 +429,7 @@ __device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Gram
         const int j = (x >> 1) * 8 + qj + (x & 1);
         const Token tj = s.token[r * 16 + j];
         const float y = j < i ? acc[x >> 1][half * 2 + (x & 1)] * (ti.fk * tj.fk) * decay(ti, tj) : 0.0f;
-        m.square[r][j * kSquarePitch + i] = y * s.beta[r * 16 + j];
+        q.at[r][j * kSquarePitch + i] = y * s.beta[r * 16 + j];
         if (gram) gram->at[r * 16 + i][r * 16 + j] = y;
       }
     }
@@ -409,18 +437,18 @@ __device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Gram
   __syncwarp();
   float t[16];
   const int c = lane & 15, r = lane >> 4;
-  const float* sq = m.square[r];
+  const float* sq = q.at[r];
 #pragma unroll
   for (int i = 0; i < 16; ++i) t[i] = i == c ? 1.0f : 0.0f;
 #pragma unroll
   for (int j = 0; j < 15; ++j) {
 #pragma unroll
-    for (int q = (j + 1) & ~3; q < 16; q += 4) {
-      const float4 n = *reinterpret_cast<const float4*>(sq + j * kSquarePitch + q);
+    for (int i = (j + 1) & ~3; i < 16; i += 4) {
+      const float4 n = *reinterpret_cast<const float4*>(sq + j * kSquarePitch + i);
       const float w[4] = {n.x, n.y, n.z, n.w};
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        if (q + x > j) t[q + x] = fmaf(-w[x], t[j], t[q + x]);
+        if (i + x > j) t[i + x] = fmaf(-w[x], t[j], t[i + x]);
     }
   }
   float most = 0.0f;
@@ -536,11 +564,11 @@ __device__ __forceinline__ void score_columns(const Gates& s, Pairs& m, const __
 
 // All warps: the three kinds of matrices, spread over the warps.
 template <int DK, int NW, int LIMBS, bool BACKWARD>
-__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Gram* gram, const __half* qp, const __half* kp, int warp, int lane) {
+__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* qp, const __half* kp, int warp, int lane) {
 #pragma unroll 1
   for (int job = warp; job < 4; job += NW) {
     if (job == 0) {
-      diagonal_inverses<DK, LIMBS>(s, m, gram, kp, lane);
+      diagonal_inverses<DK, LIMBS>(s, m, q, gram, kp, lane);
     } else if (job < 3) {
       if (BACKWARD) score_columns<DK, LIMBS>(s, m, qp, kp, job - 1, lane);
       else score_rows<DK, LIMBS>(s, m, qp, kp, 2 - job, lane);
