@@ -300,11 +300,11 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       } else if (has_state) {
         for_state<DK, VC>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
       }
-      if (has_state) raise(&sm.most_state, sm.gates.state_bad, most_of<DK / 8>(st));
       Eight raw_out[2];
 #pragma unroll 1
       for (;;) {
-        if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
+        GateIn gates{};
+        if (warp == 0) gates = fetch_gates(p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int j = tid + u * NW * 32, row = j / (VC / 8), at = (j % (VC / 8)) * 8;
@@ -313,6 +313,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           if (t >= lo && t < hi && at < dv) raw_out[u] = fetch8(d_out + t * d.d_out.stride[1] + at, dv - at, vec_do);
         }
         load_rows<DK, NW, T, true>(sm.gates, p, rows, sm.q[0], sm.k[0], early.v, 0, t0, lo, hi, tid);
+        if (warp == 0) scan_gates(sm.gates, gates, lane);
         float most = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -322,6 +323,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(x[i]));
         }
         raise(&sm.most_out, sm.gates.bad, most);
+        if (has_state) raise(&sm.most_state, sm.gates.state_bad, most_of<DK / 8>(st));
         __syncthreads();
         // A value that is not finite must not reach another episode through a product with
         // zero: such a chunk is taken episode by episode.
@@ -331,6 +333,17 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         __syncthreads();
         if (tid == 0) sm.most_out = 0;
         __syncthreads();
+      }
+      if (chunk > 0) {  // the next chunk on its way
+        prefetch_rows<NW>(p, rows, t0 - C, 0, tid);
+        if (tid < C) {
+          const T* at = d_out + (t0 - C + tid) * d.d_out.stride[1];
+          for (int c = 0; c < dv; c += 128 / int(sizeof(T))) prefetch(at + c);
+        }
+        if (chunk > 1) {
+          const float* at = p.saved + ((int64_t(blockIdx.x) * (chunks - 1) + chunk - 2) * VC) * DK;
+          for (int c = tid * 32; c < VC * DK; c += NW * 32 * 32) prefetch(at + c);
+        }
       }
       const int e_out = pow2_exp(__uint_as_float(sm.most_out));
       const float u_out = pow2_unscale(e_out) * p.scale;

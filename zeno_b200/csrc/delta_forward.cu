@@ -72,8 +72,10 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
       if (!row_exps_finite<DK / 8>(st, e0, e1)) sm.gates.state_bad = 1;
 #pragma unroll 1
       for (;;) {
-        if (warp == 0) scan_gates(sm.gates, p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
+        GateIn gates{};
+        if (warp == 0) gates = fetch_gates(p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
         load_rows<DK, NW, T, false>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, t0, lo, hi, tid);
+        if (warp == 0) scan_gates(sm.gates, gates, lane);
         __syncthreads();
         // A value that is not finite must not reach another episode, nor an earlier token,
         // through a product with zero: such a chunk is taken token by token.
@@ -81,6 +83,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         hi = lo + 1;
         __syncthreads();
       }
+      if (t1 < T_) prefetch_rows<NW>(p, rows, t1, v0, tid);
       pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, sm.squares, nullptr, sm.q[0], sm.k[0], warp, lane);
       __syncthreads();
 

@@ -175,15 +175,27 @@ __device__ __forceinline__ Rows<T> rows_of(const ZenoDeltaRule& p, uint32_t b, u
   return r;
 }
 
-// Warp 0: the gates of tokens [t0, t0 + C) that lie in [lo, hi); the others are absent
-// (no decay, nothing written).  Returns with the token's own `bad` in every lane.
-__device__ __forceinline__ void scan_gates(Gates& s, const ZenoDeltaRule& p, const float* g, const float* beta,
-                                           const uint8_t* reset, int64_t t0, int64_t lo, int64_t hi, int lane) {
+// Warp 0: the gates of tokens [t0, t0 + C) that lie in [lo, hi), a token a lane; the others are
+// absent (no decay, nothing written).  Fetched first, scanned when the rows are under way.
+struct GateIn {
+  float g, beta;
+  bool here, mark;
+};
+__device__ __forceinline__ GateIn fetch_gates(const ZenoDeltaRule& p, const float* g, const float* beta, const uint8_t* reset, int64_t t0,
+                                              int64_t lo, int64_t hi, int lane) {
   const int64_t t = t0 + lane;
-  const bool here = t >= lo && t < hi;
-  float x = here ? g[t * p.g.stride[1]] : 0.0f;
-  const float be = here ? beta[t * p.beta.stride[1]] : 0.0f;
-  const bool mark = here && reset && reset[t * p.reset.stride[1]];
+  GateIn r;
+  r.here = t >= lo && t < hi;
+  r.g = r.here ? g[t * p.g.stride[1]] : 0.0f;
+  r.beta = r.here ? beta[t * p.beta.stride[1]] : 0.0f;
+  r.mark = r.here && reset && reset[t * p.reset.stride[1]];
+  return r;
+}
+
+__device__ __forceinline__ void scan_gates(Gates& s, const GateIn& in, int lane) {
+  float x = in.g;
+  const float be = in.beta;
+  const bool here = in.here, mark = in.mark;
   const bool clear = mark || expf(x) == 0.0f;  // a decay to nothing is a reset: the sums behind it stay finite
   if (clear) x = 0.0f;
   double sum = x;
@@ -218,12 +230,9 @@ struct Eight {
   uint4 a, b;  // b: the second half of 32-bit values
 };
 template <class T>
-__device__ __forceinline__ Eight fetch8(const T* at, int n, bool vec) {
+__device__ __noinline__ Eight fetch8_slow(const T* at, int n) {  // rows that are not 16-byte aligned, ragged ends
   Eight r;
-  if (vec && n >= 8) {
-    r.a = __ldg(reinterpret_cast<const uint4*>(at));
-    if (sizeof(T) == 4) r.b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
-  } else {
+  {
     uint32_t w[8] = {};
     if constexpr (sizeof(T) == 2) {
       const unsigned short* u = reinterpret_cast<const unsigned short*>(at);
@@ -238,6 +247,28 @@ __device__ __forceinline__ Eight fetch8(const T* at, int n, bool vec) {
     r.a = make_uint4(w[0], w[1], w[2], w[3]), r.b = make_uint4(w[4], w[5], w[6], w[7]);
   }
   return r;
+}
+template <class T>
+__device__ __forceinline__ Eight fetch8(const T* at, int n, bool vec) {
+  if (!vec || n < 8) return fetch8_slow<T>(at, n);
+  Eight r;
+  r.a = __ldg(reinterpret_cast<const uint4*>(at));
+  if (sizeof(T) == 4) r.b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+  return r;
+}
+__device__ __forceinline__ void prefetch(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
+// The rows of Q, K and V of the chunk at t0 (only its first address of each row and 128 bytes: a hint).
+template <int NW, class T>
+__device__ __forceinline__ void prefetch_rows(const ZenoDeltaRule& p, const Rows<T>& r, int64_t t0, int v0, int tid) {
+  constexpr int LINE = 128 / int(sizeof(T));
+  const int64_t t = t0 + tid % C;
+  if (t < 0 || t >= p.tokens) return;
+  for (int part = tid / C; part < 3 * 128 / LINE; part += NW) {
+    const int c = part / 3 * LINE;
+    if (part % 3 == 0 && c < int(p.key_dim)) prefetch(r.q + t * p.q.stride[1] + c);
+    if (part % 3 == 1 && c < int(p.key_dim)) prefetch(r.k + t * p.k.stride[1] + c);
+    if (part % 3 == 2 && v0 + c < int(p.value_dim)) prefetch(r.v + t * p.v.stride[1] + v0 + c);
+  }
 }
 template <class T>
 __device__ __forceinline__ void unpack8(float (&x)[8], const Eight& r) {
@@ -364,7 +395,7 @@ __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, cons
 template <int DK, int LIMBS>
 __device__ __forceinline__ void rows_times_rows(float (&acc)[2][4], const __half* x, const __half* y, int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
-#pragma unroll 2
+#pragma unroll
   for (int kk = 0; kk < DK; kk += 16) {
     uint32_t a[4], b[4];
     a_rows(a, x + kk, PITCH, lane);
