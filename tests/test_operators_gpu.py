@@ -126,6 +126,38 @@ def test_not_normalised_and_scale(dtype):
     check_gradients(x, dtype, normalize=False, scale=0.3)
 
 
+# few long rollouts, which are split over the tokens
+LONG = [(1, 1000, 1, 2, 64, 64, 0.01, True), (1, 4099, 1, 1, 128, 128, 0.001, True), (1, 777, 1, 1, 40, 24, 0.0, False),
+        (1, 1025, 1, 1, 33, 100, 0.003, True), (2, 600, 1, 2, 128, 32, None, True), (5, 288, 1, 2, 16, 16, 0.005, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,Hk,H,dk,dv,reset,initial", LONG)
+def test_long(B, T, Hk, H, dk, dv, reset, initial, dtype):
+    x = inputs(B, T, Hk, H, dk, dv, dtype, seed=T, reset=reset, initial=initial)
+    check_forward(x, dtype)
+    check_gradients(x, dtype)
+
+
+def test_long_with_an_episode_that_is_not_finite():
+    x = list(inputs(1, 1200, 1, 1, 32, 32, torch.float32, reset=0.0))
+    for t in (300, 700):
+        x[5][:, t] = 1
+    d_out, d_fin = torch.ones_like(x[2]), torch.ones((1, 1, 32, 32), device=DEV)
+    want, state = plain.delta_rule(*x)
+    grads = gradients(plain.delta_rule, [t.double() if t.is_floating_point() else t for t in x], d_out, d_fin)
+    x[2][0, 400, 0, 5] = float("nan")
+    out, final = zeno_b200.delta_rule(*x)
+    got = gradients(zeno_b200.delta_rule, x, d_out, d_fin)
+    check(final, state, torch.float32, "state")
+    for part in (slice(0, 400), slice(700, 1200)):
+        check(out[:, part], want[:, part], torch.float32, "outside the episode")
+    for a, b in zip(got[:5], grads[:5]):
+        for part in (slice(0, 300), slice(700, 1200)):
+            check(a[:, part], b[:, part], torch.float32, "gradients outside the episode")
+    check(got[5], grads[5], torch.float32, "d_initial")
+
+
 @pytest.mark.parametrize("reset", [None, 0.0, 0.3, 1.0])
 @pytest.mark.parametrize("initial", [False, True])
 def test_episodes(reset, initial):

@@ -26,7 +26,8 @@ def __getattr__(name):
     if name in _ENV_NAMES:
         return getattr(importlib.import_module(".env", __name__), name)
     if name in _OPERATOR_NAMES:
-        return getattr(importlib.import_module(".operators", __name__), name)
+        value = globals()[name] = getattr(importlib.import_module(".operators", __name__), name)  # looked up once
+        return value
     raise AttributeError(f"module 'zeno_b200' has no attribute {name!r}")
 
 

@@ -39,7 +39,7 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math"
 CU_SOURCES = ["step_kernel.cu", "fast_step.cu", "noalloc.cu", "math_eval.cu"]
 # the policy operators are ordinary floating-point code: fused multiply-adds are welcome
 OP_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
-OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_backward.cu", "delta_backward_f32.cu", "newton_schulz.cu",
+OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_walk.cu", "delta_backward.cu", "delta_backward_f32.cu", "newton_schulz.cu",
               "newton_schulz_small.cu"]
 CXX_SOURCES = ["mjcf.cpp", "model.cpp", "fast_model.cpp", "world.cpp", "capi.cpp", "policy_ops.cpp"]
 HEADERS = ["zeno_types.h", "devmath.cuh", "physics.cuh", "model_access.cuh", "stage_clock.cuh", "fast_model.h", "step_kernel.h", "scene.h", "model.h", "world.h",

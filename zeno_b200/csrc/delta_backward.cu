@@ -5,9 +5,10 @@ namespace zb {
 
 cudaError_t launch_delta_backward_f32(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream);
 
-// Shared key heads: 32-bit rows of dq and dk for each value head.
+// A split rollout's states; for shared key heads, 32-bit rows of dq and dk for each value head.
 uint64_t delta_backward_workspace(const ZenoDeltaRule& p) {
-  return p.key_heads == p.value_heads ? 0 : 2 * uint64_t(p.batch) * p.tokens * p.value_heads * p.key_dim * 4;
+  const uint64_t shared = p.key_heads == p.value_heads ? 0 : 2 * uint64_t(p.batch) * p.tokens * p.value_heads * p.key_dim * 4;
+  return delta::split_bytes(p) + shared;
 }
 
 cudaError_t launch_delta_backward(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream) {

@@ -17,6 +17,10 @@
 // accumulators for the whole rollout.  Phase B sums over the value channels, so W, dE, S0
 // and R pass through shared memory as limb planes, and a warp has 16 tokens and a share of
 // the key channels.
+//
+// Few long rollouts are cut into segments here too (see the forward pass): all but the first are run
+// for the R they leave alone, a walk back over the segments gives the R behind each, and all
+// segments run at once for the gradients.
 #pragma once
 #include "delta_mma.cuh"
 
@@ -240,14 +244,23 @@ __device__ __forceinline__ bool even(const ZenoTensor& t, int width) {
          ((t.stride[0] | t.stride[1] | t.stride[2]) & 1) == 0;
 }
 
-// Blocks of an SM.
+// Blocks of an SM: 384 threads of it where the registers allow (64 x 64, 4096 x 32 tokens: 1.9 ms with 256 threads,
+// before other changes), 256 where a warp's share of the key channels or the state takes 64 registers.
 template <int DK, int NW>
 constexpr int kBlocks = (DK == 32 || (DK == 64 && NW > 2) ? 384 : 256) / (NW * 32);
+
+struct BackSplit {
+  uint32_t segments, chunks;  // chunks of a segment
+  bool r_only;                // no gradients: the R in front of each segment, from zero behind it (the last: from d_final)
+  float* n;                   // ... [batch * heads][segments][dk][dv]
+  const float* state;         // else, with more than one segment: the R behind each
+};
 
 // OUT: type of the dq and dk rows (float: the workspace of shared heads, reduced afterwards).
 template <int DK, int NW, class T, class OUT>
 __global__ void __launch_bounds__(NW * 32, kBlocks<DK, NW>)
-delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_constant__ ZenoDeltaRuleGrads d) {
+delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_constant__ ZenoDeltaRuleGrads d,
+                      const __grid_constant__ BackSplit sp) {
   extern __shared__ __align__(16) unsigned char raw[];
   using Smem = BackwardSmem<DK, NW, T>;
   constexpr int L = In<T>::limbs, VC = 16 * NW, VP = VC + 16 / int(sizeof(T)), DP = VC + 8, SP = DK + 8;
@@ -274,23 +287,34 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
   float* d_beta = static_cast<float*>(d.d_beta.data) + int64_t(b) * d.d_beta.stride[0] + int64_t(h) * d.d_beta.stride[2];
   const int64_t state_at = int64_t(blockIdx.x) * dk * dv;
 
+  const bool r_only = sp.r_only;
+  const uint32_t segment = blockIdx.z;
+  if (r_only && segment == 0) return;
+  const int64_t segment_at = (int64_t(blockIdx.x) * sp.segments + segment) * dk * dv;
+  const float* r_from = !r_only && sp.segments > 1                          ? sp.state + segment_at
+                        : d.d_final && segment + 1 == sp.segments ? d.d_final + state_at
+                                                                  : nullptr;
+  float* r_to = r_only ? sp.n + segment_at : d.d_initial && segment == 0 ? d.d_initial + state_at : nullptr;
+
   float rt[DK / 8][4] = {};  // R^T
-  if (d.d_final) for_state<DK, VC>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { x = d.d_final[state_at + at]; });
-  bool has_r = d.d_final != nullptr;  // R is not zero
+  if (r_from) for_state<DK>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { x = r_from[at]; });
+  bool has_r = r_from != nullptr;  // R is not zero
   if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0, sm.r_bad = 0, sm.most_out = sm.most_state = sm.most_r = sm.most_w = sm.most_e = 0;
   __syncthreads();
   if (has_r) raise(&sm.most_r, sm.r_bad, most_of<DK / 8>(rt));
 
   const int64_t T_ = p.tokens;
   const int64_t chunks = (T_ + C - 1) / C;
-  for (int64_t chunk = chunks - 1; chunk >= 0; --chunk) {
+  const int64_t first = int64_t(segment) * sp.chunks, last = min(chunks, first + sp.chunks);
+  for (int64_t chunk = last - 1; chunk >= first; --chunk) {
     const int64_t t0 = chunk * C, t1 = min(t0 + C, T_);
     for (int64_t hi = t1; hi > t0;) {
       int64_t lo = t0;
       // ---- loads
-      bool has_state = chunk > 0 || p.initial_state != nullptr;
+      bool has_state = !r_only && (chunk > 0 || p.initial_state != nullptr);
       float st[DK / 8][4] = {};  // S0^T
-      if (chunk > 0) {
+      if (r_only) {
+      } else if (chunk > 0) {
         const float4* from = reinterpret_cast<const float4*>(p.saved + ((int64_t(blockIdx.x) * (chunks - 1) + chunk - 1) * VC + c0) * DK);
 #pragma unroll
         for (int n = 0; n < DK / 8; ++n) {
@@ -298,7 +322,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           st[n][0] = x.x, st[n][1] = x.y, st[n][2] = x.z, st[n][3] = x.w;
         }
       } else if (has_state) {
-        for_state<DK, VC>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
+        for_state<DK>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
       }
       Eight raw_out[2];
 #pragma unroll 1
@@ -312,7 +336,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           raw_out[u] = Eight{};
           if (t >= lo && t < hi && at < dv) raw_out[u] = fetch8(d_out + t * d.d_out.stride[1] + at, dv - at, vec_do);
         }
-        load_rows<DK, NW, T, true>(sm.gates, p, rows, sm.q[0], sm.k[0], early.v, 0, t0, lo, hi, tid);
+        load_rows<DK, NW, T, true>(sm.gates, p, rows, sm.q[0], sm.k[0], early.v, 0, r_only ? 0 : dv, t0, lo, hi, tid);
         if (warp == 0) scan_gates(sm.gates, gates, lane);
         float most = 0.0f;
 #pragma unroll
@@ -334,13 +358,13 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         if (tid == 0) sm.most_out = 0;
         __syncthreads();
       }
-      if (chunk > 0) {  // the next chunk on its way
+      if (chunk > first) {  // the next chunk on its way
         prefetch_rows<NW>(p, rows, t0 - C, 0, tid);
         if (tid < C) {
           const T* at = d_out + (t0 - C + tid) * d.d_out.stride[1];
           for (int c = 0; c < dv; c += 128 / int(sizeof(T))) prefetch(at + c);
         }
-        if (chunk > 1) {
+        if (chunk > 1 && !r_only) {
           const float* at = p.saved + ((int64_t(blockIdx.x) * (chunks - 1) + chunk - 2) * VC) * DK;
           for (int c = tid * 32; c < VC * DK; c += NW * 32 * 32) prefetch(at + c);
         }
@@ -367,7 +391,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         const float fk = sm.gates.token[tid].fk;
         sm.fk[tid] = fk, sm.inv_fk[tid] = 1.0f / fk, sm.inv_fq[tid] = 1.0f / sm.gates.fq[tid];
       }
-      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], warp, lane);
+      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], true, warp, lane);
 
       // S0^T times K^T as the limbs are made; they also go to shared memory, for phase B
       float w[4][4] = {}, e[4][4] = {};
@@ -411,18 +435,25 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       __syncthreads();
 
       // ---- phase A: this warp's value channels
-      {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float2 zk = *reinterpret_cast<const float2*>(&sm.gates.zk[n * 8 + qj]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float z = x & 1 ? zk.y : zk.x;
+          e[n][x] = z == 0.0f ? 0.0f : e[n][x] * (u_r * z);
+        }
+      }
+      if (!r_only) {
         float v[4][4];
         load_values(v, early.v + c0, VP, lane);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const float2 ak = *reinterpret_cast<const float2*>(&sm.gates.ak[n * 8 + qj]);
-          const float2 zk = *reinterpret_cast<const float2*>(&sm.gates.zk[n * 8 + qj]);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const float a = x & 1 ? ak.y : ak.x, z = x & 1 ? zk.y : zk.x;
+            const float a = x & 1 ? ak.y : ak.x;
             w[n][x] = a == 0.0f ? v[n][x] : fmaf(-w[n][x], u_state * a, v[n][x]);
-            e[n][x] = z == 0.0f ? 0.0f : e[n][x] * (u_r * z);
           }
         }
         solve_forward(w, early.pairs, lane);
@@ -462,15 +493,18 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float s = fmaf(e[n][x], w[n][x], e[n][x + 2] * w[n][x + 2]);
-          s += __shfl_xor_sync(kAll, s, 4);
-          s += __shfl_xor_sync(kAll, s, 8);
-          s += __shfl_xor_sync(kAll, s, 16);
-          if (gi == 0) sm.beta_part[warp][n * 8 + qj + x] = s;
+          if (!r_only) {
+            float s = fmaf(e[n][x], w[n][x], e[n][x + 2] * w[n][x + 2]);
+            s += __shfl_xor_sync(kAll, s, 4);
+            s += __shfl_xor_sync(kAll, s, 8);
+            s += __shfl_xor_sync(kAll, s, 16);
+            if (gi == 0) sm.beta_part[warp][n * 8 + qj + x] = s;
+          }
           const float be = sm.gates.beta[n * 8 + qj + x];
           e[n][x] *= be, e[n][x + 2] *= be;
         }
       solve_backward(e, early.pairs, lane);  // now dE^T
+      if (!r_only) {
       store_out(e, d_v, d.d_v.stride[1], t0, lo, hi, c0, dv, dv_pairs, lane);
       int unused;
       raise(&sm.most_w, unused, most_of<4>(w));
@@ -637,8 +671,10 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           d_beta[t * d.d_beta.stride[1]] = db;
         }
       }
+      }
+
       // ---- R^T <- a_C R^T + (a dO)^T Q - (a dE)^T K, where something still asks for it
-      const bool more = chunk > 0 || lo > t0 || d.d_initial != nullptr;
+      const bool more = chunk > first || lo > t0 || r_to != nullptr;
       if (more) {
         float x[4][4];
 #pragma unroll
@@ -666,7 +702,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       hi = lo;
     }
   }
-  if (d.d_initial) for_state<DK, VC>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { d.d_initial[state_at + at] = x; });
+  if (r_to) for_state<DK>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { r_to[at] = x; });
 }
 
 // dq and dk of a key head: the sum over its value heads, in their order.
@@ -687,50 +723,88 @@ shared_heads_kernel(const float* part, ZenoTensor out, uint64_t rows, uint32_t t
   }
 }
 
+// Segments of a call: as many as fill the SMs with blocks, each of at least 4 chunks.
+// (8 environments x 8 heads of 128 x 128, 1000 tokens, with the forward pass: 979 us in 2 segments, 1161 whole.)
+inline uint32_t back_segments(const ZenoDeltaRule& p) {
+  const uint64_t chunks = (uint64_t(p.tokens) + C - 1) / C, blocks = uint64_t(p.batch) * p.value_heads;
+  const int warps = value_groups(p), width = key_width(p);
+  const uint64_t slots = 148ull * ((width == 32 || (width == 64 && warps > 2) ? 12 : 8) / warps);
+  uint64_t n = blocks ? slots / blocks : 1;
+  if (n > chunks / 4) n = chunks / 4;
+  return n < 2 ? 1 : uint32_t(n);
+}
+
 template <int DK, int NW, class T, class OUT>
-cudaError_t launch(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, cudaStream_t stream) {
+cudaError_t launch(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, char* workspace, cudaStream_t stream) {
   const auto kernel = delta_backward_kernel<DK, NW, T, OUT>;
   constexpr int smem = int(sizeof(BackwardSmem<DK, NW, T>));
   static_assert(smem <= 227 * 1024, "shared memory of a block");
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e = allow_smem(kernel, smem, allowed);
+  cudaError_t e = allow_smem(kernel, smem, allowed);
   if (e != cudaSuccess) return e;
-  kernel<<<p.batch * p.value_heads, NW * 32, smem, stream>>>(p, d);
+  const uint32_t rows = p.batch * p.value_heads, segments = back_segments(p);
+  BackSplit sp{};
+  sp.segments = 1, sp.chunks = (p.tokens + C - 1) / C;
+  if (segments > 1) {
+    const DeltaSplitLayout lay(p, segments);
+    float* m = reinterpret_cast<float*>(workspace);
+    float* state = reinterpret_cast<float*>(workspace + lay.m + lay.n);
+    int* cleared = reinterpret_cast<int*>(workspace + lay.m + 2 * lay.n);
+    sp.n = reinterpret_cast<float*>(workspace + lay.m);
+    sp.chunks = (sp.chunks + segments - 1) / segments;
+    sp.segments = ((p.tokens + C - 1) / C + sp.chunks - 1) / sp.chunks;  // none of them empty
+    if (sp.segments > 2) e = launch_delta_transitions(p, m, cleared, sp.segments, sp.chunks, stream);
+    if (e != cudaSuccess) return e;
+    sp.r_only = true;
+    kernel<<<dim3(rows, 1, sp.segments), NW * 32, smem, stream>>>(p, d, sp);
+    e = cudaGetLastError();
+    if (e == cudaSuccess)
+      e = launch_delta_walk(DeltaWalk{m, sp.n, state, cleared, d.d_final, sp.segments, p.key_dim, p.value_dim, true}, rows, stream);
+    if (e != cudaSuccess) return e;
+    sp.r_only = false, sp.state = state;
+  }
+  kernel<<<dim3(rows, 1, sp.segments), NW * 32, smem, stream>>>(p, d, sp);
   return cudaGetLastError();
 }
 
 template <int DK, class T, class OUT>
-cudaError_t by_width(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, cudaStream_t stream) {
-  switch (value_warps(p)) {
+cudaError_t by_width(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, char* workspace, cudaStream_t stream) {
+  switch (value_groups(p)) {
     case 2:
-      if constexpr (DK < 128) return launch<DK, 2, T, OUT>(p, d, stream);
-    case 4: return launch<DK, 4, T, OUT>(p, d, stream);
-    default: return launch<DK, 8, T, OUT>(p, d, stream);
+      if constexpr (DK < 128) return launch<DK, 2, T, OUT>(p, d, workspace, stream);
+    case 4: return launch<DK, 4, T, OUT>(p, d, workspace, stream);
+    default: return launch<DK, 8, T, OUT>(p, d, workspace, stream);
   }
 }
 
 template <class T, class OUT>
-cudaError_t by_rows(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, cudaStream_t stream) {
+cudaError_t by_rows(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, char* workspace, cudaStream_t stream) {
   switch (key_width(p)) {
-    case 32: return by_width<32, T, OUT>(p, d, stream);
-    case 64: return by_width<64, T, OUT>(p, d, stream);
-    default: return by_width<128, T, OUT>(p, d, stream);
+    case 32: return by_width<32, T, OUT>(p, d, workspace, stream);
+    case 64: return by_width<64, T, OUT>(p, d, workspace, stream);
+    default: return by_width<128, T, OUT>(p, d, workspace, stream);
   }
+}
+
+inline uint64_t split_bytes(const ZenoDeltaRule& p) {
+  const uint32_t segments = back_segments(p);
+  return segments > 1 ? DeltaSplitLayout(p, segments).total : 0;
 }
 
 template <class T>
 cudaError_t by_heads(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream) {
-  if (p.key_heads == p.value_heads) return by_rows<T, T>(p, d, stream);
+  if (p.key_heads == p.value_heads) return by_rows<T, T>(p, d, static_cast<char*>(workspace), stream);
   const uint64_t rows = uint64_t(p.batch) * p.tokens * p.key_heads;
   const uint32_t group = p.value_heads / p.key_heads;
-  float* part_q = static_cast<float*>(workspace);
+  char* at = static_cast<char*>(workspace);  // the segments' part, then the rows'
+  float* part_q = reinterpret_cast<float*>(at + split_bytes(p));
   float* part_k = part_q + rows * group * p.key_dim;
   ZenoDeltaRuleGrads x = d;
   const int64_t width = p.key_dim;
   for (ZenoTensor* t : {&x.d_q, &x.d_k})
     t->stride[2] = width, t->stride[1] = width * p.value_heads, t->stride[0] = width * p.value_heads * int64_t(p.tokens);
   x.d_q.data = part_q, x.d_k.data = part_k;
-  cudaError_t e = by_rows<T, float>(p, x, stream);
+  cudaError_t e = by_rows<T, float>(p, x, at, stream);
   if (e != cudaSuccess || rows == 0) return e;
   const uint64_t blocks = (rows * p.key_dim + 255) / 256;
   const unsigned grid = unsigned(blocks < 148 * 8 ? blocks : 148 * 8);

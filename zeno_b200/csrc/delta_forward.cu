@@ -12,11 +12,28 @@
 // (W^T = E^T (I + N)^-T, O^T = S^T Q^T + U^T P^T, S^T <- S^T + U^T K) each product's left
 // operand is the previous one's accumulators, so state, errors and outputs never leave the
 // registers, and warps meet only where the token-by-token matrices are made.
+//
+// Few long rollouts.  A stretch of tokens takes the state in front of it to M S + N.  Where the
+// environments and heads alone do not fill the GPU, the tokens are cut into segments; one launch
+// runs every segment from the identity with V = 0 (its M) and from zero (its N), one walks over the
+// segments' states, and one runs all segments again, each from its own state, for the outputs:
+// about 2.5 times the work on the SMs that would have stood idle.
 #include "delta_mma.cuh"
 
 namespace zb {
 namespace delta {
 namespace {
+
+enum Mode { kWhole, kTransitions, kOutputs };
+struct Split {
+  Mode mode;
+  uint32_t segments, chunks;  // chunks of a segment
+  float* m;        // [batch * heads][segments][dk][dk]
+  float* n;        // ... [dk][dv]: what a segment leaves of nothing (the first one: of initial_state)
+  float* state;    // ... [dk][dv]: the state in front of a segment
+  int* cleared;    // ... whether the segment drops the state in front of it
+  uint32_t value_blocks;  // kTransitions: blocks of N in the grid's second dimension, those of M behind them
+};
 
 template <int DK, int NW, class T>
 struct ForwardSmem {
@@ -32,7 +49,7 @@ struct ForwardSmem {
 template <int DK, int NW, class T>
 // Threads of an SM: 512 where the state is 32 registers a thread (4096 x 32 tokens, 64 x 64: 461 us against 544 with
 // 384 and 714 with 256), 384 where it is 64 (2 x 4096 tokens, 128 x 128: 1250 us against 1405 with 512).
-__global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) delta_forward_kernel(const __grid_constant__ ZenoDeltaRule p) {
+__global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) delta_forward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_constant__ Split sp) {
   extern __shared__ __align__(16) unsigned char raw[];
   using Smem = ForwardSmem<DK, NW, T>;
   constexpr int L = In<T>::limbs;
@@ -40,27 +57,47 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qj = (lane & 3) * 2;
   const uint32_t h = blockIdx.x % p.value_heads, b = blockIdx.x / p.value_heads;
-  const int dk = int(p.key_dim), dv = int(p.value_dim);
-  const int v0 = int(blockIdx.y) * 16 * NW;
+  const int dk = int(p.key_dim);
+  const uint32_t segment = blockIdx.z;
+  const bool outputs = sp.mode != kTransitions, is_m = !outputs && blockIdx.y >= sp.value_blocks;
+  if (is_m && segment == 0) return;
+  const int dv = is_m ? dk : int(p.value_dim);  // columns of this block's state
+  const int v0 = int(blockIdx.y - (is_m ? sp.value_blocks : 0)) * 16 * NW;
   const int c0 = v0 + warp * 16;  // the warp's first channel
   const Rows<T> rows = rows_of<T>(p, b, h);
   T* out = static_cast<T*>(p.out.data) + int64_t(b) * p.out.stride[0] + int64_t(h) * p.out.stride[2];
   const bool pairs_ok = sizeof(T) == 2 && dv % 2 == 0 && reinterpret_cast<uintptr_t>(p.out.data) % 4 == 0 &&
                         ((p.out.stride[0] | p.out.stride[1] | p.out.stride[2]) & 1) == 0;
-  const int64_t state_at = int64_t(blockIdx.x) * dk * dv;
+  const int64_t state_size = int64_t(dk) * dv, row_at = int64_t(blockIdx.x) * state_size;
+  const int64_t segment_at = (int64_t(blockIdx.x) * sp.segments + segment) * state_size;
+  const float* initial = sp.mode == kOutputs                                     ? sp.state + segment_at
+                         : p.initial_state && !is_m && segment == 0 ? p.initial_state + row_at
+                                                                    : nullptr;
+  float* final_state = sp.mode == kTransitions     ? (is_m ? sp.m : sp.n) + segment_at
+                       : p.final_state && segment + 1 == sp.segments ? p.final_state + row_at
+                                                                     : nullptr;
 
   float st[DK / 8][4] = {};
-  if (p.initial_state)
-    for_state<DK, 16 * NW>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = p.initial_state[state_at + at]; });
-  bool has_state = p.initial_state != nullptr;  // there is a state in front of the chunk
+  if (initial) {
+    for_state<DK>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { x = initial[at]; });
+  } else if (is_m) {
+    const int gi = lane >> 2;
+#pragma unroll
+    for (int n = 0; n < DK / 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) st[n][x] = c0 + gi + (x >> 1) * 8 == n * 8 + qj + (x & 1) ? 1.0f : 0.0f;
+  }
+  bool has_state = initial || is_m;  // there is a state in front of the chunk
+  bool cleared = false;              // (M) some token has dropped it
   if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;
   __syncthreads();
 
   const int64_t T_ = p.tokens;
   const int64_t chunks = (T_ + C - 1) / C;
-  for (int64_t chunk = 0; chunk < chunks; ++chunk) {
+  const int64_t last = min(chunks, (int64_t(segment) + 1) * sp.chunks);
+  for (int64_t chunk = int64_t(segment) * sp.chunks; chunk < last; ++chunk) {
     const int64_t t0 = chunk * C, t1 = min(t0 + C, T_);
-    if (p.saved && chunk > 0) {
+    if (p.saved && outputs && chunk > 0) {
       const int64_t width = int64_t(gridDim.y) * 16 * NW;
       float4* to = reinterpret_cast<float4*>(p.saved + ((int64_t(blockIdx.x) * (chunks - 1) + chunk - 1) * width + c0) * DK);
 #pragma unroll
@@ -74,7 +111,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
       for (;;) {
         GateIn gates{};
         if (warp == 0) gates = fetch_gates(p, rows.g, rows.beta, rows.reset, t0, lo, hi, lane);
-        load_rows<DK, NW, T, false>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, t0, lo, hi, tid);
+        load_rows<DK, NW, T, false>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, is_m ? 0 : dv, t0, lo, hi, tid);
         if (warp == 0) scan_gates(sm.gates, gates, lane);
         __syncthreads();
         // A value that is not finite must not reach another episode, nor an earlier token,
@@ -84,7 +121,8 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         __syncthreads();
       }
       if (t1 < T_) prefetch_rows<NW>(p, rows, t1, v0, tid);
-      pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, sm.squares, nullptr, sm.q[0], sm.k[0], warp, lane);
+      pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, sm.squares, nullptr, sm.q[0], sm.k[0], outputs, warp, lane);
+      cleared |= sm.gates.marks != 0;
       __syncthreads();
 
       // E^T = V^T - a (S0^T K^T), O^T = a (S0^T Q^T)
@@ -96,7 +134,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
           uint32_t ah[4], al[4];
           split_a(ah, al, st[kk / 8], st[kk / 8 + 1], s0, s1);
           state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, lane);
-          state_times_rows<DK, L>(o, ah, al, sm.q[0], kk, lane);
+          if (outputs) state_times_rows<DK, L>(o, ah, al, sm.q[0], kk, lane);
         }
       }
       const float f0 = pow2_unscale(e0), f1 = pow2_unscale(e1);
@@ -121,7 +159,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
 #pragma unroll
         for (int x = 0; x < 4; ++x) e[n][x] *= x & 1 ? be.y : be.x;  // U^T
       }
-      {  // O^T += U^T P^T
+      if (outputs) {  // O^T += U^T P^T
         row_exps<4>(e, e0, e1);
         const float s0 = pow2_scale(e0), s1 = pow2_scale(e1), g0 = pow2_unscale(e0), g1 = pow2_unscale(e1);
         uint32_t uh[2][4], ul[2][4];
@@ -151,7 +189,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
           }
         }
       }
-      store_out(o, out, p.out.stride[1], t0, lo, hi, c0, dv, pairs_ok, lane);
+      if (outputs) store_out(o, out, p.out.stride[1], t0, lo, hi, c0, dv, pairs_ok, lane);
       // S^T <- a_C S^T + (D_C U)^T K
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -167,38 +205,86 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
       lo = hi;
     }
   }
-  if (p.final_state)
-    for_state<DK, 16 * NW>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { p.final_state[state_at + at] = x; });
+  if (final_state) for_state<DK>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { final_state[at] = x; });
+  if (is_m && v0 == 0 && tid == 0) sp.cleared[int64_t(blockIdx.x) * sp.segments + segment] = cleared;
+}
+
+// Segments of a call: enough to give every SM three blocks of 128 threads, each of at least 4 chunks;
+// 1 (not split) below 4 of them.  (2 environments x 8 heads of 128 x 128, 4096 tokens: 407 us in 13 segments, 963 whole.)
+inline uint32_t segments_of(const ZenoDeltaRule& p) {
+  const uint64_t chunks = (uint64_t(p.tokens) + C - 1) / C;
+  const int groups = value_groups(p), warps = groups < 4 ? groups : 4;
+  const uint64_t blocks = uint64_t(p.batch) * p.value_heads * (groups / warps);
+  uint64_t n = blocks ? uint64_t(148) * 12 / (blocks * warps) : 1;
+  if (n > chunks / 4) n = chunks / 4;
+  return n < 4 ? 1 : uint32_t(n);
 }
 
 template <int DK, int NW, class T>
-cudaError_t launch(const ZenoDeltaRule& p, cudaStream_t stream) {
+cudaError_t launch(const ZenoDeltaRule& p, const Split& sp, dim3 grid, cudaStream_t stream) {
   const auto kernel = delta_forward_kernel<DK, NW, T>;
   constexpr int smem = int(sizeof(ForwardSmem<DK, NW, T>));
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kernel, smem, allowed);
   if (e != cudaSuccess) return e;
-  const dim3 grid(p.batch * p.value_heads, (p.value_dim + 16 * NW - 1) / (16 * NW));
-  kernel<<<grid, NW * 32, smem, stream>>>(p);
+  kernel<<<grid, NW * 32, smem, stream>>>(p, sp);
   return cudaGetLastError();
 }
 
+template <int DK, int NW, class T>
+cudaError_t launch(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream) {
+  const uint32_t rows = p.batch * p.value_heads, segments = segments_of(p), blocks = uint32_t(value_groups(p) / NW);
+  Split sp{};
+  sp.segments = 1, sp.chunks = (p.tokens + C - 1) / C;
+  if (segments == 1) return launch<DK, NW, T>(p, sp, dim3(rows, blocks), stream);
+  const DeltaSplitLayout lay(p, segments);
+  char* at = static_cast<char*>(workspace);
+  sp.m = reinterpret_cast<float*>(at), sp.n = reinterpret_cast<float*>(at + lay.m), sp.state = reinterpret_cast<float*>(at + lay.m + lay.n);
+  sp.cleared = reinterpret_cast<int*>(at + lay.m + 2 * lay.n);
+  sp.mode = kTransitions, sp.chunks = (sp.chunks + segments - 1) / segments;
+  sp.segments = ((p.tokens + C - 1) / C + sp.chunks - 1) / sp.chunks;  // none of them empty
+  sp.value_blocks = blocks;
+  // nothing is asked of the last segment's transition
+  cudaError_t e = launch<DK, NW, T>(p, sp, dim3(rows, blocks + (DK + 16 * NW - 1) / (16 * NW), sp.segments - 1), stream);
+  if (e != cudaSuccess) return e;
+  e = launch_delta_walk(DeltaWalk{sp.m, sp.n, sp.state, sp.cleared, p.initial_state, sp.segments, p.key_dim, p.value_dim, false}, rows, stream);
+  if (e != cudaSuccess) return e;
+  sp.mode = kOutputs;
+  return launch<DK, NW, T>(p, sp, dim3(rows, blocks, sp.segments), stream);
+}
+
 template <int DK, class T>
-cudaError_t by_width(const ZenoDeltaRule& p, cudaStream_t stream) {
-  switch (value_warps(p)) {
+cudaError_t by_width(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream) {
+  const int groups = value_groups(p);
+  switch (groups == 8 && segments_of(p) > 1 ? 4 : groups) {
     case 2:
-      if constexpr (DK < 128) return launch<DK, 2, T>(p, stream);
-    case 4: return launch<DK, 4, T>(p, stream);
-    default: return launch<DK, 8, T>(p, stream);
+      if constexpr (DK < 128) return launch<DK, 2, T>(p, workspace, stream);
+    case 4: return launch<DK, 4, T>(p, workspace, stream);
+    default: return launch<DK, 8, T>(p, workspace, stream);
+  }
+}
+
+// The M of the segments of a backward pass.
+template <int DK, class T>
+cudaError_t transitions(const ZenoDeltaRule& p, const Split& sp, cudaStream_t stream) {
+  constexpr int NW = DK == 32 ? 2 : 4;
+  return launch<DK, NW, T>(p, sp, dim3(p.batch * p.value_heads, (DK + 16 * NW - 1) / (16 * NW), sp.segments - 1), stream);
+}
+template <class T>
+cudaError_t transitions_by_width(const ZenoDeltaRule& p, const Split& sp, cudaStream_t stream) {
+  switch (key_width(p)) {
+    case 32: return transitions<32, T>(p, sp, stream);
+    case 64: return transitions<64, T>(p, sp, stream);
+    default: return transitions<128, T>(p, sp, stream);
   }
 }
 
 template <class T>
-cudaError_t by_type(const ZenoDeltaRule& p, cudaStream_t stream) {
+cudaError_t by_type(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream) {
   switch (key_width(p)) {
-    case 32: return by_width<32, T>(p, stream);
-    case 64: return by_width<64, T>(p, stream);
-    default: return by_width<128, T>(p, stream);
+    case 32: return by_width<32, T>(p, workspace, stream);
+    case 64: return by_width<64, T>(p, workspace, stream);
+    default: return by_width<128, T>(p, workspace, stream);
   }
 }
 
@@ -209,12 +295,27 @@ cudaError_t by_type(const ZenoDeltaRule& p, cudaStream_t stream) {
 // accumulators' order: [batch * heads][chunks - 1][channels / 16][DK / 8][32 lanes][4].
 uint64_t delta_saved_bytes(const ZenoDeltaRule& p) {
   const uint64_t chunks = (uint64_t(p.tokens) + kDeltaChunk - 1) / kDeltaChunk;
-  const uint64_t rows = delta::key_width(p), channels = 16 * delta::value_warps(p);
+  const uint64_t rows = delta::key_width(p), channels = 16 * delta::value_groups(p);
   return chunks > 1 ? uint64_t(p.batch) * p.value_heads * (chunks - 1) * rows * channels * 4 : 0;
 }
 
-cudaError_t launch_delta_forward(const ZenoDeltaRule& p, cudaStream_t stream) {
-  return p.dtype == ZENO_DTYPE_BF16 ? delta::by_type<__nv_bfloat16>(p, stream) : delta::by_type<float>(p, stream);
+cudaError_t launch_delta_transitions(const ZenoDeltaRule& p, float* m, int* cleared, uint32_t segments, uint32_t chunks,
+                                     cudaStream_t stream) {
+  delta::Split sp{};
+  sp.mode = delta::kTransitions, sp.segments = segments, sp.chunks = chunks, sp.m = m, sp.cleared = cleared;
+  ZenoDeltaRule q = p;
+  q.saved = nullptr;
+  return p.dtype == ZENO_DTYPE_BF16 ? delta::transitions_by_width<__nv_bfloat16>(q, sp, stream)
+                                    : delta::transitions_by_width<float>(q, sp, stream);
+}
+
+uint64_t delta_forward_workspace(const ZenoDeltaRule& p) {
+  const uint32_t segments = delta::segments_of(p);
+  return segments == 1 ? 0 : DeltaSplitLayout(p, segments).total;
+}
+
+cudaError_t launch_delta_forward(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream) {
+  return p.dtype == ZENO_DTYPE_BF16 ? delta::by_type<__nv_bfloat16>(p, workspace, stream) : delta::by_type<float>(p, workspace, stream);
 }
 
 }  // namespace zb

@@ -287,7 +287,7 @@ __device__ __forceinline__ void unpack8(float (&x)[8], const Eight& r) {
 }
 
 // All warps: rows of Q and K as scaled limb planes [C][DK + 8], their factors, and V as it is
-// [C][16 NW + 16 / sizeof(T)], zero for absent tokens and past the widths.  All loads of a batch are
+// [C][16 NW + 16 / sizeof(T)], zero for absent tokens and past the widths (dv: V's).  All loads of a batch are
 // under way before the first is used.
 //
 // A row is scaled by its own largest value.  With normalised rows that leaves factors of nearly
@@ -297,12 +297,12 @@ __device__ __forceinline__ void unpack8(float (&x)[8], const Eight& r) {
 // pass of its own.
 template <int DK, int NW, class T, bool UNIFORM>
 __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, const Rows<T>& r, __half* qp, __half* kp, T* vp,
-                                          int v0, int64_t t0, int64_t lo, int64_t hi, int tid) {
+                                          int v0, int dv, int64_t t0, int64_t lo, int64_t hi, int tid) {
   constexpr int LR = DK / 8, PITCH = DK + 8, PLANE = C * PITCH, THREADS = NW * 32;
   constexpr int VC = 16 * NW, VP = VC + 16 / int(sizeof(T));
   constexpr int JOBS = 2 * C * LR / THREADS < 1 ? 1 : 2 * C * LR / THREADS, VJOBS = C * VC / 8 / THREADS;
   constexpr int BATCH = sizeof(T) == 2 ? (JOBS < 4 ? JOBS : 4) : (JOBS < 2 ? JOBS : 2);
-  const int dk = int(p.key_dim), dv = int(p.value_dim);
+  const int dk = int(p.key_dim);
   bool bad = false;
   if (UNIFORM && !p.normalize) {
     if (tid < 2) s.most[tid] = 0;
@@ -593,14 +593,16 @@ __device__ __forceinline__ void score_columns(const Gates& s, Pairs& m, const __
   }
 }
 
-// All warps: the three kinds of matrices, spread over the warps.
+// All warps: the three kinds of matrices, spread over the warps (P only where it is asked for).
 template <int DK, int NW, int LIMBS, bool BACKWARD>
-__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* qp, const __half* kp, int warp, int lane) {
+__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* qp, const __half* kp, bool scores, int warp,
+                                              int lane) {
 #pragma unroll 1
   for (int job = warp; job < 4; job += NW) {
     if (job == 0) {
       diagonal_inverses<DK, LIMBS>(s, m, q, gram, kp, lane);
     } else if (job < 3) {
+      if (!scores) continue;
       if (BACKWARD) score_columns<DK, LIMBS>(s, m, qp, kp, job - 1, lane);
       else score_rows<DK, LIMBS>(s, m, qp, kp, 2 - job, lane);
     } else {
@@ -713,16 +715,17 @@ __device__ __forceinline__ void load_values(float (&t)[4][4], const float* v, in
 #pragma unroll
     for (int x = 0; x < 4; ++x) t[n][x] = v[(n * 8 + (lane & 3) * 2 + (x & 1)) * pitch + (lane >> 2) + (x >> 1) * 8];
 }
-// A state [dk][dv] to and from a warp's transposed accumulators.  FULL: the widths are the kernel's own.
-template <int DK, int VC, class F>
+// A state [dk][dv] to and from a warp's transposed accumulators.
+template <int DK, class F>
 __device__ __forceinline__ void for_state(float (&st)[DK / 8][4], int dk, int dv, int c0, int lane, F f) {
   const int gi = lane >> 2, qj = (lane & 3) * 2;
-  if (dk == DK && dv == VC) {  // offsets known when compiled
-    const int64_t at = int64_t(qj) * VC + c0 + gi;
+  if (dk == DK && dv % 16 == 0) {  // nothing to leave out
+    if (c0 >= dv) return;
+    int64_t at = int64_t(qj) * dv + c0 + gi;
 #pragma unroll
-    for (int n = 0; n < DK / 8; ++n)
+    for (int n = 0; n < DK / 8; ++n, at += 8 * dv)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) f(st[n][x], at + (n * 8 + (x & 1)) * VC + (x >> 1) * 8);
+      for (int x = 0; x < 4; ++x) f(st[n][x], at + (x & 1 ? dv : 0) + (x >> 1) * 8);
   } else {
 #pragma unroll
     for (int n = 0; n < DK / 8; ++n)
@@ -830,9 +833,9 @@ __device__ __forceinline__ void store_out(const float (&o)[4][4], T* out, int64_
   }
 }
 
-// Padded widths of a call's kernels: key channels, and warps of 16 value channels.
+// Padded widths of a call's kernels: key channels, and value channels in groups of 16, a warp each.
 inline int key_width(const ZenoDeltaRule& p) { return p.key_dim <= 32 ? 32 : p.key_dim <= 64 ? 64 : 128; }
-inline int value_warps(const ZenoDeltaRule& p) {
+inline int value_groups(const ZenoDeltaRule& p) {
   const int nw = p.value_dim <= 32 ? 2 : p.value_dim <= 64 ? 4 : 8;
   return key_width(p) == 128 && nw < 4 ? 4 : nw;  // backward: a warp's share of the key channels is 64 at most
 }

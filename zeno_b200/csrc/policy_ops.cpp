@@ -90,7 +90,7 @@ uint64_t zeno_delta_rule_saved_bytes(const ZenoDeltaRule* p) {
 
 uint64_t zeno_delta_rule_workspace_bytes(const ZenoDeltaRule* p, uint32_t pass) {
   if (!p || !zb::shape_fault(*p).empty()) return 0;
-  return pass == ZENO_DELTA_BACKWARD ? zb::delta_backward_workspace(*p) : 0;
+  return pass == ZENO_DELTA_BACKWARD ? zb::delta_backward_workspace(*p) : zb::delta_forward_workspace(*p);
 }
 
 int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream) {
@@ -101,7 +101,7 @@ int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t wo
   if (workspace_bytes < zeno_delta_rule_workspace_bytes(p, ZENO_DELTA_FORWARD)) return zb::refuse(what, "workspace is too small");
   if (!zb::aligned(p->saved, 16) || !zb::aligned(workspace, 16)) return zb::refuse(what, "saved and workspace must be aligned to 16 bytes");
   if (!p->batch) return ZENO_SUCCESS;
-  return zb::status(what, zb::launch_delta_forward(*p, static_cast<cudaStream_t>(cuda_stream)));
+  return zb::status(what, zb::launch_delta_forward(*p, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 
 int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d, void* workspace, uint64_t workspace_bytes,

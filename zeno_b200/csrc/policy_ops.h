@@ -28,10 +28,29 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& devices)
   return e;
 }
 
+// A rollout in segments: what takes the state over a segment is M S + N.
+struct DeltaWalk {
+  const float* m;      // [rows][segments][dk][dk]
+  const float* n;      // [rows][segments][dk][dv]
+  float* state;        // written, same shape: in front of each segment (behind it in reverse)
+  const int* cleared;  // [rows][segments]: the segment drops the state
+  const float* initial;  // [rows][dk][dv] or NULL
+  uint32_t segments, dk, dv;
+  bool reverse;
+};
+struct DeltaSplitLayout {  // bytes of m, of n and of state, and of all with cleared behind them
+  uint64_t m, n, total;
+  DeltaSplitLayout(const ZenoDeltaRule& p, uint32_t segments);
+};
+cudaError_t launch_delta_walk(const DeltaWalk& w, uint32_t rows, cudaStream_t stream);
+cudaError_t launch_delta_transitions(const ZenoDeltaRule& p, float* m, int* cleared, uint32_t segments, uint32_t chunks,
+                                     cudaStream_t stream);
+
 uint64_t delta_saved_bytes(const ZenoDeltaRule& p);
 uint64_t delta_backward_workspace(const ZenoDeltaRule& p);
 cudaError_t launch_delta_recurrent(const ZenoDeltaRule& p, cudaStream_t stream);
-cudaError_t launch_delta_forward(const ZenoDeltaRule& p, cudaStream_t stream);
+uint64_t delta_forward_workspace(const ZenoDeltaRule& p);
+cudaError_t launch_delta_forward(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream);
 cudaError_t launch_delta_backward(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream);
 
 uint64_t orthogonalize_workspace(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype);
