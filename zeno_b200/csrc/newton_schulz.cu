@@ -199,7 +199,12 @@ __device__ __forceinline__ void tensor_load(float (&r)[32], uint32_t at) {
         "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
         "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(at));
+}
+// The loads in front of it have their values.  They pass through here, so that no use of them moves up.
+__device__ __forceinline__ void tensor_wait(float (&a)[32], float (&b)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i]));
 }
 
 // Four 8 x 8 tiles of 16-bit values to shared memory, lane l giving the address of row l % 8 of tile l / 8.
@@ -370,18 +375,21 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
 #pragma unroll 1
       for (int part = 0; part < 2; ++part) {
         const uint32_t r0 = quarter * 32 + part * 16, c0 = ((warp >> 2) - 1) * 64;
-        float v[32];
+        float v[32], w[32];
         const uint32_t at = tmem + (r0 << 16) + c0;
         tensor_load(v, at);
+        if (LIMBS == 2) tensor_load(w, at + 3 * kTile);
+        tensor_wait(v, w);
         if (LIMBS == 2) {
-          float w[32];
-#pragma unroll 1
-          for (int u = 1; u < 4; ++u) {
-            if (u < 3 && u >= stages) continue;
-            tensor_load(w, at + u * kTile);
+          float x[32];
+          const bool third = stages > 2;
+          tensor_load(x, at + kTile);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] += w[e];
-          }
+          for (int e = 0; e < 32; ++e) v[e] += w[e];
+          if (third) tensor_load(w, at + 2 * kTile);
+          tensor_wait(x, w);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] += third ? x[e] + w[e] : x[e];
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
