@@ -434,7 +434,8 @@ def matrix(shape, dtype, seed=0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (29, 64), (64, 29), (64, 64), (65, 100), (127, 129), (128, 512), (200, 513),
-                                   (300, 100), (512, 512), (3, 64, 80), (2, 2, 40, 130), (5, 260, 140), (1100, 700)])
+                                   (300, 100), (512, 512), (3, 64, 80), (2, 2, 40, 130), (5, 260, 140), (1100, 700),
+                                   (3, 20, 257), (2, 64, 512), (64, 513), (900, 33), (2, 17, 2049), (40, 4096), (50, 4100)])
 def test_orthogonalize(shape, dtype):
     m = matrix(shape, dtype)
     got = zeno_b200.orthogonalize(m)

@@ -33,7 +33,7 @@ __device__ __forceinline__ int first_extra(double inverse) {
 // ... and in front of step k
 __device__ __forceinline__ int extra_at(int first, uint32_t k) { return max(0, first - 2 * int(k)); }
 
-constexpr uint32_t kSmallRows = 64, kSmallCols = 512;
+constexpr uint32_t kSmallRows = 64, kSmallCols = 4096;
 cudaError_t launch_small(const void* update, const Matrix& s, bool transposed, void* out, uint32_t dtype, uint32_t steps,
                          cudaStream_t stream);
 

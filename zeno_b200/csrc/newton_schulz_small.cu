@@ -1,9 +1,14 @@
-// Newton-Schulz orthogonalisation of small matrices (64 x 512 at most): one block has one
-// matrix in shared memory from the norm to the last step.
+// Newton-Schulz orthogonalisation of matrices of at most 64 rows (or columns) by 4096: a cluster
+// of blocks has one matrix in shared memory from the norm to the last step, each block a share of
+// its columns.
 //
 // The same products as newton_schulz.cu, operands always in two f16 limbs, on mma.sync: at these
 // sizes a step's three products are a few hundred instructions a warp and the time is their
-// latency and the block's barriers, which launches of a tiled product would multiply.
+// latency and the blocks' barriers, which launches of a tiled product would multiply (and whose one
+// tile would walk over all columns by itself).  A = X X^T is a sum over the blocks, read from
+// one another's shared memory; A A and B are the same in all of them; B X needs a block's own columns.
+#include <cooperative_groups.h>
+
 #include "delta_mma.cuh"
 #include "newton_schulz.h"
 
@@ -38,20 +43,26 @@ __device__ __forceinline__ void join(float (&acc)[2][4], const float (&low)[2][4
   for (int x = 0; x < 8; ++x) acc[x >> 2][x & 3] += low[x >> 2][x & 3];
 }
 
-// WARPS warps; np <= 32 WARPS columns.
+// WARPS warps; at most 32 WARPS columns a block, `per` tiles of 16.
 template <int WARPS, class T>
 __global__ void __launch_bounds__(WARPS * 32)
-small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed) {
+small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed, int per) {
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ double sums[WARPS];
+  __shared__ double sums[WARPS], total;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, qj = (lane & 3) * 2;
-  const int m = int(s.m), n = int(s.n), mt = (m + 15) / 16, nt = (n + 15) / 16, pitch = nt * 16 + 8;
+  const auto cluster = cooperative_groups::this_cluster();
+  const int ranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const uint32_t matrix = blockIdx.x / ranks;
+  const int j0 = rank * per * 16;  // the block's first column
+  const int m = int(s.m), n = max(0, min(int(s.n) - j0, per * 16));
+  const int mt = (m + 15) / 16, nt = (n + 15) / 16, pitch = per * 16 + 8;
   __half* x = reinterpret_cast<__half*>(raw);
   const int xs = mt * 16 * pitch, as = mt * 16 * kPitch;  // a plane
   __half* a = x + 2 * xs;
   __half* b = a + 2 * as;
-  const T* at = from + int64_t(blockIdx.x) * s.matrix;
-  out += int64_t(blockIdx.x) * m * n;
+  float* part = reinterpret_cast<float*>(b);  // this block's part of A, before B is made
+  const T* at = from + int64_t(matrix) * s.matrix + j0 * s.col;
+  out += int64_t(matrix) * m * s.n + (transposed ? int64_t(j0) * m : j0);
   const bool by_row = s.col <= s.row;
 
   double sum = 0.0;
@@ -65,13 +76,21 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed) {
   __syncthreads();
   sum = 0.0;
   for (int w = 0; w < WARPS; ++w) sum += sums[w];
+  if (ranks > 1) {
+    if (tid == 0) total = sum;
+    cluster.sync();
+    sum = 0.0;
+    for (int r = 0; r < ranks; ++r) sum += *cluster.map_shared_rank(&total, r);
+    cluster.sync();
+  }
   const double inverse = 1.0 / (sqrt(sum) + kEps);
   if (steps == 0) {
     for (int e = tid; e < m * n; e += WARPS * 32) {
       const int i = transposed ? e % m : e / n, j = transposed ? e / m : e % n;
       const float y = float(inverse * up(at[i * s.row + j * s.col]));
-      if constexpr (sizeof(T) == 2) out[e] = __float2bfloat16_rn(y);
-      else out[e] = y;
+      T* to = out + (transposed ? int64_t(j) * m + i : int64_t(i) * s.n + j);
+      if constexpr (sizeof(T) == 2) *to = __float2bfloat16_rn(y);
+      else *to = y;
     }
     return;
   }
@@ -100,10 +119,30 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed) {
         products(acc, low, ah, al, bh, bl);
       }
       join(acc, low);
+      if (ranks > 1) {
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+          part[(r + gi + ((h >> 1) & 1) * 8) * kSmallRows + c + (h >> 2) * 8 + qj + (h & 1)] = acc[h >> 2][h & 3];
+        continue;
+      }
 #pragma unroll
       for (int h = 0; h < 4; ++h)
         store_split(a, a + as, (r + gi + (h & 1) * 8) * kPitch + c + (h >> 1) * 8 + qj, acc[h >> 1][(h & 1) * 2] * kUnscale,
                     acc[h >> 1][(h & 1) * 2 + 1] * kUnscale);
+    }
+    if (ranks > 1) {
+      cluster.sync();
+      for (int e = tid; e < mt * 16 * mt * 8; e += WARPS * 32) {
+        const int i = e / (mt * 8), j = e % (mt * 8) * 2;
+        float2 y = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+        for (int q = 0; q < ranks; ++q) {
+          const float2 z = *reinterpret_cast<const float2*>(cluster.map_shared_rank(part, q) + i * kSmallRows + j);
+          y.x += z.x, y.y += z.y;
+        }
+        store_split(a, a + as, i * kPitch + j, y.x * kUnscale, y.y * kUnscale);
+      }
+      cluster.sync();  // all have read: B may take the parts' place
     }
     __syncthreads();
     // B = b A + c A A
@@ -170,7 +209,7 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed) {
 #pragma unroll
             for (int q = 0; q < 2; ++q)
               if (i < m && j + q < n) {
-                T* to = out + (transposed ? int64_t(j + q) * m + i : int64_t(i) * n + j + q);
+                T* to = out + (transposed ? int64_t(j + q) * m + i : int64_t(i) * s.n + j + q);
                 if constexpr (sizeof(T) == 2) *to = __float2bfloat16_rn(v[q]);
                 else *to = v[q];
               }
@@ -183,22 +222,29 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed) {
 }
 
 template <int WARPS, class T>
-cudaError_t launch(const void* update, const Matrix& s, bool transposed, void* out, uint32_t steps, cudaStream_t stream) {
-  const int mp = int(s.m + 15) / 16 * 16, np = int(s.n + 15) / 16 * 16;
-  const int smem = 4 * mp * (np + 8 + 2 * kPitch);
+cudaError_t launch(const void* update, const Matrix& s, bool transposed, void* out, uint32_t steps, int ranks, int per, cudaStream_t stream) {
+  const int mp = int(s.m + 15) / 16 * 16;
+  // A and B always have room for 64 rows: the parts of A are kept in B's place
+  const int smem = 4 * mp * (per * 16 + 8) + 2 * 4 * int(kSmallRows) * kPitch;
   const auto kernel = small_kernel<WARPS, T>;
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e = allow_smem(kernel, 4 * int(kSmallRows) * int(kSmallCols + 8 + 2 * kPitch), allowed);
+  const cudaError_t e = allow_smem(kernel, 4 * int(kSmallRows) * (32 * WARPS + 8 + 2 * kPitch), allowed);
   if (e != cudaSuccess) return e;
-  kernel<<<s.count, WARPS * 32, smem, stream>>>(static_cast<const T*>(update), s, static_cast<T*>(out), steps, transposed);
-  return cudaGetLastError();
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(s.count * ranks), c.blockDim = dim3(WARPS * 32), c.dynamicSmemBytes = size_t(smem), c.stream = stream;
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeClusterDimension;
+  a.val.clusterDim.x = unsigned(ranks), a.val.clusterDim.y = 1, a.val.clusterDim.z = 1;
+  c.attrs = &a, c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, static_cast<const T*>(update), s, static_cast<T*>(out), steps, transposed, per);
 }
 
 template <class T>
 cudaError_t by_width(const void* update, const Matrix& s, bool transposed, void* out, uint32_t steps, cudaStream_t stream) {
-  // 8 tiles of 16 x 16 a warp are held in the registers
-  if (s.n <= 256) return launch<8, T>(update, s, transposed, out, steps, stream);
-  return launch<16, T>(update, s, transposed, out, steps, stream);
+  // 256 columns a block and 8 tiles of 16 x 16 a warp, held in its registers; past 2048 columns 512 and 16 warps
+  const int tiles = int(s.n + 15) / 16, ranks = tiles > 128 ? 8 : (tiles + 15) / 16, per = (tiles + ranks - 1) / ranks;
+  if (per <= 16) return launch<8, T>(update, s, transposed, out, steps, ranks, per, stream);
+  return launch<16, T>(update, s, transposed, out, steps, ranks, per, stream);
 }
 
 }  // namespace
