@@ -9,6 +9,8 @@
 // one another's shared memory; A A and B are the same in all of them; B X needs a block's own columns.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "delta_mma.cuh"
 #include "newton_schulz.h"
 
@@ -43,8 +45,10 @@ __device__ __forceinline__ void join(float (&acc)[2][4], const float (&low)[2][4
   for (int x = 0; x < 8; ++x) acc[x >> 2][x & 3] += low[x >> 2][x & 3];
 }
 
-// WARPS warps; at most 32 WARPS columns a block, `per` tiles of 16.
-template <int WARPS, class T>
+// 16 warps (with 8: 64 x 256 in 52 us against 43, 200 of them in 146 against 123); a block has `per`
+// tiles of 16 columns, 32 at most: a warp holds 8 tiles of 16 x 16 in its registers.
+constexpr int WARPS = 16;
+template <class T>
 __global__ void __launch_bounds__(WARPS * 32)
 small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed, int per) {
   extern __shared__ __align__(16) unsigned char raw[];
@@ -221,12 +225,12 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed, i
   }
 }
 
-template <int WARPS, class T>
+template <class T>
 cudaError_t launch(const void* update, const Matrix& s, bool transposed, void* out, uint32_t steps, int ranks, int per, cudaStream_t stream) {
   const int mp = int(s.m + 15) / 16 * 16;
   // A and B always have room for 64 rows: the parts of A are kept in B's place
   const int smem = 4 * mp * (per * 16 + 8) + 2 * 4 * int(kSmallRows) * kPitch;
-  const auto kernel = small_kernel<WARPS, T>;
+  const auto kernel = small_kernel<T>;
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kernel, 4 * int(kSmallRows) * (32 * WARPS + 8 + 2 * kPitch), allowed);
   if (e != cudaSuccess) return e;
@@ -241,10 +245,11 @@ cudaError_t launch(const void* update, const Matrix& s, bool transposed, void* o
 
 template <class T>
 cudaError_t by_width(const void* update, const Matrix& s, bool transposed, void* out, uint32_t steps, cudaStream_t stream) {
-  // 256 columns a block and 8 tiles of 16 x 16 a warp, held in its registers; past 2048 columns 512 and 16 warps
-  const int tiles = int(s.n + 15) / 16, ranks = tiles > 128 ? 8 : (tiles + 15) / 16, per = (tiles + ranks - 1) / ranks;
-  if (per <= 16) return launch<8, T>(update, s, transposed, out, steps, ranks, per, stream);
-  return launch<16, T>(update, s, transposed, out, steps, ranks, per, stream);
+  // 64 columns a block while all blocks run at once (64 x 256, 8 warps: 52 us against 73 in one block), else 256
+  // (200 of them: 146 us against 358); past 2048 columns up to 512.
+  const int tiles = int(s.n + 15) / 16, fine = std::min((tiles + 3) / 4, 8), coarse = std::min((tiles + 15) / 16, 8);
+  const int ranks = uint64_t(s.count) * fine <= 148 ? fine : coarse, per = (tiles + ranks - 1) / ranks;
+  return launch<T>(update, s, transposed, out, steps, ranks, per, stream);
 }
 
 }  // namespace
