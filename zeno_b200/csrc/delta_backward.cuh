@@ -105,11 +105,11 @@ __device__ __forceinline__ void mma2(float (&acc0)[4], float (&acc1)[4], const u
 // of its own, each row of the result a factor.
 template <int DK, int N, int L, bool TRANSPOSED>
 __device__ __forceinline__ void pairs_times_rows(float (&out)[N][4], const __half* plane, const float* scales, const float* row_factor,
-                                                 const __half* x, int r, int c0, int lane) {
+                                                 const __half* x, int r, int halves, int c0, int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
   const float r0 = row_factor[r * 16 + (lane >> 2)], r1 = row_factor[r * 16 + (lane >> 2) + 8];
 #pragma unroll 1
-  for (int j = TRANSPOSED ? r : 0; j < (TRANSPOSED ? 2 : r + 1); ++j) {
+  for (int j = TRANSPOSED ? r : 0; j < (TRANSPOSED ? halves : r + 1); ++j) {
     uint32_t ah[4], al[4];
     if (TRANSPOSED) {
       a_cols(ah, plane + j * 16 * CP + r * 16, CP, lane);
@@ -369,6 +369,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           for (int c = tid * 32; c < VC * DK; c += NW * 32 * 32) prefetch(at + c);
         }
       }
+      const int halves = hi - t0 <= 16 ? 1 : 2;
       const int e_out = pow2_exp(__uint_as_float(sm.most_out));
       const float u_out = pow2_unscale(e_out) * p.scale;
       {
@@ -391,7 +392,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         const float fk = sm.gates.token[tid].fk;
         sm.fk[tid] = fk, sm.inv_fk[tid] = 1.0f / fk, sm.inv_fq[tid] = 1.0f / sm.gates.fq[tid];
       }
-      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], true, warp, lane);
+      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], true, halves, warp, lane);
 
       // S0^T times K^T as the limbs are made; they also go to shared memory, for phase B
       float w[4][4] = {}, e[4][4] = {};
@@ -412,7 +413,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         for (int kk = 0; kk < DK; kk += 16) {
           uint32_t ah[4], al[4];
           split_a(ah, al, st[kk / 8], st[kk / 8 + 1], sc, sc);
-          state_times_rows<DK, L>(w, ah, al, sm.k[0], kk, lane);
+          state_times_rows<DK, L>(w, ah, al, sm.k[0], kk, halves, lane);
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             const int at = (c0 + gi + (h & 1) * 8) * SP + kk + (h >> 1) * 8 + qj;
@@ -429,7 +430,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         for (int kk = 0; kk < DK; kk += 16) {
           uint32_t ah[4], al[4];
           split_a(ah, al, rt[kk / 8], rt[kk / 8 + 1], sc, sc);
-          state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, lane);
+          state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, halves, lane);
         }
       }
       __syncthreads();
@@ -456,7 +457,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
             w[n][x] = a == 0.0f ? v[n][x] : fmaf(-w[n][x], u_state * a, v[n][x]);
           }
         }
-        solve_forward(w, early.pairs, lane);
+        solve_forward(w, early.pairs, halves, lane);
         if (has_r) {
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
@@ -472,9 +473,11 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       // dU^T += dO^T P
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
+        if (r == 1 && halves == 1) break;
         float acc[2][4] = {};
 #pragma unroll
         for (int i = r; i < 2; ++i) {
+          if (i == 1 && halves == 1) break;
           uint32_t ah[4], al[4] = {}, bh[4], bl[4];
           a_cols(ah, sm.d_out[0] + i * 16 * DP + c0, DP, lane);
           if (L == 2) a_cols(al, sm.d_out[L - 1] + i * 16 * DP + c0, DP, lane);
@@ -503,7 +506,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           const float be = sm.gates.beta[n * 8 + qj + x];
           e[n][x] *= be, e[n][x + 2] *= be;
         }
-      solve_backward(e, early.pairs, lane);  // now dE^T
+      solve_backward(e, early.pairs, halves, lane);  // now dE^T
       if (!r_only) {
       store_out(e, d_v, d.d_v.stride[1], t0, lo, hi, c0, dv, dv_pairs, lane);
       int unused;
@@ -518,7 +521,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
 
       // ---- M and X, one 16 x 16 block a job: rows later tokens i, columns earlier tokens j
 #pragma unroll 1
-      for (int job = warp; job < 3; job += NW) {
+      for (int job = warp; job < (halves == 1 ? 1 : 3); job += NW) {
         const int r = (job + 1) >> 1, c = job >> 1;  // (0,0), (1,0), (1,1)
         float am[2][4] = {}, ax[2][4] = {};
 #pragma unroll 2
@@ -583,7 +586,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       // ---- phase B: 16 tokens and a share of the key channels
       constexpr int DKW = 2 * DK / NW < 16 ? 16 : 2 * DK / NW, N = DKW / 8, GROUPS = DK / DKW;
       const int r = warp & 1, group = warp >> 1, k0 = group * DKW;
-      const bool works = group < GROUPS;
+      const bool works = group < GROUPS && r < halves;
       float gq[N][4] = {}, g_row[N][4] = {}, g_col[N][4] = {};
       if (works) {
         if (has_state) {
@@ -607,10 +610,10 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
               g_row[n][x] = a == 0.0f ? 0.0f : acc[n][x] * (-a * u_e * u_state);
             }
         }
-        pairs_times_rows<DK, N, L, false>(gq, late.m[0], sm.fm, sm.inv_fq, sm.k[0], r, k0, lane);
-        pairs_times_rows<DK, N, L, false>(g_row, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, k0, lane);
-        pairs_times_rows<DK, N, L, true>(g_col, late.m[0], sm.fm, sm.inv_fk, sm.q[0], r, k0, lane);
-        pairs_times_rows<DK, N, L, true>(g_col, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, false>(gq, late.m[0], sm.fm, sm.inv_fq, sm.k[0], r, halves, k0, lane);
+        pairs_times_rows<DK, N, L, false>(g_row, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, halves, k0, lane);
+        pairs_times_rows<DK, N, L, true>(g_col, late.m[0], sm.fm, sm.inv_fk, sm.q[0], r, halves, k0, lane);
+        pairs_times_rows<DK, N, L, true>(g_col, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, halves, k0, lane);
       }
       if (has_r) {
         if (has_state) __syncthreads();
@@ -652,8 +655,10 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
                                   d.d_k.stride[1], t0, lo, hi, r, k0, dk, dk_pairs, lane);
       }
       if (warp == 0) {  // gates
-        float dg = 0.0f, db = sm.beta_pairs[1][lane] + (lane < 16 ? sm.beta_pairs[0][lane] : 0.0f);
-        for (int g = 0; g < GROUPS; ++g) dg += sm.dot_q[g][lane] + sm.dot_row[g][lane] - sm.dot_col[g][lane];
+        const bool made = lane < 16 * halves;
+        float dg = 0.0f, db = lane < 16 ? sm.beta_pairs[0][lane] : 0.0f;
+        if (halves == 2) db += sm.beta_pairs[1][lane];
+        for (int g = 0; g < GROUPS && made; ++g) dg += sm.dot_q[g][lane] + sm.dot_row[g][lane] - sm.dot_col[g][lane];
         for (int v = 0; v < NW; ++v) db += sm.beta_part[v][lane];
         const int mine = sm.gates.token[lane].episode;
         if (lane == 31)
@@ -691,8 +696,8 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
             e[n][c] = fk == 0.0f ? 0.0f : e[n][c] * -fk;
           }
         }
-        state_update<DK, L>(rt, keep, x, sm.q[0], lane);
-        state_update<DK, L>(rt, 1.0f, e, sm.k[0], lane);
+        state_update<DK, L>(rt, keep, x, sm.q[0], halves, lane);
+        state_update<DK, L>(rt, 1.0f, e, sm.k[0], halves, lane);
         has_r = true;
       }
       __syncthreads();

@@ -120,8 +120,9 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         hi = lo + 1;
         __syncthreads();
       }
+      const int halves = hi - t0 <= 16 ? 1 : 2;
       if (t1 < T_) prefetch_rows<NW>(p, rows, t1, v0, tid);
-      pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, sm.squares, nullptr, sm.q[0], sm.k[0], outputs, warp, lane);
+      pair_matrices<DK, NW, L, false>(sm.gates, sm.pairs, sm.squares, nullptr, sm.q[0], sm.k[0], outputs, halves, warp, lane);
       cleared |= sm.gates.marks != 0;
       __syncthreads();
 
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         for (int kk = 0; kk < DK; kk += 16) {
           uint32_t ah[4], al[4];
           split_a(ah, al, st[kk / 8], st[kk / 8 + 1], s0, s1);
-          state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, lane);
-          if (outputs) state_times_rows<DK, L>(o, ah, al, sm.q[0], kk, lane);
+          state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, halves, lane);
+          if (outputs) state_times_rows<DK, L>(o, ah, al, sm.q[0], kk, halves, lane);
         }
       }
       const float f0 = pow2_unscale(e0), f1 = pow2_unscale(e1);
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
           o[n][x] = a == 0.0f ? 0.0f : o[n][x] * (f * b);
         }
       }
-      solve_forward(e, sm.pairs, lane);  // now W^T
+      solve_forward(e, sm.pairs, halves, lane);  // now W^T
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const float2 be = *reinterpret_cast<const float2*>(&sm.gates.beta[n * 8 + qj]);
@@ -167,6 +168,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         for (int r = 0; r < 2; ++r) split_a(uh[r], ul[r], e[2 * r], e[2 * r + 1], s0, s1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          if (i == 1 && halves == 1) break;
           float acc[2][4] = {};
 #pragma unroll
           for (int r = 0; r <= i; ++r) {
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
 #pragma unroll
         for (int x = 0; x < 4; ++x) e[n][x] *= x & 1 ? zk.y : zk.x;
       }
-      state_update<DK, L>(st, sm.gates.keep, e, sm.k[0], lane);
+      state_update<DK, L>(st, sm.gates.keep, e, sm.k[0], halves, lane);
       has_state = true;
       __syncthreads();
       if (tid == 0) sm.gates.bad = 0, sm.gates.state_bad = 0;

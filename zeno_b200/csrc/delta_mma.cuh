@@ -444,11 +444,13 @@ __device__ __forceinline__ void store_split(__half* hi, __half* lo, int at, floa
 // One warp: N of both diagonal blocks and the inverses of I + N.  Lane c + 16 r solves column c of
 // block r by forward substitution, right-looking: a step's updates do not wait for one another.
 template <int DK, int LIMBS>
-__device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* kp, int lane) {
+__device__ __forceinline__ void diagonal_inverses(const Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* kp, int halves,
+                                                  int lane) {
   constexpr int PITCH = DK + 8;
   const int gi = lane >> 2, qj = (lane & 3) * 2;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
+    if (r == halves) break;
     float acc[2][4] = {};
     rows_times_rows<DK, LIMBS>(acc, kp + r * 16 * PITCH, kp + r * 16 * PITCH, lane);
 #pragma unroll
@@ -593,20 +595,22 @@ __device__ __forceinline__ void score_columns(const Gates& s, Pairs& m, const __
   }
 }
 
-// All warps: the three kinds of matrices, spread over the warps (P only where it is asked for).
+// All warps: the three kinds of matrices, spread over the warps (P only where it is asked for).  halves: 1 where
+// the chunk has no tokens past the 16th; nothing of the second half is made then, nor read (8192 rollouts of 8
+// tokens with gradients: 2.28 -> 1.94 ms; whole chunks pay for the branches, 4096 of 32 tokens 1.28 -> 1.30 ms).
 template <int DK, int NW, int LIMBS, bool BACKWARD>
-__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* qp, const __half* kp, bool scores, int warp,
+__device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* qp, const __half* kp, bool scores, int halves, int warp,
                                               int lane) {
 #pragma unroll 1
   for (int job = warp; job < 4; job += NW) {
     if (job == 0) {
-      diagonal_inverses<DK, LIMBS>(s, m, q, gram, kp, lane);
+      diagonal_inverses<DK, LIMBS>(s, m, q, gram, kp, halves, lane);
     } else if (job < 3) {
-      if (!scores) continue;
+      if (!scores || (halves == 1 && job == (BACKWARD ? 2 : 1))) continue;
       if (BACKWARD) score_columns<DK, LIMBS>(s, m, qp, kp, job - 1, lane);
       else score_rows<DK, LIMBS>(s, m, qp, kp, 2 - job, lane);
     } else {
-      lower_block<DK, LIMBS>(s, m, gram, kp, lane);
+      if (halves == 2) lower_block<DK, LIMBS>(s, m, gram, kp, lane);
       join_factors(s, lane);
     }
   }
@@ -633,13 +637,14 @@ __device__ __forceinline__ void times_block(float (&out)[2][4], const float (&t0
   }
 }
 
-__device__ __forceinline__ void solve_forward(float (&e)[4][4], const Pairs& m, int lane) {
+__device__ __forceinline__ void solve_forward(float (&e)[4][4], const Pairs& m, int halves, int lane) {
   float f0, f1, x[2][4];
   times_block(x, e[0], e[1], m.t[0], m.t[1], true, lane, f0, f1);  // W_0 = E_0 T_00^T
 #pragma unroll
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int c = 0; c < 4; ++c) e[n][c] = x[n][c] * ((c < 2 ? f0 : f1) * m.ft[0]);
+  if (halves == 1) return;
   times_block(x, e[0], e[1], m.n[0], m.n[1], true, lane, f0, f1);  // E_1 -= W_0 N_10^T
 #pragma unroll
   for (int n = 0; n < 2; ++n)
@@ -653,18 +658,20 @@ __device__ __forceinline__ void solve_forward(float (&e)[4][4], const Pairs& m, 
 }
 
 // dE^T = dW^T (I + N)^-1, in place: from the chunk's end to its begin.
-__device__ __forceinline__ void solve_backward(float (&e)[4][4], const Pairs& m, int lane) {
+__device__ __forceinline__ void solve_backward(float (&e)[4][4], const Pairs& m, int halves, int lane) {
   float f0, f1, x[2][4];
-  times_block(x, e[2], e[3], m.t[0] + 16 * TP, m.t[1] + 16 * TP, false, lane, f0, f1);
+  if (halves == 2) {
+    times_block(x, e[2], e[3], m.t[0] + 16 * TP, m.t[1] + 16 * TP, false, lane, f0, f1);
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) e[2 + n][c] = x[n][c] * ((c < 2 ? f0 : f1) * m.ft[1]);
-  times_block(x, e[2], e[3], m.n[0], m.n[1], false, lane, f0, f1);
+      for (int c = 0; c < 4; ++c) e[2 + n][c] = x[n][c] * ((c < 2 ? f0 : f1) * m.ft[1]);
+    times_block(x, e[2], e[3], m.n[0], m.n[1], false, lane, f0, f1);
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) e[n][c] -= x[n][c] * ((c < 2 ? f0 : f1) * m.fn);
+      for (int c = 0; c < 4; ++c) e[n][c] -= x[n][c] * ((c < 2 ? f0 : f1) * m.fn);
+  }
   times_block(x, e[0], e[1], m.t[0], m.t[1], false, lane, f0, f1);
 #pragma unroll
   for (int n = 0; n < 2; ++n)
@@ -740,10 +747,11 @@ __device__ __forceinline__ void for_state(float (&st)[DK / 8][4], int dk, int dv
 // out[4][4] += S^T X^T for the chunk's rows X (limb planes [C][DK + 8]), S scaled by s0, s1: [16 channels][C tokens].
 template <int DK, int LIMBS>
 __device__ __forceinline__ void state_times_rows(float (&out)[4][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                                 const __half* x, int kk, int lane) {
+                                                 const __half* x, int kk, int halves, int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
+    if (n == 1 && halves == 1) break;
     uint32_t b[4];
     b_rows(b, x + n * 16 * PITCH + kk, PITCH, lane);
     mma(out[2 * n], hi, b[0], b[1]);
@@ -760,7 +768,8 @@ __device__ __forceinline__ void state_times_rows(float (&out)[4][4], const uint3
 
 // S^T <- keep S^T + A X, A^T[16 channels][C tokens] unscaled accumulator tiles, X rows [C][DK + 8].
 template <int DK, int LIMBS>
-__device__ __forceinline__ void state_update(float (&st)[DK / 8][4], float keep, const float (&a)[4][4], const __half* x, int lane) {
+__device__ __forceinline__ void state_update(float (&st)[DK / 8][4], float keep, const float (&a)[4][4], const __half* x, int halves,
+                                             int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
   int e0, e1;
   row_exps<4>(a, e0, e1);
@@ -773,6 +782,7 @@ __device__ __forceinline__ void state_update(float (&st)[DK / 8][4], float keep,
     float acc[2][4] = {};
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (r == 1 && halves == 1) break;
       uint32_t b[4];
       b_cols(b, x + r * 16 * PITCH + kk, PITCH, lane);
       mma(acc[0], hi[r], b[0], b[1]);
