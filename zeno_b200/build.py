@@ -39,7 +39,8 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math"
 CU_SOURCES = ["step_kernel.cu", "fast_step.cu", "noalloc.cu", "math_eval.cu"]
 # the policy operators are ordinary floating-point code: fused multiply-adds are welcome
 OP_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
-OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_walk.cu", "delta_backward.cu", "delta_backward_f32.cu", "newton_schulz.cu",
+OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_walk.cu", "delta_backward.cu", "delta_backward_shared.cu",
+              "delta_backward_f32.cu", "newton_schulz.cu",
               "newton_schulz_small.cu"]
 CXX_SOURCES = ["mjcf.cpp", "model.cpp", "fast_model.cpp", "world.cpp", "capi.cpp", "policy_ops.cpp"]
 HEADERS = ["zeno_types.h", "devmath.cuh", "physics.cuh", "model_access.cuh", "stage_clock.cuh", "fast_model.h", "step_kernel.h", "scene.h", "model.h", "world.h",
@@ -77,6 +78,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
              for src in OP_SOURCES]
     jobs += [[cxx, *CXX_FLAGS, "-c", str(CSRC / src), "-o", str(OBJ_DIR / (src + ".o"))] for src in CXX_SOURCES]
     objs = [cmd[-1] for cmd in jobs]
+    jobs.sort(key=lambda cmd: "delta_" not in cmd[-3])  # the longest first
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as pool:
         for f in [pool.submit(run, cmd) for cmd in jobs]:
             f.result()

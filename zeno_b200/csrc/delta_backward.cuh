@@ -796,9 +796,15 @@ inline uint64_t split_bytes(const ZenoDeltaRule& p) {
   return segments > 1 ? DeltaSplitLayout(p, segments).total : 0;
 }
 
+// Rows of a gradient of their own: dq and dk of the call's type, written by the kernel itself.
 template <class T>
-cudaError_t by_heads(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream) {
-  if (p.key_heads == p.value_heads) return by_rows<T, T>(p, d, static_cast<char*>(workspace), stream);
+cudaError_t own_heads(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream) {
+  return by_rows<T, T>(p, d, static_cast<char*>(workspace), stream);
+}
+
+// Shared key heads: 32-bit rows for each value head, then their sums.
+template <class T>
+cudaError_t shared_heads(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream) {
   const uint64_t rows = uint64_t(p.batch) * p.tokens * p.key_heads;
   const uint32_t group = p.value_heads / p.key_heads;
   char* at = static_cast<char*>(workspace);  // the segments' part, then the rows'

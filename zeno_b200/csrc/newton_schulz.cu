@@ -534,7 +534,9 @@ cudaError_t launch(const Maps& m, const Product& p, uint32_t tiles, uint32_t cou
 
 template <Kind KIND, class T>
 cudaError_t launch(int limbs, const Maps& m, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
-  return limbs == 2 ? launch<2, KIND, T>(m, p, tiles, count, stream) : launch<1, KIND, T>(m, p, tiles, count, stream);
+  if constexpr (sizeof(T) == 2 && KIND != kLast)
+    if (limbs == 1) return launch<1, KIND, T>(m, p, tiles, count, stream);
+  return launch<2, KIND, T>(m, p, tiles, count, stream);
 }
 
 template <class T>

@@ -156,8 +156,7 @@ class _DeltaRule(torch.autograd.Function):
     def backward(ctx, d_out, d_final):
         q, k, v, g, beta, reset, initial, saved = ctx.saved_tensors
         if d_out is None:
-            d_out = torch.zeros((1,) * v.dim(), dtype=v.dtype, device=v.device).expand(v.shape)
-            d_out = d_out if v.shape[-1] == 1 else d_out.contiguous()
+            d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
         d_out = _rows(d_out)
         if d_final is not None:
             d_final = d_final.contiguous()
