@@ -105,11 +105,11 @@ __device__ __forceinline__ void mma2(float (&acc0)[4], float (&acc1)[4], const u
 // of its own, each row of the result a factor.
 template <int DK, int N, int L, bool TRANSPOSED>
 __device__ __forceinline__ void pairs_times_rows(float (&out)[N][4], const __half* plane, const float* scales, const float* row_factor,
-                                                 const __half* x, int r, int halves, int c0, int lane) {
+                                                 const __half* x, int r, int c0, int lane) {
   constexpr int PITCH = DK + 8, PLANE = C * PITCH;
   const float r0 = row_factor[r * 16 + (lane >> 2)], r1 = row_factor[r * 16 + (lane >> 2) + 8];
 #pragma unroll 1
-  for (int j = TRANSPOSED ? r : 0; j < (TRANSPOSED ? halves : r + 1); ++j) {
+  for (int j = TRANSPOSED ? r : 0; j < (TRANSPOSED ? 2 : r + 1); ++j) {
     uint32_t ah[4], al[4];
     if (TRANSPOSED) {
       a_cols(ah, plane + j * 16 * CP + r * 16, CP, lane);
@@ -369,7 +369,6 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           for (int c = tid * 32; c < VC * DK; c += NW * 32 * 32) prefetch(at + c);
         }
       }
-      const int halves = hi - t0 <= 16 ? 1 : 2;
       const int e_out = pow2_exp(__uint_as_float(sm.most_out));
       const float u_out = pow2_unscale(e_out) * p.scale;
       {
@@ -392,7 +391,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         const float fk = sm.gates.token[tid].fk;
         sm.fk[tid] = fk, sm.inv_fk[tid] = 1.0f / fk, sm.inv_fq[tid] = 1.0f / sm.gates.fq[tid];
       }
-      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], true, halves, warp, lane);
+      pair_matrices<DK, NW, L, true>(sm.gates, early.pairs, squares, &sm.gram, sm.q[0], sm.k[0], true, 2, warp, lane);
 
       // S0^T times K^T as the limbs are made; they also go to shared memory, for phase B
       float w[4][4] = {}, e[4][4] = {};
@@ -413,7 +412,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         for (int kk = 0; kk < DK; kk += 16) {
           uint32_t ah[4], al[4];
           split_a(ah, al, st[kk / 8], st[kk / 8 + 1], sc, sc);
-          state_times_rows<DK, L>(w, ah, al, sm.k[0], kk, halves, lane);
+          state_times_rows<DK, L>(w, ah, al, sm.k[0], kk, 2, lane);
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             const int at = (c0 + gi + (h & 1) * 8) * SP + kk + (h >> 1) * 8 + qj;
@@ -430,7 +429,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         for (int kk = 0; kk < DK; kk += 16) {
           uint32_t ah[4], al[4];
           split_a(ah, al, rt[kk / 8], rt[kk / 8 + 1], sc, sc);
-          state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, halves, lane);
+          state_times_rows<DK, L>(e, ah, al, sm.k[0], kk, 2, lane);
         }
       }
       __syncthreads();
@@ -457,7 +456,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
             w[n][x] = a == 0.0f ? v[n][x] : fmaf(-w[n][x], u_state * a, v[n][x]);
           }
         }
-        solve_forward(w, early.pairs, halves, lane);
+        solve_forward(w, early.pairs, 2, lane);
         if (has_r) {
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
@@ -473,11 +472,9 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       // dU^T += dO^T P
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if (r == 1 && halves == 1) break;
         float acc[2][4] = {};
 #pragma unroll
         for (int i = r; i < 2; ++i) {
-          if (i == 1 && halves == 1) break;
           uint32_t ah[4], al[4] = {}, bh[4], bl[4];
           a_cols(ah, sm.d_out[0] + i * 16 * DP + c0, DP, lane);
           if (L == 2) a_cols(al, sm.d_out[L - 1] + i * 16 * DP + c0, DP, lane);
@@ -506,7 +503,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
           const float be = sm.gates.beta[n * 8 + qj + x];
           e[n][x] *= be, e[n][x + 2] *= be;
         }
-      solve_backward(e, early.pairs, halves, lane);  // now dE^T
+      solve_backward(e, early.pairs, lane);  // now dE^T
       if (!r_only) {
       store_out(e, d_v, d.d_v.stride[1], t0, lo, hi, c0, dv, dv_pairs, lane);
       int unused;
@@ -521,7 +518,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
 
       // ---- M and X, one 16 x 16 block a job: rows later tokens i, columns earlier tokens j
 #pragma unroll 1
-      for (int job = warp; job < (halves == 1 ? 1 : 3); job += NW) {
+      for (int job = warp; job < 3; job += NW) {
         const int r = (job + 1) >> 1, c = job >> 1;  // (0,0), (1,0), (1,1)
         float am[2][4] = {}, ax[2][4] = {};
 #pragma unroll 2
@@ -586,7 +583,7 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
       // ---- phase B: 16 tokens and a share of the key channels
       constexpr int DKW = 2 * DK / NW < 16 ? 16 : 2 * DK / NW, N = DKW / 8, GROUPS = DK / DKW;
       const int r = warp & 1, group = warp >> 1, k0 = group * DKW;
-      const bool works = group < GROUPS && r < halves;
+      const bool works = group < GROUPS;
       float gq[N][4] = {}, g_row[N][4] = {}, g_col[N][4] = {};
       if (works) {
         if (has_state) {
@@ -610,10 +607,10 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
               g_row[n][x] = a == 0.0f ? 0.0f : acc[n][x] * (-a * u_e * u_state);
             }
         }
-        pairs_times_rows<DK, N, L, false>(gq, late.m[0], sm.fm, sm.inv_fq, sm.k[0], r, halves, k0, lane);
-        pairs_times_rows<DK, N, L, false>(g_row, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, halves, k0, lane);
-        pairs_times_rows<DK, N, L, true>(g_col, late.m[0], sm.fm, sm.inv_fk, sm.q[0], r, halves, k0, lane);
-        pairs_times_rows<DK, N, L, true>(g_col, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, halves, k0, lane);
+        pairs_times_rows<DK, N, L, false>(gq, late.m[0], sm.fm, sm.inv_fq, sm.k[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, false>(g_row, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, true>(g_col, late.m[0], sm.fm, sm.inv_fk, sm.q[0], r, k0, lane);
+        pairs_times_rows<DK, N, L, true>(g_col, late.x[0], sm.fx, sm.inv_fk, sm.k[0], r, k0, lane);
       }
       if (has_r) {
         if (has_state) __syncthreads();
@@ -655,10 +652,8 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
                                   d.d_k.stride[1], t0, lo, hi, r, k0, dk, dk_pairs, lane);
       }
       if (warp == 0) {  // gates
-        const bool made = lane < 16 * halves;
-        float dg = 0.0f, db = lane < 16 ? sm.beta_pairs[0][lane] : 0.0f;
-        if (halves == 2) db += sm.beta_pairs[1][lane];
-        for (int g = 0; g < GROUPS && made; ++g) dg += sm.dot_q[g][lane] + sm.dot_row[g][lane] - sm.dot_col[g][lane];
+        float dg = 0.0f, db = sm.beta_pairs[1][lane] + (lane < 16 ? sm.beta_pairs[0][lane] : 0.0f);
+        for (int g = 0; g < GROUPS; ++g) dg += sm.dot_q[g][lane] + sm.dot_row[g][lane] - sm.dot_col[g][lane];
         for (int v = 0; v < NW; ++v) db += sm.beta_part[v][lane];
         const int mine = sm.gates.token[lane].episode;
         if (lane == 31)
@@ -696,8 +691,8 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
             e[n][c] = fk == 0.0f ? 0.0f : e[n][c] * -fk;
           }
         }
-        state_update<DK, L>(rt, keep, x, sm.q[0], halves, lane);
-        state_update<DK, L>(rt, 1.0f, e, sm.k[0], halves, lane);
+        state_update<DK, L>(rt, keep, x, sm.q[0], 2, lane);
+        state_update<DK, L>(rt, 1.0f, e, sm.k[0], 2, lane);
         has_r = true;
       }
       __syncthreads();
@@ -710,21 +705,27 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
   if (r_to) for_state<DK>(rt, dk, dv, c0, lane, [&](float& x, int64_t at) { r_to[at] = x; });
 }
 
-// dq and dk of a key head: the sum over its value heads, in their order.
+// dq (grid y 0) and dk (1) of a key head: the sum over its value heads, in their order.  A warp a row.
 template <class T>
 __global__ void __launch_bounds__(256)
-shared_heads_kernel(const float* part, ZenoTensor out, uint64_t rows, uint32_t tokens, uint32_t key_heads, uint32_t group, uint32_t dk) {
-  const uint64_t n = rows * dk;
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += uint64_t(gridDim.x) * 256) {
-    const uint64_t row = i / dk;  // (b, t, key head)
-    const uint32_t c = uint32_t(i % dk), kh = uint32_t(row % key_heads);
+shared_heads_kernel(const float* part_q, const float* part_k, ZenoTensor d_q, ZenoTensor d_k, uint64_t rows, uint32_t tokens,
+                    uint32_t key_heads, uint32_t group, uint32_t dk) {
+  const float* part = blockIdx.y ? part_k : part_q;
+  const ZenoTensor& out = blockIdx.y ? d_k : d_q;
+  const uint32_t lane = threadIdx.x & 31;
+  for (uint64_t row = blockIdx.x * 8ull + (threadIdx.x >> 5); row < rows; row += uint64_t(gridDim.x) * 8) {  // (b, t, key head)
     const uint64_t bt = row / key_heads;
-    float sum = 0.0f;
-    for (uint32_t g = 0; g < group; ++g) sum += part[((bt * key_heads + kh) * group + g) * dk + c];
-    T* at = static_cast<T*>(out.data) + int64_t(bt / tokens) * out.stride[0] + int64_t(bt % tokens) * out.stride[1] +
-            int64_t(kh) * out.stride[2] + c;
-    if constexpr (sizeof(T) == 2) *at = __float2bfloat16_rn(sum);
-    else *at = sum;
+    const uint32_t kh = uint32_t(row - bt * key_heads);
+    const uint64_t b = bt / tokens;
+    T* at = static_cast<T*>(out.data) + int64_t(b) * out.stride[0] + int64_t(bt - b * tokens) * out.stride[1] + int64_t(kh) * out.stride[2];
+    const float* in = part + row * group * dk;
+#pragma unroll 4
+    for (uint32_t c = lane; c < dk; c += 32) {
+      float sum = 0.0f;
+      for (uint32_t g = 0; g < group; ++g) sum += in[g * dk + c];
+      if constexpr (sizeof(T) == 2) at[c] = __float2bfloat16_rn(sum);
+      else at[c] = sum;
+    }
   }
 }
 
@@ -817,10 +818,9 @@ cudaError_t shared_heads(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, vo
   x.d_q.data = part_q, x.d_k.data = part_k;
   cudaError_t e = by_rows<T, float>(p, x, at, stream);
   if (e != cudaSuccess || rows == 0) return e;
-  const uint64_t blocks = (rows * p.key_dim + 255) / 256;
-  const unsigned grid = unsigned(blocks < 148 * 8 ? blocks : 148 * 8);
-  shared_heads_kernel<T><<<grid, 256, 0, stream>>>(part_q, d.d_q, rows, p.tokens, p.key_heads, group, p.key_dim);
-  shared_heads_kernel<T><<<grid, 256, 0, stream>>>(part_k, d.d_k, rows, p.tokens, p.key_heads, group, p.key_dim);
+  const uint64_t blocks = (rows + 7) / 8;
+  shared_heads_kernel<T><<<dim3(unsigned(blocks < 148 * 8 ? blocks : 148 * 8), 2), 256, 0, stream>>>(part_q, part_k, d.d_q, d.d_k, rows,
+                                                                                                   p.tokens, p.key_heads, group, p.key_dim);
   return cudaGetLastError();
 }
 

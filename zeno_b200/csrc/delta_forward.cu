@@ -29,6 +29,7 @@ struct Split {
   Mode mode;
   uint32_t segments, chunks;  // chunks of a segment
   float* m;        // [batch * heads][segments][dk][dk]
+  bool m_transposed;
   float* n;        // ... [dk][dv]: what a segment leaves of nothing (the first one: of initial_state)
   float* state;    // ... [dk][dv]: the state in front of a segment
   int* cleared;    // ... whether the segment drops the state in front of it
@@ -207,7 +208,10 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
       lo = hi;
     }
   }
-  if (final_state) for_state<DK>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { final_state[at] = x; });
+  if (final_state && is_m && sp.m_transposed)
+    for_state<DK>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { final_state[int(at) % dk * dk + int(at) / dk] = x; });
+  else if (final_state)
+    for_state<DK>(st, dk, dv, c0, lane, [&](float& x, int64_t at) { final_state[at] = x; });
   if (is_m && v0 == 0 && tid == 0) sp.cleared[int64_t(blockIdx.x) * sp.segments + segment] = cleared;
 }
 
@@ -245,7 +249,7 @@ cudaError_t launch(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream)
   sp.cleared = reinterpret_cast<int*>(at + lay.m + 2 * lay.n);
   sp.mode = kTransitions, sp.chunks = (sp.chunks + segments - 1) / segments;
   sp.segments = ((p.tokens + C - 1) / C + sp.chunks - 1) / sp.chunks;  // none of them empty
-  sp.value_blocks = blocks;
+  sp.value_blocks = blocks, sp.m_transposed = true;
   // nothing is asked of the last segment's transition
   cudaError_t e = launch<DK, NW, T>(p, sp, dim3(rows, blocks + (DK + 16 * NW - 1) / (16 * NW), sp.segments - 1), stream);
   if (e != cudaSuccess) return e;

@@ -596,8 +596,9 @@ __device__ __forceinline__ void score_columns(const Gates& s, Pairs& m, const __
 }
 
 // All warps: the three kinds of matrices, spread over the warps (P only where it is asked for).  halves: 1 where
-// the chunk has no tokens past the 16th; nothing of the second half is made then, nor read (8192 rollouts of 8
-// tokens with gradients: 2.28 -> 1.94 ms; whole chunks pay for the branches, 4096 of 32 tokens 1.28 -> 1.30 ms).
+// the chunk has no tokens past the 16th; nothing of the second half is made then, nor read (forward: 8192 rollouts of
+// 16 tokens 650 -> 560 us, 4096 of 32 tokens 342 -> 344 us; the backward pass always takes 2, because its whole
+// chunks lost 5 % to the branches).
 template <int DK, int NW, int LIMBS, bool BACKWARD>
 __device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gram* gram, const __half* qp, const __half* kp, bool scores, int halves, int warp,
                                               int lane) {
@@ -606,7 +607,7 @@ __device__ __forceinline__ void pair_matrices(Gates& s, Pairs& m, Squares& q, Gr
     if (job == 0) {
       diagonal_inverses<DK, LIMBS>(s, m, q, gram, kp, halves, lane);
     } else if (job < 3) {
-      if (!scores || (halves == 1 && job == (BACKWARD ? 2 : 1))) continue;
+      if (!scores || (halves == 1 && job == 1)) continue;
       if (BACKWARD) score_columns<DK, LIMBS>(s, m, qp, kp, job - 1, lane);
       else score_rows<DK, LIMBS>(s, m, qp, kp, 2 - job, lane);
     } else {
@@ -658,20 +659,18 @@ __device__ __forceinline__ void solve_forward(float (&e)[4][4], const Pairs& m, 
 }
 
 // dE^T = dW^T (I + N)^-1, in place: from the chunk's end to its begin.
-__device__ __forceinline__ void solve_backward(float (&e)[4][4], const Pairs& m, int halves, int lane) {
+__device__ __forceinline__ void solve_backward(float (&e)[4][4], const Pairs& m, int lane) {
   float f0, f1, x[2][4];
-  if (halves == 2) {
-    times_block(x, e[2], e[3], m.t[0] + 16 * TP, m.t[1] + 16 * TP, false, lane, f0, f1);
+  times_block(x, e[2], e[3], m.t[0] + 16 * TP, m.t[1] + 16 * TP, false, lane, f0, f1);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) e[2 + n][c] = x[n][c] * ((c < 2 ? f0 : f1) * m.ft[1]);
-    times_block(x, e[2], e[3], m.n[0], m.n[1], false, lane, f0, f1);
+    for (int c = 0; c < 4; ++c) e[2 + n][c] = x[n][c] * ((c < 2 ? f0 : f1) * m.ft[1]);
+  times_block(x, e[2], e[3], m.n[0], m.n[1], false, lane, f0, f1);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) e[n][c] -= x[n][c] * ((c < 2 ? f0 : f1) * m.fn);
-  }
+    for (int c = 0; c < 4; ++c) e[n][c] -= x[n][c] * ((c < 2 ? f0 : f1) * m.fn);
   times_block(x, e[0], e[1], m.t[0], m.t[1], false, lane, f0, f1);
 #pragma unroll
   for (int n = 0; n < 2; ++n)

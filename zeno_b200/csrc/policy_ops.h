@@ -30,7 +30,7 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& devices)
 
 // A rollout in segments: what takes the state over a segment is M S + N.
 struct DeltaWalk {
-  const float* m;      // [rows][segments][dk][dk]
+  const float* m;      // [rows][segments][dk][dk]: M, in the forward walk M^T
   const float* n;      // [rows][segments][dk][dv]
   float* state;        // written, same shape: in front of each segment (behind it in reverse)
   const int* cleared;  // [rows][segments]: the segment drops the state
