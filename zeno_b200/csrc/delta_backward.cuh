@@ -730,7 +730,7 @@ shared_heads_kernel(const float* part_q, const float* part_k, ZenoTensor d_q, Ze
 }
 
 // Segments of a call: as many as fill the SMs with blocks, each of at least 4 chunks.
-// (8 environments x 8 heads of 128 x 128, 1000 tokens, with the forward pass: 979 us in 2 segments, 1161 whole.)
+// (8 environments x 8 heads of 128 x 128, 1000 tokens, with the forward pass: 961 us in 2 segments, 1161 whole.)
 inline uint32_t back_segments(const ZenoDeltaRule& p) {
   const uint64_t chunks = (uint64_t(p.tokens) + C - 1) / C, blocks = uint64_t(p.batch) * p.value_heads;
   const int warps = value_groups(p), width = key_width(p);

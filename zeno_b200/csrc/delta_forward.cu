@@ -48,7 +48,7 @@ struct ForwardSmem {
 };
 
 template <int DK, int NW, class T>
-// Threads of an SM: 512 where the state is 32 registers a thread (4096 x 32 tokens, 64 x 64: 461 us against 544 with
+// Threads of an SM: 512 where the state is 32 registers a thread (4096 x 32 tokens, 64 x 64, when first measured: 461 us against 544 with
 // 384 and 714 with 256), 384 where it is 64 (2 x 4096 tokens, 128 x 128: 1250 us against 1405 with 512).
 __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) delta_forward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_constant__ Split sp) {
   extern __shared__ __align__(16) unsigned char raw[];
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
 }
 
 // Segments of a call: enough to give every SM three blocks of 128 threads, each of at least 4 chunks;
-// 1 (not split) below 4 of them.  (2 environments x 8 heads of 128 x 128, 4096 tokens: 407 us in 13 segments, 963 whole.)
+// 1 (not split) below 4 of them.  (2 environments x 8 heads of 128 x 128, 4096 tokens: 375 us in 13 segments, 963 whole.)
 inline uint32_t segments_of(const ZenoDeltaRule& p) {
   const uint64_t chunks = (uint64_t(p.tokens) + C - 1) / C;
   const int groups = value_groups(p), warps = groups < 4 ? groups : 4;
