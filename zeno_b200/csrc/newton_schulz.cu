@@ -11,13 +11,9 @@
 // much smaller than 1e-7 keeps |X| << 1 for many steps; its X carries 2^E more, with E falling
 // by 2 a step (a < 4), A and B carry 2^2E.
 //
-// Precision.  X is kept in two limbs, hi and lo, 22 bits together.  float32 updates: all
-// operands are, and a product is hi hi + hi lo + lo hi.  bfloat16 updates of more than 128 rows:
-// the products of all steps but the last take the hi limbs alone (11 bits), a third of the
-// work; a X always takes both, because a rounding of X in a direction that X does not have
-// would be multiplied by 3.4 in each step (a matrix of rank 4 in 200 rows is then 6e-2
-// off, and 4e-4 with both limbs).  For Gaussian matrices of 256 to 1024 rows this leaves
-// 1.3e-3 of the result's norm, below the 1.7e-3 of rounding the result to bfloat16.
+// Precision.  All operands are kept in two limbs, hi and lo, 22 bits together, and a product is
+// hi hi + hi lo + lo hi, for bfloat16 updates too: the result is rounded to 16 bits once, at the end.
+// (A rounding of X in a direction that X does not have would be multiplied by 3.4 in each step.)
 //
 // A, B are symmetric: only tiles on and below the diagonal are computed, and stored twice.
 // X is kept in both orientations, so that all operands are read along the contracted index.
@@ -228,7 +224,6 @@ enum Kind { kGram, kSquare, kApply, kLast };  // A; B; X in both orientations; X
 struct Product {
   uint32_t depth;         // contracted length, a multiple of kDeep
   uint32_t cols;          // padded columns of the result
-  int add_limbs, out_limbs, out_t_limbs;
   uint32_t step;
   const int* extra;       // first extra exponents
   void* last;             // kLast: the caller's array
@@ -237,13 +232,12 @@ struct Product {
   uint32_t* failed;       // set where a barrier was waited for in vain
 };
 
-// Shared memory: a ring of 6 units of 32 KB; a stage is one unit (both operands' hi limbs) or two (hi
-// and lo).  Behind the last stage come two units with the tile that the epilogue adds, and the
+// Shared memory: a ring of 6 units of 32 KB; a stage is two units, both operands' hi and lo limbs.
+// Behind the last stage come two units with the tile that the epilogue adds, and the
 // other four, once the products are done, hold the result's limb planes in both orientations.
-constexpr int kUnits = 6, kUnit = 2 * kPlane;
+constexpr int kLimbs = 2, kUnits = 6, kUnit = 2 * kPlane;
 constexpr int kSmem = kUnits * kUnit + 1024 + 256;
-template <int LIMBS>
-constexpr int kColumns = LIMBS == 2 ? 4 * kTile : kTile;  // of TMEM
+constexpr int kColumns = 4 * kTile;  // of TMEM
 
 // Byte of element (row, col) in a unit that holds a 128 x 128 tile as two swizzled boxes of 64 columns.
 __device__ __forceinline__ uint32_t in_unit(uint32_t row, uint32_t col) {
@@ -253,11 +247,11 @@ __device__ __forceinline__ uint32_t in_unit(uint32_t row, uint32_t col) {
 // One block: one 128 x 128 tile of L R^T (rows of both along the contracted index), then the
 // step's epilogue.  Warp 0 loads, warp 1 issues the matrix instructions, warps 4 to 11 read
 // the accumulators, 32 rows and 64 columns each.
-template <int LIMBS, Kind KIND, class T>
+template <Kind KIND, class T>
 __global__ void __launch_bounds__(384, 1)
 product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__ CUtensorMap right, const __grid_constant__ CUtensorMap add,
                const __grid_constant__ CUtensorMap out, const __grid_constant__ CUtensorMap out_t, const __grid_constant__ Product p) {
-  constexpr int S = kUnits / LIMBS;
+  constexpr int S = kUnits / kLimbs;
   extern __shared__ unsigned char raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + kUnits * kUnit);  // full[S], empty[S], done, added
@@ -282,7 +276,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(tmem_slot)), "n"(kColumns<LIMBS>) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(tmem_slot)), "n"(kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -291,7 +285,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   const uint32_t tmem = *tmem_slot;
   const int stages = int(p.depth / kDeep);
   const uint32_t unit0 = smem_at(base);
-  const int first_add = stages * LIMBS % kUnits;
+  const int first_add = stages * kLimbs % kUnits;
   const uint32_t done = smem_at(bars + 2 * S), added = smem_at(bars + 2 * S + 1);
   wait_for_previous();
   let_next_start();
@@ -304,20 +298,19 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       const int s = k % S;
       if (k >= S) ok = barrier_wait(smem_at(bars + S + s), (k / S - 1) & 1);
       if (!ok) break;
-      const uint32_t bar = smem_at(bars + s), at = unit0 + s * LIMBS * kUnit;
-      barrier_expect(bar, LIMBS * kUnit);
+      const uint32_t bar = smem_at(bars + s), at = unit0 + s * kLimbs * kUnit;
+      barrier_expect(bar, kLimbs * kUnit);
 #pragma unroll
-      for (int l = 0; l < LIMBS; ++l) {
+      for (int l = 0; l < kLimbs; ++l) {
         tma_load(at + l * kPlane, &left, bar, k * kDeep, int(ti * kTile), int(z * 2 + l));
-        tma_load(at + (LIMBS + l) * kPlane, &right, bar, k * kDeep, int(tj * kTile), int(z * 2 + l));
+        tma_load(at + (kLimbs + l) * kPlane, &right, bar, k * kDeep, int(tj * kTile), int(z * 2 + l));
       }
     }
     if (KIND != kGram && ok) {
-      for (int j = stages; j < stages + 2 / LIMBS && ok; ++j)
-        if (j >= S) ok = barrier_wait(smem_at(bars + S + j % S), (j / S - 1) & 1);
+      if (stages >= S) ok = barrier_wait(smem_at(bars + S + stages % S), (stages / S - 1) & 1);
       if (ok) {
-        barrier_expect(added, p.add_limbs * kUnit);
-        for (int l = 0; l < p.add_limbs; ++l)
+        barrier_expect(added, kLimbs * kUnit);
+        for (int l = 0; l < kLimbs; ++l)
           for (int half = 0; half < 2; ++half)
             tma_load(unit0 + (first_add + l) % kUnits * kUnit + half * kPlane, &add, added, int(tj * kTile) + half * kDeep, int(ti * kTile),
                      int(z * 2 + l));
@@ -334,21 +327,17 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       ok = barrier_wait(smem_at(bars + s), (k / S) & 1);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t at = unit0 + s * LIMBS * kUnit;
+      const uint32_t at = unit0 + s * kLimbs * kUnit;
 #pragma unroll
       for (int kk = 0; kk < kDeep; kk += 16) {
-        const uint64_t a = operand(at + kk * 2), b = operand(at + LIMBS * kPlane + kk * 2);
-        if (LIMBS == 1) {
-          tensor_mma(tmem, a, b, k > 0 || kk > 0);
-        } else {
-          // The tensor cores' sums drop what is below 2^-24 of the running sum, always towards zero;
-          // three sums for hi hi in turn and one for the small products keep that below the operands' 2^-23
-          // (2048 x 2048: one sum of 3 x 2048 products leaves 1.4e-5 of the result, these 4.5e-6, 32-bit torch 3.7e-6).
-          const uint64_t al = operand(at + kPlane + kk * 2), bl = operand(at + (LIMBS + 1) * kPlane + kk * 2);
-          tensor_mma(tmem + (k % 3) * kTile, a, b, k >= 3 || kk > 0);
-          tensor_mma(tmem + 3 * kTile, a, bl, k > 0 || kk > 0);
-          tensor_mma(tmem + 3 * kTile, al, b, true);
-        }
+        // The tensor cores' sums drop what is below 2^-24 of the running sum, always towards zero;
+        // three sums for hi hi in turn and one for the small products keep that below the operands' 2^-23
+        // (2048 x 2048: one sum of 3 x 2048 products leaves 1.4e-5 of the result, these 4.5e-6, 32-bit torch 3.7e-6).
+        const uint64_t a = operand(at + kk * 2), b = operand(at + kLimbs * kPlane + kk * 2);
+        const uint64_t al = operand(at + kPlane + kk * 2), bl = operand(at + (kLimbs + 1) * kPlane + kk * 2);
+        tensor_mma(tmem + (k % 3) * kTile, a, b, k >= 3 || kk > 0);
+        tensor_mma(tmem + 3 * kTile, a, bl, k > 0 || kk > 0);
+        tensor_mma(tmem + 3 * kTile, al, b, true);
       }
       tensor_commit(smem_at(bars + S + s));
     }
@@ -369,7 +358,6 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int quarter = warp & 3, gi = lane >> 2, qj = (lane & 3) * 2;
       const bool mirror = KIND == kApply || (kSymmetric && ti != tj);
-      const int limbs_t = KIND == kApply ? p.out_t_limbs : p.out_limbs;
       const unsigned char* add0 = base + first_add * kUnit;
       const unsigned char* add1 = base + (first_add + 1) % kUnits * kUnit;
 #pragma unroll 1
@@ -378,31 +366,26 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
         float v[32], w[32];
         const uint32_t at = tmem + (r0 << 16) + c0;
         tensor_load(v, at);
-        if (LIMBS == 2) tensor_load(w, at + 3 * kTile);
+        tensor_load(w, at + 3 * kTile);
         tensor_wait(v, w);
-        if (LIMBS == 2) {
-          float x[32];
-          const bool third = stages > 2;
-          tensor_load(x, at + kTile);
+        float x[32];
+        const bool third = stages > 2;
+        tensor_load(x, at + kTile);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] += w[e];
-          if (third) tensor_load(w, at + 2 * kTile);
-          tensor_wait(x, w);
+        for (int e = 0; e < 32; ++e) v[e] += w[e];
+        if (third) tensor_load(w, at + 2 * kTile);
+        tensor_wait(x, w);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] += third ? x[e] + w[e] : x[e];
-        }
+        for (int e = 0; e < 32; ++e) v[e] += third ? x[e] + w[e] : x[e];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const uint32_t row = r0 + gi + ((e >> 1) & 1) * 8, col = c0 + (e >> 2) * 8 + qj;
           if (KIND == kGram) {
             v[e] *= f, v[e + 1] *= f;
           } else {
-            float2 y = __half22float2(*reinterpret_cast<const __half2*>(add0 + in_unit(row, col)));
-            if (p.add_limbs == 2) {
-              const float2 w = __half22float2(*reinterpret_cast<const __half2*>(add1 + in_unit(row, col)));
-              y.x += w.x, y.y += w.y;
-            }
-            v[e] = fmaf(v[e], f, g * y.x), v[e + 1] = fmaf(v[e + 1], f, g * y.y);
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(add0 + in_unit(row, col)));
+            const float2 z = __half22float2(*reinterpret_cast<const __half2*>(add1 + in_unit(row, col)));
+            v[e] = fmaf(v[e], f, g * (y.x + z.x)), v[e + 1] = fmaf(v[e + 1], f, g * (y.y + z.y));
           }
           if constexpr (KIND == kLast) {
             const uint32_t i = ti * kTile + row, j = tj * kTile + col;
@@ -419,8 +402,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
         if constexpr (KIND != kLast) {
           const uint32_t tile_row = lane & 7, right_tile = (lane >> 4) * 8, low_tile = ((lane >> 3) & 1) * 8;
 #pragma unroll
-          for (int l = 0; l < 2; ++l) {
-            if (l >= p.out_limbs) break;
+          for (int l = 0; l < kLimbs; ++l) {
             const uint32_t u_row = unit0 + (first_add + 2 + l) % kUnits * kUnit, u_col = unit0 + (first_add + 4 + l) % kUnits * kUnit;
 #pragma unroll
             for (int c = 0; c < 64; c += 16) {
@@ -434,7 +416,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
                 h[e] = *reinterpret_cast<const uint32_t*>(&y);
               }
               store_tiles(u_row + in_unit(r0 + low_tile + tile_row, c0 + c + right_tile), h);
-              if (mirror && l < limbs_t) store_tiles_transposed(u_col + in_unit(c0 + c + right_tile + tile_row, r0 + low_tile), h);
+              if (mirror) store_tiles_transposed(u_col + in_unit(c0 + c + right_tile + tile_row, r0 + low_tile), h);
             }
           }
         }
@@ -448,12 +430,11 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (warp == 4 && lane == 0 && ok) {
         const bool mirror = KIND == kApply || ti != tj;
-        const int limbs_t = KIND == kApply ? p.out_t_limbs : p.out_limbs;
-        for (int l = 0; l < p.out_limbs; ++l)
+        for (int l = 0; l < kLimbs; ++l)
           for (int half = 0; half < 2; ++half) {
             tma_store(&out, unit0 + (first_add + 2 + l) % kUnits * kUnit + half * kPlane, int(tj * kTile) + half * kDeep, int(ti * kTile),
                       int(z * 2 + l));
-            if (mirror && l < limbs_t)
+            if (mirror)
               tma_store(&out_t, unit0 + (first_add + 4 + l) % kUnits * kUnit + half * kPlane, int(ti * kTile) + half * kDeep,
                         int(tj * kTile), int(z * 2 + l));
           }
@@ -465,7 +446,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns<LIMBS>));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns));
   }
 }
 
@@ -523,20 +504,13 @@ struct Maps {
   CUtensorMap left, right, add, out, out_t;
 };
 
-template <int LIMBS, Kind KIND, class T>
+template <Kind KIND, class T = float>  // T: the caller's type, of kLast
 cudaError_t launch(const Maps& m, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
-  const auto kernel = product_kernel<LIMBS, KIND, T>;
+  const auto kernel = product_kernel<KIND, T>;
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kernel, kSmem, allowed);
   if (e != cudaSuccess) return e;
   return launch_after(kernel, dim3(tiles, count), 384, kSmem, stream, m.left, m.right, m.add, m.out, m.out_t, p);
-}
-
-template <Kind KIND, class T>
-cudaError_t launch(int limbs, const Maps& m, const Product& p, uint32_t tiles, uint32_t count, cudaStream_t stream) {
-  if constexpr (sizeof(T) == 2 && KIND != kLast)
-    if (limbs == 1) return launch<1, KIND, T>(m, p, tiles, count, stream);
-  return launch<2, KIND, T>(m, p, tiles, count, stream);
 }
 
 template <class T>
@@ -571,20 +545,18 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
   if (e == cudaSuccess) e = make_map(&ma, a, mp, mp, layers);
   if (e == cudaSuccess) e = make_map(&mb, b, mp, mp, layers);
   const uint32_t mt = mp / kTile, nt = np / kTile, lower = mt * (mt + 1) / 2;
-  // limbs of a step's products
-  const auto limbs_of = [&](uint32_t i) { return sizeof(T) == 4 || mt == 1 || i + 1 >= steps ? 2 : 1; };
   for (uint32_t i = 0; i < steps && e == cudaSuccess; ++i) {
-    const int now = i & 1, next = now ^ 1, limbs = limbs_of(i);
+    const int now = i & 1, next = now ^ 1;
     Product p{};
     p.m = s.m, p.n = s.n, p.transposed = transposed, p.failed = failed, p.extra = extra, p.step = i, p.last = out;
-    p.depth = np, p.cols = mp, p.add_limbs = p.out_limbs = limbs;
-    e = launch<kGram, T>(limbs, Maps{mx[now], mx[now], ma, ma, ma}, p, lower, s.count, stream);
+    p.depth = np, p.cols = mp;
+    e = launch<kGram>(Maps{mx[now], mx[now], ma, ma, ma}, p, lower, s.count, stream);
     p.depth = mp;
-    if (e == cudaSuccess) e = launch<kSquare, T>(limbs, Maps{ma, ma, ma, mb, mb}, p, lower, s.count, stream);
-    p.cols = np, p.add_limbs = p.out_limbs = 2, p.out_t_limbs = limbs_of(i + 1);
+    if (e == cudaSuccess) e = launch<kSquare>(Maps{ma, ma, ma, mb, mb}, p, lower, s.count, stream);
+    p.cols = np;
     const Maps m{mb, mxt[now], mx[now], mx[next], mxt[next]};
     if (e == cudaSuccess)
-      e = i + 1 < steps ? launch<kApply, T>(limbs, m, p, mt * nt, s.count, stream) : launch<kLast, T>(limbs, m, p, mt * nt, s.count, stream);
+      e = i + 1 < steps ? launch<kApply>(m, p, mt * nt, s.count, stream) : launch<kLast, T>(m, p, mt * nt, s.count, stream);
   }
   return e;
 }
