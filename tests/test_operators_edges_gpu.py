@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import zeno_b200
+from zeno_b200._ffi import _lib, ffi
 import operators_plain as plain
 from test_operators_gpu import DEV, TOL, check, gradients, inputs, matrix
 
@@ -28,3 +29,48 @@ def test_orthogonalize_bfloat16_of_low_rank(shape):
     left, right = (torch.randint(-1, 2, s, generator=gen, device=DEV).float() for s in ((shape[0], 4), (4, shape[1])))
     m = (left @ right).bfloat16()  # whole numbers up to 4: of rank 4 to the last bit
     assert plain.off(zeno_b200.orthogonalize(m), plain.orthogonalize(m).bfloat16()) <= 1.2e-3
+
+
+def c_step(x, initial, final, out, tokens):
+    """zeno_delta_rule_step on [batch, tokens, ...] tensors; None: no data."""
+    q, k, v, g, beta, reset = x
+    p = ffi.new("ZenoDeltaRule*")
+    p.batch, p.tokens, p.key_heads, p.key_dim, p.value_heads, p.value_dim = q.shape[0], tokens, *q.shape[2:], *v.shape[2:]
+    p.dtype, p.normalize, p.scale = int(q.dtype == torch.bfloat16), 1, q.shape[3] ** -0.5
+    for name, t in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta), ("reset", reset), ("out", out)):
+        if t is not None and tokens:
+            getattr(p, name).data = ffi.cast("void*", t.data_ptr())
+            getattr(p, name).stride = (list(t.stride()) + [0])[:3]
+    if reset is not None:
+        p.reset.data = ffi.cast("void*", reset.data_ptr())
+    p.initial_state, p.final_state = (ffi.cast("float*", 0 if t is None else t.data_ptr()) for t in (initial, final))
+    assert _lib.zeno_delta_rule_step(p, ffi.cast("void*", torch.cuda.current_stream().cuda_stream)) == 0
+
+
+@pytest.mark.parametrize("dk,dv", [(16, 16), (33, 30), (128, 64)])
+def test_step_of_no_tokens_keeps_the_state(dk, dv):
+    q, k, v, g, beta, _, state = inputs(3, 1, 1, 2, dk, dv, torch.float32)
+    marks = torch.ones((3, 1), dtype=torch.uint8, device=DEV)  # of the token that is not there
+    keep, final = state.clone(), torch.full_like(state, 7.0)
+    c_step((q, k, v, g, beta, marks), state, state, v, 0)
+    c_step((q, k, v, g, beta, marks), state, final, v, 0)
+    assert torch.equal(state, keep) and torch.equal(final, keep)
+    c_step((q, k, v, g, beta, marks), None, final, v, 0)
+    assert not final.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,Hk,H,dk,dv", [(3, 2, 1, 2, 16, 16), (2, 41, 2, 4, 33, 30), (140, 7, 1, 1, 128, 64)])
+def test_step_of_several_tokens(B, T, Hk, H, dk, dv, dtype):
+    *x, state = inputs(B, T, Hk, H, dk, dv, dtype, reset=0.2)
+    want, after = plain.delta_rule(*x, state)
+    out, final = torch.empty_like(x[2]), torch.empty_like(state)
+    c_step(x, state, final, out, T)
+    check(out, want, dtype, "out")
+    check(final, after, torch.float32, "state")
+    c_step(x, state, state, out, T)
+    assert torch.equal(state, final)
+    c_step(x, None, final, out, T)
+    want, after = plain.delta_rule(*x)
+    check(out, want, dtype, "out from nothing")
+    check(final, after, torch.float32, "state from nothing")

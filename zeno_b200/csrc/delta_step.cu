@@ -188,6 +188,11 @@ cudaError_t by_rows(const ZenoDeltaRule& p, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_delta_recurrent(const ZenoDeltaRule& p, cudaStream_t stream) {
+  if (p.tokens == 0 && p.reset.data) {  // the kernel looks at the first token's flag before it walks: there is none
+    ZenoDeltaRule q = p;
+    q.reset.data = nullptr;
+    return launch_delta_recurrent(q, stream);
+  }
   return p.dtype == ZENO_DTYPE_BF16 ? by_rows<__nv_bfloat16>(p, stream) : by_rows<float>(p, stream);
 }
 
