@@ -74,3 +74,24 @@ def test_step_of_several_tokens(B, T, Hk, H, dk, dv, dtype):
     want, after = plain.delta_rule(*x)
     check(out, want, dtype, "out from nothing")
     check(final, after, torch.float32, "state from nothing")
+
+
+def test_backward_after_a_step_on_its_initial_state_is_refused():
+    q, k, v, g, beta, _, state = inputs(3, 5, 1, 2, 16, 16, torch.float32)
+    leaf = v.clone().requires_grad_(True)
+    out, _ = zeno_b200.delta_rule(q, k, leaf, g, beta, None, state)
+    before = state._version
+    zeno_b200.delta_rule_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], state)
+    assert state._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_step_in_inference_mode():
+    with torch.inference_mode():
+        q, k, v, g, beta, _, state = inputs(3, 1, 1, 2, 16, 16, torch.float32)
+        want, after = plain.delta_rule(q, k, v, g, beta, None, state)
+        args = (q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0])
+        check(zeno_b200.delta_rule_step(*args, state), want[:, 0], torch.float32, "out")
+        check(state, after, torch.float32, "state")
+    zeno_b200.delta_rule_step(*args, state)  # a state made there, used outside

@@ -14,6 +14,7 @@ from contextlib import nullcontext
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ._ffi import _lib, ffi
 
@@ -216,7 +217,8 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, st
 
     ``q``, ``k`` [B, Hk, dk], ``v`` [B, H, dv], ``g``, ``beta`` [B, H], ``reset`` [B] (a
     world's ``dones`` buffer can be passed as it is).  ``state`` [B, H, dk, dv] float32,
-    contiguous, is updated in place."""
+    contiguous, is updated in place, and autograd knows: a rollout that was given the same
+    tensor as its initial state and is yet to be differentiated needs a clone of it."""
     _expect("state", state, _check_inputs(q, k, v, g, beta, reset, 1), (torch.float32,), q.device)
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is updated in place")
@@ -229,6 +231,8 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, st
     index = q.device.index
     with _on(index):
         _check(_lib.zeno_delta_rule_step(p, _stream(index)), "delta_rule_step")
+    if not state.is_inference():  # (those have no version, and are never saved for a backward pass)
+        increment_version(state)
     return out
 
 

@@ -49,9 +49,10 @@ class MemoryPolicy(nn.Module):
 
     @torch.no_grad()
     def act(self, obs: torch.Tensor, state: torch.Tensor, begins: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Actions [E, action_dim] for observations [E, obs_dim].  ``state`` is updated in place;
-        ``begins`` [E] marks environments whose observation is the first of an episode (the
-        ``dones`` of the step that returned it, with automatic resets)."""
+        """Actions [E, action_dim] for observations [E, obs_dim].  ``state`` is updated in place (keep
+        a clone for ``forward`` to start from); ``begins`` [E] marks environments whose observation
+        is the first of an episode (the ``dones`` of the step that returned it, with automatic
+        resets)."""
         x, q, k, v, g, beta = self._inputs(obs)
         return self._actions(x, delta_rule_step(q, k, v, g, beta, state, begins))
 
