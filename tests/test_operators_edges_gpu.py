@@ -95,3 +95,33 @@ def test_step_in_inference_mode():
         check(zeno_b200.delta_rule_step(*args, state), want[:, 0], torch.float32, "out")
         check(state, after, torch.float32, "state")
     zeno_b200.delta_rule_step(*args, state)  # a state made there, used outside
+
+
+HUGE = [(3, 1e17), (9, 1e19), (20, 1e22), (21, 1e30), (40, 3e37)]  # squares that leave 32 bits from 1.8e19 on
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_whose_squares_overflow(dtype):
+    x = list(inputs(2, 70, 1, 2, 64, 48, dtype, seed=4, reset=0.03))
+    for t, f in HUGE:
+        x[0][:, t] *= f
+        x[1][:, t + 1] *= f
+    out, final = zeno_b200.delta_rule(*x)
+    want, state = plain.delta_rule(*x)
+    check(out, want, dtype, "out")
+    check(final, state, torch.float32, "state")
+    s = x[6].clone()
+    for t in range(70):
+        check(zeno_b200.delta_rule_step(*(y[:, t] for y in x[:5]), s, x[5][:, t]), want[:, t], dtype, "step %d" % t)
+    check(s, state, torch.float32, "state of the steps")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_rows_whose_squares_overflow(dtype):
+    x = list(inputs(2, 70, 1, 2, 64, 48, dtype, seed=4, reset=0.03))
+    x[0], x[1] = x[0] * 1e30, x[1] * 1e25  # all of them, so that their own gradients (of 1e-30) are seen
+    d_out, d_fin = torch.randn_like(x[2]), torch.randn((2, 2, 64, 48), device=DEV)
+    got = gradients(zeno_b200.delta_rule, x, d_out, d_fin)
+    want = gradients(plain.delta_rule, [t.double() if t.is_floating_point() else t for t in x], d_out, d_fin)
+    for name, a, b in zip(["q", "k", "v", "g", "beta", "initial"], got, want):
+        check(a, b, a.dtype, "d_" + name)

@@ -349,6 +349,10 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
         raise(&sm.most_out, sm.gates.bad, most);
         if (has_state) raise(&sm.most_state, sm.gates.state_bad, most_of<DK / 8>(st));
         __syncthreads();
+        if (sm.gates.bad && p.normalize) {
+          mend_norms<NW, T>(sm.gates, p, rows, t0, lo, hi, tid);
+          __syncthreads();
+        }
         // A value that is not finite must not reach another episode through a product with
         // zero: such a chunk is taken episode by episode.
         if (lo > t0 || !(sm.gates.bad || sm.gates.state_bad || sm.r_bad) || (sm.gates.marks >> 1) == 0) break;

@@ -115,6 +115,10 @@ __global__ void __launch_bounds__(NW * 32, (DK <= 64 ? 512 : 384) / (NW * 32)) d
         load_rows<DK, NW, T, false>(sm.gates, p, rows, sm.q[0], sm.k[0], sm.v, v0, is_m ? 0 : dv, t0, lo, hi, tid);
         if (warp == 0) scan_gates(sm.gates, gates, lane);
         __syncthreads();
+        if (sm.gates.bad && p.normalize) {
+          mend_norms<NW, T>(sm.gates, p, rows, t0, lo, hi, tid);
+          __syncthreads();
+        }
         // A value that is not finite must not reach another episode, nor an earlier token,
         // through a product with zero: such a chunk is taken token by token.
         if (hi - lo == 1 || !(sm.gates.bad || (sm.gates.state_bad && sm.gates.marks != 0))) break;

@@ -391,6 +391,36 @@ __device__ __forceinline__ void load_rows(Gates& s, const ZenoDeltaRule& p, cons
   if (bad) s.bad = 1;
 }
 
+// All warps, where a chunk has rows that are not finite or whose squares are not: the factors of the latter,
+// from values 2^80 times smaller.  load_rows' planes are right for them.  A warp a row.
+template <int NW, class T>
+__device__ __forceinline__ void mend_norms(Gates& s, const ZenoDeltaRule& p, const Rows<T>& r, int64_t t0, int64_t lo, int64_t hi, int tid) {
+  const int lane = tid & 31;
+#pragma unroll 1
+  for (int j = tid >> 5; j < 2 * C; j += NW) {
+    const int row = j % C;
+    const int64_t t = t0 + row;
+    if (t < lo || t >= hi) continue;
+    const T* at = j >= C ? r.k + t * p.k.stride[1] : r.q + t * p.q.stride[1];
+    float sum = 0.0f, most = 0.0f;
+#pragma unroll 1
+    for (int c = lane; c < int(p.key_dim); c += 32) {
+      const float x = In<T>::up(at[c]), y = x * 0x1p-80f;
+      sum = fmaf(y, y, sum), most = max_nan(most, fabsf(x));
+    }
+#pragma unroll 1
+    for (int d = 1; d < 32; d <<= 1) {
+      sum += __shfl_xor_sync(kAll, sum, d);
+      most = max_nan(most, __shfl_xor_sync(kAll, most, d));
+    }
+    // below 2^60 the squares of 128 values stay in 32 bits
+    if (!(most >= 0x1p60f && most < INFINITY) || lane != 0) continue;
+    const float n = inverse_sqrt(sum), f = n * (pow2_unscale(pow2_exp(most)) * 0x1p-80f);
+    if (j >= C) s.token[row].fk = f, s.nk[row] = n * 0x1p-80f;
+    else s.fq[row] = f, s.nq[row] = n * 0x1p-80f;
+  }
+}
+
 // Products of 16 rows of X with 16 rows of Y over the key channels: acc[2] tiles (n8 each).
 template <int DK, int LIMBS>
 __device__ __forceinline__ void rows_times_rows(float (&acc)[2][4], const __half* x, const __half* y, int lane) {

@@ -28,7 +28,7 @@ constexpr int kStepWarps = 4;
 
 // RG: row groups in a warp; 16 RG >= key_dim, and a warp holds 4 (32 / RG) columns.
 template <int RG, class T, bool VEC>
-__global__ void __launch_bounds__(kStepWarps * 32)
+__global__ void __launch_bounds__(kStepWarps * 32, !VEC || (sizeof(T) == 2 && RG >= 4) ? 4 : 3)
 delta_recurrent_kernel(const __grid_constant__ ZenoDeltaRule p, uint32_t slices, uint64_t jobs) {
   constexpr int DK = 16 * RG, CG = 32 / RG;
   __shared__ __align__(16) float sk[kStepWarps][DK], sq[kStepWarps][DK];
@@ -83,15 +83,24 @@ delta_recurrent_kernel(const __grid_constant__ ZenoDeltaRule p, uint32_t slices,
   for (uint32_t t = 0; t < p.tokens; ++t) {
     float nq = 0.0f, nk = 0.0f;
     __syncwarp();
+    float xq[(DK + 31) / 32], xk[(DK + 31) / 32];
+    bool big_q = false, big_k = false;
 #pragma unroll
     for (int i = 0; i < (DK + 31) / 32; ++i) {
       const int r = i * 32 + lane;
-      if (r < DK) {
-        const float xq = r < dk ? to_f(q[int64_t(t) * p.q.stride[1] + r]) : 0.0f;
-        const float xk = r < dk ? to_f(k[int64_t(t) * p.k.stride[1] + r]) : 0.0f;
-        sq[warp][r] = xq, sk[warp][r] = xk;
-        nq = fmaf(xq, xq, nq), nk = fmaf(xk, xk, nk);
-      }
+      xq[i] = r < dk ? to_f(q[int64_t(t) * p.q.stride[1] + r]) : 0.0f;
+      xk[i] = r < dk ? to_f(k[int64_t(t) * p.k.stride[1] + r]) : 0.0f;
+      big_q |= fabsf(xq[i]) >= 0x1p60f, big_k |= fabsf(xk[i]) >= 0x1p60f;
+    }
+    // rows whose squares could leave 32 bits are normalised from a 2^80th of themselves
+    const float lq = p.normalize && __any_sync(0xffffffffu, big_q) ? 0x1p-80f : 1.0f;
+    const float lk = p.normalize && __any_sync(0xffffffffu, big_k) ? 0x1p-80f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < (DK + 31) / 32; ++i) {
+      const int r = i * 32 + lane;
+      xq[i] *= lq, xk[i] *= lk;
+      if (r < DK) sq[warp][r] = xq[i], sk[warp][r] = xk[i];
+      nq = fmaf(xq[i], xq[i], nq), nk = fmaf(xk[i], xk[i], nk);
     }
     float fq = p.scale, fk = 1.0f;
     if (p.normalize) {
@@ -100,7 +109,7 @@ delta_recurrent_kernel(const __grid_constant__ ZenoDeltaRule p, uint32_t slices,
         nq += __shfl_xor_sync(0xffffffffu, nq, d);
         nk += __shfl_xor_sync(0xffffffffu, nk, d);
       }
-      fq = p.scale / sqrtf(nq + kNormEps), fk = 1.0f / sqrtf(nk + kNormEps);
+      fq = p.scale / sqrtf(nq + kNormEps * lq * lq), fk = 1.0f / sqrtf(nk + kNormEps * lk * lk);
     }
     __syncwarp();
     const bool clear = rs && rs[int64_t(t) * p.reset.stride[1]];
