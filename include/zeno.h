@@ -382,6 +382,10 @@ uint64_t zeno_orthogonalize_workspace_bytes(uint32_t count, uint32_t rows, uint3
 int zeno_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows,
                        uint32_t cols, uint32_t dtype, uint32_t steps, void* workspace, uint64_t workspace_bytes,
                        void* cuda_stream);
+/* A product that waits longer than this for its own copies or matrix instructions gives up, and
+ * what builds on it comes out as NaN.  Sets the limit of later calls in nanoseconds (2e9 at
+ * first; 0: nothing is waited for, so all give up) and returns the one before. */
+uint64_t zeno_orthogonalize_wait_limit(uint64_t nanoseconds);
 
 #ifdef __cplusplus
 }

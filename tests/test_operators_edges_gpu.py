@@ -125,3 +125,21 @@ def test_gradients_of_rows_whose_squares_overflow(dtype):
     want = gradients(plain.delta_rule, [t.double() if t.is_floating_point() else t for t in x], d_out, d_fin)
     for name, a, b in zip(["q", "k", "v", "g", "beta", "initial"], got, want):
         check(a, b, a.dtype, "d_" + name)
+
+
+@pytest.mark.parametrize("steps", [1, 5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(100, 290), (700, 130), (3, 260, 140)])
+def test_orthogonalize_that_gives_up_is_not_a_number(shape, dtype, steps):
+    m = matrix(shape, dtype)
+    want = zeno_b200.orthogonalize(m, steps)
+    assert torch.isfinite(want).all()
+    before = _lib.zeno_orthogonalize_wait_limit(0)  # no product waits for anything
+    try:
+        got = zeno_b200.orthogonalize(m, steps)
+        torch.cuda.synchronize()
+    finally:
+        assert _lib.zeno_orthogonalize_wait_limit(before) == 0
+    assert before == 2_000_000_000
+    assert torch.isnan(got).all()
+    assert torch.equal(zeno_b200.orthogonalize(m, steps), want)

@@ -135,6 +135,7 @@ ffi.cdef("""
     int zeno_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows,
                            uint32_t cols, uint32_t dtype, uint32_t steps, void* workspace, uint64_t workspace_bytes,
                            void* cuda_stream);
+    uint64_t zeno_orthogonalize_wait_limit(uint64_t nanoseconds);
 """)
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libzeno.so"

@@ -32,6 +32,7 @@ constexpr int kTile = 128;     // rows and columns of a product's tile, and the 
 constexpr int kDeep = 64;      // contracted values of a stage: 128 bytes, the swizzle's width
 constexpr int kPlane = kTile * kDeep * 2;  // bytes of one operand's stage, one limb
 constexpr uint64_t kPatience = 2000000000;  // nanoseconds at a barrier before a block gives up
+std::atomic<uint64_t> wait_limit{kPatience};
 
 __host__ __device__ constexpr uint64_t padded(uint64_t x) { return (x + kTile - 1) / kTile * kTile; }
 
@@ -81,18 +82,21 @@ __device__ __forceinline__ double inverse_norm(const double* part, uint32_t part
   return 1.0 / (sqrt(block_sum(threadIdx.x < parts ? part[threadIdx.x] : 0.0)) + kEps);
 }
 
-// X's planes in both orientations, zero in the padding: [count][2 limbs][mp][np] and [count][2 limbs][np][mp],
-// and the first extra exponent of each matrix.  A block has 64 x 64 elements.
+// X's planes in both orientations, zero in the padding: [count][2 limbs][mp][np] and [count][2 limbs][np][mp];
+// the first extra exponent of each matrix, and no failure yet.  A block has 64 x 64 elements.
 template <class T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* from, Matrix s, const double* part, uint32_t parts, __half* x, __half* xt,
-                                                     int* extra) {
+                                                     uint32_t* failed, int* extra) {
   __shared__ float tile[64][65];
   wait_for_previous();
   let_next_start();
   const uint32_t mp = uint32_t(padded(s.m)), np = uint32_t(padded(s.n));
   const double inverse = inverse_norm(part + uint64_t(blockIdx.z) * parts, parts);
   const int more = first_extra(inverse);
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) extra[blockIdx.z] = more;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    extra[blockIdx.z] = more;
+    if (blockIdx.z == 0) *failed = 0;
+  }
   const double f = inverse * scalbn(double(kScale), more);
   const T* at = from + int64_t(blockIdx.z) * s.matrix;
   const uint32_t i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
@@ -144,8 +148,10 @@ __device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+// Whether the phase ended within `patience` nanoseconds (0: not waited for at all).
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, uint64_t patience) {
   uint64_t began = 0, now;
+  if (patience == 0) return false;
   for (;;) {
     uint32_t done;
     asm volatile(
@@ -156,7 +162,7 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     if (done) return true;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (began == 0) began = now;
-    else if (now - began > kPatience) return false;
+    else if (now - began > patience) return false;
   }
 }
 __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
@@ -219,6 +225,16 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t from,
                : "memory");
 }
 
+// Barrier of the 256 threads of the epilogue: whether all of them say yes.
+__device__ __forceinline__ bool all_of_256(bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.and.pred q, 1, 256, p;\nselp.u32 %0, 1, 0, q;\n}"
+      : "=r"(all) : "r"(uint32_t(yes)) : "memory");
+  return all != 0;
+}
+
 enum Kind { kGram, kSquare, kApply, kLast };  // A; B; X in both orientations; X to the caller
 
 struct Product {
@@ -229,7 +245,8 @@ struct Product {
   void* last;             // kLast: the caller's array
   uint32_t m, n;          // kLast: X's sizes
   uint32_t transposed;    // kLast: the caller's matrices are X^T
-  uint32_t* failed;       // set where a barrier was waited for in vain
+  uint32_t* failed;       // set where a barrier was waited for in vain; kLast writes NaN then
+  uint64_t patience;
 };
 
 // Shared memory: a ring of 6 units of 32 KB; a stage is two units, both operands' hi and lo limbs.
@@ -254,8 +271,8 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   constexpr int S = kUnits / kLimbs;
   extern __shared__ unsigned char raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kUnits * kUnit);  // full[S], empty[S], done, added
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + kUnits * kUnit);  // full[S], empty[S], done, added, drained
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 3);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr bool kSymmetric = KIND == kGram || KIND == kSquare;
 
@@ -272,7 +289,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   const uint32_t z = blockIdx.y;
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < 2 * S + 2; ++s) barrier_init(smem_at(bars + s), 1);
+    for (int s = 0; s < 2 * S + 3; ++s) barrier_init(smem_at(bars + s), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -286,7 +303,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   const int stages = int(p.depth / kDeep);
   const uint32_t unit0 = smem_at(base);
   const int first_add = stages * kLimbs % kUnits;
-  const uint32_t done = smem_at(bars + 2 * S), added = smem_at(bars + 2 * S + 1);
+  const uint32_t done = smem_at(bars + 2 * S), added = smem_at(bars + 2 * S + 1), drained = smem_at(bars + 2 * S + 2);
   wait_for_previous();
   let_next_start();
   asm volatile("fence.proxy.async;" ::: "memory");  // the planes may come from ordinary stores
@@ -296,7 +313,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
     bool ok = true;
     for (; k < stages; ++k) {
       const int s = k % S;
-      if (k >= S) ok = barrier_wait(smem_at(bars + S + s), (k / S - 1) & 1);
+      if (k >= S) ok = barrier_wait(smem_at(bars + S + s), (k / S - 1) & 1, p.patience);
       if (!ok) break;
       const uint32_t bar = smem_at(bars + s), at = unit0 + s * kLimbs * kUnit;
       barrier_expect(bar, kLimbs * kUnit);
@@ -307,7 +324,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       }
     }
     if (KIND != kGram && ok) {
-      if (stages >= S) ok = barrier_wait(smem_at(bars + S + stages % S), (stages / S - 1) & 1);
+      if (stages >= S) ok = barrier_wait(smem_at(bars + S + stages % S), (stages / S - 1) & 1, p.patience);
       if (ok) {
         barrier_expect(added, kLimbs * kUnit);
         for (int l = 0; l < kLimbs; ++l)
@@ -316,15 +333,15 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
                      int(z * 2 + l));
       }
     }
-    if (!ok) {  // let the copies in flight land before the block ends
-      atomicExch(p.failed, 1u);
-      for (int j = k > S ? k - S : 0; j < k; ++j) barrier_wait(smem_at(bars + j % S), (j / S) & 1);
-    }
+    if (!ok) atomicExch(p.failed, 1u);
+    // the copies in flight land before the block ends, whoever gave up
+    for (int j = k > S ? k - S : 0; j < k; ++j) barrier_wait(smem_at(bars + j % S), (j / S) & 1, kPatience);
+    if (KIND != kGram && ok) barrier_wait(added, 0, kPatience);
   } else if (warp == 1 && lane == 0) {
     bool ok = true;
     for (int k = 0; k < stages; ++k) {
       const int s = k % S;
-      ok = barrier_wait(smem_at(bars + s), (k / S) & 1);
+      ok = barrier_wait(smem_at(bars + s), (k / S) & 1, p.patience);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t at = unit0 + s * kLimbs * kUnit;
@@ -341,8 +358,11 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       }
       tensor_commit(smem_at(bars + S + s));
     }
-    if (ok) tensor_commit(done);
-    else atomicExch(p.failed, 1u);
+    if (!ok) atomicExch(p.failed, 1u);
+    // ... and the products under way end before the accumulators are given back
+    const uint32_t end = ok ? done : drained;
+    tensor_commit(end);
+    barrier_wait(end, 0, kPatience);
   } else if (warp >= 4) {
     // Scales: X 2^(12 + E), A and B 2^(12 + 2 E), their products the sums of the two.
     const int first = p.extra[z], now = extra_at(first, p.step), next = extra_at(first, p.step + 1);
@@ -351,9 +371,10 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
                     : KIND == kApply  ? exp2f(float(-12 - 3 * now + next))
                                       : exp2f(float(-24 - 3 * now));
     const float g = KIND == kSquare ? kB : KIND == kApply ? kA * exp2f(float(next - now)) : kA * exp2f(float(-12 - now));
-    bool ok = barrier_wait(done, 0);
-    if (KIND != kGram && ok) ok = barrier_wait(added, 0);
-    ok = __all_sync(0xffffffffu, ok);
+    const bool earlier = KIND == kLast && *p.failed != 0;  // a product that this one builds on gave up
+    bool ok = barrier_wait(done, 0, p.patience);
+    if (KIND != kGram && ok) ok = barrier_wait(added, 0, p.patience);
+    ok = __all_sync(0xffffffffu, ok && !earlier);
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int quarter = warp & 3, gi = lane >> 2, qj = (lane & 3) * 2;
@@ -422,13 +443,19 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    } else if (lane == 0) {
-      atomicExch(p.failed, 1u);
+    } else {
+      if (lane == 0) atomicExch(p.failed, 1u);
+      if constexpr (KIND == kLast) {  // what cannot be computed is not a number
+        T* to = static_cast<T*>(p.last) + uint64_t(z) * p.m * p.n;
+        const uint32_t i = ti * kTile + (warp & 3) * 32 + lane, j0 = tj * kTile + ((warp >> 2) - 1) * 64;
+        if (i < p.m)
+          for (uint32_t j = j0; j < min(j0 + 64, p.n); ++j)
+            to[p.transposed ? uint64_t(j) * p.m + i : uint64_t(i) * p.n + j] = T(__int_as_float(0x7fffffff));
+      }
     }
     if (KIND != kLast) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (warp == 4 && lane == 0 && ok) {
+      if (all_of_256(ok) && warp == 4 && lane == 0) {
         const bool mirror = KIND == kApply || ti != tj;
         for (int l = 0; l < kLimbs; ++l)
           for (int half = 0; half < 2; ++half) {
@@ -535,7 +562,7 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
     return launch_after(normalise_kernel<T>, dim3(s.count, 64), 256, 0, stream, from, s, static_cast<const double*>(part), parts,
                         static_cast<T*>(out), transposed);
   e = launch_after(planes_kernel<T>, dim3(np / 64, mp / 64, s.count), 256, 0, stream, from, s, static_cast<const double*>(part), parts, x[0],
-                   xt[0], extra);
+                   xt[0], failed, extra);
   CUtensorMap mx[2], mxt[2], ma, mb;
   const uint64_t layers = uint64_t(s.count) * 2;
   for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
@@ -549,6 +576,7 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
     const int now = i & 1, next = now ^ 1;
     Product p{};
     p.m = s.m, p.n = s.n, p.transposed = transposed, p.failed = failed, p.extra = extra, p.step = i, p.last = out;
+    p.patience = wait_limit.load(std::memory_order_relaxed);
     p.depth = np, p.cols = mp;
     e = launch<kGram>(Maps{mx[now], mx[now], ma, ma, ma}, p, lower, s.count, stream);
     p.depth = mp;
@@ -563,6 +591,8 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
 
 }  // namespace
 }  // namespace ns
+
+uint64_t orthogonalize_wait_limit(uint64_t nanoseconds) { return ns::wait_limit.exchange(nanoseconds); }
 
 uint64_t orthogonalize_workspace(uint32_t count, uint32_t rows, uint32_t cols, uint32_t) {
   const uint64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;

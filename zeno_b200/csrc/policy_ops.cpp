@@ -127,6 +127,8 @@ int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d
   return zb::status(what, zb::launch_delta_backward(*p, *d, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
 
+uint64_t zeno_orthogonalize_wait_limit(uint64_t nanoseconds) { return zb::orthogonalize_wait_limit(nanoseconds); }
+
 uint64_t zeno_orthogonalize_workspace_bytes(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype) {
   return zb::matrix_fault(count, rows, cols, dtype).empty() ? zb::orthogonalize_workspace(count, rows, cols, dtype) : 0;
 }

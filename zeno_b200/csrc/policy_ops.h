@@ -53,6 +53,7 @@ uint64_t delta_forward_workspace(const ZenoDeltaRule& p);
 cudaError_t launch_delta_forward(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream);
 cudaError_t launch_delta_backward(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream);
 
+uint64_t orthogonalize_wait_limit(uint64_t nanoseconds);
 uint64_t orthogonalize_workspace(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype);
 cudaError_t launch_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows, uint32_t cols,
                                  uint32_t dtype, uint32_t steps, void* workspace, cudaStream_t stream);
