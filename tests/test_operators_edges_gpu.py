@@ -143,3 +143,21 @@ def test_orthogonalize_that_gives_up_is_not_a_number(shape, dtype, steps):
     assert before == 2_000_000_000
     assert torch.isnan(got).all()
     assert torch.equal(zeno_b200.orthogonalize(m, steps), want)
+
+
+def test_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    q, k, v, g, beta, _, state = inputs(2, 3, 1, 1, 8, 8, torch.float32)
+    with forward_ad.dual_level():
+        for i in range(6):
+            x = [q, k, v, g, beta, state]
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                zeno_b200.delta_rule(*x[:5], None, x[5])
+            one = [y[:, 0] for y in x[:5]]
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                zeno_b200.delta_rule_step(*one, x[5])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            zeno_b200.orthogonalize(forward_ad.make_dual(state[0, 0], state[1, 0]))
+        zeno_b200.delta_rule(q, k, v, g, beta, None, state)  # none of these has a tangent
+        zeno_b200.orthogonalize(state)

@@ -14,6 +14,7 @@ from contextlib import nullcontext
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from ._ffi import _lib, ffi
@@ -46,6 +47,12 @@ def _stream(index: int):
 def _on(index: int):
     """A context in which the device is the current one."""
     return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _refuse_tangents(what: str, *tensors: Optional[Tensor]) -> None:
+    """The kernels see values alone: a tangent would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivatives")
 
 
 def _expect(name: str, x: Tensor, shape: Tuple[int, ...], dtypes, device: torch.device) -> None:
@@ -198,11 +205,13 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: 
     Any strides are taken (a time-major buffer's transposed view needs no copy) as long as
     the last axis is contiguous.  The state is held in 32 bits.  Gradients flow to q, k, v,
     g, beta and initial_state; they are sums in a fixed order, so they repeat bit for bit.
+    (Once, and in reverse mode only.)
     """
     state = _check_inputs(q, k, v, g, beta, reset, 2)
     if initial_state is not None:
         _expect("initial_state", initial_state, state, (torch.float32,), q.device)
         initial_state = initial_state.contiguous()
+    _refuse_tangents("delta_rule", q, k, v, g, beta, initial_state)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     q, k, v = _rows(q), _rows(k), _rows(v)
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, initial_state)):
@@ -224,6 +233,7 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, st
         raise ValueError("state must be contiguous: it is updated in place")
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, g, beta, state)):
         raise RuntimeError("delta_rule_step has no gradients: call it under torch.no_grad(), and delta_rule to learn")
+    _refuse_tangents("delta_rule_step", q, k, v, g, beta, state)
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
@@ -250,6 +260,7 @@ def orthogonalize(update: Tensor, steps: int = 5) -> Tensor:
         raise TypeError(f"update must be float32 or bfloat16, got {update.dtype}")
     if not 0 <= steps <= 100:
         raise ValueError(f"steps must be 0 to 100, got {steps}")
+    _refuse_tangents("orthogonalize", update)
     m, n = update.shape[-2:]
     x = update.detach()
     x = x.unsqueeze(0) if x.dim() == 2 else x if x.dim() == 3 else x.reshape(-1, m, n)
