@@ -161,3 +161,17 @@ def test_forward_mode_derivatives_are_refused():
             zeno_b200.orthogonalize(forward_ad.make_dual(state[0, 0], state[1, 0]))
         zeno_b200.delta_rule(q, k, v, g, beta, None, state)  # none of these has a tangent
         zeno_b200.orthogonalize(state)
+
+
+# 2e-5 as at other widths: what a sum of n terms loses may not grow with n
+@pytest.mark.parametrize("shape", [(70, 4200), (70, 20000), (130, 262144), (300000, 33), (4300, 4400)])
+def test_orthogonalize_long_sums(shape):
+    m = matrix(shape, torch.float32, seed=2)
+    assert plain.off(zeno_b200.orthogonalize(m), plain.orthogonalize(m)) <= 2e-5
+
+
+@pytest.mark.parametrize("steps", [1, 2])
+def test_orthogonalize_long_sums_of_one_and_two_steps(steps):
+    for shape in [(4300, 4400), (8, 9000)]:
+        m = matrix(shape, torch.float32, seed=2)
+        assert plain.off(zeno_b200.orthogonalize(m, steps), plain.orthogonalize(m, steps)) <= 2e-5

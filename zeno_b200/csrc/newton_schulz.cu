@@ -31,6 +31,10 @@ constexpr uint32_t kNormBlocks = 256;  // of a matrix, at most
 constexpr int kTile = 128;     // rows and columns of a product's tile, and the padding of every matrix
 constexpr int kDeep = 64;      // contracted values of a stage: 128 bytes, the swizzle's width
 constexpr int kPlane = kTile * kDeep * 2;  // bytes of one operand's stage, one limb
+// Contracted values of one launch at most: the tensor cores' truncating sums lose in proportion to their length, rounded
+// sums of such parts do not (130 x 262144 in one sum: 9.3e-4 of the result, 16.2 ms; in parts 1.0e-5, 18.5 ms; 2048 x 8192:
+// 1.7e-5, 1776 us and 6.9e-6, 1804 us).
+constexpr uint32_t kLongest = 4096;
 constexpr uint64_t kPatience = 2000000000;  // nanoseconds at a barrier before a block gives up
 std::atomic<uint64_t> wait_limit{kPatience};
 
@@ -238,7 +242,9 @@ __device__ __forceinline__ bool all_of_256(bool yes) {
 enum Kind { kGram, kSquare, kApply, kLast };  // A; B; X in both orientations; X to the caller
 
 struct Product {
-  uint32_t depth;         // contracted length, a multiple of kDeep
+  uint32_t depth;         // contracted length, a multiple of kDeep,
+  uint32_t from;          // from this index on
+  uint32_t more;          // further part of a long sum: the result so far is what is added to
   uint32_t cols;          // padded columns of the result
   uint32_t step;
   const int* extra;       // first extra exponents
@@ -301,6 +307,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const int stages = int(p.depth / kDeep);
+  const bool adds = KIND != kGram || p.more;
   const uint32_t unit0 = smem_at(base);
   const int first_add = stages * kLimbs % kUnits;
   const uint32_t done = smem_at(bars + 2 * S), added = smem_at(bars + 2 * S + 1), drained = smem_at(bars + 2 * S + 2);
@@ -319,11 +326,11 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
       barrier_expect(bar, kLimbs * kUnit);
 #pragma unroll
       for (int l = 0; l < kLimbs; ++l) {
-        tma_load(at + l * kPlane, &left, bar, k * kDeep, int(ti * kTile), int(z * 2 + l));
-        tma_load(at + (kLimbs + l) * kPlane, &right, bar, k * kDeep, int(tj * kTile), int(z * 2 + l));
+        tma_load(at + l * kPlane, &left, bar, int(p.from) + k * kDeep, int(ti * kTile), int(z * 2 + l));
+        tma_load(at + (kLimbs + l) * kPlane, &right, bar, int(p.from) + k * kDeep, int(tj * kTile), int(z * 2 + l));
       }
     }
-    if (KIND != kGram && ok) {
+    if (adds && ok) {
       if (stages >= S) ok = barrier_wait(smem_at(bars + S + stages % S), (stages / S - 1) & 1, p.patience);
       if (ok) {
         barrier_expect(added, kLimbs * kUnit);
@@ -336,7 +343,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
     if (!ok) atomicExch(p.failed, 1u);
     // the copies in flight land before the block ends, whoever gave up
     for (int j = k > S ? k - S : 0; j < k; ++j) barrier_wait(smem_at(bars + j % S), (j / S) & 1, kPatience);
-    if (KIND != kGram && ok) barrier_wait(added, 0, kPatience);
+    if (adds && ok) barrier_wait(added, 0, kPatience);
   } else if (warp == 1 && lane == 0) {
     bool ok = true;
     for (int k = 0; k < stages; ++k) {
@@ -370,10 +377,13 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
                     : KIND == kSquare ? kC * exp2f(float(-12 - 2 * now))
                     : KIND == kApply  ? exp2f(float(-12 - 3 * now + next))
                                       : exp2f(float(-24 - 3 * now));
-    const float g = KIND == kSquare ? kB : KIND == kApply ? kA * exp2f(float(next - now)) : kA * exp2f(float(-12 - now));
+    const float g = KIND == kLast ? (p.more ? exp2f(float(-12 - next)) : kA * exp2f(float(-12 - now)))
+                    : p.more      ? 1.0f
+                    : KIND == kSquare ? kB
+                                      : kA * exp2f(float(next - now));
     const bool earlier = KIND == kLast && *p.failed != 0;  // a product that this one builds on gave up
     bool ok = barrier_wait(done, 0, p.patience);
-    if (KIND != kGram && ok) ok = barrier_wait(added, 0, p.patience);
+    if (adds && ok) ok = barrier_wait(added, 0, p.patience);
     ok = __all_sync(0xffffffffu, ok && !earlier);
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -401,7 +411,7 @@ product_kernel(const __grid_constant__ CUtensorMap left, const __grid_constant__
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const uint32_t row = r0 + gi + ((e >> 1) & 1) * 8, col = c0 + (e >> 2) * 8 + qj;
-          if (KIND == kGram) {
+          if (!adds) {
             v[e] *= f, v[e + 1] *= f;
           } else {
             const float2 y = __half22float2(*reinterpret_cast<const __half2*>(add0 + in_unit(row, col)));
@@ -577,14 +587,22 @@ cudaError_t run(const void* update, const Matrix& s, bool transposed, void* out,
     Product p{};
     p.m = s.m, p.n = s.n, p.transposed = transposed, p.failed = failed, p.extra = extra, p.step = i, p.last = out;
     p.patience = wait_limit.load(std::memory_order_relaxed);
-    p.depth = np, p.cols = mp;
-    e = launch<kGram>(Maps{mx[now], mx[now], ma, ma, ma}, p, lower, s.count, stream);
-    p.depth = mp;
-    if (e == cudaSuccess) e = launch<kSquare>(Maps{ma, ma, ma, mb, mb}, p, lower, s.count, stream);
+    // The parts of a product, each added to what the ones in front of it left in `sum`.
+    const auto in_parts = [&](uint32_t depth, const CUtensorMap& sum, Maps m, const auto& launch_part) {
+      const uint32_t parts = (depth + kLongest - 1) / kLongest, each = (depth / kTile + parts - 1) / parts * kTile;
+      for (p.from = p.more = 0; p.from < depth && e == cudaSuccess; p.from += each, p.more = 1, m.add = sum) {
+        p.depth = depth - p.from < each ? depth - p.from : each;
+        e = launch_part(m, p.from + each >= depth);
+      }
+    };
+    p.cols = mp;
+    in_parts(np, ma, Maps{mx[now], mx[now], ma, ma, ma},
+             [&](const Maps& m, bool) { return launch<kGram>(m, p, lower, s.count, stream); });
+    in_parts(mp, mb, Maps{ma, ma, ma, mb, mb}, [&](const Maps& m, bool) { return launch<kSquare>(m, p, lower, s.count, stream); });
     p.cols = np;
-    const Maps m{mb, mxt[now], mx[now], mx[next], mxt[next]};
-    if (e == cudaSuccess)
-      e = i + 1 < steps ? launch<kApply>(m, p, mt * nt, s.count, stream) : launch<kLast, T>(m, p, mt * nt, s.count, stream);
+    in_parts(mp, mx[next], Maps{mb, mxt[now], mx[now], mx[next], mxt[next]}, [&](const Maps& m, bool end) {
+      return end && i + 1 == steps ? launch<kLast, T>(m, p, mt * nt, s.count, stream) : launch<kApply>(m, p, mt * nt, s.count, stream);
+    });
   }
   return e;
 }
