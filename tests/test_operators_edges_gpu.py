@@ -175,3 +175,12 @@ def test_orthogonalize_long_sums_of_one_and_two_steps(steps):
     for shape in [(4300, 4400), (8, 9000)]:
         m = matrix(shape, torch.float32, seed=2)
         assert plain.off(zeno_b200.orthogonalize(m, steps), plain.orthogonalize(m, steps)) <= 2e-5
+
+
+@pytest.mark.parametrize("shape", [(30, 40), (90, 150)])
+@pytest.mark.parametrize("size", [1e-21, 1e-23, 1e-26, 1e-30, 1e-36])
+def test_orthogonalize_of_next_to_nothing(size, shape):
+    m = matrix(shape, torch.float32) * size
+    want = plain.orthogonalize(m)
+    got = zeno_b200.orthogonalize(m)
+    assert got.any() and plain.off(got * 2.0 ** 40, want * 2.0 ** 40) <= 2e-5

@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(256) norm_kernel(const T* from, Matrix s, doub
 }
 
 // By a whole block of 256 threads; parts <= 256.
-__device__ __forceinline__ double inverse_norm(const double* part, uint32_t parts) {
-  return 1.0 / (sqrt(block_sum(threadIdx.x < parts ? part[threadIdx.x] : 0.0)) + kEps);
+__device__ __forceinline__ double norm_of(const double* part, uint32_t parts) {
+  return sqrt(block_sum(threadIdx.x < parts ? part[threadIdx.x] : 0.0));
 }
 
 // X's planes in both orientations, zero in the padding: [count][2 limbs][mp][np] and [count][2 limbs][np][mp];
@@ -95,13 +95,13 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* from, Matrix s, co
   wait_for_previous();
   let_next_start();
   const uint32_t mp = uint32_t(padded(s.m)), np = uint32_t(padded(s.n));
-  const double inverse = inverse_norm(part + uint64_t(blockIdx.z) * parts, parts);
-  const int more = first_extra(inverse);
+  const double norm = norm_of(part + uint64_t(blockIdx.z) * parts, parts);
+  const int more = first_extra(norm);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     extra[blockIdx.z] = more;
     if (blockIdx.z == 0) *failed = 0;
   }
-  const double f = inverse * scalbn(double(kScale), more);
+  const double f = scalbn(double(kScale), more) / (norm + kEps);
   const T* at = from + int64_t(blockIdx.z) * s.matrix;
   const uint32_t i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
   const bool by_row = s.col <= s.row;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* from, Matrix s, co
 template <class T>
 __global__ void __launch_bounds__(256) normalise_kernel(const T* from, Matrix s, const double* part, uint32_t parts, T* out, bool transposed) {
   wait_for_previous();
-  const double f = inverse_norm(part + uint64_t(blockIdx.x) * parts, parts);
+  const double f = 1.0 / (norm_of(part + uint64_t(blockIdx.x) * parts, parts) + kEps);
   const T* at = from + int64_t(blockIdx.x) * s.matrix;
   const uint64_t n = uint64_t(s.m) * s.n;
   for (uint64_t e = blockIdx.y * 256ull + threadIdx.x; e < n; e += 256ull * gridDim.y) {

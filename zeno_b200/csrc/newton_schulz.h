@@ -22,13 +22,12 @@ __device__ __forceinline__ float up(T x) { return float(x); }
 template <>
 __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// The extra exponent of X in front of the first step: 2^-E >= |X|_F = 1 - 1e-7 / (|M| + 1e-7).
-// `inverse` is 1 / (|M| + 1e-7).  At most 100, where a A A X has long left the 32-bit range.
-__device__ __forceinline__ int first_extra(double inverse) {
-  const double size = 1.0 - kEps * inverse;
+// The extra exponent of X in front of the first step: 2^-E >= |X|_F = |M| / (|M| + 1e-7).  At most
+// 125, for the least 32-bit number (B X has long left the 32-bit range then, a X is what counts).
+__device__ __forceinline__ int first_extra(double norm) {
+  const double size = norm / (norm + kEps);
   if (!(size > 0.0)) return 0;
-  const int e = -ilogb(size) - 1;
-  return e < 0 ? 0 : e > 100 ? 100 : e;
+  return max(0, -ilogb(size) - 1);
 }
 // ... and in front of step k
 __device__ __forceinline__ int extra_at(int first, uint32_t k) { return max(0, first - 2 * int(k)); }

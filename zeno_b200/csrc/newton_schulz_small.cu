@@ -87,7 +87,7 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed, i
     for (int r = 0; r < ranks; ++r) sum += *cluster.map_shared_rank(&total, r);
     cluster.sync();
   }
-  const double inverse = 1.0 / (sqrt(sum) + kEps);
+  const double norm = sqrt(sum), inverse = 1.0 / (norm + kEps);
   if (steps == 0) {
     for (int e = tid; e < m * n; e += WARPS * 32) {
       const int i = transposed ? e % m : e / n, j = transposed ? e / m : e % n;
@@ -98,7 +98,7 @@ small_kernel(const T* from, Matrix s, T* out, uint32_t steps, bool transposed, i
     }
     return;
   }
-  const int first = first_extra(inverse);
+  const int first = first_extra(norm);
   const double f = inverse * scalbn(double(kScale), first);
   for (int e = tid; e < mt * nt * 256; e += WARPS * 32) {
     const int i = by_row ? e / (nt * 16) : e % (mt * 16), j = by_row ? e % (nt * 16) : e / (mt * 16);
