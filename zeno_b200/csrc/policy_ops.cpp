@@ -98,7 +98,9 @@ int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t wo
   if (!p) return zb::refuse(what, "NULL arguments");
   const std::string why = zb::data_fault(*p);
   if (!why.empty()) return zb::refuse(what, why);
-  if (workspace_bytes < zeno_delta_rule_workspace_bytes(p, ZENO_DELTA_FORWARD)) return zb::refuse(what, "workspace is too small");
+  const uint64_t need = zeno_delta_rule_workspace_bytes(p, ZENO_DELTA_FORWARD);
+  if (workspace_bytes < need) return zb::refuse(what, "workspace is too small");
+  if (need && !workspace) return zb::refuse(what, "workspace is NULL");
   if (!zb::aligned(p->saved, 16) || !zb::aligned(workspace, 16)) return zb::refuse(what, "saved and workspace must be aligned to 16 bytes");
   if (!p->batch) return ZENO_SUCCESS;
   return zb::status(what, zb::launch_delta_forward(*p, workspace, static_cast<cudaStream_t>(cuda_stream)));
@@ -122,7 +124,9 @@ int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d
   if (!zb::aligned(d->d_final, 4) || !zb::aligned(d->d_initial, 4)) return zb::refuse(what, "a state is not aligned to its elements");
   if (!zb::aligned(p->saved, 16) || !zb::aligned(workspace, 16)) return zb::refuse(what, "saved and workspace must be aligned to 16 bytes");
   if (!p->saved && zb::delta_saved_bytes(*p)) return zb::refuse(what, "saved is NULL");
-  if (workspace_bytes < zeno_delta_rule_workspace_bytes(p, ZENO_DELTA_BACKWARD)) return zb::refuse(what, "workspace is too small");
+  const uint64_t need = zeno_delta_rule_workspace_bytes(p, ZENO_DELTA_BACKWARD);
+  if (workspace_bytes < need) return zb::refuse(what, "workspace is too small");
+  if (need && !workspace) return zb::refuse(what, "workspace is NULL");
   if (!p->batch) return ZENO_SUCCESS;
   return zb::status(what, zb::launch_delta_backward(*p, *d, workspace, static_cast<cudaStream_t>(cuda_stream)));
 }
