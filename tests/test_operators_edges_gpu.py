@@ -7,7 +7,7 @@ import torch
 import zeno_b200
 from zeno_b200._ffi import _lib, ffi
 import operators_plain as plain
-from test_operators_gpu import DEV, TOL, check, gradients, inputs, matrix
+from test_operators_gpu import DEV, check, check_forward, check_gradients, gradients, inputs, matrix
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,92 @@ def test_orthogonalize_of_next_to_nothing(size, shape):
     want = plain.orthogonalize(m)
     got = zeno_b200.orthogonalize(m)
     assert got.any() and plain.off(got * 2.0 ** 40, want * 2.0 ** 40) <= 2e-5
+
+
+@pytest.mark.parametrize("B,T,Hk,H,dk,dv,dtype", [(600, 100, 1, 2, 32, 32, torch.float32), (300, 130, 2, 2, 64, 64, torch.bfloat16),
+                                                  (5000, 33, 1, 1, 16, 16, torch.bfloat16)])
+def test_many_environments_of_several_chunks(B, T, Hk, H, dk, dv, dtype):
+    x = inputs(B, T, Hk, H, dk, dv, dtype, seed=T, reset=0.02)
+    check_forward(x, dtype)
+    check_gradients(x, dtype)
+
+
+def test_in_a_cuda_graph():
+    x = [inputs(5, 300, 1, 2, 64, 64, torch.bfloat16, seed=s) for s in (1, 2)]
+    d = [torch.randn_like(x[0][2]), torch.randn_like(x[0][6])]
+    m = [matrix((2, 200, 300), torch.float32, seed=s) for s in (1, 2)]
+    small = [matrix((3, 40, 300), torch.float32, seed=s) for s in (1, 2)]
+
+    def work(x, m, small):
+        state = x[6].clone()
+        out = zeno_b200.delta_rule_step(*(t[:, 0] for t in x[:5]), state, x[5][:, 0])
+        return [out, state, *gradients(zeno_b200.delta_rule, x, *d), zeno_b200.orthogonalize(m), zeno_b200.orthogonalize(small)]
+    want = work(x[1], m[1], small[1])
+    still = [[t.clone() for t in x[0]], m[0].clone(), small[0].clone()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(*still)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(*still)
+    for a, b in zip([*still[0], still[1], still[2]], [*x[1], m[1], small[1]]):
+        a.copy_(b)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_threads_with_streams_of_their_own():
+    import threading
+    x = [inputs(6, 200, 1, 2, 64, 64, torch.bfloat16, seed=s) for s in range(4)]
+    m = [matrix((2, 150, 200), torch.float32, seed=s) for s in range(4)]
+
+    def work(i):
+        d = torch.ones_like(x[i][2]), torch.ones_like(x[i][6])
+        return [*zeno_b200.delta_rule(*x[i]), *gradients(zeno_b200.delta_rule, x[i], *d), zeno_b200.orthogonalize(m[i])]
+    want = [work(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got, wrong = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i] = work(i)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # seen by the test, not lost in the thread
+            wrong.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for a, b in zip(got, want):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
+
+
+def test_muon_is_momentum_orthogonalised():
+    from zeno_b200.policy import Muon
+    shapes = [(20, 70), (300, 90), (3, 40, 50), (17,)]
+    params = [torch.zeros(s, device=DEV, requires_grad=True) for s in shapes]
+    optimiser = Muon(params, lr=0.1, momentum=0.9)
+    plain_params, moments = [[torch.zeros(s, device=DEV, dtype=torch.float64) for s in shapes] for _ in range(2)]
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(7)
+    for _ in range(2):
+        for p, want, mom in zip(params, plain_params, moments):
+            p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+            mom.mul_(0.9).add_(p.grad)
+            update = p.grad.double() + 0.9 * mom
+            if p.dim() > 1:
+                update = plain.orthogonalize(update) * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5
+            want.sub_(0.1 * update)
+        optimiser.step()
+    for p, want in zip(params, plain_params):
+        assert plain.off(p, want) <= 4e-5  # two orthogonalised updates
