@@ -334,7 +334,9 @@ typedef struct {
  *   u  = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
  * normalize: q and k are divided by sqrt(|x|^2 + 1e-6) first.  Value head h reads key head
  * h / (value_heads / key_heads).  A reset clears the state whatever it held, infinities
- * and NaN included.  Widths are 1..128, any strides. */
+ * and NaN included.  Widths are 1..128, any strides.
+ * The state and all sums are 32-bit floats; the products of forward and backward take 22 bits of their
+ * operands, counted from the largest value of a row, in backward from that of 32 tokens of a head. */
 typedef struct {
   uint32_t batch, tokens, key_heads, value_heads, key_dim, value_dim;
   uint32_t dtype;     /* of q, k, v, out and their gradients: ZENO_DTYPE_* */
@@ -364,6 +366,8 @@ typedef struct {
 #define ZENO_DELTA_FORWARD 0u
 #define ZENO_DELTA_BACKWARD 1u
 uint64_t zeno_delta_rule_workspace_bytes(const ZenoDeltaRule* p, uint32_t pass);
+/* (ceil(tokens / 32) - 1) states of every environment and head, their widths rounded up to 32, 64 or 128 (128 rows
+ * have 64 columns at least): 0.8 GB for 4096 environments, 128 tokens and 4 heads of 64 x 64. */
 uint64_t zeno_delta_rule_saved_bytes(const ZenoDeltaRule* p);
 int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d, void* workspace,

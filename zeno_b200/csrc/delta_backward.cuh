@@ -738,7 +738,7 @@ shared_heads_kernel(const float* part_q, const float* part_k, ZenoTensor d_q, Ze
 inline uint32_t back_segments(const ZenoDeltaRule& p) {
   const uint64_t chunks = (uint64_t(p.tokens) + C - 1) / C, blocks = uint64_t(p.batch) * p.value_heads;
   const int warps = value_groups(p), width = key_width(p);
-  const uint64_t slots = 148ull * ((width == 32 || (width == 64 && warps > 2) ? 12 : 8) / warps);
+  const uint64_t slots = uint64_t(kSms) * ((width == 32 || (width == 64 && warps > 2) ? 12 : 8) / warps);
   uint64_t n = blocks ? slots / blocks : 1;
   if (n > chunks / 4) n = chunks / 4;
   return n < 2 ? 1 : uint32_t(n);
@@ -823,7 +823,7 @@ cudaError_t shared_heads(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, vo
   cudaError_t e = by_rows<T, float>(p, x, at, stream);
   if (e != cudaSuccess || rows == 0) return e;
   const uint64_t blocks = (rows + 7) / 8;
-  shared_heads_kernel<T><<<dim3(unsigned(blocks < 148 * 8 ? blocks : 148 * 8), 2), 256, 0, stream>>>(part_q, part_k, d.d_q, d.d_k, rows,
+  shared_heads_kernel<T><<<dim3(unsigned(blocks < kSms * 8 ? blocks : kSms * 8), 2), 256, 0, stream>>>(part_q, part_k, d.d_q, d.d_k, rows,
                                                                                                    p.tokens, p.key_heads, group, p.key_dim);
   return cudaGetLastError();
 }

@@ -225,7 +225,7 @@ inline uint32_t segments_of(const ZenoDeltaRule& p) {
   const uint64_t chunks = (uint64_t(p.tokens) + C - 1) / C;
   const int groups = value_groups(p), warps = groups < 4 ? groups : 4;
   const uint64_t blocks = uint64_t(p.batch) * p.value_heads * (groups / warps);
-  uint64_t n = blocks ? uint64_t(148) * 12 / (blocks * warps) : 1;
+  uint64_t n = blocks ? uint64_t(kSms) * 12 / (blocks * warps) : 1;
   if (n > chunks / 4) n = chunks / 4;
   return n < 4 ? 1 : uint32_t(n);
 }

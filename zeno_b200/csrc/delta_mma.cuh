@@ -7,6 +7,9 @@
 // values 2^-16 of it still keep all of theirs.  Products are hi hi + lo hi + hi lo with
 // 32-bit sums (lo lo is below 2^-22).  bfloat16 inputs are exact in one limb once their
 // row is scaled, so a product of an input with a computed value takes two instructions.
+// The backward pass gives dO, W, dE, S0 and R one scale for all channels and tokens of a chunk
+// (their products contract over either): what lies 2^-16 below its largest value loses bits
+// there, and below 2^-38 is dropped.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -248,7 +248,7 @@ cudaError_t by_width(const void* update, const Matrix& s, bool transposed, void*
   // 64 columns a block while all blocks run at once (64 x 256, 8 warps: 52 us against 73 in one block), else 256
   // (200 of them: 146 us against 358); past 2048 columns up to 512.
   const int tiles = int(s.n + 15) / 16, fine = std::min((tiles + 3) / 4, 8), coarse = std::min((tiles + 15) / 16, 8);
-  const int ranks = uint64_t(s.count) * fine <= 148 ? fine : coarse, per = (tiles + ranks - 1) / ranks;
+  const int ranks = uint64_t(s.count) * fine <= kSms ? fine : coarse, per = (tiles + ranks - 1) / ranks;
   return launch<T>(update, s, transposed, out, steps, ranks, per, stream);
 }
 

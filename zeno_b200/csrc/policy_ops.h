@@ -13,6 +13,7 @@ namespace zb {
 constexpr int kDeltaMaxDim = 128;  // largest key or value width of a head
 constexpr int kDeltaChunk = 32;    // tokens of one chunk (one lane each in the gate scan)
 constexpr float kNormEps = 1e-6f;  // under the root of the norms of q and k
+constexpr uint32_t kSms = 148;     // of a B200
 
 // Lets a kernel use `bytes` of dynamic shared memory, once for each device.
 template <class Kernel>

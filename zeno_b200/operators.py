@@ -205,7 +205,10 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: 
     Any strides are taken (a time-major buffer's transposed view needs no copy) as long as
     the last axis is contiguous.  The state is held in 32 bits.  Gradients flow to q, k, v,
     g, beta and initial_state; they are sums in a fixed order, so they repeat bit for bit.
-    (Once, and in reverse mode only.)
+    (Once, and in reverse mode only.)  g's is a difference of sums over q, k and the state and
+    carries their 32-bit error, which may exceed it where decays leave next to nothing.
+    For the gradients a call keeps the state in front of every 32 tokens but the first,
+    widths rounded up to 32, 64 or 128: 0.8 GB for 4096 x 128 tokens and 4 heads of 64 x 64.
     """
     state = _check_inputs(q, k, v, g, beta, reset, 2)
     if initial_state is not None:
