@@ -372,8 +372,8 @@ uint64_t zeno_delta_rule_saved_bytes(const ZenoDeltaRule* p);
 int zeno_delta_rule_forward(const ZenoDeltaRule* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d, void* workspace,
                              uint64_t workspace_bytes, void* cuda_stream);
-/* The recurrent form, for acting: tokens is usually 1, final_state usually initial_state
- * (updated in place).  Same results as forward up to rounding. */
+/* The recurrent form, for acting: tokens is usually 1 (0: the state is passed on), final_state
+ * usually initial_state (updated in place).  Same results as forward up to rounding. */
 int zeno_delta_rule_step(const ZenoDeltaRule* p, void* cuda_stream);
 
 /* Newton-Schulz orthogonalisation of `count` matrices [rows, cols], as the Muon optimiser
