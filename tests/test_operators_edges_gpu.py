@@ -273,3 +273,35 @@ def test_muon_is_momentum_orthogonalised():
         optimiser.step()
     for p, want in zip(params, plain_params):
         assert plain.off(p, want) <= 4e-5  # two orthogonalised updates
+
+
+def test_offsets_that_pass_32_bits():
+    """Rows of one buffer of 5 GB, the environments' 1.2e9 elements apart."""
+    x = list(inputs(3, 40, 1, 2, 32, 16, torch.bfloat16))
+    far = torch.zeros(2_500_000_000, dtype=torch.bfloat16, device=DEV)
+    at, y = 0, list(x)
+    for i in range(3):
+        s = list(x[i].stride())
+        s[0] = 1_200_000_000
+        y[i] = torch.as_strided(far, x[i].shape, s, at)
+        y[i].copy_(x[i])
+        at += x[i][0].numel()
+    for a, b in zip(zeno_b200.delta_rule(*y), zeno_b200.delta_rule(*x)):
+        assert torch.equal(a, b)
+    d = torch.ones_like(x[2]), torch.ones_like(x[6])
+    want = gradients(zeno_b200.delta_rule, x, *d)
+    leaves = [t.detach().requires_grad_(True) if t.is_floating_point() else t for t in y]
+    got = torch.autograd.grad(zeno_b200.delta_rule(*leaves), [t for t in leaves if t.requires_grad], d)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    states = x[6].clone(), x[6].clone()
+    outs = [zeno_b200.delta_rule_step(*(t[:, 3] for t in z[:5]), s) for z, s in zip((x, y), states)]
+    assert torch.equal(*outs) and torch.equal(*states)
+    for shape in [(3, 20, 30), (3, 140, 150)]:
+        m = matrix(shape, torch.bfloat16)
+        wide = torch.as_strided(far, shape, (1_200_000_000, shape[2], 1))
+        wide.copy_(m)
+        assert torch.equal(zeno_b200.orthogonalize(wide), zeno_b200.orthogonalize(m))
+        rows = torch.as_strided(far, shape[1:], (17_000_000, 1))
+        rows.copy_(m[0])
+        assert torch.equal(zeno_b200.orthogonalize(rows), zeno_b200.orthogonalize(m[0]))
