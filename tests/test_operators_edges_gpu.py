@@ -305,3 +305,24 @@ def test_offsets_that_pass_32_bits():
         rows = torch.as_strided(far, shape[1:], (17_000_000, 1))
         rows.copy_(m[0])
         assert torch.equal(zeno_b200.orthogonalize(rows), zeno_b200.orthogonalize(m[0]))
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("name,value", [("q", "nan"), ("q", "inf"), ("k", "nan"), ("k", "-inf"), ("v", "inf"), ("g", "nan"), ("beta", "nan")])
+@pytest.mark.parametrize("T,resets,bad_at", [(70, (20, 45), 30), (70, (20, 32), 40), (33, (32,), 32), (900, (300, 500), 310)])
+def test_gradients_outside_an_episode_that_is_not_finite(T, resets, bad_at, name, value, norm):
+    x = list(inputs(2, T, 1, 2, 64, 40, torch.float32, reset=0.0, norm=norm))
+    for t in resets:
+        x[5][:, t] = 1
+    d = torch.ones_like(x[2]), torch.ones_like(x[6])
+    want = gradients(plain.delta_rule, [t.double() if t.is_floating_point() else t for t in x], *d, normalize=norm)
+    i = "q k v g beta".split().index(name)
+    x[i][0, bad_at, 0] = float(value)
+    got = gradients(zeno_b200.delta_rule, x, *d, normalize=norm)
+    begin = max((0, *(t for t in resets if t <= bad_at)))
+    end = min((T, *(t for t in resets if t > bad_at)))
+    for a, b in zip(got[:5], want[:5]):
+        check(a[1], b[1], torch.float32, "another environment")
+        check(a[0, end:], b[0, end:], torch.float32, "behind the episode")
+        check(a[0, :begin], b[0, :begin], torch.float32, "in front of the episode")
+    check(got[5], want[5], torch.float32, "d_initial")

@@ -679,6 +679,16 @@ delta_backward_kernel(const __grid_constant__ ZenoDeltaRule p, const __grid_cons
 
       // ---- R^T <- a_C R^T + (a dO)^T Q - (a dE)^T K, where something still asks for it
       const bool more = chunk > first || lo > t0 || r_to != nullptr;
+      if (sm.gates.bad && (sm.gates.marks >> int(lo - t0)) & 1) {
+        // The first token drops the state, and the products below give zeros, but not from rows that are not finite: they
+        // have done their part.
+        __syncthreads();
+        uint4* at[2] = {reinterpret_cast<uint4*>(sm.q[0]), reinterpret_cast<uint4*>(sm.k[0])};
+#pragma unroll 1
+        for (int j = tid; j < L * C * SP / 8; j += NW * 32) at[0][j] = at[1][j] = make_uint4(0, 0, 0, 0);
+        if (tid < C) sm.gates.ak[tid] = sm.gates.aq[tid] = 0.0f;
+        __syncthreads();
+      }
       if (more) {
         float x[4][4];
 #pragma unroll
