@@ -376,6 +376,79 @@ int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d
  * usually initial_state (updated in place).  Same results as forward up to rounding. */
 int zeno_delta_rule_step(const ZenoDeltaRule* p, void* cuda_stream);
 
+/* Linear attention with a decay for each head, per environment and value head, with a state S [key_dim, value_dim]:
+ *   S <- exp(g) S, or 0 where an episode begins (reset != 0, or exp(g) == 0)
+ *   S <- S + k v^T;  out = scale S^T q
+ * Heads, resets, widths and strides as for the delta rule; q and k are taken as they are.  One log decay for
+ * each head is a g whose first two strides are 0.  The state and all sums are 32-bit floats.  A product with a
+ * 32-bit value keeps 24 bits of it where its result is 32-bit, 16 where it is a bfloat16. */
+typedef struct {
+  uint32_t batch, tokens, key_heads, value_heads, key_dim, value_dim;
+  uint32_t dtype; /* of q, k, v, out and their gradients: ZENO_DTYPE_* */
+  float scale;
+  ZenoTensor q, k;  /* [batch, tokens, key_heads, key_dim] */
+  ZenoTensor v;     /* [batch, tokens, value_heads, value_dim] */
+  ZenoTensor g;     /* float [batch, tokens, value_heads] */
+  ZenoTensor reset; /* uint8 [batch, tokens]; data NULL: no episode begins */
+  const float* initial_state; /* [batch, value_heads, key_dim, value_dim], contiguous; NULL: zero */
+  float* final_state;         /* same shape; may be initial_state; NULL: not written */
+  ZenoTensor out;             /* [batch, tokens, value_heads, value_dim] */
+  float* saved; /* written by forward for backward: zeno_linear_attention_saved_bytes; NULL: no gradients wanted */
+} ZenoLinearAttention;
+
+/* What backward reads and writes besides the ZenoLinearAttention of its forward call (whose
+ * inputs and saved are unchanged, initial_state too; out is not read).  d_final, d_initial, d_g.data and d_decay may
+ * be NULL. */
+typedef struct {
+  ZenoTensor d_out;     /* read, as out */
+  const float* d_final; /* read, as final_state */
+  ZenoTensor d_q, d_k, d_v;  /* written, as q, k, v */
+  ZenoTensor d_g;       /* written, as g */
+  float* d_decay;       /* written, [value_heads]: the sum of g's gradients over batch and tokens */
+  float* d_initial;     /* written, as initial_state */
+} ZenoLinearAttentionGrads;
+
+#define ZENO_LINEAR_FORWARD 0u
+#define ZENO_LINEAR_BACKWARD 1u
+uint64_t zeno_linear_attention_workspace_bytes(const ZenoLinearAttention* p, uint32_t pass);
+/* The state in front of every 64 tokens but the first (32 in 32-bit calls) of every environment and head: 0.27 GB for 4096
+ * environments, 128 tokens and 4 heads of 64 x 64 in bfloat16. */
+uint64_t zeno_linear_attention_saved_bytes(const ZenoLinearAttention* p);
+int zeno_linear_attention_forward(const ZenoLinearAttention* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+int zeno_linear_attention_backward(const ZenoLinearAttention* p, const ZenoLinearAttentionGrads* d, void* workspace,
+                                   uint64_t workspace_bytes, void* cuda_stream);
+/* The recurrent form, for acting: tokens is usually 1 (0: the state is passed on), final_state usually
+ * initial_state (updated in place).  Same results as forward up to rounding. */
+int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
+
+/* Layer norm of rows of `width` values: out = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps), mean and
+ * variance in 32 bits, the variance from the differences to the mean. */
+typedef struct {
+  uint64_t rows[3];  /* the rows are [rows[0], rows[1], rows[2]] */
+  uint32_t width;    /* at least 1 */
+  uint32_t dtype;    /* of x, out and their gradients: ZENO_DTYPE_* */
+  uint32_t affine_dtype; /* of weight, bias and their gradients */
+  float eps;
+  ZenoTensor x;      /* strides of the three axes of rows, in elements; the values of a row are contiguous */
+  const void* weight; /* [width], contiguous; NULL: 1 */
+  const void* bias;   /* [width], contiguous; NULL: 0 */
+  ZenoTensor out;
+  float* saved;       /* written by forward for backward: mean (in two parts) and rstd of every row, [3][rows]; NULL: no gradients wanted */
+} ZenoLayerNorm;
+
+/* out and bias are not read.  d_x.data, d_weight and d_bias may be NULL: not wanted. */
+typedef struct {
+  ZenoTensor d_out; /* read, as out */
+  ZenoTensor d_x;   /* written, as x */
+  void* d_weight;   /* written, as weight: sums over the rows in a fixed order */
+  void* d_bias;
+} ZenoLayerNormGrads;
+
+int zeno_layer_norm_forward(const ZenoLayerNorm* p, void* cuda_stream);
+uint64_t zeno_layer_norm_workspace_bytes(const ZenoLayerNorm* p); /* of backward */
+int zeno_layer_norm_backward(const ZenoLayerNorm* p, const ZenoLayerNormGrads* d, void* workspace, uint64_t workspace_bytes,
+                             void* cuda_stream);
+
 /* Newton-Schulz orthogonalisation of `count` matrices [rows, cols], as the Muon optimiser
  * applies it to an update M: X = M / (|M|_F + 1e-7), then `steps` times
  *   X <- a X + (b A + c A A) X,  A = X X^T,  (a, b, c) = (3.4445, -4.7750, 2.0315)

@@ -3,8 +3,8 @@
 The physics step runs as one fused CUDA kernel per World.step behind Zeno's C ABI
 (``zeno_b200/lib/libzeno.so``, declared in ``include/zeno.h``).  This package is the
 Python side of that boundary: ``ZenoWorld`` and ``ZenoEnv``/``make`` keep the reference
-package's interface.  ``delta_rule``, ``delta_rule_step`` and ``orthogonalize`` are
-operators for the policies that act in the worlds (they take PyTorch tensors).
+package's interface.  ``delta_rule``, ``delta_rule_step``, ``linear_attention``,
+``linear_attention_step``, ``layer_norm`` and ``orthogonalize`` are operators for the policies that act in the worlds (they take PyTorch tensors).
 
 The library is loaded on first use of a name that needs it (``ZenoWorld``,
 ``is_cuda_available``, ...), not at import, so that the pure-Python modules (``scenes``,
@@ -17,7 +17,7 @@ import importlib
 _FFI_NAMES = ("CONTACT_DTYPE", "CudaArray", "ZenoWorld", "ZeroCopyArray", "is_cuda_available", "is_metal_available",
               "version")
 _ENV_NAMES = ("ZenoEnv", "make")
-_OPERATOR_NAMES = ("delta_rule", "delta_rule_step", "orthogonalize")
+_OPERATOR_NAMES = ("delta_rule", "delta_rule_step", "layer_norm", "linear_attention", "linear_attention_step", "orthogonalize")
 
 
 def __getattr__(name):

@@ -131,6 +131,31 @@ ffi.cdef("""
     int zeno_delta_rule_backward(const ZenoDeltaRule* p, const ZenoDeltaRuleGrads* d, void* workspace,
                                  uint64_t workspace_bytes, void* cuda_stream);
     int zeno_delta_rule_step(const ZenoDeltaRule* p, void* cuda_stream);
+    typedef struct {
+        uint32_t batch; uint32_t tokens; uint32_t key_heads; uint32_t value_heads; uint32_t key_dim; uint32_t value_dim;
+        uint32_t dtype; float scale;
+        ZenoTensor q; ZenoTensor k; ZenoTensor v; ZenoTensor g; ZenoTensor reset;
+        const float* initial_state; float* final_state; ZenoTensor out; float* saved;
+    } ZenoLinearAttention;
+    typedef struct {
+        ZenoTensor d_out; const float* d_final; ZenoTensor d_q; ZenoTensor d_k; ZenoTensor d_v;
+        ZenoTensor d_g; float* d_decay; float* d_initial;
+    } ZenoLinearAttentionGrads;
+    uint64_t zeno_linear_attention_workspace_bytes(const ZenoLinearAttention* p, uint32_t pass);
+    uint64_t zeno_linear_attention_saved_bytes(const ZenoLinearAttention* p);
+    int zeno_linear_attention_forward(const ZenoLinearAttention* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+    int zeno_linear_attention_backward(const ZenoLinearAttention* p, const ZenoLinearAttentionGrads* d, void* workspace,
+                                       uint64_t workspace_bytes, void* cuda_stream);
+    int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
+    typedef struct {
+        uint64_t rows[3]; uint32_t width; uint32_t dtype; uint32_t affine_dtype; float eps;
+        ZenoTensor x; const void* weight; const void* bias; ZenoTensor out; float* saved;
+    } ZenoLayerNorm;
+    typedef struct { ZenoTensor d_out; ZenoTensor d_x; void* d_weight; void* d_bias; } ZenoLayerNormGrads;
+    int zeno_layer_norm_forward(const ZenoLayerNorm* p, void* cuda_stream);
+    uint64_t zeno_layer_norm_workspace_bytes(const ZenoLayerNorm* p);
+    int zeno_layer_norm_backward(const ZenoLayerNorm* p, const ZenoLayerNormGrads* d, void* workspace, uint64_t workspace_bytes,
+                                 void* cuda_stream);
     uint64_t zeno_orthogonalize_workspace_bytes(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype);
     int zeno_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows,
                            uint32_t cols, uint32_t dtype, uint32_t steps, void* workspace, uint64_t workspace_bytes,

@@ -41,10 +41,12 @@ CU_SOURCES = ["step_kernel.cu", "fast_step.cu", "noalloc.cu", "math_eval.cu"]
 OP_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_walk.cu", "delta_backward.cu", "delta_backward_shared.cu",
               "delta_backward_f32.cu", "newton_schulz.cu",
-              "newton_schulz_small.cu"]
+              "newton_schulz_small.cu", "linear_step.cu", "linear_forward.cu", "linear_forward_f32.cu", "linear_backward.cu",
+              "linear_backward_f32.cu", "linear_walk.cu", "layer_norm.cu"]
 CXX_SOURCES = ["mjcf.cpp", "model.cpp", "fast_model.cpp", "world.cpp", "capi.cpp", "policy_ops.cpp"]
 HEADERS = ["zeno_types.h", "devmath.cuh", "physics.cuh", "model_access.cuh", "stage_clock.cuh", "fast_model.h", "step_kernel.h", "scene.h", "model.h", "world.h",
-           "policy_ops.h", "delta_mma.cuh", "delta_backward.cuh", "newton_schulz.h"]
+           "policy_ops.h", "delta_mma.cuh", "delta_backward.cuh", "newton_schulz.h", "linear_mma.cuh", "linear_forward.cuh", "linear_backward.cuh",
+           "linear_launch.h", "linear_forward_impl.cuh", "linear_backward_impl.cuh"]
 
 
 def _newer(target: Path, deps) -> bool:

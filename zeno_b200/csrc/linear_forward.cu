@@ -1,0 +1,21 @@
+// Linear attention, forward, of bfloat16 calls, and the sizes of all.
+#include "linear_forward_impl.cuh"
+
+namespace zb {
+namespace linear {
+template cudaError_t forward<bf16>(const ZenoLinearAttention&, void*, cudaStream_t);
+extern template cudaError_t forward<float>(const ZenoLinearAttention&, void*, cudaStream_t);
+}  // namespace linear
+
+uint64_t linear_saved_bytes(const ZenoLinearAttention& p) {
+  const uint64_t C = uint64_t(linear::chunk_of(p)), chunks = (p.tokens + C - 1) / C;
+  return chunks < 2 ? 0 : (chunks - 1) * p.batch * p.value_heads * p.key_dim * p.value_dim * 4;
+}
+
+uint64_t linear_forward_workspace(const ZenoLinearAttention& p) { return linear::cut_of(p, linear::fill_of(p)).total; }
+
+cudaError_t launch_linear_forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t stream) {
+  return p.dtype == ZENO_DTYPE_BF16 ? linear::forward<linear::bf16>(p, workspace, stream) : linear::forward<float>(p, workspace, stream);
+}
+
+}  // namespace zb

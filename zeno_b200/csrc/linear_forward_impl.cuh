@@ -1,0 +1,33 @@
+// Launches of the forward pass for one element type.
+#pragma once
+#include "linear_launch.h"
+
+namespace zb {
+namespace linear {
+
+template <class T>
+cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t stream) {
+  return with_shape<T>(p, [&](auto shape) {
+    using S = decltype(shape);
+    const Cut c = cut_of(p, fill_of(p));
+    Segments sg{c.count, c.chunks, static_cast<float*>(workspace), nullptr};
+    cudaError_t e;
+    if (c.count > 1) {
+      sg.keep = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.state);
+      e = cut_states<S>(p, p.k, p.v, sg, p.initial_state, false, stream);
+      if (e != cudaSuccess) return e;
+    }
+    constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
+    auto kernel = linear_forward_kernel<S, BLOCKS>;
+    // the first chunk of a rollout from nothing has no state in front of it
+    const int bytes = ForwardSmem<S>::bytes(p.initial_state || c.count > 1 || p.tokens > uint32_t(S::C));
+    static std::atomic<uint64_t> devices{0};
+    e = allow_smem(kernel, ForwardSmem<S>::bytes(true), devices);
+    if (e != cudaSuccess) return e;
+    kernel<<<p.batch * p.value_heads * c.count, S::THREADS, bytes, stream>>>(p, sg);
+    return cudaGetLastError();
+  });
+}
+
+}  // namespace linear
+}  // namespace zb

@@ -1,0 +1,84 @@
+// Which instance of the chunked linear attention serves a call, and how a rollout is cut into segments.
+#pragma once
+#include "linear_backward.cuh"
+
+namespace zb {
+namespace linear {
+
+// Chunks of 64 tokens in bfloat16, so that what a chunk costs whatever its length (the state's limbs, its traffic in
+// training) comes half as often; rollouts of up to 32 tokens and 32-bit calls (three limbs of everything in shared
+// memory) take 32.
+inline int chunk_of(const ZenoLinearAttention& p) { return p.dtype == ZENO_DTYPE_BF16 && p.tokens > 32 ? 64 : 32; }
+inline int width_of(const ZenoLinearAttention& p) {
+  const uint32_t w = p.key_dim > p.value_dim ? p.key_dim : p.value_dim;
+  return w <= 32 ? 32 : w <= 64 ? 64 : 128;
+}
+
+struct Cut {
+  uint32_t count, chunks;  // segments, and chunks of each
+  uint64_t state, keep, total;  // bytes
+};
+// `fill`: blocks that fill the GPU.  Segments cost a second reading of two of the inputs and a walk over the states, so
+// a rollout is cut only where it at least doubles the blocks.
+inline Cut cut_of(const ZenoLinearAttention& p, uint32_t fill) {
+  const uint32_t C = uint32_t(chunk_of(p)), chunks = (p.tokens + C - 1) / C;
+  const uint64_t rows = uint64_t(p.batch) * p.value_heads;
+  Cut c{1, chunks, 0, 0, 0};
+  if (rows == 0 || 2 * rows > fill || chunks < 2) return c;
+  const uint32_t want = uint32_t(fill / rows);
+  const uint32_t count = want < chunks ? want : chunks;
+  c.chunks = (chunks + count - 1) / count;
+  c.count = (chunks + c.chunks - 1) / c.chunks;
+  if (c.count == 1) return c;
+  c.state = (rows * c.count * p.key_dim * p.value_dim * 4 + 15) / 16 * 16;
+  c.keep = (rows * c.count * 4 + 15) / 16 * 16;
+  c.total = c.state + c.keep;
+  return c;
+}
+inline uint32_t fill_of(const ZenoLinearAttention& p) {
+  const int w = width_of(p);
+  return kSms * (w == 128 ? 1 : 2);
+}
+
+// f(shape) of the call's instance, for one element type.
+template <class T, class F>
+cudaError_t with_shape(const ZenoLinearAttention& p, F&& f) {
+  const int w = width_of(p);
+  if constexpr (sizeof(T) == 2) {
+    if (chunk_of(p) == 32) {
+      if (w == 32) return f(Shape<T, 32, 32, 4>{});
+      if (w == 64) return f(Shape<T, 64, 32, 4>{});
+      return f(Shape<T, 128, 32, 8>{});
+    }
+    if (w == 32) return f(Shape<T, 32, 64, 4>{});
+    if (w == 64) return f(Shape<T, 64, 64, 8>{});
+    return f(Shape<T, 128, 64, 16>{});
+  } else {
+    if (w == 32) return f(Shape<T, 32, 32, 4>{});
+    if (w == 64) return f(Shape<T, 64, 32, 8>{});
+    return f(Shape<T, 128, 32, 8>{});
+  }
+}
+
+template <class T>
+cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t stream);
+template <class T>
+cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream);
+
+// What each segment adds, then the states in front of (behind) them.
+template <class S>
+cudaError_t cut_states(const ZenoLinearAttention& p, const ZenoTensor& x, const ZenoTensor& y, const Segments& sg, const float* initial, bool reverse,
+                       cudaStream_t stream) {
+  static std::atomic<uint64_t> devices{0};
+  const int bytes = ForwardSmem<S>::gates + 2 * 2 * S::L * S::PLANE;
+  cudaError_t e = allow_smem(linear_segment_kernel<S>, bytes, devices);
+  if (e != cudaSuccess) return e;
+  const uint32_t rows = p.batch * p.value_heads;
+  linear_segment_kernel<S><<<rows * (sg.count - 1), S::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_linear_walk(LinearWalk{sg.state, sg.keep, initial, sg.count, p.key_dim * p.value_dim, reverse}, rows, stream);
+}
+
+}  // namespace linear
+}  // namespace zb

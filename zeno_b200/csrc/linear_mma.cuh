@@ -1,0 +1,516 @@
+// Building blocks of the chunked linear attention with decays: the chunk's rows in shared memory, matrix
+// products on split operands, the gates of a chunk, and the state in the warps' accumulators.
+//
+// Precision.  The matrix instructions take bfloat16 operands and sum in 32 bits.  bfloat16 inputs enter as
+// they are.  A 32-bit value x enters as limbs of 8 bits each: hi = x cut to bfloat16, then the same of what
+// is left; three limbs are x exactly, and since a bfloat16 has the exponents of a float nothing is scaled and
+// nothing leaves the range.  What ends in a 32-bit result (the states, the decays' gradient, all of a 32-bit call)
+// takes three limbs, products of two such values the six terms above 2^-24.  What ends in a bfloat16 result (P in
+// out and dV, dP in dQ and dK of a bfloat16 call) takes two, the second one rounded: 2^-17 against the result's 2^-9.
+// The instructions' sums truncate, so the state is not summed in them: each chunk's contribution is, and
+// is added to the state by an ordinary multiply-add.
+//
+// Not finite values.  A masked pair is a product with zero, which an infinity or a NaN would leave the mask through.
+// Every present token meets itself, so such an input leaves a result that is not finite; where a chunk has one,
+// its results are taken again element by element over the pairs that the mask leaves.
+#pragma once
+#include <cuda_bf16.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "delta_mma.cuh"
+#include "policy_ops.h"
+
+namespace zb {
+namespace linear {
+
+using delta::kAll;
+using bf16 = __nv_bfloat16;
+using plane_t = uint16_t;  // bfloat16 bits
+
+// D: the widths of a head, padded.  C: tokens of a chunk.  NW: warps.  The warps lie over a chunk's products as
+// [C / 16 row tiles][NH groups of columns] and over the state as [D / 16 row tiles][MG groups of columns].
+template <class T_, int D_, int C_, int NW_>
+struct Shape {
+  using T = T_;
+  static constexpr int D = D_, C = C_, NW = NW_, THREADS = NW_ * 32;
+  static constexpr int L = sizeof(T) == 2 ? 1 : 3;   // limbs of an input
+  static constexpr int PL = sizeof(T) == 2 ? 2 : 3;  // limbs of P and dP
+  static constexpr int P = D + 8, PLANE = C * P;     // rows 16 bytes apart in banks
+  static constexpr int CP = C + 8, CPLANE = C * CP;
+  static constexpr int SPLANE = D * P;
+  static constexpr int RT = C / 16, NH = NW / RT, NHS = NH < RT ? NH : RT, SP = RT / NHS;
+  static constexpr int NO = D / NH / 16;  // pairs of 8 columns of a warp's part of a product
+  static constexpr int MR = D / 16, MG = NW / MR, NM = D / MG / 16;
+  static_assert(NW % RT == 0 && NW % MR == 0 && NO >= 1 && NM >= 1 && SP >= 1);
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Fragments of a 16 x 16 operand in shared memory, as in delta_mma.cuh.  TR: stored with the contracted axis first.
+template <bool TR>
+__device__ __forceinline__ void frag_a(uint32_t (&r)[4], const plane_t* at, int pitch, int lane) {
+  if (TR) delta::ldsm4t(r, delta::smem_at(at + ((lane >> 4) * 8 + (lane & 7)) * pitch + ((lane >> 3) & 1) * 8));
+  else delta::ldsm4(r, delta::smem_at(at + (lane & 15) * pitch + (lane >> 4) * 8));
+}
+template <bool TR>
+__device__ __forceinline__ void frag_b(uint32_t (&r)[4], const plane_t* at, int pitch, int lane) {
+  if (TR) delta::ldsm4t(r, delta::smem_at(at + (lane & 15) * pitch + (lane >> 4) * 8));
+  else delta::ldsm4(r, delta::smem_at(at + ((lane >> 4) * 8 + (lane & 7)) * pitch + ((lane >> 3) & 1) * 8));
+}
+
+__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_cut(float x, float y) {  // the upper halves: x low, y high
+  return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+}
+__device__ __forceinline__ uint32_t pack_round(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two values as N packed limbs; three are exact, of two the second is rounded.
+template <int N>
+__device__ __forceinline__ void split(float x, float y, uint32_t (&r)[N]) {
+  if constexpr (N == 1) {
+    r[0] = pack_round(x, y);
+  } else {
+    r[0] = pack_cut(x, y);
+    x -= cut(x), y -= cut(y);
+    if constexpr (N == 2) {
+      r[1] = pack_round(x, y);
+    } else {
+      r[1] = pack_cut(x, y);
+      r[2] = pack_cut(x - cut(x), y - cut(y));
+    }
+  }
+}
+__device__ __forceinline__ float lower(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float upper(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// The value that N planes hold at `at`; the first alone where it is not finite.
+template <int N>
+__device__ __forceinline__ float value(const plane_t* at, int plane) {
+  float x = __uint_as_float(uint32_t(at[0]) << 16);
+  if (fabsf(x) < INFINITY) {
+#pragma unroll
+    for (int l = 1; l < N; ++l) x += __uint_as_float(uint32_t(at[l * plane]) << 16);
+  }
+  return x;
+}
+// Two neighbouring ones.
+template <int N>
+__device__ __forceinline__ float2 values(const plane_t* at, int plane) {
+  uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+  float2 x = make_float2(lower(w), upper(w));
+#pragma unroll
+  for (int l = 1; l < N; ++l) {
+    w = *reinterpret_cast<const uint32_t*>(at + l * plane);
+    x.x += lower(w), x.y += upper(w);
+  }
+  return x;
+}
+
+// One 16-wide step: d += the products of the first limbs, low += the other terms above 2^-24 of the largest, smallest
+// first.  The instructions' sums truncate at 2^-23 of what they hold, which is 2^-8 less for `low`.
+template <int LA, int LB>
+__device__ __forceinline__ void mma_terms(float (&d)[2][4], float (&low)[2][4], const uint32_t (&a)[LA][4], const uint32_t (&b)[LB][4]) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)
+#pragma unroll
+    for (int l = 0; l < LA; ++l)
+      if (s - l >= 0 && s - l < LB) {
+        float(&to)[2][4] = s ? low : d;
+        mma(to[0], a[l], b[s - l][0], b[s - l][1]);
+        mma(to[1], a[l], b[s - l][2], b[s - l][3]);
+      }
+}
+
+// acc[j] += A B over the 16-wide steps [k0, k1): A 16 x 16 tiles of LA planes, B of LB planes.  pairs: 16-column tiles of B
+// that exist.  Products of two limbs (of P and dP, for bfloat16 results) share one sum.
+template <int LA, int LB, bool TA, bool TB, int N>
+__device__ __forceinline__ void product(float (&acc)[N][2][4], const plane_t* a, int a_pitch, int a_plane, const plane_t* b, int b_pitch,
+                                        int b_plane, int k0, int k1, int pairs, int lane) {
+  constexpr bool APART = LA * LB > 2;
+  float low[APART ? N : 1][2][4] = {};
+#pragma unroll 2
+  for (int kk = k0; kk < k1; ++kk) {
+    uint32_t fa[LA][4];
+#pragma unroll
+    for (int l = 0; l < LA; ++l) frag_a<TA>(fa[l], a + l * a_plane + (TA ? kk * 16 * a_pitch : kk * 16), a_pitch, lane);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j >= pairs) break;
+      uint32_t fb[LB][4];
+#pragma unroll
+      for (int l = 0; l < LB; ++l)
+        frag_b<TB>(fb[l], b + l * b_plane + (TB ? kk * 16 * b_pitch + j * 16 : j * 16 * b_pitch + kk * 16), b_pitch, lane);
+      mma_terms<LA, LB>(acc[j], APART ? low[APART ? j : 0] : acc[j], fa, fb);
+    }
+  }
+  if (APART) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc[j][x >> 2][x & 3] += low[APART ? j : 0][x >> 2][x & 3];
+  }
+}
+
+// ---------------------------------------------------------------- gates
+template <int C>
+struct Gates {
+  float hi[C], lo[C];  // sum of the log decays since the last reset, base 2, in two parts (differences of long sums are exact enough)
+  int episode[C];      // resets up to and including this token
+  float carried[C];    // c_i: decay from the state in front of the chunk; 0 behind a reset, and for absent tokens
+  float to_end[C];     // e_j: decay from token j to the chunk's end; 0 in front of a reset, and for absent tokens
+  float keep;          // what is left of the state in front of the chunk
+};
+
+// One warp: the gates of n tokens, C / 32 neighbouring ones a lane.
+template <int C>
+__device__ __forceinline__ void load_gates(Gates<C>& s, const float* g, int64_t g_stride, const uint8_t* reset, int64_t reset_stride, int64_t t0,
+                                           int n, int lane) {
+  constexpr int U = C / 32;
+  float x[U];
+  bool mark[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = lane * U + u;
+    x[u] = i < n ? g[(t0 + i) * g_stride] : 0.0f;
+    mark[u] = i < n && reset && reset[(t0 + i) * reset_stride];
+  }
+  unsigned marks[U];
+  double sum[U];  // from the last reset on, so that what one episode's decays are, not finite included, stays in it
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    mark[u] = mark[u] || expf(x[u]) == 0.0f;  // a decay to nothing is a reset: the sums behind it stay finite
+    sum[u] = mark[u] ? 0.0 : double(x[u]) + (u ? sum[u - 1] : 0.0);
+    any |= mark[u];
+    marks[u] = __ballot_sync(kAll, mark[u]);
+  }
+  double run = sum[U - 1];
+  bool cut = any;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const double y = __shfl_up_sync(kAll, run, d);
+    const bool z = __shfl_up_sync(kAll, int(cut), d);
+    if (lane >= d) {
+      if (!cut) run += y;
+      cut |= z;
+    }
+  }
+  const double last = __shfl_sync(kAll, run, 31) * 1.4426950408889634;
+  double before = __shfl_up_sync(kAll, run, 1);
+  if (lane == 0) before = 0.0;
+  int all = 0, episode = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) all += __popc(marks[u]), episode += __popc(marks[u] & ((1u << lane) - 1));
+  any = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = lane * U + u;
+    any |= mark[u];
+    const double y = (any ? sum[u] : before + sum[u]) * 1.4426950408889634;
+    episode += mark[u];
+    s.hi[i] = float(y);
+    s.lo[i] = float(y - float(y));
+    s.episode[i] = episode;
+    s.carried[i] = i < n && episode == 0 ? ex2(float(y)) : 0.0f;
+    s.to_end[i] = i < n && episode == all ? ex2(float(last - y)) : 0.0f;
+  }
+  if (lane == 0) s.keep = all == 0 ? ex2(float(last)) : 0.0f;
+}
+
+// ---------------------------------------------------------------- rows
+__device__ __forceinline__ void copy16(plane_t* to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(delta::smem_at(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// All threads: n rows of `width` values as planes [16 nt][P], zero for absent tokens and past the width up to
+// the next 16 columns.
+template <class S>
+__device__ __forceinline__ void load_rows(plane_t* to, const typename S::T* from, int64_t stride, int width, bool vec, int n, int nt, int tid) {
+  constexpr int LR = S::D / 8;
+  const int cols = (width + 15) & ~15;
+  if (S::L == 1 && vec) {
+#pragma unroll 4
+    for (int j = tid; j < nt * 16 * LR; j += S::THREADS) {
+      const int row = j / LR, c = j % LR * 8;
+      if (c >= cols) continue;
+      const bool there = row < n && c < width;
+      copy16(to + row * S::P + c, there ? from + row * stride + c : from, there);
+    }
+    return;
+  }
+#pragma unroll 2
+  for (int j = tid; j < nt * 16 * LR; j += S::THREADS) {
+    const int row = j / LR, c = j % LR * 8;
+    if (c >= cols) continue;
+    delta::Eight raw{};
+    if (row < n && c < width) raw = delta::fetch8(from + row * stride + c, width - c, vec);
+    plane_t* at = to + row * S::P + c;
+    if constexpr (S::L == 1) {
+      *reinterpret_cast<uint4*>(at) = raw.a;
+    } else {
+      float x[8];
+      delta::unpack8<float>(x, raw);
+      uint32_t w[3][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t r[3];
+        // an infinity or a NaN is its first limb alone
+        const float x0 = x[2 * i], x1 = x[2 * i + 1];
+        const bool f0 = fabsf(x0) < INFINITY, f1 = fabsf(x1) < INFINITY;
+        split<3>(x0, x1, r);
+        if (!f0 || !f1) {
+          split<3>(f0 ? x0 : 0.0f, f1 ? x1 : 0.0f, r);
+          if (!f0) r[0] = (r[0] & 0xffff0000u) | (x0 != x0 ? 0x7fc0u : __float_as_uint(x0) >> 16);
+          if (!f1) r[0] = (r[0] & 0xffffu) | (x1 != x1 ? 0x7fc00000u : __float_as_uint(x1));
+        }
+        w[0][i] = r[0], w[1][i] = r[1], w[2][i] = r[2];
+      }
+#pragma unroll
+      for (int l = 0; l < 3; ++l) *reinterpret_cast<uint4*>(at + l * S::PLANE) = make_uint4(w[l][0], w[l][1], w[l][2], w[l][3]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the state in the warps' accumulators
+// A warp's part: rows [16 (warp % MR), +16), columns [16 NM (warp / MR), +16 NM) of a state [dk][dv].
+template <class S>
+struct Part {
+  int row, col;    // first row and column
+  int pairs;       // 16-column tiles that exist (0: none, or no rows)
+  __device__ __forceinline__ Part(int warp, int dk, int dv) {
+    row = warp % S::MR * 16, col = warp / S::MR * S::NM * 16;
+    pairs = row < dk && col < dv ? (dv - col + 15) / 16 : 0;
+  }
+};
+
+// f(element of row, column, value reference) over pairs of neighbouring columns of a part that exist.
+template <class S, class F>
+__device__ __forceinline__ void each_pair(float (&m)[S::NM][2][4], const Part<S>& part, int dk, int dv, int lane, F&& f) {
+#pragma unroll
+  for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = part.row + (lane >> 2) + r * 8, col = part.col + j * 16 + h * 8 + (lane & 3) * 2;
+        if (row < dk && col < dv) f(row, col, m[j][h][2 * r], m[j][h][2 * r + 1]);
+      }
+}
+
+template <class S>
+__device__ __forceinline__ void clear(float (&m)[S::NM][2][4]) {
+#pragma unroll
+  for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) m[j][x >> 2][x & 3] = 0.0f;
+}
+
+// `even`: pairs of columns are 8-byte aligned
+__device__ __forceinline__ bool pairs_aligned(const void* p, int dv) { return dv % 2 == 0 && reinterpret_cast<uintptr_t>(p) % 8 == 0; }
+__device__ __forceinline__ float2 read_pair(const float* at, int col, int dv, bool even) {
+  if (even) return *reinterpret_cast<const float2*>(at);
+  return make_float2(at[0], col + 1 < dv ? at[1] : 0.0f);
+}
+__device__ __forceinline__ void write_pair(float* at, int col, int dv, bool even, float x, float y) {
+  if (even) {
+    *reinterpret_cast<float2*>(at) = make_float2(x, y);
+  } else {
+    at[0] = x;
+    if (col + 1 < dv) at[1] = y;
+  }
+}
+
+template <class S>
+__device__ __forceinline__ void read_state(float (&m)[S::NM][2][4], const float* from, const Part<S>& part, int dk, int dv, int lane) {
+  const bool even = pairs_aligned(from, dv);
+  clear<S>(m);
+  each_pair<S>(m, part, dk, dv, lane, [&](int row, int col, float& x, float& y) {
+    const float2 v = read_pair(from + row * dv + col, col, dv, even);
+    x = v.x, y = v.y;
+  });
+}
+template <class S>
+__device__ __forceinline__ void write_state(float (&m)[S::NM][2][4], float* to, const Part<S>& part, int dk, int dv, int lane) {
+  const bool even = pairs_aligned(to, dv);
+  each_pair<S>(m, part, dk, dv, lane,
+               [&](int row, int col, float& x, float& y) { write_pair(to + row * dv + col, col, dv, even, x, y); });
+}
+
+// The part's limbs into planes [D][P] (whole 16 x 16 tiles).
+template <class S, int N>
+__device__ __forceinline__ void dump_state(const float (&m)[S::NM][2][4], plane_t* to, const Part<S>& part, int lane) {
+#pragma unroll
+  for (int j = 0; j < S::NM; ++j) {
+    if (j >= part.pairs) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t w[N];
+        split<N>(m[j][h][2 * r], m[j][h][2 * r + 1], w);
+        plane_t* at = to + (part.row + (lane >> 2) + r * 8) * S::P + part.col + j * 16 + h * 8 + (lane & 3) * 2;
+#pragma unroll
+        for (int l = 0; l < N; ++l) *reinterpret_cast<uint32_t*>(at + l * S::SPLANE) = w[l];
+      }
+  }
+}
+
+// m = keep m + sum_j factor weight[j] x_j y_j^T over a chunk's tokens, 32 of them at a time.  The weight goes into x's
+// fragments, which then have three limbs.
+template <class S>
+__device__ __forceinline__ void update(float (&m)[S::NM][2][4], const plane_t* x, const plane_t* y, const float* weight, float factor,
+                                       float keep, int nt, const Part<S>& part, int lane) {
+#pragma unroll
+  for (int half = 0; half < S::RT; half += 2) {
+    if (half >= nt || !part.pairs) break;
+    uint32_t a[2][3][4];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      if (half + kk >= nt) break;
+      const int t = (half + kk) * 16;
+      uint32_t raw[S::L][4];
+#pragma unroll
+      for (int l = 0; l < S::L; ++l) frag_a<true>(raw[l], x + l * S::PLANE + t * S::P + part.row, S::P, lane);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float2 w = *reinterpret_cast<const float2*>(weight + t + (r >> 1) * 8 + (lane & 3) * 2);
+        float x0 = lower(raw[0][r]), x1 = upper(raw[0][r]);
+#pragma unroll
+        for (int l = 1; l < S::L; ++l) x0 += lower(raw[l][r]), x1 += upper(raw[l][r]);
+        uint32_t limbs[3];
+        split<3>(x0 * (w.x * factor), x1 * (w.y * factor), limbs);
+        a[kk][0][r] = limbs[0], a[kk][1][r] = limbs[1], a[kk][2][r] = limbs[2];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < S::NM; ++j) {
+      if (j >= part.pairs) break;
+      float acc[2][4] = {}, low[2][4] = {};
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        if (half + kk >= nt) break;
+        uint32_t b[S::L][4];
+#pragma unroll
+        for (int l = 0; l < S::L; ++l) frag_b<true>(b[l], y + l * S::PLANE + (half + kk) * 16 * S::P + part.col + j * 16, S::P, lane);
+        mma_terms<3, S::L>(acc, low, a[kk], b);
+      }
+      const float k = half ? 1.0f : keep;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float add = acc[h][e] + low[h][e];
+          m[j][h][e] = k == 0.0f ? add : fmaf(k, m[j][h][e], add);
+        }
+    }
+  }
+}
+// The same, element by element, leaving out tokens of no weight.
+template <class S>
+__device__ __noinline__ float update_slow(float old, const plane_t* x, const plane_t* y, const float* weight, float factor, float keep, int n) {
+  float sum = 0.0f;
+  for (int j = 0; j < n; ++j)
+    if (weight[j] != 0.0f) sum = fmaf(weight[j] * factor * value<S::L>(x + j * S::P, S::PLANE), value<S::L>(y + j * S::P, S::PLANE), sum);
+  return keep == 0.0f ? sum : fmaf(keep, old, sum);
+}
+template <class S>
+__device__ __forceinline__ void update_masked(float (&m)[S::NM][2][4], const plane_t* x, const plane_t* y, const float* weight, float factor,
+                                              float keep, int n, const Part<S>& part, int dk, int dv, int lane) {
+#pragma unroll
+  for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = part.row + (lane >> 2) + ((e >> 1) & 1) * 8, col = part.col + j * 16 + (e >> 2) * 8 + (lane & 3) * 2 + (e & 1);
+      if (row < dk && col < dv) m[j][e >> 2][e & 3] = update_slow<S>(m[j][e >> 2][e & 3], x + row, y + col, weight, factor, keep, n);
+    }
+}
+
+// Whether any of a warp's accumulators is not finite (a sum that overflows counts too).
+template <int N>
+__device__ __forceinline__ bool not_finite(const float (&acc)[N][2][4]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sum = fmaf(acc[j][x >> 2][x & 3], 0.0f, sum);
+  return sum != sum;
+}
+
+// ---------------------------------------------------------------- results
+// A warp's part of a product, rows [16 r, +16) and columns [col, col + 16 N), rounded into rows of bfloat16.
+template <class S, int N>
+__device__ __forceinline__ void stage(plane_t* to, const float (&acc)[N][2][4], int row, int col, int pairs, int lane) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (j >= pairs) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        *reinterpret_cast<uint32_t*>(to + (row + (lane >> 2) + r * 8) * S::P + col + j * 16 + h * 8 + (lane & 3) * 2) =
+            pack_round(acc[j][h][2 * r], acc[j][h][2 * r + 1]);
+  }
+}
+// All threads: staged rows to memory.
+template <class S>
+__device__ __forceinline__ void store_rows(bf16* to, int64_t stride, const plane_t* from, int width, bool vec, int n, int tid) {
+  constexpr int LR = S::D / 8;
+  for (int j = tid; j < n * LR; j += S::THREADS) {
+    const int row = j / LR, c = j % LR * 8;
+    if (c >= width) continue;
+    bf16* at = to + row * stride + c;
+    const plane_t* x = from + row * S::P + c;
+    if (vec) {
+      *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < width) reinterpret_cast<plane_t*>(at)[i] = x[i];
+    }
+  }
+}
+// A warp's part of a product as 32-bit values straight to memory (four lanes fill a 32-byte sector).
+template <int N>
+__device__ __forceinline__ void store_float(float* to, int64_t stride, const float (&acc)[N][2][4], int row, int col, int n, int width, int lane) {
+  const bool even = reinterpret_cast<uintptr_t>(to) % 8 == 0 && stride % 2 == 0 && width % 2 == 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = row + (lane >> 2) + r * 8, c = col + j * 16 + h * 8 + (lane & 3) * 2;
+        if (i < n && c < width) write_pair(to + i * stride + c, c, width, even, acc[j][h][2 * r], acc[j][h][2 * r + 1]);
+      }
+}
+
+// Where one (environment, value head) is in a tensor.
+template <class T>
+__device__ __forceinline__ T* place(const ZenoTensor& t, int64_t b, int64_t h) {
+  return static_cast<T*>(t.data) + b * t.stride[0] + h * t.stride[2];
+}
+
+// Rollouts in segments of `chunks` chunks, one block each.
+struct Segments {
+  uint32_t count, chunks;
+  float* state;  // [rows][count][dk][dv]: first what a segment adds, then the state in front of it (behind it in reverse)
+  float* keep;   // [rows][count]: what a segment leaves of the state in front of it
+};
+
+}  // namespace linear
+}  // namespace zb

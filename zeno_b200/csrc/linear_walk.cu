@@ -1,0 +1,89 @@
+// The state over the segments of a rollout, element by element: S <- keep S + what the segment adds.  In place: what a
+// segment adds is read, the state in front of it (in reverse, behind it) is written.  Bound by the bytes of the states.
+#include <cuda_bf16.h>
+
+#include "policy_ops.h"
+
+namespace zb {
+namespace {
+
+__global__ void __launch_bounds__(256) linear_walk_kernel(const LinearWalk w) {
+  const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+  const uint64_t row = blockIdx.y;
+  if (i >= w.size) return;
+  float run = w.initial ? w.initial[row * w.size + i] : 0.0f;
+  float* state = w.state + row * w.segments * w.size + i;
+  const float* keep = w.keep + row * w.segments;
+#pragma unroll 4
+  for (uint32_t step = 0; step < w.segments; ++step) {
+    const uint32_t seg = w.reverse ? w.segments - 1 - step : step;
+    // the last one's sum is not asked for, and was not taken
+    const float add = step + 1 < w.segments ? state[seg * w.size] : 0.0f;
+    const float k = step + 1 < w.segments ? keep[seg] : 1.0f;
+    state[seg * w.size] = run;
+    run = k == 0.0f ? add : fmaf(k, run, add);
+  }
+}
+
+// out[t][kh][c] = sum over the value heads that share key head kh, in their order, rounded once.
+template <class T>
+__device__ __forceinline__ T rounded(float x);
+template <>
+__device__ __forceinline__ float rounded<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <class T>
+__global__ void __launch_bounds__(256) linear_shared_kernel(const LinearShared s, const uint64_t total) {
+  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+    const uint32_t c = uint32_t(i % s.width);
+    const uint64_t rest = i / s.width;
+    const uint32_t kh = uint32_t(rest % s.key_heads);
+    const uint64_t token = rest / s.key_heads;  // batch and token
+    const uint64_t b = token / s.tokens, t = token % s.tokens;
+    const float* from = s.from + (token * s.key_heads * s.group + uint64_t(kh) * s.group) * s.width + c;
+    float sum = from[0];
+    for (uint32_t g = 1; g < s.group; ++g) sum += from[g * s.width];
+    static_cast<T*>(s.to.data)[int64_t(b) * s.to.stride[0] + int64_t(t) * s.to.stride[1] + int64_t(kh) * s.to.stride[2] + c] = rounded<T>(sum);
+  }
+}
+
+// One block a head: its decay's gradient from those of the environments and segments, in a fixed order, in 64 bits.
+__global__ void __launch_bounds__(256) linear_decay_kernel(const double* from, uint32_t batch, uint32_t heads, uint32_t segments, float* to) {
+  __shared__ double part[256];
+  const uint32_t h = blockIdx.x;
+  double sum = 0.0;
+  for (uint64_t i = threadIdx.x; i < uint64_t(batch) * segments; i += 256)
+    sum += from[(i / segments * heads + h) * segments + i % segments];
+  part[threadIdx.x] = sum;
+  for (uint32_t d = 128; d > 0; d >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
+  }
+  if (threadIdx.x == 0) to[h] = float(part[0]);
+}
+
+}  // namespace
+
+cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t stream) {
+  // at most a few hundred rows are cut into segments
+  linear_walk_kernel<<<dim3((w.size + 255) / 256, rows), 256, 0, stream>>>(w);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_linear_shared(const LinearShared& s, uint32_t batch, uint32_t dtype, cudaStream_t stream) {
+  const uint64_t total = uint64_t(batch) * s.tokens * s.key_heads * s.width;
+  const uint64_t blocks = (total + 1023) / 1024;
+  const unsigned grid = unsigned(blocks < 16 * kSms ? blocks : 16 * kSms);
+  if (!grid) return cudaSuccess;
+  if (dtype == ZENO_DTYPE_BF16) linear_shared_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(s, total);
+  else linear_shared_kernel<float><<<grid, 256, 0, stream>>>(s, total);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_linear_decay(const double* from, uint32_t batch, uint32_t heads, uint32_t segments, float* to, cudaStream_t stream) {
+  linear_decay_kernel<<<heads, 256, 0, stream>>>(from, batch, heads, segments, to);
+  return cudaGetLastError();
+}
+
+}  // namespace zb

@@ -54,6 +54,33 @@ uint64_t delta_forward_workspace(const ZenoDeltaRule& p);
 cudaError_t launch_delta_forward(const ZenoDeltaRule& p, void* workspace, cudaStream_t stream);
 cudaError_t launch_delta_backward(const ZenoDeltaRule& p, const ZenoDeltaRuleGrads& d, void* workspace, cudaStream_t stream);
 
+// Linear attention over the segments of few long rollouts: S <- keep S + what the segment adds.
+struct LinearWalk {
+  float* state;          // [rows][segments][size]: read as what a segment adds, written as the state in front of it
+  const float* keep;     // [rows][segments]
+  const float* initial;  // [rows][size] or NULL
+  uint32_t segments, size;
+  bool reverse;          // from the last segment back; written is the state behind a segment
+};
+struct LinearShared {  // gradients of a key head's rows from those of its value heads
+  const float* from;   // [batch][tokens][key_heads * group][width]
+  ZenoTensor to;
+  uint32_t tokens, key_heads, group, width;
+};
+cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t stream);
+cudaError_t launch_linear_shared(const LinearShared& s, uint32_t batch, uint32_t dtype, cudaStream_t stream);
+cudaError_t launch_linear_decay(const double* from, uint32_t batch, uint32_t heads, uint32_t segments, float* to, cudaStream_t stream);
+uint64_t linear_saved_bytes(const ZenoLinearAttention& p);
+uint64_t linear_forward_workspace(const ZenoLinearAttention& p);
+uint64_t linear_backward_workspace(const ZenoLinearAttention& p);
+cudaError_t launch_linear_forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t stream);
+cudaError_t launch_linear_backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream);
+cudaError_t launch_linear_step(const ZenoLinearAttention& p, cudaStream_t stream);
+
+uint64_t layer_norm_workspace(const ZenoLayerNorm& p);
+cudaError_t launch_layer_norm_forward(const ZenoLayerNorm& p, cudaStream_t stream);
+cudaError_t launch_layer_norm_backward(const ZenoLayerNorm& p, const ZenoLayerNormGrads& d, void* workspace, cudaStream_t stream);
+
 uint64_t orthogonalize_wait_limit(uint64_t nanoseconds);
 uint64_t orthogonalize_workspace(uint32_t count, uint32_t rows, uint32_t cols, uint32_t dtype);
 cudaError_t launch_orthogonalize(const void* update, const int64_t* strides, void* out, uint32_t count, uint32_t rows, uint32_t cols,
