@@ -22,7 +22,7 @@ struct BackwardSmem {
     float state[S::NW];                    // <S, R> over each warp's part
   };
   static constexpr int row = S::L * S::PLANE, pairs = S::PL * S::CPLANE, state = 3 * S::SPLANE;
-  static constexpr int front = (int(sizeof(Gates<S::C>)) + 15) / 16 * 16 + (int(sizeof(Sums)) + 15) / 16 * 16;
+  static constexpr int front = int(sizeof(Gates<S::C>)) + (int(sizeof(Sums)) + 15) / 16 * 16;
   static int bytes(bool with_state) { return front + 2 * (4 * row + 2 * pairs + (with_state ? state : 0)); }
 };
 
@@ -31,12 +31,14 @@ struct BackwardOut {
   double* decay;               // [rows][segments], where all tokens of a head have one decay
 };
 
-// acc's rows by f[i] (what f is zero for is left out), and the products of the rows with those of X: x_i
+// acc's rows by f[i] (what f is zero for is left out).  Returns the products of the lane's two rows with those of X over its columns:
+// summed over the 4 lanes of a row and the groups of columns they are x_i.
 template <class S>
-__device__ __forceinline__ void scale_and_dot(float (&acc)[S::NO][2][4], const float* f, float scale, const plane_t* x, float* to, int rt, int ct,
-                                              int pairs, int lane) {
+__device__ __forceinline__ float2 scale_and_dot(float (&acc)[S::NO][2][4], const float* f, float scale, const plane_t* x, int rt, int ct, int pairs,
+                                                int lane) {
   const int i0 = rt * 16 + (lane >> 2);
   const float f0 = f[i0], f1 = f[i0 + 8];
+  const float s0 = f0 * scale, s1 = f1 * scale;
   float d0 = 0.0f, d1 = 0.0f;
 #pragma unroll
   for (int j = 0; j < S::NO; ++j) {
@@ -46,17 +48,18 @@ __device__ __forceinline__ void scale_and_dot(float (&acc)[S::NO][2][4], const f
       float(&y)[4] = acc[j][h];
       const plane_t* at = x + i0 * S::P + (ct * S::NO + j) * 16 + h * 8 + (lane & 3) * 2;
       const float2 x0 = values<S::L>(at, S::PLANE), x1 = values<S::L>(at + 8 * S::P, S::PLANE);
-      y[0] = f0 == 0.0f ? 0.0f : y[0] * (f0 * scale), y[1] = f0 == 0.0f ? 0.0f : y[1] * (f0 * scale);
-      y[2] = f1 == 0.0f ? 0.0f : y[2] * (f1 * scale), y[3] = f1 == 0.0f ? 0.0f : y[3] * (f1 * scale);
+      y[0] = f0 == 0.0f ? 0.0f : y[0] * s0, y[1] = f0 == 0.0f ? 0.0f : y[1] * s0;
+      y[2] = f1 == 0.0f ? 0.0f : y[2] * s1, y[3] = f1 == 0.0f ? 0.0f : y[3] * s1;
       d0 = fmaf(x0.x, y[0], fmaf(x0.y, y[1], d0)), d1 = fmaf(x1.x, y[2], fmaf(x1.y, y[3], d1));
     }
   }
-  d0 += __shfl_xor_sync(kAll, d0, 1), d1 += __shfl_xor_sync(kAll, d1, 1);
-  d0 += __shfl_xor_sync(kAll, d0, 2), d1 += __shfl_xor_sync(kAll, d1, 2);
-  if ((lane & 3) == 0) {  // f == 0: the row of x may hold anything
-    to[i0] = f0 == 0.0f ? 0.0f : d0;
-    to[i0 + 8] = f1 == 0.0f ? 0.0f : d1;
-  }
+  // f == 0: the row of x may hold anything
+  return make_float2(f0 == 0.0f ? 0.0f : d0, f1 == 0.0f ? 0.0f : d1);
+}
+__device__ __forceinline__ void keep_rows(float* to, float2 x, int rt, int lane) {
+  x.x += __shfl_xor_sync(kAll, x.x, 1), x.y += __shfl_xor_sync(kAll, x.y, 1);
+  x.x += __shfl_xor_sync(kAll, x.x, 2), x.y += __shfl_xor_sync(kAll, x.y, 2);
+  if ((lane & 3) == 0) to[rt * 16 + (lane >> 2)] = x.x, to[rt * 16 + (lane >> 2) + 8] = x.y;
 }
 
 // One element of a gradient over the pairs that the mask leaves: factor (state row . x) + sum over the pairs.
@@ -71,7 +74,7 @@ __device__ __noinline__ float masked_element(const Gates<S::C>& s, float f, cons
   }
   for (int o = ROWS ? 0 : at; o < (ROWS ? at + 1 : n); ++o) {
     const int i = ROWS ? at : o, j = ROWS ? o : at;
-    if (pair_decay<S>(s, i, j, 1.0f) != 0.0f) sum = fmaf(value<S::PL>(pairs + i * S::CP + j, S::CPLANE), value<S::L>(y + o * S::P, S::PLANE), sum);
+    if (pair_decay(s.token[i], s.token[j], meets(s.token[i], s.token[j], i, j)) != 0.0f) sum = fmaf(value<S::PL>(pairs + i * S::CP + j, S::CPLANE), value<S::L>(y + o * S::P, S::PLANE), sum);
   }
   return sum;
 }
@@ -97,22 +100,21 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
   using M = BackwardSmem<S>;
   extern __shared__ __align__(16) char smem[];
   Gates<S::C>& s = *reinterpret_cast<Gates<S::C>*>(smem);
-  typename M::Sums& sums = *reinterpret_cast<typename M::Sums*>(smem + (sizeof(Gates<S::C>) + 15) / 16 * 16);
+  typename M::Sums& sums = *reinterpret_cast<typename M::Sums*>(smem + sizeof(Gates<S::C>));
   plane_t* q = reinterpret_cast<plane_t*>(smem + M::front);
   plane_t *k = q + M::row, *v = k + M::row, *o = v + M::row, *pr = o + M::row, *dp = pr + M::pairs, *st = dp + M::pairs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = warp % S::RT, ct = warp / S::RT;
   const int dk = int(p.key_dim), dv = int(p.value_dim), nk = (dk + 15) / 16, nv = (dv + 15) / 16;
-  const At a = block_at(p, sg.count, sg.chunks, 0, sg.count, S::C);
+  const At a = block_at(p, sg, 0, S::C);
+  if (a.b >= p.batch) return;
+  const Mover<S> mv(tid);
   const int64_t state_size = int64_t(dk) * dv;
   const bool shared = extra.shared_q != nullptr;
   const T *gq = place<T>(p.q, a.b, a.kh), *gk = place<T>(p.k, a.b, a.kh), *gv = place<T>(p.v, a.b, a.h), *go = place<T>(d.d_out, a.b, a.h);
   const float* gg = place<float>(p.g, a.b, a.h);
   const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
-  const bool vq = vec_rows<S, T>(p.q, p.key_dim), vk = vec_rows<S, T>(p.k, p.key_dim), vv = vec_rows<S, T>(p.v, p.value_dim);
-  const bool vo = vec_rows<S, T>(d.d_out, p.value_dim);
   T *wq = place<T>(d.d_q, a.b, a.kh), *wk = place<T>(d.d_k, a.b, a.kh), *wv = place<T>(d.d_v, a.b, a.h);
-  const bool vwq = vec_rows<S, T>(d.d_q, p.key_dim), vwk = vec_rows<S, T>(d.d_k, p.key_dim), vwv = vec_rows<S, T>(d.d_v, p.value_dim);
   const int64_t shared_stride = int64_t(p.value_heads) * dk;
 
   const Part<S> part(warp, dk, dv);
@@ -122,7 +124,8 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
                                       : d.d_final ? d.d_final + int64_t(a.row) * state_size : nullptr;
   if (behind) read_state<S>(m, behind, part, dk, dv, lane);
   else clear<S>(m);
-  double decay_sum = 0.0;  // of one lane's tokens
+  const bool each = d.d_g.data != nullptr;  // every token's decay has a gradient of its own
+  double decay_sum = 0.0;
   const int col = ct * S::NO * 16;
 
   for (int c = a.c1 - 1; c >= a.c0; --c) {
@@ -132,11 +135,12 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
                                : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
     const bool have_r = c + 1 < a.c1 || behind;
     __syncthreads();  // the last chunk's results have left
-    load_rows<S>(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, vq, n, nt, tid);
-    load_rows<S>(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, vk, n, nt, tid);
-    load_rows<S>(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, vv, n, nt, tid);
-    load_rows<S>(o, go + t0 * d.d_out.stride[1], d.d_out.stride[1], dv, vo, n, nt, tid);
+    load_rows<S>(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, nt, mv);
+    load_rows<S>(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, nt, mv);
+    load_rows<S>(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, nt, mv);
+    load_rows<S>(o, go + t0 * d.d_out.stride[1], d.d_out.stride[1], dv, sg.vec & kVecOut, n, nt, mv);
     if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    float state_dot = 0.0f;  // <S, R> over this thread's elements
     if (front) {
       const bool even = pairs_aligned(front, dv);
       float dot = 0.0f;
@@ -158,14 +162,19 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
             for (int l = 0; l < 3; ++l) *reinterpret_cast<uint32_t*>(at + l * S::SPLANE) = w[l];
           }
       }
+      state_dot = have_r ? dot : 0.0f;
+      if (each) {
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(kAll, dot, x);
-      if (lane == 0) sums.state[warp] = dot;
+        for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(kAll, dot, x);
+        if (lane == 0) sums.state[warp] = dot;
+      }
     }
     copies_landed();
     __syncthreads();
 
     // P, D, and what the pairs give the decays
+    // this thread's part of their gradient, where all tokens of the head have one
+    float decays = each || s.keep == 0.0f ? 0.0f : state_dot * s.keep * float(n);
     if (ct < S::NHS) {
       float sp[S::SP][2][4] = {}, so[S::SP][2][4] = {};
       const int pairs = rt < nt ? min(S::SP, rt - ct * S::SP + 1) : 0;
@@ -173,34 +182,49 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
         product<S::L, S::L, false, false>(sp, q + rt * 16 * S::P, S::P, S::PLANE, k + ct * S::SP * 16 * S::P, S::P, S::PLANE, 0, nk, pairs, lane);
         product<S::L, S::L, false, false>(so, o + rt * 16 * S::P, S::P, S::PLANE, v + ct * S::SP * 16 * S::P, S::P, S::PLANE, 0, nv, pairs, lane);
       }
+      const int i0 = rt * 16 + (lane >> 2);
+      const Token ti[2] = {s.token[i0], s.token[i0 + 8]};
       float before[2] = {0.0f, 0.0f};  // of the group's columns so far, for each of the lane's two rows
 #pragma unroll
       for (int j = 0; j < S::SP; ++j) {
         const int c0 = (ct * S::SP + j) * 16;
         if (j >= pairs) {
           // nothing lies in front of these columns' tokens but what lies to the left
-          if (lane < 16) sums.pairs[rt][c0 + lane] = 0.0f;
+          if (each && lane < 16) sums.pairs[rt][c0 + lane] = 0.0f;
           continue;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int cc = c0 + h * 8 + (lane & 3) * 2;
-          float passes[2] = {0.0f, 0.0f};  // tokens cc and cc + 1, over the lane's rows
+          const Token t0 = s.token[cc], t1 = s.token[cc + 1];
+          float pass[2][2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int i = rt * 16 + (lane >> 2) + r * 8;
-            const float f0 = pair_decay<S>(s, i, cc, p.scale), f1 = pair_decay<S>(s, i, cc + 1, p.scale);
-            const float p0 = f0 == 0.0f ? 0.0f : sp[j][h][2 * r] * f0, p1 = f1 == 0.0f ? 0.0f : sp[j][h][2 * r + 1] * f1;
-            const float a0 = f0 == 0.0f ? 0.0f : p0 * so[j][h][2 * r], a1 = f1 == 0.0f ? 0.0f : p1 * so[j][h][2 * r + 1];
+            const int i = i0 + r * 8;
+            const bool m0 = meets(ti[r], t0, i, cc), m1 = meets(ti[r], t1, i, cc + 1);
+            const float f0 = pair_decay(ti[r], t0, m0) * p.scale, f1 = pair_decay(ti[r], t1, m1) * p.scale;
+            const float o0 = so[j][h][2 * r], o1 = so[j][h][2 * r + 1];
+            const float p0 = m0 ? sp[j][h][2 * r] * f0 : 0.0f, p1 = m1 ? sp[j][h][2 * r + 1] * f1 : 0.0f;
             uint32_t w[S::PL];
             split<S::PL>(p0, p1, w);
 #pragma unroll
             for (int l = 0; l < S::PL; ++l) *reinterpret_cast<uint32_t*>(pr + l * S::CPLANE + i * S::CP + cc) = w[l];
-            split<S::PL>(f0 == 0.0f ? 0.0f : so[j][h][2 * r] * f0, f1 == 0.0f ? 0.0f : so[j][h][2 * r + 1] * f1, w);
+            split<S::PL>(m0 ? o0 * f0 : 0.0f, m1 ? o1 * f1 : 0.0f, w);
 #pragma unroll
             for (int l = 0; l < S::PL; ++l) *reinterpret_cast<uint32_t*>(dp + l * S::CPLANE + i * S::CP + cc) = w[l];
+            pass[r][0] = m0 ? p0 * o0 : 0.0f, pass[r][1] = m1 ? p1 * o1 : 0.0f;
+          }
+          if (!each) {  // a pair passes i - j tokens
+            const float far = float(i0 - cc);
+            decays = fmaf(pass[0][0], far, fmaf(pass[0][1], far - 1.0f, fmaf(pass[1][0], far + 8.0f, fmaf(pass[1][1], far + 7.0f, decays))));
+            continue;
+          }
+          float passes[2] = {0.0f, 0.0f};  // tokens cc and cc + 1, over the lane's rows
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int i = i0 + r * 8;
             // the sum of A in front of each column, over the 4 lanes of the row
-            float sum = a0 + a1;
+            float sum = pass[r][0] + pass[r][1];
             const float x1 = __shfl_up_sync(kAll, sum, 1, 4);
             if ((lane & 3) >= 1) sum += x1;
             const float x2 = __shfl_up_sync(kAll, sum, 2, 4);
@@ -209,7 +233,7 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
             left = (lane & 3) ? before[r] + left : before[r];
             before[r] += __shfl_sync(kAll, sum, 3, 4);
             if (i >= cc) passes[0] += left;
-            if (i >= cc + 1) passes[1] += left + a0;
+            if (i >= cc + 1) passes[1] += left + pass[r][0];
           }
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
@@ -219,9 +243,9 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
           if (lane < 4) sums.pairs[rt][cc] = passes[0], sums.pairs[rt][cc + 1] = passes[1];
         }
       }
-      if ((lane & 3) == 0) {
-        sums.row[ct][rt * 16 + (lane >> 2)] = before[0];
-        sums.row[ct][rt * 16 + (lane >> 2) + 8] = before[1];
+      if (each && (lane & 3) == 0) {
+        sums.row[ct][i0] = before[0];
+        sums.row[ct][i0 + 8] = before[1];
       }
     }
     __syncthreads();
@@ -233,7 +257,10 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
     if (pk > 0) {
       if (front) {
         product<S::L, 3, false, false>(dq, o + rt * 16 * S::P, S::P, S::PLANE, st + col * S::P, S::P, S::SPLANE, 0, nv, pk, lane);
-        scale_and_dot<S>(dq, s.carried, p.scale, q, sums.x[ct], rt, ct, pk, lane);
+        const float2 x = scale_and_dot<S>(dq, s.carried, p.scale, q, rt, ct, pk, lane);
+        const float i = float(rt * 16 + (lane >> 2));
+        if (each) keep_rows(sums.x[ct], x, rt, lane);
+        else decays = fmaf(x.x, i + 1.0f, fmaf(x.y, i + 9.0f, decays));  // the state in front passes every token up to this one
       }
       product<S::PL, S::L, false, true>(dq, dp + rt * 16 * S::CP, S::CP, S::CPLANE, k + col, S::P, S::PLANE, 0, rt + 1, pk, lane);
       bad = not_finite(dq);
@@ -256,7 +283,10 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
     if (pk > 0) {
       if (have_r) {
         product<S::L, 3, false, false>(dk_, v + rt * 16 * S::P, S::P, S::PLANE, st + col * S::P, S::P, S::SPLANE, 0, nv, pk, lane);
-        scale_and_dot<S>(dk_, s.to_end, 1.0f, k, sums.y[ct], rt, ct, pk, lane);
+        const float2 y = scale_and_dot<S>(dk_, s.to_end, 1.0f, k, rt, ct, pk, lane);
+        const float rest = float(n - 1 - rt * 16 - (lane >> 2));
+        if (each) keep_rows(sums.y[ct], y, rt, lane);
+        else decays = fmaf(y.x, rest, fmaf(y.y, rest - 8.0f, decays));  // what begins here passes the tokens behind it
       }
       product<S::PL, S::L, true, true>(dk_, dp + rt * 16, S::CP, S::CPLANE, q + col, S::P, S::PLANE, rt, nt, pk, lane);
       bad = not_finite(dk_);
@@ -309,7 +339,8 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
       store_float(extra.shared_k + at, shared_stride, dk_, rt * 16, col, n, dk, lane);
     }
     // the decays: a warp, C / 32 neighbouring tokens a lane
-    if (warp == S::NW - 1) {
+    decay_sum += double(decays);
+    if (each && warp == S::NW - 1) {
       constexpr int U = S::C / 32;
       float z = 0.0f;
       if (front && have_r && s.keep != 0.0f) {
@@ -381,8 +412,8 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
       for (int u = 0; u < U; ++u) {
         const int t = lane * U + u;
         if (t < n) {
-          decay_sum += dg[u];
-          if (d.d_g.data) place<float>(d.d_g, a.b, a.h)[(t0 + t) * d.d_g.stride[1]] = dg[u];
+          decay_sum += double(dg[u]);
+          place<float>(d.d_g, a.b, a.h)[(t0 + t) * d.d_g.stride[1]] = dg[u];
         }
       }
     }
@@ -393,17 +424,24 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
     if constexpr (sizeof(T) == 2) {
       __syncthreads();
       if (!shared) {
-        store_rows<S>(wq + t0 * d.d_q.stride[1], d.d_q.stride[1], k, dk, vwq, n, tid);
-        store_rows<S>(wk + t0 * d.d_k.stride[1], d.d_k.stride[1], v, dk, vwk, n, tid);
+        store_rows<S>(wq + t0 * d.d_q.stride[1], d.d_q.stride[1], k, dk, sg.vec & kVecDq, n, mv);
+        store_rows<S>(wk + t0 * d.d_k.stride[1], d.d_k.stride[1], v, dk, sg.vec & kVecDk, n, mv);
       }
-      store_rows<S>(wv + t0 * d.d_v.stride[1], d.d_v.stride[1], pr, dv, vwv, n, tid);
+      store_rows<S>(wv + t0 * d.d_v.stride[1], d.d_v.stride[1], pr, dv, sg.vec & kVecDv, n, mv);
     }
   }
   if (a.c0 == 0 && d.d_initial) write_state<S>(m, d.d_initial + int64_t(a.row) * state_size, part, dk, dv, lane);
-  if (extra.decay && warp == S::NW - 1) {
+  if (extra.decay) {
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) decay_sum += __shfl_xor_sync(kAll, decay_sum, x);
-    if (lane == 0) extra.decay[int64_t(a.row) * sg.count + a.seg] = decay_sum;
+    double* part_sum = reinterpret_cast<double*>(smem);  // (where the gates were)
+    __syncthreads();
+    if (lane == 0) part_sum[warp] = decay_sum;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < S::NW; ++w) decay_sum += part_sum[w];
+      extra.decay[int64_t(a.row) * sg.count + a.seg] = decay_sum;
+    }
   }
 }
 

@@ -23,7 +23,9 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
     const Cut c = cut_of(p, fill_of(p));
     const BackwardLayout l = backward_layout(p);
     char* at = static_cast<char*>(workspace);
-    Segments sg{c.count, c.chunks, reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + c.state)};
+    const uint32_t vec = vec_of(p, d.d_out) | vec_of(d.d_q, p.key_dim, p.dtype, kVecDq) | vec_of(d.d_k, p.key_dim, p.dtype, kVecDk) |
+                         vec_of(d.d_v, p.value_dim, p.dtype, kVecDv);
+    Segments sg{c.count, c.chunks, vec, reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + c.state)};
     BackwardOut extra{};
     if (l.shared) {
       extra.shared_q = reinterpret_cast<float*>(at + l.cut);
@@ -44,7 +46,7 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
     if (e != cudaSuccess) return e;
     static_assert(sizeof(T) == 4 || S::C * S::P <= 2 * S::PL * S::CPLANE, "dV is staged where P and D were");
     static_assert(BackwardSmem<S>::front + 2 * (4 * S::L * S::PLANE + 2 * S::PL * S::CPLANE + 3 * S::SPLANE) <= 232448, "shared memory of a block");
-    kernel<<<p.batch * p.value_heads * c.count, S::THREADS, bytes, stream>>>(p, d, sg, extra);
+    kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, d, sg, extra);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     if (l.shared) {

@@ -10,37 +10,33 @@
 namespace zb {
 namespace linear {
 
-// Rows and head of a block.
+// Rows and head of a block: the grid is [batch / kBatchAxis][batch][segments of a head][heads], the last the fastest, so that neighbouring
+// blocks read neighbouring rows.
+constexpr uint32_t kBatchAxis = 32768;
 struct At {
   uint32_t row, b, h, kh, seg;
   int c0, c1, chunks;
 };
-__device__ __forceinline__ At block_at(const ZenoLinearAttention& p, uint32_t count, uint32_t per, uint32_t first, uint32_t blocks, int C) {
+__device__ __forceinline__ At block_at(const ZenoLinearAttention& p, const Segments& sg, uint32_t first, int C) {
   At a;
-  a.row = blockIdx.x / blocks;
-  a.seg = first + blockIdx.x % blocks;
-  a.b = a.row / p.value_heads;
-  a.h = a.row % p.value_heads;
-  a.kh = a.h / (p.value_heads / p.key_heads);
-  a.chunks = int((p.tokens + C - 1) / C);
-  a.c0 = int(a.seg * per);
-  a.c1 = a.seg + 1 == count ? a.chunks : a.c0 + int(per);
+  a.b = blockIdx.z * kBatchAxis + blockIdx.y;
+  a.h = blockIdx.x, a.seg = first;
+  if (sg.count > 1) a.seg += blockIdx.x / p.value_heads, a.h = blockIdx.x % p.value_heads;
+  a.row = a.b * p.value_heads + a.h;
+  a.kh = p.value_heads == p.key_heads ? a.h : a.h / (p.value_heads / p.key_heads);
+  a.chunks = (int(p.tokens) + C - 1) / C;
+  a.c0 = int(a.seg * sg.chunks);
+  a.c1 = a.seg + 1 == sg.count ? a.chunks : a.c0 + int(sg.chunks);
   return a;
 }
-
-template <class S, class T>
-__device__ __forceinline__ bool vec_rows(const ZenoTensor& t, uint32_t width) { return delta::vec_ok<T>(t, int(width)); }
-
-// P_ij = scale a_ij (q_i . k_j), its limbs into planes [C][CP]; tiles above the diagonal are not written.
-template <class S>
-__device__ __forceinline__ float pair_decay(const Gates<S::C>& s, int i, int j, float scale) {
-  return j <= i && s.episode[i] == s.episode[j] ? scale * ex2((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j])) : 0.0f;
+inline dim3 grid_of(const ZenoLinearAttention& p, uint32_t segments) {
+  return dim3(p.value_heads * segments, p.batch < kBatchAxis ? p.batch : kBatchAxis, (p.batch + kBatchAxis - 1) / kBatchAxis);
 }
 
 template <class S>
 struct ForwardSmem {
   static constexpr int rows = 3 * S::L * S::PLANE, pairs = S::PL * S::CPLANE, state = S::PL * S::SPLANE;
-  static constexpr int gates = (int(sizeof(Gates<S::C>)) + 15) / 16 * 16;
+  static constexpr int gates = int(sizeof(Gates<S::C>));
   static int bytes(bool with_state) { return gates + 2 * (rows + pairs + (with_state ? state : 0)); }
 };
 
@@ -55,14 +51,14 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = warp % S::RT, ct = warp / S::RT;
   const int dk = int(p.key_dim), dv = int(p.value_dim), nk = (dk + 15) / 16;
-  const At a = block_at(p, sg.count, sg.chunks, 0, sg.count, S::C);
+  const At a = block_at(p, sg, 0, S::C);
+  if (a.b >= p.batch) return;
+  const Mover<S> mv(tid);
   const int64_t state_size = int64_t(dk) * dv;
   const T *gq = place<T>(p.q, a.b, a.kh), *gk = place<T>(p.k, a.b, a.kh), *gv = place<T>(p.v, a.b, a.h);
   const float* gg = place<float>(p.g, a.b, a.h);
   const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
   T* go = place<T>(p.out, a.b, a.h);
-  const bool vq = vec_rows<S, T>(p.q, p.key_dim), vk = vec_rows<S, T>(p.k, p.key_dim), vv = vec_rows<S, T>(p.v, p.value_dim);
-  const bool vo = vec_rows<S, T>(p.out, p.value_dim);
 
   const Part<S> part(warp, dk, dv);
   float m[S::NM][2][4];
@@ -76,9 +72,9 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
     const int n = int(min(int64_t(S::C), int64_t(p.tokens) - t0)), nt = (n + 15) / 16;
     const bool have = c > a.c0 || first;
     __syncthreads();  // the last chunk's results have left
-    load_rows<S>(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, vq, n, nt, tid);
-    load_rows<S>(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, vk, n, nt, tid);
-    load_rows<S>(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, vv, n, nt, tid);
+    load_rows<S>(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, nt, mv);
+    load_rows<S>(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, nt, mv);
+    load_rows<S>(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, nt, mv);
     if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     if (have) dump_state<S, S::PL>(m, st, part, lane);
     if (p.saved && c > 0) write_state<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane);
@@ -90,17 +86,25 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
       const int pairs = min(S::SP, rt - ct * S::SP + 1);  // up to the diagonal
       if (pairs > 0)
         product<S::L, S::L, false, false>(acc, q + rt * 16 * S::P, S::P, S::PLANE, k + ct * S::SP * 16 * S::P, S::P, S::PLANE, 0, nk, pairs, lane);
+      const int i0 = rt * 16 + (lane >> 2);
+      const Token ti[2] = {s.token[i0], s.token[i0 + 8]};
 #pragma unroll
       for (int j = 0; j < S::SP; ++j) {
         if (j >= pairs) break;
 #pragma unroll
-        for (int x = 0; x < 8; x += 2) {
-          const int i = rt * 16 + (lane >> 2) + ((x >> 1) & 1) * 8, col = (ct * S::SP + j) * 16 + (x >> 2) * 8 + (lane & 3) * 2;
-          const float d0 = pair_decay<S>(s, i, col, p.scale), d1 = pair_decay<S>(s, i, col + 1, p.scale);
-          uint32_t w[S::PL];
-          split<S::PL>(d0 == 0.0f ? 0.0f : acc[j][x >> 2][x & 3] * d0, d1 == 0.0f ? 0.0f : acc[j][x >> 2][(x & 3) + 1] * d1, w);
+        for (int h = 0; h < 2; ++h) {
+          const int col = (ct * S::SP + j) * 16 + h * 8 + (lane & 3) * 2;
+          const Token t0 = s.token[col], t1 = s.token[col + 1];
 #pragma unroll
-          for (int l = 0; l < S::PL; ++l) *reinterpret_cast<uint32_t*>(pr + l * S::CPLANE + i * S::CP + col) = w[l];
+          for (int r = 0; r < 2; ++r) {
+            const int i = i0 + r * 8;
+            const bool m0 = meets(ti[r], t0, i, col), m1 = meets(ti[r], t1, i, col + 1);
+            const float f0 = pair_decay(ti[r], t0, m0) * p.scale, f1 = pair_decay(ti[r], t1, m1) * p.scale;
+            uint32_t w[S::PL];
+            split<S::PL>(m0 ? acc[j][h][2 * r] * f0 : 0.0f, m1 ? acc[j][h][2 * r + 1] * f1 : 0.0f, w);
+#pragma unroll
+            for (int l = 0; l < S::PL; ++l) *reinterpret_cast<uint32_t*>(pr + l * S::CPLANE + i * S::CP + col) = w[l];
+          }
         }
       }
     }
@@ -138,7 +142,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
             y *= s.carried[i] * p.scale;
           }
           for (int j = 0; j <= i; ++j)
-            if (pair_decay<S>(s, i, j, 1.0f) != 0.0f)
+            if (pair_decay(s.token[i], s.token[j], meets(s.token[i], s.token[j], i, j)) != 0.0f)
               y = fmaf(value<S::PL>(pr + i * S::CP + j, S::CPLANE), value<S::L>(v + j * S::P + cc, S::PLANE), y);
 #pragma unroll
           for (int z = 0; z < S::NO * 8; ++z)
@@ -155,7 +159,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
     }
     if constexpr (sizeof(T) == 2) {
       __syncthreads();
-      store_rows<S>(go + t0 * p.out.stride[1], p.out.stride[1], q, dv, vo, n, tid);
+      store_rows<S>(go + t0 * p.out.stride[1], p.out.stride[1], q, dv, sg.vec & kVecOut, n, mv);
     }
   }
   if (a.c1 == a.chunks && p.final_state) write_state<S>(m, p.final_state + int64_t(a.row) * state_size, part, dk, dv, lane);
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
 // state) Q, dO and scale c, from the last chunk to the first.
 template <class S>
 __global__ void __launch_bounds__(S::THREADS) linear_segment_kernel(const __grid_constant__ ZenoLinearAttention p, const ZenoTensor tx, const ZenoTensor ty,
-                                                                    const Segments sg, const bool reverse) {
+                                                                    const Segments sg, const bool reverse) {  // (at most a few hundred rows)
   using T = typename S::T;
   extern __shared__ __align__(16) char smem[];
   Gates<S::C>& s = *reinterpret_cast<Gates<S::C>*>(smem);
@@ -173,11 +177,12 @@ __global__ void __launch_bounds__(S::THREADS) linear_segment_kernel(const __grid
   plane_t* y = x + S::L * S::PLANE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int dk = int(p.key_dim), dv = int(p.value_dim);
-  const At a = block_at(p, sg.count, sg.chunks, reverse ? 1 : 0, sg.count - 1, S::C);
+  const At a = block_at(p, sg, reverse ? 1 : 0, S::C);
+  const Mover<S> mv(tid);
   const T *gx = place<T>(tx, a.b, a.kh), *gy = place<T>(ty, a.b, a.h);
   const float* gg = place<float>(p.g, a.b, a.h);
   const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
-  const bool vx = vec_rows<S, T>(tx, p.key_dim), vy = vec_rows<S, T>(ty, p.value_dim);
+  const bool vx = sg.vec & (reverse ? kVecQ : kVecK), vy = sg.vec & (reverse ? kVecOut : kVecV);
   const Part<S> part(warp, dk, dv);
   float m[S::NM][2][4];
   clear<S>(m);
@@ -186,8 +191,8 @@ __global__ void __launch_bounds__(S::THREADS) linear_segment_kernel(const __grid
     const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * S::C;
     const int n = int(min(int64_t(S::C), int64_t(p.tokens) - t0)), nt = (n + 15) / 16;
     __syncthreads();
-    load_rows<S>(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, nt, tid);
-    load_rows<S>(y, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, nt, tid);
+    load_rows<S>(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, nt, mv);
+    load_rows<S>(y, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, nt, mv);
     if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     copies_landed();
     __syncthreads();

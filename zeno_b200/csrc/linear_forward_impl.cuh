@@ -10,7 +10,7 @@ cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t 
   return with_shape<T>(p, [&](auto shape) {
     using S = decltype(shape);
     const Cut c = cut_of(p, fill_of(p));
-    Segments sg{c.count, c.chunks, static_cast<float*>(workspace), nullptr};
+    Segments sg{c.count, c.chunks, vec_of(p, p.out), static_cast<float*>(workspace), nullptr};
     cudaError_t e;
     if (c.count > 1) {
       sg.keep = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.state);
@@ -24,7 +24,7 @@ cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t 
     static std::atomic<uint64_t> devices{0};
     e = allow_smem(kernel, ForwardSmem<S>::bytes(true), devices);
     if (e != cudaSuccess) return e;
-    kernel<<<p.batch * p.value_heads * c.count, S::THREADS, bytes, stream>>>(p, sg);
+    kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, sg);
     return cudaGetLastError();
   });
 }

@@ -40,6 +40,16 @@ inline uint32_t fill_of(const ZenoLinearAttention& p) {
   return kSms * (w == 128 ? 1 : 2);
 }
 
+inline uint32_t vec_of(const ZenoTensor& t, uint32_t width, uint32_t dtype, uint32_t flag) {
+  const int64_t n = dtype == ZENO_DTYPE_BF16 ? 8 : 4;
+  const bool vec = width % 8 == 0 && reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && t.stride[0] % n == 0 && t.stride[1] % n == 0 && t.stride[2] % n == 0;
+  return vec ? flag : 0;
+}
+inline uint32_t vec_of(const ZenoLinearAttention& p, const ZenoTensor& out) {
+  return vec_of(p.q, p.key_dim, p.dtype, kVecQ) | vec_of(p.k, p.key_dim, p.dtype, kVecK) | vec_of(p.v, p.value_dim, p.dtype, kVecV) |
+         vec_of(out, p.value_dim, p.dtype, kVecOut);
+}
+
 // f(shape) of the call's instance, for one element type.
 template <class T, class F>
 cudaError_t with_shape(const ZenoLinearAttention& p, F&& f) {
@@ -74,7 +84,7 @@ cudaError_t cut_states(const ZenoLinearAttention& p, const ZenoTensor& x, const 
   cudaError_t e = allow_smem(linear_segment_kernel<S>, bytes, devices);
   if (e != cudaSuccess) return e;
   const uint32_t rows = p.batch * p.value_heads;
-  linear_segment_kernel<S><<<rows * (sg.count - 1), S::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
+  linear_segment_kernel<S><<<grid_of(p, sg.count - 1), S::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_linear_walk(LinearWalk{sg.state, sg.keep, initial, sg.count, p.key_dim * p.value_dim, reverse}, rows, stream);

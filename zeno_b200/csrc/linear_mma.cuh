@@ -166,67 +166,104 @@ __device__ __forceinline__ void product(float (&acc)[N][2][4], const plane_t* a,
 }
 
 // ---------------------------------------------------------------- gates
+// One token of a chunk, as the pairs read it.
+struct __align__(16) Token {
+  float hi, lo;  // sum of the log decays since the last reset, base 2, in two parts (differences of long sums are exact enough)
+  int episode;   // resets up to and including this token
+  int pad;
+};
 template <int C>
-struct Gates {
-  float hi[C], lo[C];  // sum of the log decays since the last reset, base 2, in two parts (differences of long sums are exact enough)
-  int episode[C];      // resets up to and including this token
-  float carried[C];    // c_i: decay from the state in front of the chunk; 0 behind a reset, and for absent tokens
-  float to_end[C];     // e_j: decay from token j to the chunk's end; 0 in front of a reset, and for absent tokens
-  float keep;          // what is left of the state in front of the chunk
+struct __align__(16) Gates {
+  Token token[C];
+  float carried[C];  // c_i: decay from the state in front of the chunk; 0 behind a reset, and for absent tokens
+  float to_end[C];   // e_j: decay from token j to the chunk's end; 0 in front of a reset, and for absent tokens
+  float keep;        // what is left of the state in front of the chunk
 };
 
-// One warp: the gates of n tokens, C / 32 neighbouring ones a lane.
+// a_ij of a pair, 0 where the mask takes it out.
+__device__ __forceinline__ bool meets(const Token& ti, const Token& tj, int i, int j) { return j <= i && ti.episode == tj.episode; }
+__device__ __forceinline__ float pair_decay(const Token& ti, const Token& tj, bool meet) {
+  return meet ? ex2((ti.hi - tj.hi) + (ti.lo - tj.lo)) : 0.0f;
+}
+
+// One warp: the gates of n tokens, C / 32 neighbouring ones a lane.  Sums run from the last reset on, so that what one
+// episode's decays are, not finite included, stays in it.  One decay for all tokens (a stride of 0) needs no sum.
 template <int C>
 __device__ __forceinline__ void load_gates(Gates<C>& s, const float* g, int64_t g_stride, const uint8_t* reset, int64_t reset_stride, int64_t t0,
                                            int n, int lane) {
   constexpr int U = C / 32;
+  constexpr double kLog2e = 1.4426950408889634;
   float x[U];
   bool mark[U];
+  unsigned marks[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = lane * U + u;
     x[u] = i < n ? g[(t0 + i) * g_stride] : 0.0f;
     mark[u] = i < n && reset && reset[(t0 + i) * reset_stride];
   }
-  unsigned marks[U];
-  double sum[U];  // from the last reset on, so that what one episode's decays are, not finite included, stays in it
-  bool any = false;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     mark[u] = mark[u] || expf(x[u]) == 0.0f;  // a decay to nothing is a reset: the sums behind it stay finite
-    sum[u] = mark[u] ? 0.0 : double(x[u]) + (u ? sum[u - 1] : 0.0);
-    any |= mark[u];
+    if (mark[u]) x[u] = 0.0f;
     marks[u] = __ballot_sync(kAll, mark[u]);
   }
-  double run = sum[U - 1];
-  bool cut = any;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const double y = __shfl_up_sync(kAll, run, d);
-    const bool z = __shfl_up_sync(kAll, int(cut), d);
-    if (lane >= d) {
-      if (!cut) run += y;
-      cut |= z;
-    }
-  }
-  const double last = __shfl_sync(kAll, run, 31) * 1.4426950408889634;
-  double before = __shfl_up_sync(kAll, run, 1);
-  if (lane == 0) before = 0.0;
+  double y[U], last;
   int all = 0, episode = 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) all += __popc(marks[u]), episode += __popc(marks[u] & ((1u << lane) - 1));
-  any = false;
+  if (g_stride == 0) {
+    int from = -1;  // the last mark in front of the lane's tokens, as a token; the sum counts from the one behind it
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned m = marks[u] & ((1u << lane) - 1);
+      if (m) from = max(from, (31 - __clz(m)) * U + u);
+    }
+    const double step = double(g[0]) * kLog2e;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = lane * U + u;
+      if (mark[u]) from = i;
+      const int steps = min(i, n - 1) - from;
+      y[u] = steps > 0 ? steps * step : 0.0;
+    }
+    last = __shfl_sync(kAll, y[U - 1], 31);
+  } else {
+    double sum[U];
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      sum[u] = mark[u] ? 0.0 : double(x[u]) + (u ? sum[u - 1] : 0.0);
+      any |= mark[u];
+    }
+    double run = sum[U - 1];
+    bool cut = any;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double z = __shfl_up_sync(kAll, run, d);
+      const bool c = __shfl_up_sync(kAll, int(cut), d);
+      if (lane >= d) {
+        if (!cut) run += z;
+        cut |= c;
+      }
+    }
+    last = __shfl_sync(kAll, run, 31) * kLog2e;
+    double before = __shfl_up_sync(kAll, run, 1);
+    if (lane == 0) before = 0.0;
+    any = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      any |= mark[u];
+      y[u] = (any ? sum[u] : before + sum[u]) * kLog2e;
+    }
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = lane * U + u;
-    any |= mark[u];
-    const double y = (any ? sum[u] : before + sum[u]) * 1.4426950408889634;
     episode += mark[u];
-    s.hi[i] = float(y);
-    s.lo[i] = float(y - float(y));
-    s.episode[i] = episode;
-    s.carried[i] = i < n && episode == 0 ? ex2(float(y)) : 0.0f;
-    s.to_end[i] = i < n && episode == all ? ex2(float(last - y)) : 0.0f;
+    s.token[i] = Token{float(y[u]), float(y[u] - float(y[u])), episode, 0};
+    s.carried[i] = i < n && episode == 0 ? ex2(float(y[u])) : 0.0f;
+    s.to_end[i] = i < n && episode == all ? ex2(float(last - y[u])) : 0.0f;
   }
   if (lane == 0) s.keep = all == 0 ? ex2(float(last)) : 0.0f;
 }
@@ -237,52 +274,82 @@ __device__ __forceinline__ void copy16(plane_t* to, const void* from, bool there
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// All threads: n rows of `width` values as planes [16 nt][P], zero for absent tokens and past the width up to
-// the next 16 columns.
+// Which 8 columns of which rows of a chunk a thread moves: rows row, row + STEP, ...
 template <class S>
-__device__ __forceinline__ void load_rows(plane_t* to, const typename S::T* from, int64_t stride, int width, bool vec, int n, int nt, int tid) {
-  constexpr int LR = S::D / 8;
-  const int cols = (width + 15) & ~15;
-  if (S::L == 1 && vec) {
-#pragma unroll 4
-    for (int j = tid; j < nt * 16 * LR; j += S::THREADS) {
-      const int row = j / LR, c = j % LR * 8;
-      if (c >= cols) continue;
-      const bool there = row < n && c < width;
-      copy16(to + row * S::P + c, there ? from + row * stride + c : from, there);
+struct Mover {
+  static constexpr int LR = S::D / 8, STEP = S::THREADS / LR, TURNS = S::C / STEP;
+  static_assert(S::THREADS % LR == 0 && S::C % STEP == 0);
+  int row, c;
+  __device__ __forceinline__ explicit Mover(int tid) : row(tid / LR), c(tid % LR * 8) {}
+};
+
+__device__ __forceinline__ void split_rows(plane_t* at, int plane, const delta::Eight& raw) {
+  float x[8];
+  delta::unpack8<float>(x, raw);
+  uint32_t w[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t r[3];
+    // an infinity or a NaN is its first limb alone
+    const float x0 = x[2 * i], x1 = x[2 * i + 1];
+    const bool f0 = fabsf(x0) < INFINITY, f1 = fabsf(x1) < INFINITY;
+    split<3>(f0 ? x0 : 0.0f, f1 ? x1 : 0.0f, r);
+    if (!f0) r[0] = (r[0] & 0xffff0000u) | (x0 != x0 ? 0x7fc0u : __float_as_uint(x0) >> 16);
+    if (!f1) r[0] = (r[0] & 0xffffu) | (x1 != x1 ? 0x7fc00000u : __float_as_uint(x1));
+    w[0][i] = r[0], w[1][i] = r[1], w[2][i] = r[2];
+  }
+#pragma unroll
+  for (int l = 0; l < 3; ++l) *reinterpret_cast<uint4*>(at + l * plane) = make_uint4(w[l][0], w[l][1], w[l][2], w[l][3]);
+}
+
+// All threads: n rows of `width` values as planes [16 nt][P], zero for absent tokens and past the width up to
+// the next 16 columns.  vec: rows are of whole 16-byte pieces.
+template <class S>
+__device__ __forceinline__ void load_rows(plane_t* to, const typename S::T* from, int64_t stride, int width, bool vec, int n, int nt, const Mover<S>& mv) {
+  using M = Mover<S>;
+  if (mv.c >= ((width + 15) & ~15)) return;
+  const typename S::T* at = from + mv.row * stride + mv.c;
+  to += mv.row * S::P + mv.c;
+  if (vec) {
+    const bool column = mv.c < width;
+    if constexpr (S::L == 1) {
+#pragma unroll
+      for (int u = 0; u < M::TURNS; ++u) {
+        const int row = mv.row + u * M::STEP;
+        if (row >= nt * 16) break;
+        const bool there = row < n && column;
+        copy16(to + u * M::STEP * S::P, there ? at : from, there);
+        at += M::STEP * stride;
+      }
+    } else {
+      constexpr int BATCH = M::TURNS < 2 ? M::TURNS : 2;
+#pragma unroll
+      for (int first = 0; first < M::TURNS; first += BATCH) {
+        delta::Eight raw[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          raw[u] = delta::Eight{};
+          if (mv.row + (first + u) * M::STEP < n && column) {
+            raw[u].a = __ldg(reinterpret_cast<const uint4*>(at));
+            raw[u].b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+          }
+          at += M::STEP * stride;
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+          if (mv.row + (first + u) * M::STEP < nt * 16) split_rows(to + (first + u) * M::STEP * S::P, S::PLANE, raw[u]);
+      }
     }
     return;
   }
-#pragma unroll 2
-  for (int j = tid; j < nt * 16 * LR; j += S::THREADS) {
-    const int row = j / LR, c = j % LR * 8;
-    if (c >= cols) continue;
+#pragma unroll 1
+  for (int row = mv.row; row < nt * 16; row += M::STEP) {
     delta::Eight raw{};
-    if (row < n && c < width) raw = delta::fetch8(from + row * stride + c, width - c, vec);
-    plane_t* at = to + row * S::P + c;
-    if constexpr (S::L == 1) {
-      *reinterpret_cast<uint4*>(at) = raw.a;
-    } else {
-      float x[8];
-      delta::unpack8<float>(x, raw);
-      uint32_t w[3][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t r[3];
-        // an infinity or a NaN is its first limb alone
-        const float x0 = x[2 * i], x1 = x[2 * i + 1];
-        const bool f0 = fabsf(x0) < INFINITY, f1 = fabsf(x1) < INFINITY;
-        split<3>(x0, x1, r);
-        if (!f0 || !f1) {
-          split<3>(f0 ? x0 : 0.0f, f1 ? x1 : 0.0f, r);
-          if (!f0) r[0] = (r[0] & 0xffff0000u) | (x0 != x0 ? 0x7fc0u : __float_as_uint(x0) >> 16);
-          if (!f1) r[0] = (r[0] & 0xffffu) | (x1 != x1 ? 0x7fc00000u : __float_as_uint(x1));
-        }
-        w[0][i] = r[0], w[1][i] = r[1], w[2][i] = r[2];
-      }
-#pragma unroll
-      for (int l = 0; l < 3; ++l) *reinterpret_cast<uint4*>(at + l * S::PLANE) = make_uint4(w[l][0], w[l][1], w[l][2], w[l][3]);
-    }
+    if (row < n && mv.c < width) raw = delta::fetch8_slow(at, width - mv.c);
+    if constexpr (S::L == 1) *reinterpret_cast<uint4*>(to) = raw.a;
+    else split_rows(to, S::PLANE, raw);
+    at += M::STEP * stride;
+    to += M::STEP * S::P;
   }
 }
 
@@ -468,20 +535,27 @@ __device__ __forceinline__ void stage(plane_t* to, const float (&acc)[N][2][4], 
 }
 // All threads: staged rows to memory.
 template <class S>
-__device__ __forceinline__ void store_rows(bf16* to, int64_t stride, const plane_t* from, int width, bool vec, int n, int tid) {
-  constexpr int LR = S::D / 8;
-  for (int j = tid; j < n * LR; j += S::THREADS) {
-    const int row = j / LR, c = j % LR * 8;
-    if (c >= width) continue;
-    bf16* at = to + row * stride + c;
-    const plane_t* x = from + row * S::P + c;
-    if (vec) {
-      *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(x);
-    } else {
+__device__ __forceinline__ void store_rows(bf16* to, int64_t stride, const plane_t* from, int width, bool vec, int n, const Mover<S>& mv) {
+  using M = Mover<S>;
+  if (mv.c >= width) return;
+  plane_t* at = reinterpret_cast<plane_t*>(to) + mv.row * stride + mv.c;
+  from += mv.row * S::P + mv.c;
+  if (vec) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < width) reinterpret_cast<plane_t*>(at)[i] = x[i];
+    for (int u = 0; u < M::TURNS; ++u) {
+      if (mv.row + u * M::STEP >= n) break;
+      *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(from + u * M::STEP * S::P);
+      at += M::STEP * stride;
     }
+    return;
+  }
+#pragma unroll 1
+  for (int row = mv.row; row < n; row += M::STEP) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (mv.c + i < width) at[i] = from[i];
+    at += M::STEP * stride;
+    from += M::STEP * S::P;
   }
 }
 // A warp's part of a product as 32-bit values straight to memory (four lanes fill a 32-byte sector).
@@ -505,9 +579,13 @@ __device__ __forceinline__ T* place(const ZenoTensor& t, int64_t b, int64_t h) {
   return static_cast<T*>(t.data) + b * t.stride[0] + h * t.stride[2];
 }
 
+// Rows of whole 16-byte pieces, of each tensor.
+enum : uint32_t { kVecQ = 1, kVecK = 2, kVecV = 4, kVecOut = 8, kVecDq = 16, kVecDk = 32, kVecDv = 64 };
+
 // Rollouts in segments of `chunks` chunks, one block each.
 struct Segments {
   uint32_t count, chunks;
+  uint32_t vec;    // kVec...
   float* state;  // [rows][count][dk][dv]: first what a segment adds, then the state in front of it (behind it in reverse)
   float* keep;   // [rows][count]: what a segment leaves of the state in front of it
 };
