@@ -39,6 +39,37 @@ __device__ __forceinline__ int64_t offset(const RowsAt& a, uint32_t row, const N
   return int64_t(rest / p.rows1) * a.stride[0] + int64_t(rest % p.rows1) * a.stride[1] + int64_t(i2) * a.stride[2];
 }
 
+// Two 32-bit values at once: sm_100 adds, multiplies and multiply-adds pairs of registers in one instruction, and the
+// arithmetic of a value is what the vector units can just keep up with.
+struct Two {
+  uint64_t bits;
+};
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 apart(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.bits));
+  return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+
 // V neighbouring values as 32-bit ones: one 16-byte vector, or a single value.
 template <class T, int V>
 __device__ __forceinline__ void fetch(float (&x)[V], const T* at) {
@@ -78,8 +109,23 @@ __device__ __forceinline__ void put(T* at, const float (&x)[V]) {
   }
 }
 
-// Sums of two values over the lanes of a row.  A block's sums pass through `box` ([2][64], taken in turns so that one
-// barrier is enough).
+// Sums over the lanes of a row.  A block's pass through `box` ([2][32], taken in turns so that one barrier is enough).
+template <bool BLOCK>
+__device__ __forceinline__ float row_sum(float s, int lanes, float2 (*box)[32], int& turn) {
+  if (BLOCK) lanes = 32;
+  for (int d = 1; d < lanes; d <<= 1) s += __shfl_xor_sync(kAll, s, d);
+  if (BLOCK) {
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) box[turn][warp].x = s;
+    __syncthreads();
+    const int i = threadIdx.x & 31;
+    s = i < warps ? box[turn][i].x : 0.0f;
+    turn ^= 1;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) s += __shfl_xor_sync(kAll, s, d);
+  }
+  return s;
+}
 template <bool BLOCK>
 __device__ __forceinline__ float2 row_sum(float2 s, int lanes, float2 (*box)[32], int& turn) {
   if (BLOCK) lanes = 32;
@@ -105,18 +151,19 @@ __device__ __forceinline__ float2 row_sum(float2 s, int lanes, float2 (*box)[32]
 
 // N vectors of V values a lane, K rows at once.  `lanes` of a warp (or the block) share a row.
 template <class T, class W, int V, int N, int K, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_forward_kernel(const __grid_constant__ Norm p, const int lanes) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_forward_kernel(const __grid_constant__ Norm p, const int lanes, const int lanes_log) {
+  constexpr int M = N * V / 2;  // pairs of values of a lane
   __shared__ float2 box[2][32];
   int turn = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
-  const int per = BLOCK ? 1 : blockDim.x / lanes;  // rows side by side in a block
+  const uint32_t per = BLOCK ? 1 : 256u >> lanes_log;  // rows side by side in a block
   const int stride = BLOCK ? blockDim.x : lanes;
-  const uint64_t row0 = uint64_t(blockIdx.x) * (per * K) + (BLOCK ? 0 : threadIdx.x / lanes);
+  const uint32_t row0 = blockIdx.x * (per * K) + (BLOCK ? 0 : threadIdx.x >> lanes_log);  // (below 2^31 + 2^10)
   float x[K][N][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const uint64_t row = row0 + uint64_t(k) * per;
-    const T* from = static_cast<const T*>(p.x) + (row < p.rows ? offset(p.at_x, uint32_t(row), p) : 0);
+    const uint32_t row = row0 + k * per;
+    const T* from = static_cast<const T*>(p.x) + (row < p.rows ? offset(p.at_x, row, p) : 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t c = uint32_t(lane + i * stride) * V;
@@ -130,61 +177,75 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_forward_kernel(const _
   }
   float mean[K], rest[K], rstd[K];
   const float inverse = 1.0f / float(p.width);
+  Two y[K][M];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    float2 s = make_float2(0.0f, 0.0f);
+    const float* values = &x[k][0][0];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int m = 0; m < M; ++m) y[k][m] = two(values[2 * m], values[2 * m + 1]);
+    Two s = y[k][0];
 #pragma unroll
-      for (int e = 0; e < V; ++e) s.x += x[k][i][e];
-    mean[k] = row_sum<BLOCK>(s, lanes, box, turn).x * inverse;
+    for (int m = 1; m < M; ++m) s = s + y[k][m];
+    const float2 t = apart(s);
+    mean[k] = row_sum<BLOCK>(t.x + t.y, lanes, box, turn) * inverse;
   }
+  // where a lane's values are not all there, what is not stays zero
+  const bool whole = uint32_t(lane + (N - 1) * stride + 1) * V <= p.width;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    float2 s = make_float2(0.0f, 0.0f);
+    const Two minus = two(-mean[k], -mean[k]);
+    Two s = two(0.0f, 0.0f), q = s;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const bool there = uint32_t(lane + i * stride) * V < p.width;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = there ? x[k][i][e] - mean[k] : 0.0f;
-        x[k][i][e] = d, s.x += d, s.y = fmaf(d, d, s.y);
+    for (int m = 0; m < M; ++m) {
+      Two d = y[k][m] + minus;
+      if (!whole) {
+        const float2 a = apart(d);
+        d = two(uint32_t(lane + 2 * m / V * stride) * V < p.width ? a.x : 0.0f, uint32_t(lane + (2 * m + 1) / V * stride) * V < p.width ? a.y : 0.0f);
       }
+      y[k][m] = d, s = s + d, q = fma2(d, d, q);
     }
-    s = row_sum<BLOCK>(s, lanes, box, turn);
+    const float2 a = apart(s), b = apart(q);
+    const float2 t = row_sum<BLOCK>(make_float2(a.x + a.y, b.x + b.y), lanes, box, turn);
     // what the sum's rounding left of the mean
-    rest[k] = s.x * inverse;
-    rstd[k] = 1.0f / sqrtf(fmaxf(fmaf(-rest[k], rest[k], s.y * inverse), 0.0f) + p.eps);
-    if (s.y != s.y) rstd[k] = s.y;
+    rest[k] = t.x * inverse;
+    rstd[k] = 1.0f / sqrtf(fmaxf(fmaf(-rest[k], rest[k], t.y * inverse), 0.0f) + p.eps);
+    if (t.y != t.y) rstd[k] = t.y;
+    const Two r = two(-rest[k], -rest[k]), f = two(rstd[k], rstd[k]);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[k][i][e] = (x[k][i][e] - rest[k]) * rstd[k];
+    for (int m = 0; m < M; ++m) y[k][m] = (y[k][m] + r) * f;
   }
+  // one pair for all of a lane's rows at a time; 1 and 0 where there is no weight or bias
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const uint32_t c = uint32_t(lane + i * stride) * V;
     if (c >= p.width) continue;
     float w[V], b[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = 1.0f, b[e] = 0.0f;
     if (p.weight) fetch(w, static_cast<const W*>(p.weight) + c);
     if (p.bias) fetch(b, static_cast<const W*>(p.bias) + c);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint64_t row = row0 + uint64_t(k) * per;
+      const uint32_t row = row0 + k * per;
       if (row >= p.rows) continue;
-      float y[V];
+      float z[V];
+      if constexpr (V == 1) {
+        const float2 a = apart(y[k][i / 2]);
+        z[0] = fmaf(i % 2 ? a.y : a.x, w[0], b[0]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        y[e] = p.weight ? x[k][i][e] * w[e] : x[k][i][e];
-        if (p.bias) y[e] += b[e];
+        for (int m = 0; m < V / 2; ++m) {
+          const float2 a = apart(fma2(y[k][i * V / 2 + m], two(w[2 * m], w[2 * m + 1]), two(b[2 * m], b[2 * m + 1])));
+          z[2 * m] = a.x, z[2 * m + 1] = a.y;
+        }
       }
-      put(static_cast<T*>(p.y) + offset(p.at_y, uint32_t(row), p) + c, y);
+      put(static_cast<T*>(p.y) + offset(p.at_y, row, p) + c, z);
     }
   }
   if (p.saved && lane == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint64_t row = row0 + uint64_t(k) * per;
+      const uint32_t row = row0 + k * per;
       if (row < p.rows) p.saved[row] = mean[k], p.saved[uint64_t(p.rows) + row] = rest[k], p.saved[2 * uint64_t(p.rows) + row] = rstd[k];
     }
   }
@@ -192,104 +253,117 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_forward_kernel(const _
 
 // Rows from blockIdx.x on in steps of the grid; a thread's sums over its columns end in the block's line of the workspace.
 template <class T, class W, int V, int N, int K, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_backward_kernel(const __grid_constant__ Norm p, const int lanes) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_backward_kernel(const __grid_constant__ Norm p, const int lanes, const int lanes_log) {
+  constexpr int M = N * V / 2;
   __shared__ float2 box[2][32];
   extern __shared__ float side[];  // sums of the rows side by side
   int turn = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
-  const int per = BLOCK ? 1 : blockDim.x / lanes;
+  const uint32_t per = BLOCK ? 1 : 256u >> lanes_log;
   const int stride = BLOCK ? blockDim.x : lanes;
-  const int own = BLOCK ? 0 : threadIdx.x / lanes;
+  const uint32_t own = BLOCK ? 0 : threadIdx.x >> lanes_log;
   const float inverse = 1.0f / float(p.width);
-  float dw[N][V] = {}, db[N][V] = {};
+  Two dw[M], db[M], w[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) dw[m] = db[m] = two(0.0f, 0.0f);
+  {
+    float v[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t c = uint32_t(lane + i * stride) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i][e] = 1.0f;
+      if (p.weight && c < p.width) fetch(v[i], static_cast<const W*>(p.weight) + c);
+    }
+    const float* values = &v[0][0];
+#pragma unroll
+    for (int m = 0; m < M; ++m) w[m] = two(values[2 * m], values[2 * m + 1]);
+  }
   for (uint64_t first = uint64_t(blockIdx.x) * (per * K); first < p.rows; first += uint64_t(gridDim.x) * (per * K)) {
-    float x[K][N][V], g[K][N][V], rstd[K];
+    Two x[K][M], g[K][M];
+    float mean[K], rest[K], rstd[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint64_t row = first + own + uint64_t(k) * per;
+      const uint32_t row = uint32_t(first) + own + k * per;
       const bool here = row < p.rows;
-      const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, uint32_t(row), p) : 0);
-      const T* grad = static_cast<const T*>(p.dy) + (here ? offset(p.at_dy, uint32_t(row), p) : 0);
+      const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, row, p) : 0);
+      const T* grad = static_cast<const T*>(p.dy) + (here ? offset(p.at_dy, row, p) : 0);
+      float a[N][V], b[N][V];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const uint32_t c = uint32_t(lane + i * stride) * V;
         if (here && c < p.width) {
-          fetch(x[k][i], from + c);
-          fetch(g[k][i], grad + c);
+          fetch(a[i], from + c);
+          fetch(b[i], grad + c);
         } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) x[k][i][e] = g[k][i][e] = 0.0f;
+          for (int e = 0; e < V; ++e) a[i][e] = b[i][e] = 0.0f;
         }
       }
+      const float *va = &a[0][0], *vb = &b[0][0];
+#pragma unroll
+      for (int m = 0; m < M; ++m) x[k][m] = two(va[2 * m], va[2 * m + 1]), g[k][m] = two(vb[2 * m], vb[2 * m + 1]);
+      mean[k] = here ? p.saved[row] : 0.0f;
+      rest[k] = here ? p.saved[uint64_t(p.rows) + row] : 0.0f;
+      rstd[k] = here ? p.saved[2 * uint64_t(p.rows) + row] : 0.0f;
     }
     float2 s[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint64_t row = first + own + uint64_t(k) * per;
-      const bool here = row < p.rows;
-      const float mean = here ? p.saved[row] : 0.0f, rest = here ? p.saved[p.rows + row] : 0.0f;
-      rstd[k] = here ? p.saved[2 * uint64_t(p.rows) + row] : 0.0f;
-      s[k] = make_float2(0.0f, 0.0f);
+      const Two minus = two(-mean[k], -mean[k]), r = two(-rest[k], -rest[k]), f = two(rstd[k], rstd[k]);
+      Two s0 = two(0.0f, 0.0f), s1 = s0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t c = uint32_t(lane + i * stride) * V;
-        if (c >= p.width) continue;
-        float w[V];
-        if (p.weight) fetch(w, static_cast<const W*>(p.weight) + c);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float hat = (x[k][i][e] - mean - rest) * rstd[k], dy = g[k][i][e];
-          x[k][i][e] = hat;
-          dw[i][e] = fmaf(dy, hat, dw[i][e]), db[i][e] += dy;
-          const float dh = p.weight ? dy * w[e] : dy;
-          g[k][i][e] = dh;
-          s[k].x += dh, s[k].y = fmaf(dh, hat, s[k].y);
-        }
+      for (int m = 0; m < M; ++m) {  // (what is not there has no gradient: it adds nothing)
+        const Two hat = (x[k][m] + minus + r) * f, dy = g[k][m], dh = dy * w[m];
+        dw[m] = fma2(dy, hat, dw[m]), db[m] = db[m] + dy;
+        s0 = s0 + dh, s1 = fma2(dh, hat, s1);
+        x[k][m] = hat, g[k][m] = dh;
       }
+      const float2 a = apart(s0), b = apart(s1);
+      s[k] = make_float2(a.x + a.y, b.x + b.y);
     }
     if (!p.dx) continue;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint64_t row = first + own + uint64_t(k) * per;
+      const uint32_t row = uint32_t(first) + own + k * per;
       const float2 t = row_sum<BLOCK>(s[k], lanes, box, turn);
       if (row >= p.rows) continue;
-      const float m0 = t.x * inverse, m1 = t.y * inverse;
-      T* to = static_cast<T*>(p.dx) + offset(p.at_dx, uint32_t(row), p);
+      const Two m0 = two(-t.x * inverse, -t.x * inverse), m1 = two(-t.y * inverse, -t.y * inverse), f = two(rstd[k], rstd[k]);
+      T* to = static_cast<T*>(p.dx) + offset(p.at_dx, row, p);
+      float z[N][V];
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const float2 a = apart((g[k][m] + fma2(x[k][m], m1, m0)) * f);
+        (&z[0][0])[2 * m] = a.x, (&z[0][0])[2 * m + 1] = a.y;
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const uint32_t c = uint32_t(lane + i * stride) * V;
-        if (c >= p.width) continue;
-        float y[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = (g[k][i][e] - fmaf(x[k][i][e], m1, m0)) * rstd[k];
-        put(to + c, y);
+        if (c < p.width) put(to + c, z[i]);
       }
     }
   }
   if (!p.partial) return;
   float* line = p.partial + uint64_t(blockIdx.x) * 2 * p.width;
-  if (BLOCK) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const uint32_t c = uint32_t(lane + i * stride) * V + e;
-        if (c < p.width) line[c] = dw[i][e], line[p.width + c] = db[i][e];
-      }
-    return;
-  }
   const int cols = lanes * N * V;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
-    __syncthreads();
+    if (!BLOCK) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int m = 0; m < M; ++m) {
+      const float2 a = apart(pass ? db[m] : dw[m]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) side[own * cols + (lane + i * stride) * V + e] = pass ? db[i][e] : dw[i][e];
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t c = uint32_t(lane + (2 * m + h) / V * stride) * V + (2 * m + h) % V;
+        if (!BLOCK) side[own * cols + c] = h ? a.y : a.x;
+        else if (c < p.width) line[pass * p.width + c] = h ? a.y : a.x;
+      }
+    }
+    if (BLOCK) continue;
     __syncthreads();
-    for (uint32_t c = threadIdx.x; c < p.width; c += blockDim.x) {
+    for (uint32_t c = threadIdx.x; c < p.width; c += 256) {
       float sum = 0.0f;
-      for (int r = 0; r < per; ++r) sum += side[r * cols + c];
+      for (uint32_t r = 0; r < per; ++r) sum += side[r * cols + c];
       line[pass * p.width + c] = sum;
     }
   }
@@ -408,7 +482,8 @@ constexpr int rows_at_once(int values, bool block, bool backward) {
 
 struct Choice {
   bool vec, block;
-  int lanes;    // of a row; threads where a block takes one
+  int lanes;    // of a row (a power of two); threads where a block takes one
+  int lanes_log;
   int vectors;  // of a lane, as one of the instances
   int values() const { return vec ? vectors * width : vectors; }
   int width;    // values of a vector
@@ -431,6 +506,7 @@ Choice choose(const ZenoLayerNorm& p, bool vec) {
     while (uint32_t(c.lanes) < pieces && c.lanes < 32) c.lanes *= 2;
     // scalars: two of a lane, so that a warp takes several short rows
     if (!vec && c.lanes > 4 && pieces <= uint32_t(c.lanes)) c.lanes /= 2;
+    while (1 << c.lanes_log < c.lanes) ++c.lanes_log;
     const uint32_t n = (pieces + c.lanes - 1) / c.lanes;
     c.vectors = vec ? (n <= 1 ? 1 : n <= 2 ? 2 : 4) : (n <= 2 ? 2 : n <= 8 ? 8 : 16);
     return c;
@@ -445,10 +521,10 @@ template <class T, class W, int V, int N, bool BLOCK>
 cudaError_t run(const Norm& p, const Choice& c, bool backward, unsigned blocks, cudaStream_t stream) {
   const int threads = BLOCK ? c.lanes : 256;
   if (!backward) {
-    norm_forward_kernel<T, W, V, N, rows_at_once(V * N, BLOCK, false), BLOCK><<<blocks, threads, 0, stream>>>(p, c.lanes);
+    norm_forward_kernel<T, W, V, N, rows_at_once(V * N, BLOCK, false), BLOCK><<<blocks, threads, 0, stream>>>(p, c.lanes, c.lanes_log);
   } else {
     const size_t side = BLOCK || !p.partial ? 0 : size_t(256) * N * V * 4;
-    norm_backward_kernel<T, W, V, N, rows_at_once(V * N, BLOCK, true), BLOCK><<<blocks, threads, side, stream>>>(p, c.lanes);
+    norm_backward_kernel<T, W, V, N, rows_at_once(V * N, BLOCK, true), BLOCK><<<blocks, threads, side, stream>>>(p, c.lanes, c.lanes_log);
   }
   return cudaGetLastError();
 }

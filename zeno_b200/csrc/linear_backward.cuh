@@ -28,7 +28,7 @@ struct BackwardSmem {
 
 struct BackwardOut {
   float *shared_q, *shared_k;  // [batch][tokens][value heads][dk], where value heads share a key head
-  double* decay;               // [rows][segments], where all tokens of a head have one decay
+  double* decay;               // [value heads][batch][segments], where all tokens of a head have one decay
 };
 
 // acc's rows by f[i] (what f is zero for is left out).  Returns the products of the lane's two rows with those of X over its columns:
@@ -142,26 +142,14 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
     if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     float state_dot = 0.0f;  // <S, R> over this thread's elements
     if (front) {
-      const bool even = pairs_aligned(front, dv);
+      float x[S::NM][2][4];
+      read_state<S>(x, front, part, dk, dv, lane);
       float dot = 0.0f;
 #pragma unroll
-      for (int j = 0; j < S::NM; ++j) {
-        if (j >= part.pairs) break;
+      for (int j = 0; j < S::NM; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int row = part.row + (lane >> 2) + r * 8, cc = part.col + j * 16 + h * 8 + (lane & 3) * 2;
-            float2 x = make_float2(0.0f, 0.0f);
-            if (row < dk && cc < dv) x = read_pair(front + row * dv + cc, cc, dv, even);
-            dot = fmaf(x.x, m[j][h][2 * r], fmaf(x.y, m[j][h][2 * r + 1], dot));
-            uint32_t w[3];
-            split<3>(x.x, x.y, w);
-            plane_t* at = st + row * S::P + cc;
-#pragma unroll
-            for (int l = 0; l < 3; ++l) *reinterpret_cast<uint32_t*>(at + l * S::SPLANE) = w[l];
-          }
-      }
+        for (int e = 0; e < 8; ++e) dot = fmaf(x[j][e >> 2][e & 3], m[j][e >> 2][e & 3], dot);
+      dump_state<S, 3>(x, st, part, lane);
       state_dot = have_r ? dot : 0.0f;
       if (each) {
 #pragma unroll
@@ -440,7 +428,7 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
     __syncthreads();
     if (tid == 0) {
       for (int w = 1; w < S::NW; ++w) decay_sum += part_sum[w];
-      extra.decay[int64_t(a.row) * sg.count + a.seg] = decay_sum;
+      extra.decay[(uint64_t(a.h) * p.batch + a.b) * sg.count + a.seg] = decay_sum;
     }
   }
 }

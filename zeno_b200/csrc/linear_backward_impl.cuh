@@ -32,7 +32,7 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
       extra.shared_k = reinterpret_cast<float*>(at + l.cut + l.shared);
     }
     if (d.d_decay) extra.decay = reinterpret_cast<double*>(at + l.cut + 2 * l.shared);
-    if (!p.batch) return launch_linear_decay(nullptr, 0, p.value_heads, 1, d.d_decay, stream);
+    if (!p.batch) return launch_linear_decay(nullptr, 0, p.value_heads, d.d_decay, stream);
     cudaError_t e;
     if (c.count > 1) {
       e = cut_states<S>(p, p.q, d.d_out, sg, d.d_final, true, stream);
@@ -55,7 +55,7 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
       if (e == cudaSuccess) e = launch_linear_shared(LinearShared{extra.shared_k, d.d_k, p.tokens, p.key_heads, group, p.key_dim}, p.batch, p.dtype, stream);
       if (e != cudaSuccess) return e;
     }
-    return d.d_decay ? launch_linear_decay(extra.decay, p.batch, p.value_heads, c.count, d.d_decay, stream) : cudaSuccess;
+    return d.d_decay ? launch_linear_decay(extra.decay, uint64_t(p.batch) * c.count, p.value_heads, d.d_decay, stream) : cudaSuccess;
   });
 }
 

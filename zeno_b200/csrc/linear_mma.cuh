@@ -365,18 +365,20 @@ struct Part {
   }
 };
 
-// f(element of row, column, value reference) over pairs of neighbouring columns of a part that exist.
+// A lane's elements of a part are pairs of neighbouring columns: (j, h, r) is at row 8 r and column 16 j + 8 h of its first.
+// f(j, h, r, offset into the state of row length dv) over the pairs that exist.
 template <class S, class F>
-__device__ __forceinline__ void each_pair(float (&m)[S::NM][2][4], const Part<S>& part, int dk, int dv, int lane, F&& f) {
+__device__ __forceinline__ void each_pair(const Part<S>& part, int dk, int dv, int lane, F&& f) {
+  const int row = part.row + (lane >> 2), col = part.col + (lane & 3) * 2;
+  const int left[2] = {row < dk ? dv - col : 0, row + 8 < dk ? dv - col : 0};
+  const int at[2] = {row * dv + col, (row + 8) * dv + col};
 #pragma unroll
   for (int j = 0; j < S::NM; ++j)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = part.row + (lane >> 2) + r * 8, col = part.col + j * 16 + h * 8 + (lane & 3) * 2;
-        if (row < dk && col < dv) f(row, col, m[j][h][2 * r], m[j][h][2 * r + 1]);
-      }
+      for (int r = 0; r < 2; ++r)
+        if (j * 16 + h * 8 < left[r]) f(j, h, r, at[r] + j * 16 + h * 8);
 }
 
 template <class S>
@@ -387,35 +389,45 @@ __device__ __forceinline__ void clear(float (&m)[S::NM][2][4]) {
     for (int x = 0; x < 8; ++x) m[j][x >> 2][x & 3] = 0.0f;
 }
 
-// `even`: pairs of columns are 8-byte aligned
+// Pairs of columns are 8-byte aligned.
 __device__ __forceinline__ bool pairs_aligned(const void* p, int dv) { return dv % 2 == 0 && reinterpret_cast<uintptr_t>(p) % 8 == 0; }
-__device__ __forceinline__ float2 read_pair(const float* at, int col, int dv, bool even) {
-  if (even) return *reinterpret_cast<const float2*>(at);
-  return make_float2(at[0], col + 1 < dv ? at[1] : 0.0f);
-}
-__device__ __forceinline__ void write_pair(float* at, int col, int dv, bool even, float x, float y) {
+__device__ __forceinline__ void write_pair(float* at, int col, int width, bool even, float x, float y) {
   if (even) {
     *reinterpret_cast<float2*>(at) = make_float2(x, y);
   } else {
     at[0] = x;
-    if (col + 1 < dv) at[1] = y;
+    if (col + 1 < width) at[1] = y;
   }
 }
 
 template <class S>
 __device__ __forceinline__ void read_state(float (&m)[S::NM][2][4], const float* from, const Part<S>& part, int dk, int dv, int lane) {
-  const bool even = pairs_aligned(from, dv);
   clear<S>(m);
-  each_pair<S>(m, part, dk, dv, lane, [&](int row, int col, float& x, float& y) {
-    const float2 v = read_pair(from + row * dv + col, col, dv, even);
-    x = v.x, y = v.y;
-  });
+  if (pairs_aligned(from, dv)) {
+    each_pair<S>(part, dk, dv, lane, [&](int j, int h, int r, int at) {
+      const float2 v = *reinterpret_cast<const float2*>(from + at);
+      m[j][h][2 * r] = v.x, m[j][h][2 * r + 1] = v.y;
+    });
+  } else {
+    const int left = dv - 1 - part.col - (lane & 3) * 2;  // of the second of a pair
+    each_pair<S>(part, dk, dv, lane, [&](int j, int h, int r, int at) {
+      m[j][h][2 * r] = from[at];
+      if (j * 16 + h * 8 < left) m[j][h][2 * r + 1] = from[at + 1];
+    });
+  }
 }
 template <class S>
-__device__ __forceinline__ void write_state(float (&m)[S::NM][2][4], float* to, const Part<S>& part, int dk, int dv, int lane) {
-  const bool even = pairs_aligned(to, dv);
-  each_pair<S>(m, part, dk, dv, lane,
-               [&](int row, int col, float& x, float& y) { write_pair(to + row * dv + col, col, dv, even, x, y); });
+__device__ __forceinline__ void write_state(const float (&m)[S::NM][2][4], float* to, const Part<S>& part, int dk, int dv, int lane) {
+  if (pairs_aligned(to, dv)) {
+    each_pair<S>(part, dk, dv, lane,
+                 [&](int j, int h, int r, int at) { *reinterpret_cast<float2*>(to + at) = make_float2(m[j][h][2 * r], m[j][h][2 * r + 1]); });
+  } else {
+    const int left = dv - 1 - part.col - (lane & 3) * 2;
+    each_pair<S>(part, dk, dv, lane, [&](int j, int h, int r, int at) {
+      to[at] = m[j][h][2 * r];
+      if (j * 16 + h * 8 < left) to[at + 1] = m[j][h][2 * r + 1];
+    });
+  }
 }
 
 // The part's limbs into planes [D][P] (whole 16 x 16 tiles).

@@ -48,19 +48,22 @@ __global__ void __launch_bounds__(256) linear_shared_kernel(const LinearShared s
   }
 }
 
-// One block a head: its decay's gradient from those of the environments and segments, in a fixed order, in 64 bits.
-__global__ void __launch_bounds__(256) linear_decay_kernel(const double* from, uint32_t batch, uint32_t heads, uint32_t segments, float* to) {
-  __shared__ double part[256];
-  const uint32_t h = blockIdx.x;
+// One block a head: its decay's gradient from those of the environments and segments, [heads][count], in a fixed order, in 64 bits.
+__global__ void __launch_bounds__(1024) linear_decay_kernel(const double* from, uint64_t count, float* to) {
+  __shared__ double part[32];
+  from += blockIdx.x * count;
   double sum = 0.0;
-  for (uint64_t i = threadIdx.x; i < uint64_t(batch) * segments; i += 256)
-    sum += from[(i / segments * heads + h) * segments + i % segments];
-  part[threadIdx.x] = sum;
-  for (uint32_t d = 128; d > 0; d >>= 1) {
-    __syncthreads();
-    if (threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
-  }
-  if (threadIdx.x == 0) to[h] = float(part[0]);
+#pragma unroll 8
+  for (uint64_t i = threadIdx.x; i < count; i += 1024) sum += from[i];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  sum = part[threadIdx.x];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (threadIdx.x == 0) to[blockIdx.x] = float(sum);
 }
 
 }  // namespace
@@ -81,8 +84,8 @@ cudaError_t launch_linear_shared(const LinearShared& s, uint32_t batch, uint32_t
   return cudaGetLastError();
 }
 
-cudaError_t launch_linear_decay(const double* from, uint32_t batch, uint32_t heads, uint32_t segments, float* to, cudaStream_t stream) {
-  linear_decay_kernel<<<heads, 256, 0, stream>>>(from, batch, heads, segments, to);
+cudaError_t launch_linear_decay(const double* from, uint64_t count, uint32_t heads, float* to, cudaStream_t stream) {
+  linear_decay_kernel<<<heads, 1024, 0, stream>>>(from, count, to);
   return cudaGetLastError();
 }
 
