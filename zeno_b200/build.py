@@ -5,6 +5,9 @@ floating-point operation is the one written in the source (explicit __fmaf_rn ca
 are the only fused operations); host model-building code is compiled with
 -ffp-contract=off for the same reason.
 
+The memory operators' PyTorch functions (zeno_b200/lib/zeno_torch.so, on libzeno.so) are compiled with g++ against the
+installed PyTorch.
+
 The library is also copied to <repo>/zig-out/lib/libzeno.so, where the reference's own
 Python package and ABI check look for it.  The sources compile in parallel.
 
@@ -12,10 +15,12 @@ Usage: python -m zeno_b200.build [--force]
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -24,6 +29,8 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 OUT_DIR = PKG / "lib"
 LIB = OUT_DIR / "libzeno.so"
+BINDING = OUT_DIR / "zeno_torch.so"
+BINDING_SOURCE = CSRC / "torch_binding.cpp"
 # where the reference's own Python package (python/zeno/_ffi.py _find_library) and its
 # tests/check_abi_contract.py look for the library: <repo>/zig-out/lib/libzeno.so
 ZIG_OUT_LIB = PKG.parent / "zig-out" / "lib" / "libzeno.so"
@@ -56,15 +63,7 @@ def _newer(target: Path, deps) -> bool:
     return all(Path(d).stat().st_mtime <= t for d in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every CUDA/C++ source and link libzeno.so; returns the library path."""
-    deps = [CSRC / s for s in CU_SOURCES + OP_SOURCES + CXX_SOURCES + HEADERS] + [INCLUDE / "zeno.h", Path(__file__)]
-    if not force and _newer(LIB, deps):
-        return LIB
-    OBJ_DIR.mkdir(exist_ok=True)
-    OUT_DIR.mkdir(exist_ok=True)
-    cxx = shutil.which("g++") or "g++"
-
+def _runner(verbose: bool):
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
@@ -73,6 +72,43 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             raise RuntimeError(f"build failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if verbose and (r.stdout or r.stderr):
             print(r.stdout, r.stderr)
+    return run
+
+
+def _compile_binding(run, cxx: str) -> Path:
+    """The object file of the PyTorch functions."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("build failed: the operators' functions need an installed PyTorch")
+    torch_dir = Path(spec.origin).parent
+    obj = OBJ_DIR / (BINDING_SOURCE.name + ".o")
+    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", CUDA_HOME / "include",
+                sysconfig.get_paths()["include"]]
+    run([cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", *(f"-I{i}" for i in includes), "-c", str(BINDING_SOURCE), "-o", str(obj)])
+    return obj
+
+
+def _link_binding(run, cxx: str, obj: Path) -> None:
+    torch_lib = Path(importlib.util.find_spec("torch").origin).parent / "lib"
+    tmp = BINDING.with_suffix(".so.tmp")
+    run([cxx, "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}", "-lzeno", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+         "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
+    os.replace(tmp, BINDING)
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every CUDA/C++ source and link libzeno.so and the PyTorch functions; returns the library path."""
+    deps = [CSRC / s for s in CU_SOURCES + OP_SOURCES + CXX_SOURCES + HEADERS] + [INCLUDE / "zeno.h", Path(__file__)]
+    binding_deps = [BINDING_SOURCE, INCLUDE / "zeno.h", Path(__file__)]
+    cxx = shutil.which("g++") or "g++"
+    run = _runner(verbose)
+    if not force and _newer(LIB, deps):
+        if not _newer(BINDING, binding_deps):
+            OBJ_DIR.mkdir(exist_ok=True)
+            _link_binding(run, cxx, _compile_binding(run, cxx))
+        return LIB
+    OBJ_DIR.mkdir(exist_ok=True)
+    OUT_DIR.mkdir(exist_ok=True)
 
     jobs = [[NVCC, *NVCC_FLAGS, f"-I{INCLUDE}", "-c", str(CSRC / src), "-o", str(OBJ_DIR / (src + ".o"))]
             for src in CU_SOURCES]
@@ -82,11 +118,14 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     objs = [cmd[-1] for cmd in jobs]
     jobs.sort(key=lambda cmd: "delta_" not in cmd[-3])  # the longest first
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as pool:
-        for f in [pool.submit(run, cmd) for cmd in jobs]:
+        running = [pool.submit(run, cmd) for cmd in jobs]
+        binding = pool.submit(_compile_binding, run, cxx)
+        for f in running:
             f.result()
     tmp = LIB.with_suffix(".so.tmp")
     run([NVCC, *ARCH, "-shared", "-o", str(tmp), *objs, "-Xlinker", "--no-undefined"])
     os.replace(tmp, LIB)
+    _link_binding(run, cxx, binding.result())
     ZIG_OUT_LIB.parent.mkdir(parents=True, exist_ok=True)
     shutil.copyfile(LIB, ZIG_OUT_LIB.with_suffix(".so.tmp"))
     os.replace(ZIG_OUT_LIB.with_suffix(".so.tmp"), ZIG_OUT_LIB)

@@ -13,6 +13,9 @@ from __future__ import annotations
 
 import struct
 from contextlib import nullcontext
+from importlib.machinery import ExtensionFileLoader
+from importlib.util import module_from_spec, spec_from_loader
+from pathlib import Path
 from typing import Optional, Tuple
 
 import torch
@@ -20,6 +23,20 @@ from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from ._ffi import _lib, ffi
+
+
+def _binding():
+    """The compiled functions of the memory operators (csrc/torch_binding.cpp)."""
+    path = Path(__file__).resolve().parent / "lib" / "zeno_torch.so"
+    if not path.exists():
+        raise ImportError(f"{path} is missing: build it with `python -m zeno_b200.build`")
+    loader = ExtensionFileLoader("zeno_torch", str(path))
+    module = module_from_spec(spec_from_loader("zeno_torch", loader))
+    loader.exec_module(module)
+    return module
+
+
+_torch = _binding()
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _FLAGS = (torch.uint8, torch.bool)
@@ -32,14 +49,6 @@ Tensor = torch.Tensor
 _RULE = struct.Struct("@8IfI" + "P3q" * 6 + "2P" + "P3q" + "P")
 _GRADS = struct.Struct("@P3qP" + "P3q" * 5 + "P")
 assert _RULE.size == ffi.sizeof("ZenoDeltaRule") and _GRADS.size == ffi.sizeof("ZenoDeltaRuleGrads")
-_LINEAR = struct.Struct("@7If" + "P3q" * 5 + "2P" + "P3q" + "P")
-_LINEAR_GRADS = struct.Struct("@P3qP" + "P3q" * 4 + "2P")
-_NORM = struct.Struct("@3Q3If" + "P3q" + "2P" + "P3q" + "P")
-_NORM_GRADS = struct.Struct("@" + "P3q" * 2 + "2P")
-assert _LINEAR.size == ffi.sizeof("ZenoLinearAttention") and _LINEAR_GRADS.size == ffi.sizeof("ZenoLinearAttentionGrads")
-assert _NORM.size == ffi.sizeof("ZenoLayerNorm") and _NORM_GRADS.size == ffi.sizeof("ZenoLayerNormGrads")
-_LINEAR_PTR, _LINEAR_GRADS_PTR = ffi.typeof("ZenoLinearAttention*"), ffi.typeof("ZenoLinearAttentionGrads*")
-_NORM_PTR, _NORM_GRADS_PTR = ffi.typeof("ZenoLayerNorm*"), ffi.typeof("ZenoLayerNormGrads*")
 _RULE_PTR, _GRADS_PTR = ffi.typeof("ZenoDeltaRule*"), ffi.typeof("ZenoDeltaRuleGrads*")
 _ADDRESS, _NO_TENSOR = ffi.typeof("void*"), (0, 0, 0, 0)
 
@@ -74,7 +83,7 @@ def _expect(name: str, x: Tensor, shape: Tuple[int, ...], dtypes, device: torch.
         raise ValueError(f"{name} is on {x.device}, q on {device}")
 
 
-def _check_heads(q: Tensor, k: Tensor, v: Tensor, lead: int):
+def _check_inputs(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: Optional[Tensor], lead: int):
     """``lead``: the axes in front of the heads (2: batch and tokens, 1: batch).  Returns the
     state's shape."""
     qs, vs, dtype, device = q.shape, v.shape, q.dtype, q.device
@@ -91,20 +100,15 @@ def _check_heads(q: Tensor, k: Tensor, v: Tensor, lead: int):
         raise ValueError(f"head widths must be 1 to {_MAX_DIM}, got {dk} and {dv}")
     if key_heads < 1 or heads < 1 or heads % key_heads:
         raise ValueError(f"the {heads} value heads must be a multiple of the {key_heads} key heads")
+    front = qs[:lead]
+    gates = vs[:-1]
     _expect("k", k, qs, (dtype,), device)
-    _expect("v", v, qs[:lead] + vs[lead:], (dtype,), device)
-    return (qs[0], heads, dk, dv)
-
-
-def _check_inputs(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, reset: Optional[Tensor], lead: int):
-    """As ``_check_heads``, with the gates of the delta rule."""
-    state = _check_heads(q, k, v, lead)
-    gates, device = v.shape[:-1], q.device
+    _expect("v", v, front + vs[lead:], (dtype,), device)
     _expect("g", g, gates, (torch.float32,), device)
     _expect("beta", beta, gates, (torch.float32,), device)
     if reset is not None:
-        _expect("reset", reset, q.shape[:lead], _FLAGS, device)
-    return state
+        _expect("reset", reset, front, _FLAGS, device)
+    return (qs[0], heads, dk, dv)
 
 
 def _rows(x: Tensor) -> Tensor:
@@ -264,84 +268,6 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, st
     return out
 
 
-def _linear(tensor, q, k, v, g, reset, initial, final, out, scale, saved=None):
-    qs, vs = q.shape, v.shape
-    return ffi.from_buffer(_LINEAR_PTR, _LINEAR.pack(
-        qs[0], qs[1] if tensor is _tokens else 1, qs[-2], vs[-2], qs[-1], vs[-1], _DTYPES[q.dtype], scale,
-        *tensor(q), *tensor(k), *tensor(v), *(_per_head(g) if g.dim() == 1 else tensor(g)), *tensor(reset), _address(initial),
-        _address(final), *tensor(out), _address(saved)))
-
-
-def _per_head(g: Tensor):
-    """A ZenoTensor of [heads], the same for all tokens."""
-    return g.data_ptr(), 0, 0, g.stride(0)
-
-
-def _check_decays(q: Tensor, k: Tensor, v: Tensor, g: Tensor, reset: Optional[Tensor], lead: int):
-    """Returns the state's shape."""
-    state = _check_heads(q, k, v, lead)
-    _expect("g", g, v.shape[lead:-1] if g.dim() == 1 else v.shape[:-1], (torch.float32,), q.device)
-    if reset is not None:
-        _expect("reset", reset, q.shape[:lead], _FLAGS, q.device)
-    return state
-
-
-def _dense_like(x: Tensor) -> Tensor:
-    """An empty tensor of x's shape, and of its order where that leaves the last axis contiguous."""
-    y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
-def _linear_forward(q, k, v, g, reset, initial, scale, save):
-    out = _dense_like(v)
-    device = q.device
-    final = torch.empty((v.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device)
-    p = _linear(_tokens, q, k, v, g, reset, initial, final, out, scale)
-    saved = None
-    with _on(device.index):
-        if save:
-            n = _lib.zeno_linear_attention_saved_bytes(p)
-            if n:
-                saved = torch.empty(n // 4, dtype=torch.float32, device=device)
-                p = _linear(_tokens, q, k, v, g, reset, initial, final, out, scale, saved)
-        n = _lib.zeno_linear_attention_workspace_bytes(p, 0)
-        w = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        _check(_lib.zeno_linear_attention_forward(p, ffi.cast(_ADDRESS, _address(w)), n, _stream(device.index)), "linear_attention")
-    return out, final, saved
-
-
-class _LinearAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, g, reset, initial, scale):
-        out, final, saved = _linear_forward(q, k, v, g, reset, initial, scale, True)
-        ctx.save_for_backward(q, k, v, g, reset, initial, saved)
-        ctx.scale = scale
-        ctx.set_materialize_grads(False)
-        return out, final
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_out, d_final):
-        q, k, v, g, reset, initial, saved = ctx.saved_tensors
-        d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if d_out is None else _rows(d_out)
-        if d_final is not None:
-            d_final = d_final.contiguous()
-        p = _linear(_tokens, q, k, v, g, reset, initial, None, d_out, ctx.scale, saved)
-        d_q, d_k, d_v = _dense_like(q), _dense_like(k), _dense_like(v)
-        d_g = torch.empty_like(g) if ctx.needs_input_grad[3] else None
-        per_head = g.dim() == 1
-        d_initial = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[5] else None
-        d = ffi.from_buffer(_LINEAR_GRADS_PTR, _LINEAR_GRADS.pack(
-            *_tokens(d_out), _address(d_final), *_tokens(d_q), *_tokens(d_k), *_tokens(d_v), *_tokens(None if per_head else d_g),
-            _address(d_g) if per_head else 0, _address(d_initial)))
-        index = q.device.index
-        with _on(index):
-            n = _lib.zeno_linear_attention_workspace_bytes(p, 1)
-            w = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-            _check(_lib.zeno_linear_attention_backward(p, d, ffi.cast(_ADDRESS, _address(w)), n, _stream(index)), "linear_attention backward")
-        return d_q, d_k, d_v, d_g, None, d_initial, None
-
-
 def linear_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, reset: Optional[Tensor] = None,
                      initial_state: Optional[Tensor] = None, *, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """Linear attention with a decay for each head over a rollout: ``(out [B, T, H, dv], final_state [B, H, dk, dv])``.
@@ -366,17 +292,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, reset: Optional
     For the gradients a call keeps the state in front of every 64 tokens but the first (32 in float32):
     0.27 GB for 4096 x 128 tokens and 4 heads of 64 x 64 in bfloat16.
     """
-    state = _check_decays(q, k, v, g, reset, 2)
-    if initial_state is not None:
-        _expect("initial_state", initial_state, state, (torch.float32,), q.device)
-        initial_state = initial_state.contiguous()
-    _refuse_tangents("linear_attention", q, k, v, g, initial_state)
-    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, initial_state)):
-        return _LinearAttention.apply(q, k, v, g, reset, initial_state, scale)
-    out, final, _ = _linear_forward(q, k, v, g, reset, initial_state, scale, False)
-    return out, final
+    return _torch.linear_attention(q, k, v, g, reset, initial_state, scale)
 
 
 def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Tensor, reset: Optional[Tensor] = None,
@@ -387,76 +303,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Ten
     world's ``dones`` buffer can be passed as it is).  ``state`` [B, H, dk, dv] float32,
     contiguous, is updated in place, and autograd knows: a rollout that was given the same
     tensor as its initial state and is yet to be differentiated needs a clone of it."""
-    _expect("state", state, _check_decays(q, k, v, g, reset, 1), (torch.float32,), q.device)
-    if not state.is_contiguous():
-        raise ValueError("state must be contiguous: it is updated in place")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, g, state)):
-        raise RuntimeError("linear_attention_step has no gradients: call it under torch.no_grad(), and linear_attention to learn")
-    _refuse_tangents("linear_attention_step", q, k, v, g, state)
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    p = _linear(_one_token, q, k, v, g, reset, state, state, out, scale)
-    index = q.device.index
-    with _on(index):
-        _check(_lib.zeno_linear_attention_step(p, _stream(index)), "linear_attention_step")
-    if not state.is_inference():  # (those have no version, and are never saved for a backward pass)
-        increment_version(state)
-    return out
-
-
-def _norm_rows(x: Optional[Tensor], axes: int):
-    """A ZenoTensor of rows, its leading axes padded to three."""
-    if x is None:
-        return _NO_TENSOR
-    return (x.data_ptr(), *(0,) * (3 - axes), *x.stride()[:axes])
-
-
-def _norm(x, weight, bias, eps, out, saved):
-    shape = x.shape
-    axes = len(shape) - 1
-    return ffi.from_buffer(_NORM_PTR, _NORM.pack(
-        *(1,) * (3 - axes), *shape[:-1], shape[-1], _DTYPES[x.dtype],
-        _DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype], eps,
-        *_norm_rows(x, axes), _address(weight), _address(bias), *_norm_rows(out, axes), _address(saved)))
-
-
-def _norm_forward(x, weight, bias, eps, save):
-    out = _dense_like(x)
-    index = x.device.index
-    saved = torch.empty(3 * (x.numel() // x.shape[-1]), dtype=torch.float32, device=x.device) if save else None
-    with _on(index):
-        _check(_lib.zeno_layer_norm_forward(_norm(x, weight, bias, eps, out, saved), _stream(index)), "layer_norm")
-    return out, saved
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        out, saved = _norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, saved)
-        ctx.eps, ctx.bias = eps, None if bias is None else bias.dtype
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_out):
-        x, weight, saved = ctx.saved_tensors
-        d_out = _rows(d_out)
-        axes, device, width = x.dim() - 1, x.device, x.shape[-1]
-        want = ctx.needs_input_grad
-        d_x = _dense_like(x) if want[0] else None
-        d_weight = torch.empty(width, dtype=weight.dtype, device=device) if want[1] else None
-        d_bias = torch.empty(width, dtype=ctx.bias, device=device) if want[2] else None
-        p = _norm(x, weight, d_bias, ctx.eps, None, saved)  # (the bias itself is not read)
-        d = ffi.from_buffer(_NORM_GRADS_PTR, _NORM_GRADS.pack(*_norm_rows(d_out, axes), *_norm_rows(d_x, axes), _address(d_weight),
-                                                              _address(d_bias)))
-        index = device.index
-        with _on(index):
-            n = _lib.zeno_layer_norm_workspace_bytes(p) if want[1] or want[2] else 0
-            w = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-            _check(_lib.zeno_layer_norm_backward(p, d, ffi.cast(_ADDRESS, _address(w)), n, _stream(index)), "layer_norm backward")
-        return d_x, d_weight, d_bias, None
+    return _torch.linear_attention_step(q, k, v, g, state, reset, scale)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, *, eps: float = 1e-5) -> Tensor:
@@ -466,37 +313,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     contiguous; the result keeps a time-major order).  ``weight`` and ``bias`` [n] are float32 or of x's type, both of one
     type; None: 1 and 0.  Mean, variance and all sums are held in 32 bits.  Gradients flow to x, weight and bias (once,
     and in reverse mode only); they are sums in a fixed order, so they repeat bit for bit."""
-    if x.device.type != "cuda":
-        raise ValueError(f"expected a CUDA tensor, got x on {x.device}")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"x must be float32 or bfloat16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x needs a last axis to be normalised over, got shape {tuple(x.shape)}")
-    for name, y in (("weight", weight), ("bias", bias)):
-        if y is None:
-            continue
-        if y.shape != x.shape[-1:]:
-            raise ValueError(f"{name} must have shape {tuple(x.shape[-1:])}, got {tuple(y.shape)}")
-        if y.dtype != torch.float32 and y.dtype != x.dtype:
-            raise TypeError(f"{name} must be float32 or {x.dtype}, got {y.dtype}")
-        if y.device != x.device:
-            raise ValueError(f"{name} is on {y.device}, x on {x.device}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
-    eps = float(eps)
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-    _refuse_tangents("layer_norm", x, weight, bias)
-    shape = x.shape
-    x = _rows(x)
-    if x.dim() > 4:
-        x = x.reshape(-1, shape[-1])
-    weight, bias = (y if y is None or y.is_contiguous() else y.contiguous() for y in (weight, bias))
-    if torch.is_grad_enabled() and any(y is not None and y.requires_grad for y in (x, weight, bias)):
-        out = _LayerNorm.apply(x, weight, bias, eps)
-    else:
-        out, _ = _norm_forward(x, weight, bias, eps, False)
-    return out if out.shape == shape else out.reshape(shape)
+    return _torch.layer_norm(x, weight, bias, eps)
 
 
 def orthogonalize(update: Tensor, steps: int = 5) -> Tensor:
