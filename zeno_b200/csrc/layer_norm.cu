@@ -70,19 +70,36 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
-// V neighbouring values as 32-bit ones: one 16-byte vector, or a single value.
+// V neighbouring values (one 16-byte vector, or a single value) as they are in memory.
 template <class T, int V>
-__device__ __forceinline__ void fetch(float (&x)[V], const T* at) {
+struct Raw {
+  using type = uint4;
+};
+template <class T>
+struct Raw<T, 1> {
+  using type = T;
+};
+template <class T, int V>
+__device__ __forceinline__ typename Raw<T, V>::type fetch_raw(const T* at) {
+  return *reinterpret_cast<const typename Raw<T, V>::type*>(at);
+}
+__device__ __forceinline__ void unpack(float (&x)[1], float w) { x[0] = w; }
+__device__ __forceinline__ void unpack(float (&x)[1], bf16 w) { x[0] = __bfloat162float(w); }
+__device__ __forceinline__ void unpack(float (&x)[4], const uint4& w) {
+  x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void unpack(float (&x)[8], const uint4& w) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+}
+// V values of a weight, of its own type.
+template <class W, int V>
+__device__ __forceinline__ void fetch(float (&x)[V], const W* at) {
   if constexpr (V == 1) {
-    x[0] = float(*at);
-  } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int h = 0; h < V; h += 8) {
-      const uint4 w = *reinterpret_cast<const uint4*>(at + h);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[h + 2 * i] = __uint_as_float(u[i] << 16), x[h + 2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
+    unpack(x, *at);
+  } else if constexpr (sizeof(W) == 2) {
+    unpack(x, *reinterpret_cast<const uint4*>(at));
   } else {
 #pragma unroll
     for (int h = 0; h < V; h += 4) {
@@ -109,11 +126,17 @@ __device__ __forceinline__ void put(T* at, const float (&x)[V]) {
   }
 }
 
-// Sums over the lanes of a row.  A block's pass through `box` ([2][32], taken in turns so that one barrier is enough).
-template <bool BLOCK>
-__device__ __forceinline__ float row_sum(float s, int lanes, float2 (*box)[32], int& turn) {
-  if (BLOCK) lanes = 32;
-  for (int d = 1; d < lanes; d <<= 1) s += __shfl_xor_sync(kAll, s, d);
+// 1 / sqrt(x): the approximation and one Newton step
+__device__ __forceinline__ float inverse_sqrt(float x) {
+  const float y = rsqrtf(x);
+  return x < INFINITY ? fmaf(0.5f * y, fmaf(-x * y, y, 1.0f), y) : y + (x - x);
+}
+
+// Sums over the LANES lanes of a row, or over a block.  A block's pass through `box` (taken in turns so that one barrier is enough).
+template <int LANES, bool BLOCK>
+__device__ __forceinline__ float row_sum(float s, float2 (*box)[32], int& turn) {
+#pragma unroll
+  for (int d = 1; d < LANES; d <<= 1) s += __shfl_xor_sync(kAll, s, d);
   if (BLOCK) {
     const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) box[turn][warp].x = s;
@@ -126,10 +149,10 @@ __device__ __forceinline__ float row_sum(float s, int lanes, float2 (*box)[32], 
   }
   return s;
 }
-template <bool BLOCK>
-__device__ __forceinline__ float2 row_sum(float2 s, int lanes, float2 (*box)[32], int& turn) {
-  if (BLOCK) lanes = 32;
-  for (int d = 1; d < lanes; d <<= 1) {
+template <int LANES, bool BLOCK>
+__device__ __forceinline__ float2 row_sum(float2 s, float2 (*box)[32], int& turn) {
+#pragma unroll
+  for (int d = 1; d < LANES; d <<= 1) {
     s.x += __shfl_xor_sync(kAll, s.x, d);
     s.y += __shfl_xor_sync(kAll, s.y, d);
   }
@@ -149,76 +172,99 @@ __device__ __forceinline__ float2 row_sum(float2 s, int lanes, float2 (*box)[32]
   return s;
 }
 
-// N vectors of V values a lane, K rows at once.  `lanes` of a warp (or the block) share a row.
-template <class T, class W, int V, int N, int K, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_forward_kernel(const __grid_constant__ Norm p, const int lanes, const int lanes_log) {
-  constexpr int M = N * V / 2;  // pairs of values of a lane
+// A row belongs to LANES lanes, or with BLOCK to all warps of a block, 32 N V neighbouring values to each.  A lane has N vectors of V
+// values, LANES V apart; K rows at once.
+template <class T_, class W_, int V_, int N_, int LANES_, bool BLOCK_>
+struct Shape {
+  using T = T_;
+  using W = W_;
+  static constexpr int V = V_, N = N_, LANES = LANES_, M = N * V / 2;  // M: pairs of values of a lane
+  static constexpr bool BLOCK = BLOCK_;
+  static constexpr int PER = BLOCK ? 1 : 256 / LANES;  // rows side by side in a block
+  // short rows several at a time, so that enough loads are under way; backward fetches ahead instead
+  static constexpr int K = BLOCK ? 1 : N * V <= 8 ? 4 : 2;
+  static constexpr int COLS = LANES * N * V;  // columns that there is room for (BLOCK: for each warp)
+  int first;   // first column
+  bool full;   // no column of this row (this warp) is past the width
+  __device__ __forceinline__ explicit Shape(uint32_t width) {
+    const int lane = BLOCK ? threadIdx.x & 31 : threadIdx.x & (LANES - 1), warp = BLOCK ? threadIdx.x >> 5 : 0;
+    first = warp * COLS + lane * V;
+    full = uint32_t((warp + 1) * COLS) <= width;
+  }
+  __device__ __forceinline__ int column(int i) const { return first + i * LANES * V; }
+};
+
+template <class S>
+__global__ void __launch_bounds__(S::BLOCK ? 512 : 256) norm_forward_kernel(const __grid_constant__ Norm p) {
+  using T = typename S::T;
+  using W = typename S::W;
+  constexpr int V = S::V, N = S::N, M = S::M, K = S::K;
   __shared__ float2 box[2][32];
   int turn = 0;
-  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
-  const uint32_t per = BLOCK ? 1 : 256u >> lanes_log;  // rows side by side in a block
-  const int stride = BLOCK ? blockDim.x : lanes;
-  const uint32_t row0 = blockIdx.x * (per * K) + (BLOCK ? 0 : threadIdx.x >> lanes_log);  // (below 2^31 + 2^10)
-  float x[K][N][V];
+  const S at(p.width);
+  const uint32_t width = p.width;
+  const uint32_t row0 = blockIdx.x * (S::PER * K) + (S::BLOCK ? 0 : threadIdx.x / S::LANES);
+  typename Raw<T, V>::type raw[K][N];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const uint32_t row = row0 + k * per;
-    const T* from = static_cast<const T*>(p.x) + (row < p.rows ? offset(p.at_x, row, p) : 0);
+    const uint32_t row = row0 + k * S::PER;
+    const bool here = row < p.rows;
+    const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, row, p) : 0) + at.first;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint32_t c = uint32_t(lane + i * stride) * V;
-      if (row < p.rows && c < p.width) {
-        fetch(x[k][i], from + c);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[k][i][e] = 0.0f;
-      }
+      raw[k][i] = typename Raw<T, V>::type{};
+      if (here && (at.full || uint32_t(at.column(i)) < width)) raw[k][i] = fetch_raw<T, V>(from + i * S::LANES * V);
     }
   }
+  const float inverse = 1.0f / float(width);
   float mean[K], rest[K], rstd[K];
-  const float inverse = 1.0f / float(p.width);
   Two y[K][M];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const float* values = &x[k][0][0];
+    float x[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack(x[i], raw[k][i]);
+    const float* values = &x[0][0];
 #pragma unroll
     for (int m = 0; m < M; ++m) y[k][m] = two(values[2 * m], values[2 * m + 1]);
     Two s = y[k][0];
 #pragma unroll
     for (int m = 1; m < M; ++m) s = s + y[k][m];
     const float2 t = apart(s);
-    mean[k] = row_sum<BLOCK>(t.x + t.y, lanes, box, turn) * inverse;
+    mean[k] = row_sum<S::LANES, S::BLOCK>(t.x + t.y, box, turn) * inverse;
   }
-  // where a lane's values are not all there, what is not stays zero
-  const bool whole = uint32_t(lane + (N - 1) * stride + 1) * V <= p.width;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const Two minus = two(-mean[k], -mean[k]);
-    Two s = two(0.0f, 0.0f), q = s;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      Two d = y[k][m] + minus;
-      if (!whole) {
-        const float2 a = apart(d);
-        d = two(uint32_t(lane + 2 * m / V * stride) * V < p.width ? a.x : 0.0f, uint32_t(lane + (2 * m + 1) / V * stride) * V < p.width ? a.y : 0.0f);
+    for (int m = 0; m < M; ++m) y[k][m] = y[k][m] + minus;
+  }
+  if (!at.full) {  // what is not there stays zero
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const float2 a = apart(y[k][m]);
+        y[k][m] = two(uint32_t(at.column(2 * m / V)) < width ? a.x : 0.0f, uint32_t(at.column((2 * m + 1) / V)) < width ? a.y : 0.0f);
       }
-      y[k][m] = d, s = s + d, q = fma2(d, d, q);
-    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Two s = y[k][0], q = y[k][0] * y[k][0];
+#pragma unroll
+    for (int m = 1; m < M; ++m) s = s + y[k][m], q = fma2(y[k][m], y[k][m], q);
     const float2 a = apart(s), b = apart(q);
-    const float2 t = row_sum<BLOCK>(make_float2(a.x + a.y, b.x + b.y), lanes, box, turn);
+    const float2 t = row_sum<S::LANES, S::BLOCK>(make_float2(a.x + a.y, b.x + b.y), box, turn);
     // what the sum's rounding left of the mean
     rest[k] = t.x * inverse;
-    rstd[k] = 1.0f / sqrtf(fmaxf(fmaf(-rest[k], rest[k], t.y * inverse), 0.0f) + p.eps);
+    rstd[k] = inverse_sqrt(fmaxf(fmaf(-rest[k], rest[k], t.y * inverse), 0.0f) + p.eps);
     if (t.y != t.y) rstd[k] = t.y;
-    const Two r = two(-rest[k], -rest[k]), f = two(rstd[k], rstd[k]);
-#pragma unroll
-    for (int m = 0; m < M; ++m) y[k][m] = (y[k][m] + r) * f;
   }
-  // one pair for all of a lane's rows at a time; 1 and 0 where there is no weight or bias
+  // one load of a weight for all of a lane's rows; 1 and 0 where there is none
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const uint32_t c = uint32_t(lane + i * stride) * V;
-    if (c >= p.width) continue;
+    const int c = at.column(i);
+    if (!at.full && uint32_t(c) >= width) continue;
     float w[V], b[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) w[e] = 1.0f, b[e] = 0.0f;
@@ -226,147 +272,161 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_forward_kernel(const _
     if (p.bias) fetch(b, static_cast<const W*>(p.bias) + c);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint32_t row = row0 + k * per;
+      const uint32_t row = row0 + k * S::PER;
       if (row >= p.rows) continue;
+      const float less = -rest[k] * rstd[k];
       float z[V];
       if constexpr (V == 1) {
         const float2 a = apart(y[k][i / 2]);
-        z[0] = fmaf(i % 2 ? a.y : a.x, w[0], b[0]);
+        z[0] = fmaf(fmaf(i % 2 ? a.y : a.x, rstd[k], less), w[0], b[0]);
       } else {
+        const Two f = two(rstd[k], rstd[k]), r = two(less, less);
 #pragma unroll
         for (int m = 0; m < V / 2; ++m) {
-          const float2 a = apart(fma2(y[k][i * V / 2 + m], two(w[2 * m], w[2 * m + 1]), two(b[2 * m], b[2 * m + 1])));
+          const float2 a = apart(fma2(fma2(y[k][i * V / 2 + m], f, r), two(w[2 * m], w[2 * m + 1]), two(b[2 * m], b[2 * m + 1])));
           z[2 * m] = a.x, z[2 * m + 1] = a.y;
         }
       }
       put(static_cast<T*>(p.y) + offset(p.at_y, row, p) + c, z);
     }
   }
-  if (p.saved && lane == 0) {
+  if (p.saved && (S::BLOCK ? threadIdx.x : threadIdx.x & (S::LANES - 1)) == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint32_t row = row0 + k * per;
+      const uint32_t row = row0 + k * S::PER;
       if (row < p.rows) p.saved[row] = mean[k], p.saved[uint64_t(p.rows) + row] = rest[k], p.saved[2 * uint64_t(p.rows) + row] = rstd[k];
     }
   }
 }
 
-// Rows from blockIdx.x on in steps of the grid; a thread's sums over its columns end in the block's line of the workspace.
-template <class T, class W, int V, int N, int K, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) norm_backward_kernel(const __grid_constant__ Norm p, const int lanes, const int lanes_log) {
-  constexpr int M = N * V / 2;
+// A row of x and dy, and what is known of it.
+template <class S>
+struct Fetched {
+  typename Raw<typename S::T, S::V>::type x[S::N], g[S::N];
+  float mean, rest, rstd;
+  __device__ __forceinline__ void fetch(const Norm& p, const S& at, uint32_t row) {
+    using T = typename S::T;
+    const bool here = row < p.rows;
+    const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, row, p) : 0) + at.first;
+    const T* grad = static_cast<const T*>(p.dy) + (here ? offset(p.at_dy, row, p) : 0) + at.first;
+#pragma unroll
+    for (int i = 0; i < S::N; ++i) {
+      x[i] = g[i] = typename Raw<T, S::V>::type{};
+      if (here && (at.full || uint32_t(at.column(i)) < p.width)) {
+        x[i] = fetch_raw<T, S::V>(from + i * S::LANES * S::V);
+        g[i] = fetch_raw<T, S::V>(grad + i * S::LANES * S::V);
+      }
+    }
+    mean = here ? p.saved[row] : 0.0f;
+    rest = here ? p.saved[uint64_t(p.rows) + row] : 0.0f;
+    rstd = here ? p.saved[2 * uint64_t(p.rows) + row] : 0.0f;
+  }
+};
+
+// Rows from blockIdx.x on in steps of the grid; a thread's sums over its columns end in the block's line of the workspace.  The next row is
+// on its way while one is worked on, where there are registers for it.
+template <class S>
+__device__ __forceinline__ void norm_backward(const Norm& p) {
+  using T = typename S::T;
+  using W = typename S::W;
+  constexpr int V = S::V, N = S::N, M = S::M;
+  constexpr bool AHEAD = N * V <= 8;
   __shared__ float2 box[2][32];
   extern __shared__ float side[];  // sums of the rows side by side
   int turn = 0;
-  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
-  const uint32_t per = BLOCK ? 1 : 256u >> lanes_log;
-  const int stride = BLOCK ? blockDim.x : lanes;
-  const uint32_t own = BLOCK ? 0 : threadIdx.x >> lanes_log;
+  const S at(p.width);
+  const uint32_t own = S::BLOCK ? 0 : threadIdx.x / S::LANES;
   const float inverse = 1.0f / float(p.width);
-  Two dw[M], db[M], w[M];
+  Two dw[M], db[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) dw[m] = db[m] = two(0.0f, 0.0f);
-  {
-    float v[N][V];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t c = uint32_t(lane + i * stride) * V;
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] = 1.0f;
-      if (p.weight && c < p.width) fetch(v[i], static_cast<const W*>(p.weight) + c);
-    }
-    const float* values = &v[0][0];
-#pragma unroll
-    for (int m = 0; m < M; ++m) w[m] = two(values[2 * m], values[2 * m + 1]);
-  }
-  for (uint64_t first = uint64_t(blockIdx.x) * (per * K); first < p.rows; first += uint64_t(gridDim.x) * (per * K)) {
-    Two x[K][M], g[K][M];
-    float mean[K], rest[K], rstd[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t row = uint32_t(first) + own + k * per;
-      const bool here = row < p.rows;
-      const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, row, p) : 0);
-      const T* grad = static_cast<const T*>(p.dy) + (here ? offset(p.at_dy, row, p) : 0);
+  Fetched<S> next;
+  if (AHEAD) next.fetch(p, at, blockIdx.x * S::PER + own);
+  for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER) {
+    const uint32_t row = uint32_t(first) + own;
+    if (!AHEAD) next.fetch(p, at, row);
+    Fetched<S> now = next;
+    const uint64_t ahead = first + uint64_t(gridDim.x) * S::PER;
+    if (AHEAD && ahead < p.rows) next.fetch(p, at, uint32_t(ahead) + own);
+    Two x[M], g[M];
+    {
       float a[N][V], b[N][V];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t c = uint32_t(lane + i * stride) * V;
-        if (here && c < p.width) {
-          fetch(a[i], from + c);
-          fetch(b[i], grad + c);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) a[i][e] = b[i][e] = 0.0f;
-        }
-      }
+      for (int i = 0; i < N; ++i) unpack(a[i], now.x[i]), unpack(b[i], now.g[i]);
       const float *va = &a[0][0], *vb = &b[0][0];
 #pragma unroll
-      for (int m = 0; m < M; ++m) x[k][m] = two(va[2 * m], va[2 * m + 1]), g[k][m] = two(vb[2 * m], vb[2 * m + 1]);
-      mean[k] = here ? p.saved[row] : 0.0f;
-      rest[k] = here ? p.saved[uint64_t(p.rows) + row] : 0.0f;
-      rstd[k] = here ? p.saved[2 * uint64_t(p.rows) + row] : 0.0f;
+      for (int m = 0; m < M; ++m) x[m] = two(va[2 * m], va[2 * m + 1]), g[m] = two(vb[2 * m], vb[2 * m + 1]);
     }
-    float2 s[K];
+    const float less = -now.rest * now.rstd;
+    const Two minus = two(-now.mean, -now.mean), r = two(less, less), f = two(now.rstd, now.rstd);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const Two minus = two(-mean[k], -mean[k]), r = two(-rest[k], -rest[k]), f = two(rstd[k], rstd[k]);
-      Two s0 = two(0.0f, 0.0f), s1 = s0;
-#pragma unroll
-      for (int m = 0; m < M; ++m) {  // (what is not there has no gradient: it adds nothing)
-        const Two hat = (x[k][m] + minus + r) * f, dy = g[k][m], dh = dy * w[m];
-        dw[m] = fma2(dy, hat, dw[m]), db[m] = db[m] + dy;
-        s0 = s0 + dh, s1 = fma2(dh, hat, s1);
-        x[k][m] = hat, g[k][m] = dh;
-      }
-      const float2 a = apart(s0), b = apart(s1);
-      s[k] = make_float2(a.x + a.y, b.x + b.y);
+    for (int m = 0; m < M; ++m) {  // (what is not there has no gradient: it adds nothing)
+      x[m] = fma2(x[m] + minus, f, r);
+      dw[m] = fma2(g[m], x[m], dw[m]), db[m] = db[m] + g[m];
     }
     if (!p.dx) continue;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t row = uint32_t(first) + own + k * per;
-      const float2 t = row_sum<BLOCK>(s[k], lanes, box, turn);
-      if (row >= p.rows) continue;
-      const Two m0 = two(-t.x * inverse, -t.x * inverse), m1 = two(-t.y * inverse, -t.y * inverse), f = two(rstd[k], rstd[k]);
-      T* to = static_cast<T*>(p.dx) + offset(p.at_dx, row, p);
-      float z[N][V];
-#pragma unroll
-      for (int m = 0; m < M; ++m) {
-        const float2 a = apart((g[k][m] + fma2(x[k][m], m1, m0)) * f);
-        (&z[0][0])[2 * m] = a.x, (&z[0][0])[2 * m + 1] = a.y;
-      }
+    if (p.weight) {
+      float w[N][V];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const uint32_t c = uint32_t(lane + i * stride) * V;
-        if (c < p.width) put(to + c, z[i]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[i][e] = 0.0f;
+        if (at.full || uint32_t(at.column(i)) < p.width) fetch(w[i], static_cast<const W*>(p.weight) + at.column(i));
       }
+      const float* values = &w[0][0];
+#pragma unroll
+      for (int m = 0; m < M; ++m) g[m] = g[m] * two(values[2 * m], values[2 * m + 1]);
     }
+    Two s0 = g[0], s1 = g[0] * x[0];
+#pragma unroll
+    for (int m = 1; m < M; ++m) s0 = s0 + g[m], s1 = fma2(g[m], x[m], s1);
+    const float2 a = apart(s0), b = apart(s1);
+    const float2 t = row_sum<S::LANES, S::BLOCK>(make_float2(a.x + a.y, b.x + b.y), box, turn);
+    if (row >= p.rows) continue;
+    const Two m0 = two(-t.x * inverse, -t.x * inverse), m1 = two(-t.y * inverse, -t.y * inverse);
+    T* to = static_cast<T*>(p.dx) + offset(p.at_dx, row, p) + at.first;
+    float z[N][V];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const float2 c = apart((g[m] + fma2(x[m], m1, m0)) * f);
+      (&z[0][0])[2 * m] = c.x, (&z[0][0])[2 * m + 1] = c.y;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at.full || uint32_t(at.column(i)) < p.width) put(to + i * S::LANES * V, z[i]);
   }
   if (!p.partial) return;
   float* line = p.partial + uint64_t(blockIdx.x) * 2 * p.width;
-  const int cols = lanes * N * V;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
-    if (!BLOCK) __syncthreads();
+    if (!S::BLOCK) __syncthreads();
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       const float2 a = apart(pass ? db[m] : dw[m]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t c = uint32_t(lane + (2 * m + h) / V * stride) * V + (2 * m + h) % V;
-        if (!BLOCK) side[own * cols + c] = h ? a.y : a.x;
+        const uint32_t c = uint32_t(at.column((2 * m + h) / V)) + (2 * m + h) % V;
+        if (!S::BLOCK) side[own * S::COLS + c] = h ? a.y : a.x;
         else if (c < p.width) line[pass * p.width + c] = h ? a.y : a.x;
       }
     }
-    if (BLOCK) continue;
+    if (S::BLOCK) continue;
     __syncthreads();
     for (uint32_t c = threadIdx.x; c < p.width; c += 256) {
       float sum = 0.0f;
-      for (uint32_t r = 0; r < per; ++r) sum += side[r * cols + c];
+      for (int r = 0; r < S::PER; ++r) sum += side[r * S::COLS + c];
       line[pass * p.width + c] = sum;
     }
   }
+}
+template <class S>
+__global__ void __launch_bounds__(256) norm_backward_kernel(const __grid_constant__ Norm p) {
+  norm_backward<S>(p);
+}
+// (104 registers, so that rows of 4096 values are two to an SM)
+template <class S>
+__global__ void __maxnreg__(104) norm_backward_block_kernel(const __grid_constant__ Norm p) {
+  norm_backward<S>(p);
 }
 
 // Rows too long for registers: one block a row, which is read three times forward (from L2 after the first).
@@ -380,15 +440,15 @@ __global__ void __launch_bounds__(1024) norm_wide_forward_kernel(const __grid_co
     T* to = static_cast<T*>(p.y) + offset(p.at_y, row, p);
     float2 s = make_float2(0.0f, 0.0f);
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) s.x += float(from[c]);
-    const float mean = row_sum<true>(s, 32, box, turn).x * inverse;
+    const float mean = row_sum<32, true>(s.x, box, turn) * inverse;
     s = make_float2(0.0f, 0.0f);
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) {
       const float d = float(from[c]) - mean;
       s.x += d, s.y = fmaf(d, d, s.y);
     }
-    s = row_sum<true>(s, 32, box, turn);
+    s = row_sum<32, true>(s, box, turn);
     const float rest = s.x * inverse;
-    float rstd = 1.0f / sqrtf(fmaxf(fmaf(-rest, rest, s.y * inverse), 0.0f) + p.eps);
+    float rstd = inverse_sqrt(fmaxf(fmaf(-rest, rest, s.y * inverse), 0.0f) + p.eps);
     if (s.y != s.y) rstd = s.y;
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) {
       float y[1] = {(float(from[c]) - mean - rest) * rstd};
@@ -419,7 +479,7 @@ __global__ void __launch_bounds__(1024) norm_wide_backward_kernel(const __grid_c
       if (line) line[c] = fmaf(dy, hat, line[c]), line[p.width + c] += dy;
     }
     if (!p.dx) continue;
-    s = row_sum<true>(s, 32, box, turn);
+    s = row_sum<32, true>(s, box, turn);
     const float m0 = s.x * inverse, m1 = s.y * inverse;
     T* to = static_cast<T*>(p.dx) + offset(p.at_dx, row, p);
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) {
@@ -473,20 +533,15 @@ RowsAt rows_at(const ZenoTensor& t, const ZenoLayerNorm& p) {
   return a;
 }
 
-// Up to 16 values a lane (backward holds four of each: x, dy and the two sums).  Short rows, a part of a warp each, are
-// taken several at a time, so that enough loads are under way.
+// Up to 16 values a lane (backward holds x, dy and the two sums of each).
 constexpr int kValues = 16;
-constexpr int rows_at_once(int values, bool block, bool backward) {
-  return block ? 1 : (values <= 8 ? 4 : 2) / (backward ? 2 : 1);
-}
 
 struct Choice {
   bool vec, block;
   int lanes;    // of a row (a power of two); threads where a block takes one
-  int lanes_log;
   int vectors;  // of a lane, as one of the instances
-  int values() const { return vec ? vectors * width : vectors; }
   int width;    // values of a vector
+  int values() const { return vectors * width; }
 };
 
 bool vec_ok(const void* data, const ZenoTensor& t, size_t item) {
@@ -502,46 +557,59 @@ Choice choose(const ZenoLayerNorm& p, bool vec) {
   c.width = vec ? int(16 / item_of(p.dtype)) : 1;
   const uint32_t v = uint32_t(c.width), pieces = (p.width + v - 1) / v, most = kValues / v;
   if (pieces <= 32 * most) {
-    c.lanes = 1;
-    while (uint32_t(c.lanes) < pieces && c.lanes < 32) c.lanes *= 2;
-    // scalars: two of a lane, so that a warp takes several short rows
-    if (!vec && c.lanes > 4 && pieces <= uint32_t(c.lanes)) c.lanes /= 2;
-    while (1 << c.lanes_log < c.lanes) ++c.lanes_log;
+    // lanes of one vector, or of two values, each; longer rows take a warp
+    const uint32_t least = vec ? 1 : 2;
+    c.lanes = vec ? 1 : 4;
+    while (uint32_t(c.lanes) * least < pieces && c.lanes < 32) c.lanes *= 2;
     const uint32_t n = (pieces + c.lanes - 1) / c.lanes;
     c.vectors = vec ? (n <= 1 ? 1 : n <= 2 ? 2 : 4) : (n <= 2 ? 2 : n <= 8 ? 8 : 16);
     return c;
   }
   c.block = true;
-  c.lanes = int(std::max(((pieces + most - 1) / most + 31) / 32 * 32, 64u));
+  c.lanes = int((pieces + 32 * most - 1) / (32 * most) * 32);
   c.vectors = int(most);
   return c;
 }
 
-template <class T, class W, int V, int N, bool BLOCK>
+template <class S>
 cudaError_t run(const Norm& p, const Choice& c, bool backward, unsigned blocks, cudaStream_t stream) {
-  const int threads = BLOCK ? c.lanes : 256;
+  const int threads = S::BLOCK ? c.lanes : 256;
   if (!backward) {
-    norm_forward_kernel<T, W, V, N, rows_at_once(V * N, BLOCK, false), BLOCK><<<blocks, threads, 0, stream>>>(p, c.lanes, c.lanes_log);
+    norm_forward_kernel<S><<<blocks, threads, 0, stream>>>(p);
+  } else if constexpr (S::BLOCK) {
+    norm_backward_block_kernel<S><<<blocks, threads, 0, stream>>>(p);
   } else {
-    const size_t side = BLOCK || !p.partial ? 0 : size_t(256) * N * V * 4;
-    norm_backward_kernel<T, W, V, N, rows_at_once(V * N, BLOCK, true), BLOCK><<<blocks, threads, side, stream>>>(p, c.lanes, c.lanes_log);
+    norm_backward_kernel<S><<<blocks, threads, p.partial ? size_t(256) * S::N * S::V * 4 : 0, stream>>>(p);
   }
   return cudaGetLastError();
 }
 
 template <class T, class W>
 cudaError_t by_values(const Norm& p, const Choice& c, bool backward, unsigned blocks, cudaStream_t stream) {
-  constexpr int V = 16 / int(sizeof(T));
-  if (c.block) return c.vec ? run<T, W, V, kValues / V, true>(p, c, backward, blocks, stream) : run<T, W, 1, kValues, true>(p, c, backward, blocks, stream);
+  constexpr int V = 16 / int(sizeof(T)), MOST = kValues / V;
+  if (c.block)
+    return c.vec ? run<Shape<T, W, V, MOST, 32, true>>(p, c, backward, blocks, stream) : run<Shape<T, W, 1, kValues, 32, true>>(p, c, backward, blocks, stream);
   if (c.vec) {
-    if (c.vectors == 1) return run<T, W, V, 1, false>(p, c, backward, blocks, stream);
+    if (c.vectors == 1) switch (c.lanes) {
+        case 1: return run<Shape<T, W, V, 1, 1, false>>(p, c, backward, blocks, stream);
+        case 2: return run<Shape<T, W, V, 1, 2, false>>(p, c, backward, blocks, stream);
+        case 4: return run<Shape<T, W, V, 1, 4, false>>(p, c, backward, blocks, stream);
+        case 8: return run<Shape<T, W, V, 1, 8, false>>(p, c, backward, blocks, stream);
+        case 16: return run<Shape<T, W, V, 1, 16, false>>(p, c, backward, blocks, stream);
+        default: return run<Shape<T, W, V, 1, 32, false>>(p, c, backward, blocks, stream);
+      }
     if constexpr (V == 4)
-      if (c.vectors == 2) return run<T, W, V, 2, false>(p, c, backward, blocks, stream);
-    return run<T, W, V, kValues / V, false>(p, c, backward, blocks, stream);
+      if (c.vectors == 2) return run<Shape<T, W, V, 2, 32, false>>(p, c, backward, blocks, stream);
+    return run<Shape<T, W, V, MOST, 32, false>>(p, c, backward, blocks, stream);
   }
-  if (c.vectors == 2) return run<T, W, 1, 2, false>(p, c, backward, blocks, stream);
-  if (c.vectors == 8) return run<T, W, 1, 8, false>(p, c, backward, blocks, stream);
-  return run<T, W, 1, 16, false>(p, c, backward, blocks, stream);
+  if (c.vectors == 2) switch (c.lanes) {
+      case 4: return run<Shape<T, W, 1, 2, 4, false>>(p, c, backward, blocks, stream);
+      case 8: return run<Shape<T, W, 1, 2, 8, false>>(p, c, backward, blocks, stream);
+      case 16: return run<Shape<T, W, 1, 2, 16, false>>(p, c, backward, blocks, stream);
+      default: return run<Shape<T, W, 1, 2, 32, false>>(p, c, backward, blocks, stream);
+    }
+  if (c.vectors == 8) return run<Shape<T, W, 1, 8, 32, false>>(p, c, backward, blocks, stream);
+  return run<Shape<T, W, 1, 16, 32, false>>(p, c, backward, blocks, stream);
 }
 
 Norm norm_of(const ZenoLayerNorm& p) {
@@ -567,7 +635,7 @@ bool is_vec(const ZenoLayerNorm& p, const ZenoTensor& out) {
 unsigned backward_blocks(const ZenoLayerNorm& p, uint32_t rows, bool vec) {
   if (p.width > kWide) return unsigned(std::min<uint32_t>(rows, kSms));
   const Choice c = choose(p, vec);
-  const uint64_t per = c.block ? 1 : uint64_t(256 / c.lanes) * rows_at_once(c.values(), c.block, true);
+  const uint64_t per = c.block ? 1 : uint64_t(256 / c.lanes);
   const uint64_t threads = c.block ? uint64_t(c.lanes) : 256;
   return unsigned(std::min<uint64_t>((rows + per - 1) / per, uint64_t(kSms) * std::max<uint64_t>(1, 1024 / threads)));
 }
@@ -581,7 +649,7 @@ cudaError_t forward(const ZenoLayerNorm& p, cudaStream_t stream) {
   }
   const bool vec = is_vec(p, p.out);
   const Choice c = choose(p, vec);
-  const uint64_t per = c.block ? 1 : uint64_t(256 / c.lanes) * rows_at_once(c.values(), c.block, false);
+  const uint64_t per = c.block ? 1 : uint64_t(256 / c.lanes) * (c.values() <= 8 ? 4 : 2);  // Shape's PER K
   return by_values<T, W>(n, c, false, unsigned((n.rows + per - 1) / per), stream);
 }
 
