@@ -173,7 +173,7 @@ __device__ __forceinline__ float2 row_sum(float2 s, float2 (*box)[32], int& turn
 }
 
 // A row belongs to LANES lanes, or with BLOCK to all warps of a block, 32 N V neighbouring values to each.  A lane has N vectors of V
-// values, LANES V apart; K rows at once.
+// values, LANES V apart.
 template <class T_, class W_, int V_, int N_, int LANES_, bool BLOCK_>
 struct Shape {
   using T = T_;
@@ -181,8 +181,7 @@ struct Shape {
   static constexpr int V = V_, N = N_, LANES = LANES_, M = N * V / 2;  // M: pairs of values of a lane
   static constexpr bool BLOCK = BLOCK_;
   static constexpr int PER = BLOCK ? 1 : 256 / LANES;  // rows side by side in a block
-  // short rows several at a time, so that enough loads are under way; backward fetches ahead instead
-  static constexpr int K = BLOCK ? 1 : N * V <= 8 ? 4 : 2;
+  static constexpr bool AHEAD = N * V <= 8;
   static constexpr int COLS = LANES * N * V;  // columns that there is room for (BLOCK: for each warp)
   int first;   // first column
   bool full;   // no column of this row (this warp) is past the width
@@ -194,108 +193,100 @@ struct Shape {
   __device__ __forceinline__ int column(int i) const { return first + i * LANES * V; }
 };
 
+// Rows from blockIdx.x on in steps of the grid; the next one is on its way while one is worked on.  Where a lane has 16 values
+// there are more blocks instead (of 4099 values: 25 us against 28).
 template <class S>
 __global__ void __launch_bounds__(S::BLOCK ? 512 : 256) norm_forward_kernel(const __grid_constant__ Norm p) {
   using T = typename S::T;
   using W = typename S::W;
-  constexpr int V = S::V, N = S::N, M = S::M, K = S::K;
+  constexpr int V = S::V, N = S::N, M = S::M;
+  constexpr bool AHEAD = S::AHEAD, HELD = AHEAD;  // weight and bias stay in registers
   __shared__ float2 box[2][32];
   int turn = 0;
   const S at(p.width);
-  const uint32_t width = p.width;
-  const uint32_t row0 = blockIdx.x * (S::PER * K) + (S::BLOCK ? 0 : threadIdx.x / S::LANES);
-  typename Raw<T, V>::type raw[K][N];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const uint32_t row = row0 + k * S::PER;
+  const uint32_t own = S::BLOCK ? 0 : threadIdx.x / S::LANES;
+  typename Raw<T, V>::type raw[N];
+  auto fetch_row = [&](uint32_t row) {
     const bool here = row < p.rows;
     const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, row, p) : 0) + at.first;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      raw[k][i] = typename Raw<T, V>::type{};
-      if (here && (at.full || uint32_t(at.column(i)) < width)) raw[k][i] = fetch_raw<T, V>(from + i * S::LANES * V);
+      raw[i] = typename Raw<T, V>::type{};
+      if (here && (at.full || uint32_t(at.column(i)) < p.width)) raw[i] = fetch_raw<T, V>(from + i * S::LANES * V);
     }
+  };
+  if (AHEAD) fetch_row(blockIdx.x * S::PER + own);
+  float w[N][V], b[N][V];
+  auto fetch_affine = [&](int i) {  // 1 and 0 where there is none
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[i][e] = 1.0f, b[i][e] = 0.0f;
+    if (!at.full && uint32_t(at.column(i)) >= p.width) return;
+    if (p.weight) fetch(w[i], static_cast<const W*>(p.weight) + at.column(i));
+    if (p.bias) fetch(b[i], static_cast<const W*>(p.bias) + at.column(i));
+  };
+  if (HELD) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) fetch_affine(i);
   }
-  const float inverse = 1.0f / float(width);
-  float mean[K], rest[K], rstd[K];
-  Two y[K][M];
+  const float inverse = 1.0f / float(p.width);
+  for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER) {
+    const uint32_t row = uint32_t(first) + own;
+    if (!AHEAD) fetch_row(row);
+    Two y[M];
+    {
+      float x[N][V];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float x[N][V];
+      for (int i = 0; i < N; ++i) unpack(x[i], raw[i]);
+      const float* values = &x[0][0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) unpack(x[i], raw[k][i]);
-    const float* values = &x[0][0];
+      for (int m = 0; m < M; ++m) y[m] = two(values[2 * m], values[2 * m + 1]);
+    }
+    const uint64_t ahead = first + uint64_t(gridDim.x) * S::PER;
+    if (AHEAD && ahead < p.rows) fetch_row(uint32_t(ahead) + own);
+    Two s = y[0];
 #pragma unroll
-    for (int m = 0; m < M; ++m) y[k][m] = two(values[2 * m], values[2 * m + 1]);
-    Two s = y[k][0];
-#pragma unroll
-    for (int m = 1; m < M; ++m) s = s + y[k][m];
+    for (int m = 1; m < M; ++m) s = s + y[m];
     const float2 t = apart(s);
-    mean[k] = row_sum<S::LANES, S::BLOCK>(t.x + t.y, box, turn) * inverse;
-  }
+    const float mean = row_sum<S::LANES, S::BLOCK>(t.x + t.y, box, turn) * inverse;
+    const Two minus = two(-mean, -mean);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const Two minus = two(-mean[k], -mean[k]);
-#pragma unroll
-    for (int m = 0; m < M; ++m) y[k][m] = y[k][m] + minus;
-  }
-  if (!at.full) {  // what is not there stays zero
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int m = 0; m < M; ++m) y[m] = y[m] + minus;
+    if (!at.full) {  // what is not there stays zero
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        const float2 a = apart(y[k][m]);
-        y[k][m] = two(uint32_t(at.column(2 * m / V)) < width ? a.x : 0.0f, uint32_t(at.column((2 * m + 1) / V)) < width ? a.y : 0.0f);
+        const float2 a = apart(y[m]);
+        y[m] = two(uint32_t(at.column(2 * m / V)) < p.width ? a.x : 0.0f, uint32_t(at.column((2 * m + 1) / V)) < p.width ? a.y : 0.0f);
       }
-  }
+    }
+    s = y[0];
+    Two q = y[0] * y[0];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    Two s = y[k][0], q = y[k][0] * y[k][0];
-#pragma unroll
-    for (int m = 1; m < M; ++m) s = s + y[k][m], q = fma2(y[k][m], y[k][m], q);
-    const float2 a = apart(s), b = apart(q);
-    const float2 t = row_sum<S::LANES, S::BLOCK>(make_float2(a.x + a.y, b.x + b.y), box, turn);
+    for (int m = 1; m < M; ++m) s = s + y[m], q = fma2(y[m], y[m], q);
+    const float2 c = apart(s), d = apart(q);
+    const float2 sums = row_sum<S::LANES, S::BLOCK>(make_float2(c.x + c.y, d.x + d.y), box, turn);
     // what the sum's rounding left of the mean
-    rest[k] = t.x * inverse;
-    rstd[k] = inverse_sqrt(fmaxf(fmaf(-rest[k], rest[k], t.y * inverse), 0.0f) + p.eps);
-    if (t.y != t.y) rstd[k] = t.y;
-  }
-  // one load of a weight for all of a lane's rows; 1 and 0 where there is none
+    const float rest = sums.x * inverse;
+    float rstd = inverse_sqrt(fmaxf(fmaf(-rest, rest, sums.y * inverse), 0.0f) + p.eps);
+    if (sums.y != sums.y) rstd = sums.y;
+    if (row >= p.rows) continue;
+    const float less = -rest * rstd;
+    const Two f = two(rstd, rstd), r = two(less, less);
+    T* to = static_cast<T*>(p.y) + offset(p.at_y, row, p) + at.first;
+    float z[N][V];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = at.column(i);
-    if (!at.full && uint32_t(c) >= width) continue;
-    float w[V], b[V];
+    for (int i = 0; i < N; ++i)
+      if (!HELD) fetch_affine(i);
 #pragma unroll
-    for (int e = 0; e < V; ++e) w[e] = 1.0f, b[e] = 0.0f;
-    if (p.weight) fetch(w, static_cast<const W*>(p.weight) + c);
-    if (p.bias) fetch(b, static_cast<const W*>(p.bias) + c);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t row = row0 + k * S::PER;
-      if (row >= p.rows) continue;
-      const float less = -rest[k] * rstd[k];
-      float z[V];
-      if constexpr (V == 1) {
-        const float2 a = apart(y[k][i / 2]);
-        z[0] = fmaf(fmaf(i % 2 ? a.y : a.x, rstd[k], less), w[0], b[0]);
-      } else {
-        const Two f = two(rstd[k], rstd[k]), r = two(less, less);
-#pragma unroll
-        for (int m = 0; m < V / 2; ++m) {
-          const float2 a = apart(fma2(fma2(y[k][i * V / 2 + m], f, r), two(w[2 * m], w[2 * m + 1]), two(b[2 * m], b[2 * m + 1])));
-          z[2 * m] = a.x, z[2 * m + 1] = a.y;
-        }
-      }
-      put(static_cast<T*>(p.y) + offset(p.at_y, row, p) + c, z);
+    for (int m = 0; m < M; ++m) {
+      const float *vw = &w[0][0] + 2 * m, *vb = &b[0][0] + 2 * m;
+      const float2 a = apart(fma2(fma2(y[m], f, r), two(vw[0], vw[1]), two(vb[0], vb[1])));
+      (&z[0][0])[2 * m] = a.x, (&z[0][0])[2 * m + 1] = a.y;
     }
-  }
-  if (p.saved && (S::BLOCK ? threadIdx.x : threadIdx.x & (S::LANES - 1)) == 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t row = row0 + k * S::PER;
-      if (row < p.rows) p.saved[row] = mean[k], p.saved[uint64_t(p.rows) + row] = rest[k], p.saved[2 * uint64_t(p.rows) + row] = rstd[k];
-    }
+    for (int i = 0; i < N; ++i)
+      if (at.full || uint32_t(at.column(i)) < p.width) put(to + i * S::LANES * V, z[i]);
+    if (p.saved && (S::BLOCK ? threadIdx.x : threadIdx.x & (S::LANES - 1)) == 0)
+      p.saved[row] = mean, p.saved[uint64_t(p.rows) + row] = rest, p.saved[2 * uint64_t(p.rows) + row] = rstd;
   }
 }
 
@@ -330,7 +321,7 @@ __device__ __forceinline__ void norm_backward(const Norm& p) {
   using T = typename S::T;
   using W = typename S::W;
   constexpr int V = S::V, N = S::N, M = S::M;
-  constexpr bool AHEAD = N * V <= 8;
+  constexpr bool AHEAD = S::AHEAD;
   __shared__ float2 box[2][32];
   extern __shared__ float side[];  // sums of the rows side by side
   int turn = 0;
@@ -631,14 +622,14 @@ bool is_vec(const ZenoLayerNorm& p, const ZenoTensor& out) {
   return p.width % (16 / item) == 0 && vec_ok(p.x.data, p.x, item) && vec_ok(out.data, out, item) && affine_ok(p);
 }
 
-// Blocks of the backward pass: enough to fill the GPU, and no more lines of sums than the rows are worth.
-unsigned backward_blocks(const ZenoLayerNorm& p, uint32_t rows, bool vec) {
+// Blocks that share the rows: enough to fill the GPU, and backward no more lines of sums than that.
+unsigned blocks_of(const ZenoLayerNorm& p, uint32_t rows, bool vec, uint32_t threads_of_sm) {
   if (p.width > kWide) return unsigned(std::min<uint32_t>(rows, kSms));
   const Choice c = choose(p, vec);
-  const uint64_t per = c.block ? 1 : uint64_t(256 / c.lanes);
-  const uint64_t threads = c.block ? uint64_t(c.lanes) : 256;
-  return unsigned(std::min<uint64_t>((rows + per - 1) / per, uint64_t(kSms) * std::max<uint64_t>(1, 1024 / threads)));
+  const uint32_t per = c.block ? 1 : 256 / c.lanes, threads = c.block ? c.lanes : 256;
+  return unsigned(std::min<uint64_t>((uint64_t(rows) + per - 1) / per, uint64_t(kSms) * std::max<uint32_t>(1, threads_of_sm / threads)));
 }
+unsigned backward_blocks(const ZenoLayerNorm& p, uint32_t rows, bool vec) { return blocks_of(p, rows, vec, 1024); }
 
 template <class T, class W>
 cudaError_t forward(const ZenoLayerNorm& p, cudaStream_t stream) {
@@ -648,9 +639,7 @@ cudaError_t forward(const ZenoLayerNorm& p, cudaStream_t stream) {
     return cudaGetLastError();
   }
   const bool vec = is_vec(p, p.out);
-  const Choice c = choose(p, vec);
-  const uint64_t per = c.block ? 1 : uint64_t(256 / c.lanes) * (c.values() <= 8 ? 4 : 2);  // Shape's PER K
-  return by_values<T, W>(n, c, false, unsigned((n.rows + per - 1) / per), stream);
+  return by_values<T, W>(n, choose(p, vec), false, blocks_of(p, n.rows, vec, choose(p, vec).values() <= 8 ? 1280 : UINT32_MAX), stream);
 }
 
 template <class T, class W>
