@@ -51,8 +51,8 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
     if (e != cudaSuccess) return e;
     if (l.shared) {
       const uint32_t group = p.value_heads / p.key_heads;
-      e = launch_linear_shared(LinearShared{extra.shared_q, d.d_q, p.tokens, p.key_heads, group, p.key_dim}, p.batch, p.dtype, stream);
-      if (e == cudaSuccess) e = launch_linear_shared(LinearShared{extra.shared_k, d.d_k, p.tokens, p.key_heads, group, p.key_dim}, p.batch, p.dtype, stream);
+      e = launch_linear_shared(LinearShared{extra.shared_q, d.d_q, p.tokens, p.key_heads, group, p.key_dim},
+                               LinearShared{extra.shared_k, d.d_k, p.tokens, p.key_heads, group, p.key_dim}, p.batch, p.dtype, stream);
       if (e != cudaSuccess) return e;
     }
     return d.d_decay ? launch_linear_decay(extra.decay, uint64_t(p.batch) * c.count, p.value_heads, d.d_decay, stream) : cudaSuccess;

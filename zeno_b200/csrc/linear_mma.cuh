@@ -58,6 +58,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // d = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // Fragments of a 16 x 16 operand in shared memory, as in delta_mma.cuh.  TR: stored with the contracted axis first.
 template <bool TR>
 __device__ __forceinline__ void frag_a(uint32_t (&r)[4], const plane_t* at, int pitch, int lane) {
@@ -122,16 +128,23 @@ __device__ __forceinline__ float2 values(const plane_t* at, int plane) {
 
 // One 16-wide step: d += the products of the first limbs, low += the other terms above 2^-24 of the largest, smallest
 // first.  The instructions' sums truncate at 2^-23 of what they hold, which is 2^-8 less for `low`.
-template <int LA, int LB>
+template <int LA, int LB, bool FIRST = false>
 __device__ __forceinline__ void mma_terms(float (&d)[2][4], float (&low)[2][4], const uint32_t (&a)[LA][4], const uint32_t (&b)[LB][4]) {
+  bool begun = !FIRST;
 #pragma unroll
   for (int s = 2; s >= 0; --s)
 #pragma unroll
     for (int l = 0; l < LA; ++l)
       if (s - l >= 0 && s - l < LB) {
         float(&to)[2][4] = s ? low : d;
-        mma(to[0], a[l], b[s - l][0], b[s - l][1]);
-        mma(to[1], a[l], b[s - l][2], b[s - l][3]);
+        if (begun && !(FIRST && s == 0)) {
+          mma(to[0], a[l], b[s - l][0], b[s - l][1]);
+          mma(to[1], a[l], b[s - l][2], b[s - l][3]);
+        } else {
+          mma_first(to[0], a[l], b[s - l][0], b[s - l][1]);
+          mma_first(to[1], a[l], b[s - l][2], b[s - l][3]);
+        }
+        begun = true;
       }
 }
 
@@ -366,19 +379,28 @@ struct Part {
 };
 
 // A lane's elements of a part are pairs of neighbouring columns: (j, h, r) is at row 8 r and column 16 j + 8 h of its first.
-// f(j, h, r, offset into the state of row length dv) over the pairs that exist.
-template <class S, class F>
-__device__ __forceinline__ void each_pair(const Part<S>& part, int dk, int dv, int lane, F&& f) {
+// f(j, h, r, at, second) over the pairs that exist; `second`: so does the second of the pair.
+template <class S, class P, class F>
+__device__ __forceinline__ void each_pair(P* state, const Part<S>& part, int dk, int dv, int lane, F&& f) {
   const int row = part.row + (lane >> 2), col = part.col + (lane & 3) * 2;
+  P* const at[2] = {state + row * dv + col, state + (row + 8) * dv + col};
+  if (part.row + 16 <= dk && part.col + S::NM * 16 <= dv) {  // all of it
+#pragma unroll
+    for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) f(j, h, r, at[r] + (j * 16 + h * 8), true);
+    return;
+  }
   const int left[2] = {row < dk ? dv - col : 0, row + 8 < dk ? dv - col : 0};
-  const int at[2] = {row * dv + col, (row + 8) * dv + col};
 #pragma unroll
   for (int j = 0; j < S::NM; ++j)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        if (j * 16 + h * 8 < left[r]) f(j, h, r, at[r] + j * 16 + h * 8);
+        if (j * 16 + h * 8 < left[r]) f(j, h, r, at[r] + (j * 16 + h * 8), j * 16 + h * 8 + 1 < left[r]);
 }
 
 template <class S>
@@ -404,28 +426,26 @@ template <class S>
 __device__ __forceinline__ void read_state(float (&m)[S::NM][2][4], const float* from, const Part<S>& part, int dk, int dv, int lane) {
   clear<S>(m);
   if (pairs_aligned(from, dv)) {
-    each_pair<S>(part, dk, dv, lane, [&](int j, int h, int r, int at) {
-      const float2 v = *reinterpret_cast<const float2*>(from + at);
+    each_pair<S>(from, part, dk, dv, lane, [&](int j, int h, int r, const float* at, bool) {
+      const float2 v = *reinterpret_cast<const float2*>(at);
       m[j][h][2 * r] = v.x, m[j][h][2 * r + 1] = v.y;
     });
   } else {
-    const int left = dv - 1 - part.col - (lane & 3) * 2;  // of the second of a pair
-    each_pair<S>(part, dk, dv, lane, [&](int j, int h, int r, int at) {
-      m[j][h][2 * r] = from[at];
-      if (j * 16 + h * 8 < left) m[j][h][2 * r + 1] = from[at + 1];
+    each_pair<S>(from, part, dk, dv, lane, [&](int j, int h, int r, const float* at, bool second) {
+      m[j][h][2 * r] = at[0];
+      if (second) m[j][h][2 * r + 1] = at[1];
     });
   }
 }
 template <class S>
 __device__ __forceinline__ void write_state(const float (&m)[S::NM][2][4], float* to, const Part<S>& part, int dk, int dv, int lane) {
   if (pairs_aligned(to, dv)) {
-    each_pair<S>(part, dk, dv, lane,
-                 [&](int j, int h, int r, int at) { *reinterpret_cast<float2*>(to + at) = make_float2(m[j][h][2 * r], m[j][h][2 * r + 1]); });
+    each_pair<S>(to, part, dk, dv, lane,
+                 [&](int j, int h, int r, float* at, bool) { *reinterpret_cast<float2*>(at) = make_float2(m[j][h][2 * r], m[j][h][2 * r + 1]); });
   } else {
-    const int left = dv - 1 - part.col - (lane & 3) * 2;
-    each_pair<S>(part, dk, dv, lane, [&](int j, int h, int r, int at) {
-      to[at] = m[j][h][2 * r];
-      if (j * 16 + h * 8 < left) to[at + 1] = m[j][h][2 * r + 1];
+    each_pair<S>(to, part, dk, dv, lane, [&](int j, int h, int r, float* at, bool second) {
+      at[0] = m[j][h][2 * r];
+      if (second) at[1] = m[j][h][2 * r + 1];
     });
   }
 }
@@ -479,14 +499,15 @@ __device__ __forceinline__ void update(float (&m)[S::NM][2][4], const plane_t* x
 #pragma unroll
     for (int j = 0; j < S::NM; ++j) {
       if (j >= part.pairs) break;
-      float acc[2][4] = {}, low[2][4] = {};
+      float acc[2][4], low[2][4];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        if (half + kk >= nt) break;
+        if (kk && half + kk >= nt) break;
         uint32_t b[S::L][4];
 #pragma unroll
         for (int l = 0; l < S::L; ++l) frag_b<true>(b[l], y + l * S::PLANE + (half + kk) * 16 * S::P + part.col + j * 16, S::P, lane);
-        mma_terms<3, S::L>(acc, low, a[kk], b);
+        if (kk) mma_terms<3, S::L>(acc, low, a[kk], b);
+        else mma_terms<3, S::L, true>(acc, low, a[kk], b);
       }
       const float k = half ? 1.0f : keep;
 #pragma unroll

@@ -33,18 +33,33 @@ __device__ __forceinline__ float rounded<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-template <class T>
-__global__ void __launch_bounds__(256) linear_shared_kernel(const LinearShared s, const uint64_t total) {
-  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
-    const uint32_t c = uint32_t(i % s.width);
-    const uint64_t rest = i / s.width;
-    const uint32_t kh = uint32_t(rest % s.key_heads);
-    const uint64_t token = rest / s.key_heads;  // batch and token
-    const uint64_t b = token / s.tokens, t = token % s.tokens;
-    const float* from = s.from + (token * s.key_heads * s.group + uint64_t(kh) * s.group) * s.width + c;
-    float sum = from[0];
-    for (uint32_t g = 1; g < s.group; ++g) sum += from[g * s.width];
-    static_cast<T*>(s.to.data)[int64_t(b) * s.to.stride[0] + int64_t(t) * s.to.stride[1] + int64_t(kh) * s.to.stride[2] + c] = rounded<T>(sum);
+// blockIdx.y is the environment, blockIdx.z the gradient; a thread takes V neighbouring channels of a token's key head.
+struct SharedPair {
+  LinearShared of[2];
+  uint32_t batch, turn;  // turn: tokens of a block
+};
+template <class T, int V>
+__global__ void __launch_bounds__(256) linear_shared_kernel(const SharedPair pair) {
+  const LinearShared s = blockIdx.z ? pair.of[1] : pair.of[0];
+  const uint32_t pieces = s.width / V, row = pieces * s.key_heads;
+  for (uint32_t j = threadIdx.x; j < pair.turn * row; j += 256) {
+    const uint32_t t = blockIdx.x * pair.turn + j / row, kh = j % row / pieces, c = j % pieces * V;
+    if (t >= s.tokens) return;
+    for (uint32_t b = blockIdx.y; b < pair.batch; b += gridDim.y) {
+      const float* from = s.from + ((uint64_t(b) * s.tokens + t) * (s.key_heads * s.group) + kh * s.group) * s.width + c;
+      T* to = static_cast<T*>(s.to.data) + int64_t(b) * s.to.stride[0] + int64_t(t) * s.to.stride[1] + int64_t(kh) * s.to.stride[2] + c;
+      float sum[V] = {};
+      for (uint32_t g = 0; g < s.group; ++g) {
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(from + uint64_t(g) * s.width);
+          sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
+        } else {
+          sum[0] += from[uint64_t(g) * s.width];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) to[e] = rounded<T>(sum[e]);
+    }
   }
 }
 
@@ -74,13 +89,19 @@ cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t 
   return cudaGetLastError();
 }
 
-cudaError_t launch_linear_shared(const LinearShared& s, uint32_t batch, uint32_t dtype, cudaStream_t stream) {
-  const uint64_t total = uint64_t(batch) * s.tokens * s.key_heads * s.width;
-  const uint64_t blocks = (total + 1023) / 1024;
-  const unsigned grid = unsigned(blocks < 16 * kSms ? blocks : 16 * kSms);
-  if (!grid) return cudaSuccess;
-  if (dtype == ZENO_DTYPE_BF16) linear_shared_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(s, total);
-  else linear_shared_kernel<float><<<grid, 256, 0, stream>>>(s, total);
+cudaError_t launch_linear_shared(const LinearShared& q, const LinearShared& k, uint32_t batch, uint32_t dtype, cudaStream_t stream) {
+  if (!batch || !q.tokens) return cudaSuccess;
+  const bool four = q.width % 4 == 0;
+  const uint32_t row = q.key_heads * (four ? q.width / 4 : q.width), turn = row < 1024 ? 1024 / row : 1;
+  const SharedPair pair{{q, k}, batch, turn};
+  const dim3 grid((q.tokens + turn - 1) / turn, batch < 65535 ? batch : 65535, 2);
+  if (dtype == ZENO_DTYPE_BF16) {
+    if (four) linear_shared_kernel<__nv_bfloat16, 4><<<grid, 256, 0, stream>>>(pair);
+    else linear_shared_kernel<__nv_bfloat16, 1><<<grid, 256, 0, stream>>>(pair);
+  } else {
+    if (four) linear_shared_kernel<float, 4><<<grid, 256, 0, stream>>>(pair);
+    else linear_shared_kernel<float, 1><<<grid, 256, 0, stream>>>(pair);
+  }
   return cudaGetLastError();
 }
 
