@@ -115,11 +115,23 @@ def test_many_environments_of_several_chunks(dtype):
     check_all(x, torch.randn(500, 70, 2, 48, device=DEV).to(dtype))
 
 
+@pytest.mark.parametrize("dk,dv", [(64, 64), (1, 1), (7, 13), (16, 32), (32, 32), (40, 24), (33, 64), (64, 9), (128, 64)])
+@pytest.mark.parametrize("T", [1, 2, 7, 15, 16, 17, 31, 32])
+def test_short_rollouts_of_many_environments(T, dk, dv):
+    """A warp a head."""
+    for i, (Hk, H, fixed, reset, initial, d_final) in enumerate([(1, 1, True, None, False, False), (2, 2, False, 0.1, True, False),
+                                                                (1, 3, True, 0.2, True, False), (1, 2, False, None, False, True)]):
+        B = (700, 311, 200, 300)[i]
+        x = inputs(B, T, Hk, H, dk, dv, torch.bfloat16, seed=T + i, fixed=fixed, reset=reset, initial=initial)
+        check_all(x, torch.randn(B, T, H, dv, device=DEV).bfloat16(), torch.randn(B, H, dk, dv, device=DEV) if d_final else None)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_strides(dtype):
+@pytest.mark.parametrize("B", [5, 350])
+def test_strides(B, dtype):
     """Time-major buffers, heads out of a packed projection, rows that are not 16-byte aligned, a last axis that is not
     contiguous: the same results as of contiguous copies, bit for bit."""
-    B, T, H, d = 5, 40, 2, 48
+    T, H, d = 40 if B == 5 else 20, 2, 48
     base = inputs(B, T, H, H, d, d, dtype)
     d_out = torch.randn(B, T, H, d, device=DEV).to(dtype)
     want = gradients(zeno_b200.linear_attention, base, d_out)
@@ -196,15 +208,19 @@ def test_large_and_small_values(dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("name,value", [("q", "nan"), ("k", "nan"), ("k", "-inf"), ("v", "inf"), ("v", "nan"), ("g", "nan"), ("d_out", "nan"), ("d_out", "inf")])
-@pytest.mark.parametrize("T,resets,bad_at", [(70, (20, 45), 30), (70, (20, 32), 40), (33, (32,), 32), (900, (300, 500), 310), (20, (7,), 3)])
-def test_what_is_not_finite_stays_in_its_episode(T, resets, bad_at, name, value, dtype):
-    B, H, d = 2, 2, 32
-    x = inputs(B, T, H, H, d, d, dtype, reset=None)
+@pytest.mark.parametrize("B,T,resets,bad_at", [(2, 70, (20, 45), 30), (2, 70, (20, 32), 40), (2, 33, (32,), 32), (2, 900, (300, 500), 310), (2, 20, (7,), 3),
+                                               (300, 20, (7,), 3), (300, 32, (5, 20), 20), (300, 32, (5, 20), 10)])
+@pytest.mark.parametrize("fixed", [False, True])
+def test_what_is_not_finite_stays_in_its_episode(B, T, resets, bad_at, fixed, name, value, dtype):
+    H, d = 2, 32
+    x = inputs(B, T, H, H, d, d, dtype, reset=None, fixed=fixed)
+    if fixed and name == "g":
+        return  # (then it is in every episode)
     x[4] = torch.zeros(B, T, device=DEV, dtype=torch.uint8)
     for r in resets:
         x[4][:, r] = 1
     d_out = torch.randn(B, T, H, d, device=DEV).to(dtype)
-    want = gradients(zeno_b200.linear_attention, x, d_out)
+    want = exact(x, d_out)
     y = [t.clone() for t in x]
     z = d_out.clone()
     bad = z if name == "d_out" else y["qkvg".index(name)]
@@ -218,13 +234,16 @@ def test_what_is_not_finite_stays_in_its_episode(T, resets, bad_at, name, value,
     outside = [t for t in range(T) if not first <= t < last]
     assert outside
     for what, a, b in zip(NAMES, got, want):
+        if fixed and what == "d_g":
+            check(a[0], b[0], what)  # (the other head's)
+            continue
         if what in ("state", "d_initial"):
             episode = last == T if what == "state" else first == 0
-            pick = [(slice(1, 2), slice(None)), (slice(0, 1), slice(0, 1))] + ([] if episode else [(slice(0, 1), slice(1, 2))])
+            pick = [(slice(1, B), slice(None)), (slice(0, 1), slice(0, 1))] + ([] if episode else [(slice(0, 1), slice(1, 2))])
             for p in pick:
                 check(a[p], b[p], what)
             continue
-        check(a[1], b[1], what)
+        check(a[1:], b[1:], what)
         check(a[0, :, 0], b[0, :, 0], what)
         check(a[0, outside, 1], b[0, outside, 1], what)
     if name != "d_out":  # and what comes before it in its episode
@@ -239,7 +258,7 @@ def test_a_dropped_state_may_hold_anything(dtype):
     x[4] = torch.zeros(3, 40, device=DEV, dtype=torch.uint8)
     x[4][:, 0] = 1
     d = torch.randn(3, 40, 1, 16, device=DEV).to(dtype)
-    want = gradients(zeno_b200.linear_attention, x, d)
+    want = exact(x, d)
     x[5][:] = float("nan")
     for a, b in zip(gradients(zeno_b200.linear_attention, x, d), want):
         check(a, b)

@@ -16,6 +16,8 @@ inline BackwardLayout backward_layout(const ZenoLinearAttention& p) {
   return l;
 }
 
+cudaError_t backward_by_warps(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, const BackwardOut& extra, uint32_t vec, cudaStream_t stream);
+
 template <class T>
 cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream) {
   return with_shape<T>(p, [&](auto shape) {
@@ -38,16 +40,20 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
       e = cut_states<S>(p, p.q, d.d_out, sg, d.d_final, true, stream);
       if (e != cudaSuccess) return e;
     }
-    constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
-    auto kernel = linear_backward_kernel<S, BLOCKS>;
-    const int bytes = BackwardSmem<S>::bytes(p.initial_state || d.d_final || p.tokens > uint32_t(S::C));
-    static std::atomic<uint64_t> devices{0};
-    e = allow_smem(kernel, BackwardSmem<S>::bytes(true), devices);
-    if (e != cudaSuccess) return e;
-    static_assert(sizeof(T) == 4 || S::C * S::P <= 2 * S::PL * S::CPLANE, "dV is staged where P and D were");
-    static_assert(BackwardSmem<S>::front + 2 * (4 * S::L * S::PLANE + 2 * S::PL * S::CPLANE + 3 * S::SPLANE) <= 232448, "shared memory of a block");
-    kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, d, sg, extra);
-    e = cudaGetLastError();
+    if (sizeof(T) == 2 && warp_a_head(p) && !d.d_final) {
+      e = backward_by_warps(p, d, extra, vec, stream);
+    } else {
+      constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
+      auto kernel = linear_backward_kernel<S, BLOCKS>;
+      const int bytes = BackwardSmem<S>::bytes(p.initial_state || d.d_final || p.tokens > uint32_t(S::C));
+      static std::atomic<uint64_t> devices{0};
+      e = allow_smem(kernel, BackwardSmem<S>::bytes(true), devices);
+      if (e != cudaSuccess) return e;
+      static_assert(sizeof(T) == 4 || S::C * S::P <= 2 * S::PL * S::CPLANE, "dV is staged where P and D were");
+      static_assert(BackwardSmem<S>::front + 2 * (4 * S::L * S::PLANE + 2 * S::PL * S::CPLANE + 3 * S::SPLANE) <= 232448, "shared memory of a block");
+      kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, d, sg, extra);
+      e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
     if (l.shared) {
       const uint32_t group = p.value_heads / p.key_heads;

@@ -1,6 +1,6 @@
 // Which instance of the chunked linear attention serves a call, and how a rollout is cut into segments.
 #pragma once
-#include "linear_backward.cuh"
+#include "linear_warp.cuh"
 
 namespace zb {
 namespace linear {
@@ -13,6 +13,8 @@ inline int width_of(const ZenoLinearAttention& p) {
   const uint32_t w = p.key_dim > p.value_dim ? p.key_dim : p.value_dim;
   return w <= 32 ? 32 : w <= 64 ? 64 : 128;
 }
+
+constexpr int kWarpWidth = 64;
 
 struct Cut {
   uint32_t count, chunks;  // segments, and chunks of each
@@ -68,6 +70,15 @@ cudaError_t with_shape(const ZenoLinearAttention& p, F&& f) {
     if (w == 64) return f(Shape<T, 64, 32, 8>{});
     return f(Shape<T, 128, 32, 8>{});
   }
+}
+
+// Short rollouts of many environments: a warp a head.  Few of them finish earlier with a block each.
+inline bool warp_a_head(const ZenoLinearAttention& p) {
+  return p.dtype == ZENO_DTYPE_BF16 && p.tokens >= 1 && p.tokens <= 32 && width_of(p) <= kWarpWidth && uint64_t(p.batch) * p.value_heads >= 4 * kSms;
+}
+template <class F>
+cudaError_t with_warp_shape(const ZenoLinearAttention& p, F&& f) {
+  return width_of(p) == 32 ? f(WarpShape<32>{}) : f(WarpShape<64>{});
 }
 
 template <class T>
