@@ -9,11 +9,11 @@ extern template cudaError_t backward<float>(const ZenoLinearAttention&, const Ze
 
 namespace linear {
 cudaError_t backward_by_warps(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, const BackwardOut& extra, uint32_t vec, cudaStream_t stream) {
-  return with_warp_shape(p, [&](auto shape) {
+  return with_warp_shape(p, [&](auto shape, auto full) {
     using S = decltype(shape);
     constexpr int WARPS = 1, BLOCKS = 11;
     constexpr int bytes = WARPS * (int(sizeof(WarpGates)) + 4 * 2 * S::PLANE);
-    auto kernel = linear_warp_backward_kernel<S::D, WARPS, BLOCKS>;
+    auto kernel = linear_warp_backward_kernel<S::D, decltype(full)::value, WARPS, BLOCKS>;
     static std::atomic<uint64_t> devices{0};
     const cudaError_t e = allow_smem(kernel, bytes, devices);
     if (e != cudaSuccess) return e;

@@ -78,7 +78,10 @@ inline bool warp_a_head(const ZenoLinearAttention& p) {
 }
 template <class F>
 cudaError_t with_warp_shape(const ZenoLinearAttention& p, F&& f) {
-  return width_of(p) == 32 ? f(WarpShape<32>{}) : f(WarpShape<64>{});
+  const uint32_t w = uint32_t(width_of(p));
+  const bool full = p.key_dim == w && p.value_dim == w;
+  if (w == 32) return full ? f(WarpShape<32>{}, std::true_type{}) : f(WarpShape<32>{}, std::false_type{});
+  return full ? f(WarpShape<64>{}, std::true_type{}) : f(WarpShape<64>{}, std::false_type{});
 }
 
 template <class T>

@@ -145,7 +145,8 @@ __device__ __noinline__ void warp_forward_slow(const ZenoLinearAttention& p, con
     }
 }
 
-template <int D, int WARPS, int BLOCKS>
+// FULL: keys and values of D channels, so that offsets are known and nothing is past an end.
+template <int D, bool FULL, int WARPS, int BLOCKS>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel(const __grid_constant__ ZenoLinearAttention p, const uint32_t vec) {
   using S = WarpShape<D>;
   constexpr int KT = S::KT;
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel
   char* mine = smem + warp * (int(sizeof(Gates<32>)) + 3 * 2 * S::PLANE);
   Gates<32>& s = *reinterpret_cast<Gates<32>*>(mine);
   plane_t *q = reinterpret_cast<plane_t*>(mine + sizeof(Gates<32>)), *k = q + S::PLANE, *v = k + S::PLANE;
-  const int dk = int(p.key_dim), dv = int(p.value_dim), n = int(p.tokens), nt = (n + 15) / 16;
+  const int dk = FULL ? D : int(p.key_dim), dv = FULL ? D : int(p.value_dim), n = int(p.tokens), nt = (n + 15) / 16;
   const Mover<S> mv(lane);
   load_rows<S>(q, place<bf16>(p.q, a.b, a.kh), p.q.stride[1], dk, vec & kVecQ, n, nt, mv);
   load_rows<S>(k, place<bf16>(p.k, a.b, a.kh), p.k.stride[1], dk, vec & kVecK, n, nt, mv);
@@ -245,8 +246,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel
           for (int e = 0; e < 2; ++e) {
             const int row = kk * 16 + h * 8 + c2 + e;
             const float* from = initial + row * dv + vt * 16 + g;
-            s0[kk][h][e] = row < dk && left > 0 ? from[0] : 0.0f;
-            s0[kk][h][2 + e] = row < dk && left > 8 ? from[8] : 0.0f;
+            s0[kk][h][e] = FULL || (row < dk && left > 0) ? from[0] : 0.0f;
+            s0[kk][h][2 + e] = FULL || (row < dk && left > 8) ? from[8] : 0.0f;
           }
       }
 #pragma unroll
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel
             for (int t = 0; t < 2; ++t) {
               float y = add[h][2 * t + e];
               if (initial && keep != 0.0f) y = fmaf(keep, s0[kk][h][2 * t + e], y);
-              if (row < dk && left > 8 * t) to[8 * t] = y;
+              if (FULL || (row < dk && left > 8 * t)) to[8 * t] = y;
             }
           }
       }
@@ -425,7 +426,7 @@ __device__ __noinline__ double warp_backward_slow(const ZenoLinearAttention& p, 
 }
 
 // Without a gradient of the final state.
-template <int D, int WARPS, int BLOCKS>
+template <int D, bool FULL, int WARPS, int BLOCKS>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS)
 linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __grid_constant__ ZenoLinearAttentionGrads d, const uint32_t vec,
                             const BackwardOut extra) {
@@ -439,7 +440,7 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
   WarpGates& all = *reinterpret_cast<WarpGates*>(mine);
   Gates<32>& s = all.gates;
   plane_t *q = reinterpret_cast<plane_t*>(mine + sizeof(WarpGates)), *k = q + S::PLANE, *v = k + S::PLANE, *o = v + S::PLANE;
-  const int dk = int(p.key_dim), dv = int(p.value_dim), n = int(p.tokens), nt = (n + 15) / 16;
+  const int dk = FULL ? D : int(p.key_dim), dv = FULL ? D : int(p.value_dim), n = int(p.tokens), nt = (n + 15) / 16;
   const Mover<S> mv(lane);
   load_rows<S>(q, place<bf16>(p.q, a.b, a.kh), p.q.stride[1], dk, vec & kVecQ, n, nt, mv);
   load_rows<S>(k, place<bf16>(p.k, a.b, a.kh), p.k.stride[1], dk, vec & kVecK, n, nt, mv);
@@ -567,7 +568,7 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
             const int c = kk * 16 + h * 8 + c2;
             const float* from = initial + (row + 8 * t) * dv + c;
             const bool there = row + 8 * t < dk;
-            split<3>(there && c < dv ? from[0] : 0.0f, there && c + 1 < dv ? from[1] : 0.0f, b[t][h]);
+            split<3>(FULL || (there && c < dv) ? from[0] : 0.0f, FULL || (there && c + 1 < dv) ? from[1] : 0.0f, b[t][h]);
           }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -635,7 +636,7 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int row = kt * 16 + g + u * 8, c = vt * 16 + h * 8 + c2;
-            if (row < dk && c < dv) {
+            if (FULL || (row < dk && c < dv)) {
               float* at = state + row * dv + c;
               write_pair(at, c, dv, dv % 2 == 0 && reinterpret_cast<uintptr_t>(at) % 8 == 0, add[h][2 * u], add[h][2 * u + 1]);
             }
