@@ -105,7 +105,7 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
   plane_t *k = q + M::row, *v = k + M::row, *o = v + M::row, *pr = o + M::row, *dp = pr + M::pairs, *st = dp + M::pairs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = warp % S::RT, ct = warp / S::RT;
-  const int dk = int(p.key_dim), dv = int(p.value_dim), nk = (dk + 15) / 16, nv = (dv + 15) / 16;
+  const int dk = S::FULL ? S::D : int(p.key_dim), dv = S::FULL ? S::D : int(p.value_dim), nk = (dk + 15) / 16, nv = (dv + 15) / 16;
   const At a = block_at(p, sg, 0, S::C);
   if (a.b >= p.batch) return;
   const Mover<S> mv(tid);
@@ -239,7 +239,7 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
     __syncthreads();
 
     // dQ
-    const int pk = rt < nt ? (dk - col + 15) / 16 : 0, pv = rt < nt ? (dv - col + 15) / 16 : 0;  // column tiles of this warp
+    const int pk = rt >= nt ? 0 : S::FULL ? S::NO : min(S::NO, (dk - col + 15) / 16), pv = rt >= nt ? 0 : S::FULL ? S::NO : min(S::NO, (dv - col + 15) / 16);  // column tiles of this warp
     float dq[S::NO][2][4] = {};
     bool bad = false;
     if (pk > 0) {

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
   plane_t *k = q + S::L * S::PLANE, *v = k + S::L * S::PLANE, *pr = v + S::L * S::PLANE, *st = pr + M::pairs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = warp % S::RT, ct = warp / S::RT;
-  const int dk = int(p.key_dim), dv = int(p.value_dim), nk = (dk + 15) / 16;
+  const int dk = S::FULL ? S::D : int(p.key_dim), dv = S::FULL ? S::D : int(p.value_dim), nk = (dk + 15) / 16;
   const At a = block_at(p, sg, 0, S::C);
   if (a.b >= p.batch) return;
   const Mover<S> mv(tid);
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
     }
     __syncthreads();
 
-    const int col = ct * S::NO * 16, pairs = rt < nt ? (dv - col + 15) / 16 : 0;
+    const int col = ct * S::NO * 16, pairs = rt >= nt ? 0 : S::FULL ? S::NO : min(S::NO, (dv - col + 15) / 16);
     float acc[S::NO][2][4] = {};
     bool bad = false;
     if (pairs > 0) {
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(S::THREADS) linear_segment_kernel(const __grid
   plane_t* x = reinterpret_cast<plane_t*>(smem + ForwardSmem<S>::gates);
   plane_t* y = x + S::L * S::PLANE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int dk = int(p.key_dim), dv = int(p.value_dim);
+  const int dk = S::FULL ? S::D : int(p.key_dim), dv = S::FULL ? S::D : int(p.value_dim);
   const At a = block_at(p, sg, reverse ? 1 : 0, S::C);
   const Mover<S> mv(tid);
   const T *gx = place<T>(tx, a.b, a.kh), *gy = place<T>(ty, a.b, a.h);

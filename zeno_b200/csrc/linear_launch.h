@@ -53,23 +53,27 @@ inline uint32_t vec_of(const ZenoLinearAttention& p, const ZenoTensor& out) {
 }
 
 // f(shape) of the call's instance, for one element type.
-template <class T, class F>
-cudaError_t with_shape(const ZenoLinearAttention& p, F&& f) {
-  const int w = width_of(p);
+template <class T, bool FULL, class F>
+cudaError_t with_shape_of(const ZenoLinearAttention& p, int w, F&& f) {
   if constexpr (sizeof(T) == 2) {
     if (chunk_of(p) == 32) {
-      if (w == 32) return f(Shape<T, 32, 32, 4>{});
-      if (w == 64) return f(Shape<T, 64, 32, 4>{});
-      return f(Shape<T, 128, 32, 8>{});
+      if (w == 32) return f(Shape<T, 32, 32, 4, FULL>{});
+      if (w == 64) return f(Shape<T, 64, 32, 4, FULL>{});
+      return f(Shape<T, 128, 32, 8, FULL>{});
     }
-    if (w == 32) return f(Shape<T, 32, 64, 4>{});
-    if (w == 64) return f(Shape<T, 64, 64, 8>{});
-    return f(Shape<T, 128, 64, 16>{});
+    if (w == 32) return f(Shape<T, 32, 64, 4, FULL>{});
+    if (w == 64) return f(Shape<T, 64, 64, 8, FULL>{});
+    return f(Shape<T, 128, 64, 16, FULL>{});
   } else {
-    if (w == 32) return f(Shape<T, 32, 32, 4>{});
-    if (w == 64) return f(Shape<T, 64, 32, 8>{});
-    return f(Shape<T, 128, 32, 8>{});
+    if (w == 32) return f(Shape<T, 32, 32, 4, FULL>{});
+    if (w == 64) return f(Shape<T, 64, 32, 8, FULL>{});
+    return f(Shape<T, 128, 32, 8, FULL>{});
   }
+}
+inline bool full_width(const ZenoLinearAttention& p) { return int(p.key_dim) == width_of(p) && int(p.value_dim) == width_of(p); }
+template <class T, class F>
+cudaError_t with_shape(const ZenoLinearAttention& p, F&& f) {
+  return full_width(p) ? with_shape_of<T, true>(p, width_of(p), f) : with_shape_of<T, false>(p, width_of(p), f);
 }
 
 // Short rollouts of many environments: a warp a head.  Few of them finish earlier with a block each.
@@ -78,8 +82,8 @@ inline bool warp_a_head(const ZenoLinearAttention& p) {
 }
 template <class F>
 cudaError_t with_warp_shape(const ZenoLinearAttention& p, F&& f) {
-  const uint32_t w = uint32_t(width_of(p));
-  const bool full = p.key_dim == w && p.value_dim == w;
+  const int w = width_of(p);
+  const bool full = full_width(p);
   if (w == 32) return full ? f(WarpShape<32>{}, std::true_type{}) : f(WarpShape<32>{}, std::false_type{});
   return full ? f(WarpShape<64>{}, std::true_type{}) : f(WarpShape<64>{}, std::false_type{});
 }

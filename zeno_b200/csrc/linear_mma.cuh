@@ -31,9 +31,11 @@ using plane_t = uint16_t;  // bfloat16 bits
 
 // D: the widths of a head, padded.  C: tokens of a chunk.  NW: warps.  The warps lie over a chunk's products as
 // [C / 16 row tiles][NH groups of columns] and over the state as [D / 16 row tiles][MG groups of columns].
-template <class T_, int D_, int C_, int NW_>
+// FULL: keys and values have D channels each, so that offsets are known and no column is past an end.
+template <class T_, int D_, int C_, int NW_, bool FULL_>
 struct Shape {
   using T = T_;
+  static constexpr bool FULL = FULL_;
   static constexpr int D = D_, C = C_, NW = NW_, THREADS = NW_ * 32;
   static constexpr int L = sizeof(T) == 2 ? 1 : 3;   // limbs of an input
   static constexpr int PL = sizeof(T) == 2 ? 2 : 3;  // limbs of P and dP
@@ -374,7 +376,7 @@ struct Part {
   int pairs;       // 16-column tiles that exist (0: none, or no rows)
   __device__ __forceinline__ Part(int warp, int dk, int dv) {
     row = warp % S::MR * 16, col = warp / S::MR * S::NM * 16;
-    pairs = row < dk && col < dv ? (dv - col + 15) / 16 : 0;
+    pairs = S::FULL ? S::NM : row < dk && col < dv ? min(S::NM, (dv - col + 15) / 16) : 0;
   }
 };
 
@@ -384,7 +386,7 @@ template <class S, class P, class F>
 __device__ __forceinline__ void each_pair(P* state, const Part<S>& part, int dk, int dv, int lane, F&& f) {
   const int row = part.row + (lane >> 2), col = part.col + (lane & 3) * 2;
   P* const at[2] = {state + row * dv + col, state + (row + 8) * dv + col};
-  if (part.row + 16 <= dk && part.col + S::NM * 16 <= dv) {  // all of it
+  if (S::FULL || (part.row + 16 <= dk && part.col + S::NM * 16 <= dv)) {  // all of it
 #pragma unroll
     for (int j = 0; j < S::NM; ++j)
 #pragma unroll

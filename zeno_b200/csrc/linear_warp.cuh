@@ -512,7 +512,7 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
             x = meet ? x * f : 0.0f;
             pass[u][e] = meet ? x * y : 0.0f;
             y = meet ? y * f : 0.0f;
-            odd = fmaf(x, 0.0f, fmaf(y, 0.0f, odd));
+            odd = fmaf(pass[u][e], 0.0f, odd);  // (x and y are finite if their product is)
           }
         }
         if (!each) {  // a pair passes i - j tokens
