@@ -1,6 +1,6 @@
 """A recurrent policy on Ant: act in every environment on the GPU, keep the rollout, learn from it.
 
-    python examples/memory_policy.py [--envs 4096] [--horizon 32] [--updates 10]
+    python examples/memory_policy.py [--envs 4096] [--horizon 32] [--updates 10] [--memory delta|decay]
 
 Each update steps the world ``horizon`` times (the policy reads the observations where the world
 wrote them, and the world reads the actions where the policy wrote them), then takes one
@@ -26,7 +26,7 @@ NOISE = 0.2  # standard deviation of the actions around the policy's
 DISCOUNT = 0.99
 
 
-def run(envs: int = 4096, horizon: int = 32, updates: int = 10, seed: int = 0, log=print):
+def run(envs: int = 4096, horizon: int = 32, updates: int = 10, seed: int = 0, log=print, memory: str = "delta"):
     torch.manual_seed(seed)
     device = torch.device("cuda")
     world = zeno_b200.ZenoWorld(mjcf_string=scenes.ant(), num_envs=envs, substeps=4)
@@ -34,7 +34,7 @@ def run(envs: int = 4096, horizon: int = 32, updates: int = 10, seed: int = 0, l
     stream = torch.cuda.Stream()
     world.set_stream(stream.cuda_stream)
     obs, rewards, dones = (torch.as_tensor(world.device_array(k), device=device) for k in ("observations", "rewards", "dones"))
-    policy = MemoryPolicy(world.obs_dim, world.action_dim).to(device)
+    policy = MemoryPolicy(world.obs_dim, world.action_dim, memory=memory).to(device)
     optimiser = Muon(policy.parameters(), lr=0.01)
     state = policy.initial_state(envs)
     means = []
@@ -82,5 +82,6 @@ if __name__ == "__main__":
     ap.add_argument("--horizon", type=int, default=32)
     ap.add_argument("--updates", type=int, default=10)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--memory", choices=("delta", "decay"), default="delta")
     a = ap.parse_args()
-    run(a.envs, a.horizon, a.updates, a.seed)
+    run(a.envs, a.horizon, a.updates, a.seed, memory=a.memory)

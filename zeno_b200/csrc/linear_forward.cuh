@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
 
 // What each segment adds to the state behind it: X, Y and weights are K, V and e; in reverse (the gradient of the
 // state) Q, dO and scale c, from the last chunk to the first.
-template <class S>
-__global__ void __launch_bounds__(S::THREADS) linear_segment_kernel(const __grid_constant__ ZenoLinearAttention p, const ZenoTensor tx, const ZenoTensor ty,
+template <class S, int BLOCKS>
+__global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_segment_kernel(const __grid_constant__ ZenoLinearAttention p, const ZenoTensor tx, const ZenoTensor ty,
                                                                     const Segments sg, const bool reverse) {  // (at most a few hundred rows)
   using T = typename S::T;
   extern __shared__ __align__(16) char smem[];
@@ -195,25 +195,12 @@ __global__ void __launch_bounds__(S::THREADS) linear_segment_kernel(const __grid
     load_rows<S>(y, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, nt, mv);
     if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     copies_landed();
-    __syncthreads();
+    const bool bad = __syncthreads_or(rows_odd<S>(x, dk, nt, mv) || rows_odd<S>(y, dv, nt, mv));
     const float* weight = reverse ? s.carried : s.to_end;
-    const float factor = reverse ? p.scale : 1.0f;
-    float add[S::NM][2][4];
-    clear<S>(add);
-    update<S>(add, x, y, weight, factor, 0.0f, nt, part, lane);
-    if (__syncthreads_or(not_finite(add))) {
-      clear<S>(add);
-      update_masked<S>(add, x, y, weight, factor, 0.0f, n, part, dk, dv, lane);
-    }
-    const float keep = s.keep;
-    kept *= keep;
-#pragma unroll
-    for (int j = 0; j < S::NM; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float& z = m[j][e >> 2][e & 3];
-        z = keep == 0.0f ? add[j][e >> 2][e & 3] : fmaf(keep, z, add[j][e >> 2][e & 3]);
-      }
+    const float factor = reverse ? p.scale : 1.0f, keep = step ? s.keep : 0.0f;
+    kept *= s.keep;
+    if (bad) update_masked<S>(m, x, y, weight, factor, keep, n, part, dk, dv, lane);
+    else update<S>(m, x, y, weight, factor, keep, nt, part, lane);
   }
   const int64_t at = int64_t(a.row) * sg.count + a.seg;
   write_state<S>(m, sg.state + at * dk * dv, part, dk, dv, lane);

@@ -94,15 +94,21 @@ template <class T>
 cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream);
 
 // What each segment adds, then the states in front of (behind) them.
+// The shape of the segments' sums: where nothing but the state is in registers, half the warps do with 128 channels, and two blocks fit.
 template <class S>
+using SegmentShape = Shape<typename S::T, S::D, S::C, S::D == 128 ? 8 : S::NW, S::FULL>;
+
+template <class Full>
 cudaError_t cut_states(const ZenoLinearAttention& p, const ZenoTensor& x, const ZenoTensor& y, const Segments& sg, const float* initial, bool reverse,
                        cudaStream_t stream) {
+  using S = SegmentShape<Full>;
+  constexpr int BLOCKS = 512 / S::THREADS;
   static std::atomic<uint64_t> devices{0};
   const int bytes = ForwardSmem<S>::gates + 2 * 2 * S::L * S::PLANE;
-  cudaError_t e = allow_smem(linear_segment_kernel<S>, bytes, devices);
+  cudaError_t e = allow_smem(linear_segment_kernel<S, BLOCKS>, bytes, devices);
   if (e != cudaSuccess) return e;
   const uint32_t rows = p.batch * p.value_heads;
-  linear_segment_kernel<S><<<grid_of(p, sg.count - 1), S::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
+  linear_segment_kernel<S, BLOCKS><<<grid_of(p, sg.count - 1), S::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_linear_walk(LinearWalk{sg.state, sg.keep, initial, sg.count, p.key_dim * p.value_dim, reverse}, rows, stream);

@@ -368,6 +368,24 @@ __device__ __forceinline__ void load_rows(plane_t* to, const typename S::T* from
   }
 }
 
+// Whether something that this thread brought is not finite (which its first limb shows).
+template <class S>
+__device__ __forceinline__ bool rows_odd(const plane_t* at, int width, int nt, const Mover<S>& mv) {
+  if (mv.c >= ((width + 15) & ~15)) return false;
+  __nv_bfloat162 z = __floats2bfloat162_rn(0.0f, 0.0f);
+  const __nv_bfloat162 nothing = z;
+#pragma unroll
+  for (int u = 0; u < Mover<S>::TURNS; ++u) {
+    if (mv.row + u * Mover<S>::STEP >= nt * 16) break;
+    const uint4 w = *reinterpret_cast<const uint4*>(at + (mv.row + u * Mover<S>::STEP) * S::P + mv.c);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), nothing, z);
+  }
+  const float sum = __low2float(z) + __high2float(z);
+  return sum != sum;
+}
+
 // ---------------------------------------------------------------- the state in the warps' accumulators
 // A warp's part: rows [16 (warp % MR), +16), columns [16 NM (warp / MR), +16 NM) of a state [dk][dv].
 template <class S>

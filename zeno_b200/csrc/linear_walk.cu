@@ -7,6 +7,8 @@
 namespace zb {
 namespace {
 
+// kAhead: segments whose sums are under way at once.
+template <uint32_t kAhead>
 __global__ void __launch_bounds__(256) linear_walk_kernel(const LinearWalk w) {
   const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
   const uint64_t row = blockIdx.y;
@@ -14,14 +16,22 @@ __global__ void __launch_bounds__(256) linear_walk_kernel(const LinearWalk w) {
   float run = w.initial ? w.initial[row * w.size + i] : 0.0f;
   float* state = w.state + row * w.segments * w.size + i;
   const float* keep = w.keep + row * w.segments;
-#pragma unroll 4
-  for (uint32_t step = 0; step < w.segments; ++step) {
-    const uint32_t seg = w.reverse ? w.segments - 1 - step : step;
-    // the last one's sum is not asked for, and was not taken
-    const float add = step + 1 < w.segments ? state[seg * w.size] : 0.0f;
-    const float k = step + 1 < w.segments ? keep[seg] : 1.0f;
-    state[seg * w.size] = run;
-    run = k == 0.0f ? add : fmaf(k, run, add);
+  for (uint32_t first = 0; first < w.segments; first += kAhead) {
+    float add[kAhead], kept[kAhead];
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) {
+      const uint32_t step = first + u, seg = w.reverse ? w.segments - 1 - step : step;
+      add[u] = 0.0f, kept[u] = 1.0f;
+      // (the last one's sum is not asked for, and was not taken)
+      if (step + 1 < w.segments) add[u] = state[seg * uint64_t(w.size)], kept[u] = keep[seg];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) {
+      const uint32_t step = first + u, seg = w.reverse ? w.segments - 1 - step : step;
+      if (step >= w.segments) break;
+      state[seg * uint64_t(w.size)] = run;
+      run = kept[u] == 0.0f ? add[u] : fmaf(kept[u], run, add[u]);
+    }
   }
 }
 
@@ -85,7 +95,9 @@ __global__ void __launch_bounds__(1024) linear_decay_kernel(const double* from, 
 
 cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t stream) {
   // at most a few hundred rows are cut into segments
-  linear_walk_kernel<<<dim3((w.size + 255) / 256, rows), 256, 0, stream>>>(w);
+  const dim3 grid((w.size + 255) / 256, rows);
+  if (w.segments <= 2) linear_walk_kernel<2><<<grid, 256, 0, stream>>>(w);
+  else linear_walk_kernel<8><<<grid, 256, 0, stream>>>(w);
   return cudaGetLastError();
 }
 

@@ -211,20 +211,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel
       as_left(pf[r + c], sc[c]);
     }
   }
-  if (mv.c < ((dv + 15) & ~15)) {  // (V: the pieces that this lane brought)
-    __nv_bfloat162 z = __floats2bfloat162_rn(0.0f, 0.0f);
-    const __nv_bfloat162 nothing = z;
-#pragma unroll
-    for (int u = 0; u < Mover<S>::TURNS; ++u) {
-      if (mv.row + u * Mover<S>::STEP >= nt * 16) break;
-      const uint4 w = *reinterpret_cast<const uint4*>(v + (mv.row + u * Mover<S>::STEP) * S::P + mv.c);
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), nothing, z);
-    }
-    odd += __low2float(z) + __high2float(z);
-  }
-  if (__any_sync(kAll, odd != odd)) {
+  if (__any_sync(kAll, odd != odd || rows_odd<S>(v, dv, nt, mv))) {
     warp_forward_slow<S>(p, s, q, k, v, out, initial, final, n, lane);
     return;
   }
