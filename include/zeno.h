@@ -421,6 +421,11 @@ int zeno_linear_attention_backward(const ZenoLinearAttention* p, const ZenoLinea
  * initial_state (updated in place).  Same results as forward up to rounding. */
 int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
 
+/* Chunks of wide heads wait for their own matrix instructions; one that waits longer than this gives up, and what
+ * builds on it comes out as NaN.  Sets the limit of later calls in nanoseconds (2e9 at first; 0: nothing is
+ * waited for, so all give up) and returns the one before. */
+uint64_t zeno_linear_attention_wait_limit(uint64_t nanoseconds);
+
 /* Layer norm of rows of `width` values: out = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps), mean and
  * variance in 32 bits, the variance from the differences to the mean. */
 typedef struct {

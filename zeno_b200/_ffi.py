@@ -146,6 +146,7 @@ ffi.cdef("""
     int zeno_linear_attention_forward(const ZenoLinearAttention* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
     int zeno_linear_attention_backward(const ZenoLinearAttention* p, const ZenoLinearAttentionGrads* d, void* workspace,
                                        uint64_t workspace_bytes, void* cuda_stream);
+    uint64_t zeno_linear_attention_wait_limit(uint64_t nanoseconds);
     int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
     typedef struct {
         uint64_t rows[3]; uint32_t width; uint32_t dtype; uint32_t affine_dtype; float eps;

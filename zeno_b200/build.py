@@ -53,7 +53,7 @@ OP_SOURCES = ["delta_step.cu", "delta_forward.cu", "delta_walk.cu", "delta_backw
 CXX_SOURCES = ["mjcf.cpp", "model.cpp", "fast_model.cpp", "world.cpp", "capi.cpp", "policy_ops.cpp"]
 HEADERS = ["zeno_types.h", "devmath.cuh", "physics.cuh", "model_access.cuh", "stage_clock.cuh", "fast_model.h", "step_kernel.h", "scene.h", "model.h", "world.h",
            "policy_ops.h", "delta_mma.cuh", "delta_backward.cuh", "newton_schulz.h", "linear_mma.cuh", "linear_forward.cuh", "linear_backward.cuh",
-           "linear_warp.cuh", "linear_launch.h", "linear_forward_impl.cuh", "linear_backward_impl.cuh"]
+           "linear_warp.cuh", "linear_tensor.cuh", "linear_launch.h", "linear_forward_impl.cuh", "linear_backward_impl.cuh"]
 
 
 def _newer(target: Path, deps) -> bool:

@@ -17,14 +17,21 @@ cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t 
       e = cut_states<S>(p, p.k, p.v, sg, p.initial_state, false, stream);
       if (e != cudaSuccess) return e;
     }
-    constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
-    auto kernel = linear_forward_kernel<S, BLOCKS>;
-    // the first chunk of a rollout from nothing has no state in front of it
-    const int bytes = ForwardSmem<S>::bytes(p.initial_state || c.count > 1 || p.tokens > uint32_t(S::C));
     static std::atomic<uint64_t> devices{0};
-    e = allow_smem(kernel, ForwardSmem<S>::bytes(true), devices);
-    if (e != cudaSuccess) return e;
-    kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, sg);
+    if constexpr (kTensor<S>) {
+      auto kernel = tensor::linear_tensor_forward_kernel<S>;
+      e = allow_smem(kernel, tensor::kForwardBytes, devices);
+      if (e != cudaSuccess) return e;
+      kernel<<<grid_of(p, c.count), S::THREADS, tensor::kForwardBytes, stream>>>(p, sg, linear_patience());
+    } else {
+      constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
+      auto kernel = linear_forward_kernel<S, BLOCKS>;
+      // the first chunk of a rollout from nothing has no state in front of it
+      const int bytes = ForwardSmem<S>::bytes(p.initial_state || c.count > 1 || p.tokens > uint32_t(S::C));
+      e = allow_smem(kernel, ForwardSmem<S>::bytes(true), devices);
+      if (e != cudaSuccess) return e;
+      kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, sg);
+    }
     return cudaGetLastError();
   });
 }

@@ -1,5 +1,6 @@
 // Which instance of the chunked linear attention serves a call, and how a rollout is cut into segments.
 #pragma once
+#include "linear_tensor.cuh"
 #include "linear_warp.cuh"
 
 namespace zb {
@@ -94,21 +95,30 @@ template <class T>
 cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream);
 
 // What each segment adds, then the states in front of (behind) them.
-// The shape of the segments' sums: where nothing but the state is in registers, half the warps do with 128 channels, and two blocks fit.
+// Wide heads in chunks of 64: on tcgen05.
 template <class S>
-using SegmentShape = Shape<typename S::T, S::D, S::C, S::D == 128 ? 8 : S::NW, S::FULL>;
+constexpr bool kTensor = sizeof(typename S::T) == 2 && S::D == tensor::D && S::C == tensor::C;
 
 template <class Full>
 cudaError_t cut_states(const ZenoLinearAttention& p, const ZenoTensor& x, const ZenoTensor& y, const Segments& sg, const float* initial, bool reverse,
                        cudaStream_t stream) {
-  using S = SegmentShape<Full>;
-  constexpr int BLOCKS = 512 / S::THREADS;
-  static std::atomic<uint64_t> devices{0};
-  const int bytes = ForwardSmem<S>::gates + 2 * 2 * S::L * S::PLANE;
-  cudaError_t e = allow_smem(linear_segment_kernel<S, BLOCKS>, bytes, devices);
-  if (e != cudaSuccess) return e;
   const uint32_t rows = p.batch * p.value_heads;
-  linear_segment_kernel<S, BLOCKS><<<grid_of(p, sg.count - 1), S::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
+  static std::atomic<uint64_t> devices{0};
+  cudaError_t e;
+  if constexpr (kTensor<Full>) {
+    using S = tensor::SegmentShape<Full::FULL>;
+    auto kernel = tensor::linear_tensor_segment_kernel<S>;
+    e = allow_smem(kernel, tensor::kSegmentBytes, devices);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid_of(p, sg.count - 1), S::THREADS, tensor::kSegmentBytes, stream>>>(p, x, y, sg, reverse, linear_patience());
+  } else {
+    constexpr int BLOCKS = 512 / Full::THREADS;
+    auto kernel = linear_segment_kernel<Full, BLOCKS>;
+    const int bytes = ForwardSmem<Full>::gates + 2 * 2 * Full::L * Full::PLANE;
+    e = allow_smem(kernel, bytes, devices);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid_of(p, sg.count - 1), Full::THREADS, bytes, stream>>>(p, x, y, sg, reverse);
+  }
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_linear_walk(LinearWalk{sg.state, sg.keep, initial, sg.count, p.key_dim * p.value_dim, reverse}, rows, stream);

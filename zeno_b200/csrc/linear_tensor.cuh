@@ -1,0 +1,564 @@
+// Long rollouts of wide heads (more than 64 channels, bfloat16): the chunked linear attention of linear_forward.cuh with its products on
+// tcgen05.
+//
+// A chunk of 64 tokens is products of 64 and 128 rows, too few instructions apart for mma.sync to be fed: loading and holding its operands
+// was two thirds of the instructions that the general kernels issue for such a head (1800 a warp and chunk forward).  Here operands are
+// tiles of 64 columns in shared memory with the 128-byte swizzle, read along either axis, one thread issues the products,
+// and the warps do what is left: decays, limbs, the state's sum.  The accumulators come back in the same fragments as those of mma.sync, so that
+// the formulas are written as there.  Sums of a chunk are taken in TMEM, the state itself is summed in registers (the tensor cores truncate).
+//
+// Waits end after a limit; a block whose products do not finish writes NaN.
+#pragma once
+#include "linear_backward.cuh"
+
+namespace zb {
+namespace linear {
+namespace tensor {
+
+constexpr int C = 64, D = 128;
+constexpr int kTok = C * D;          // elements of a tile of token rows: two blocks [64 rows][64 columns]
+constexpr int kPair = C * C;         // of a token-by-token tile: one block
+constexpr int kState = D * D;        // of a state: two blocks [128 rows][64 columns]
+constexpr uint64_t kPatience = 2000000000;  // nanoseconds at a barrier before a block gives up
+
+// Where an element is: blocks of 64 columns, rows of 128 bytes whose 16-byte pieces are swapped within groups of 8 rows.
+template <int ROWS>
+__device__ __forceinline__ int spot(int row, int col) {
+  return (col >> 6) * (ROWS * 64) + row * 64 + ((((col >> 3) & 7) ^ (row & 7)) << 3) + (col & 7);
+}
+
+// Operands of tcgen05.mma.  ALONG: rows hold the contracted index (step k: 16 columns of a block).  ACROSS: rows are the contracted index, the
+// operand's own index lies along them (step k: 16 rows), its blocks of 64 are ROWS * 128 bytes apart.
+__device__ __forceinline__ uint64_t descriptor(uint32_t at, uint32_t leading) {
+  return uint64_t((at & 0x3ffff) >> 4) | uint64_t(leading >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+template <int ROWS>
+__device__ __forceinline__ uint64_t along(uint32_t at, int k) {
+  return descriptor(at + (k >> 2) * (ROWS * 128) + (k & 3) * 32, 16);
+}
+template <int ROWS>
+__device__ __forceinline__ uint64_t across(uint32_t at, int k) {
+  return descriptor(at + k * 2048, ROWS * 128);
+}
+// bfloat16 operands, 32-bit sums, M x N; TA, TB: A, B are read across.
+template <int M, int N, bool TA, bool TB>
+constexpr uint32_t kInstruction = 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(TA) << 15 | uint32_t(TB) << 16 | uint32_t(N >> 3) << 17 |
+                                  uint32_t(M >> 4) << 24;
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(uint32_t(add))
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Whether the phase ended within `patience` nanoseconds (0: not waited for at all).
+__device__ __forceinline__ bool ended(uint32_t bar, uint32_t parity, uint64_t patience) {
+  uint64_t began = 0, now;
+  if (patience == 0) return false;
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (began == 0) began = now;
+    else if (now - began > patience) return false;
+  }
+}
+
+// 16 rows and 8 X columns of accumulators: r[4 c + x] is column 8 c + 2 (lane % 4) + (x & 1) of row lane / 4 + 8 (x >> 1), as the tiles of
+// mma.sync have it.
+__device__ __forceinline__ void fetch2(float* r, uint32_t at) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(at));
+}
+__device__ __forceinline__ void fetch4(float* r, uint32_t at) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+                 "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+               : "r"(at));
+}
+// The loads in front of it have their values; these pass through here, so that no use of them moves up.
+template <int N>
+__device__ __forceinline__ void fetched(float (&r)[N][2][4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm volatile("" : "+f"(r[j][e >> 2][e & 3]));
+}
+
+// The value that N planes hold; the first alone where it is not finite.
+template <int N, int ROWS>
+__device__ __forceinline__ float value_at(const plane_t* at, int plane, int row, int col) { return value<N>(at + spot<ROWS>(row, col), plane); }
+
+// Which 8 columns of which rows of a chunk a thread moves.
+template <int THREADS>
+struct Mover {
+  static constexpr int STEP = THREADS / 16, TURNS = C / STEP;
+  int row, c;
+  __device__ __forceinline__ explicit Mover(int tid) : row(tid >> 4), c((tid & 15) * 8) {}
+};
+
+// All threads: a chunk's rows as a tile, zero for absent tokens and past the width.
+template <int THREADS>
+__device__ __forceinline__ void load_tile(plane_t* to, const bf16* from, int64_t stride, int width, bool vec, int n, const Mover<THREADS>& mv) {
+  using M = Mover<THREADS>;
+  const bf16* at = from + mv.row * stride + mv.c;
+#pragma unroll
+  for (int u = 0; u < M::TURNS; ++u) {
+    const int row = mv.row + u * M::STEP;
+    const bool there = row < n && mv.c < width;
+    plane_t* spot_at = to + spot<C>(row, mv.c);
+    if (vec) {
+      copy16(spot_at, there ? at : from, there);
+    } else {
+      delta::Eight raw{};
+      if (there) raw = delta::fetch8_slow(at, width - mv.c);
+      *reinterpret_cast<uint4*>(spot_at) = raw.a;
+    }
+    at += M::STEP * stride;
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void store_tile(bf16* to, int64_t stride, const plane_t* from, int width, bool vec, int n, const Mover<THREADS>& mv) {
+  using M = Mover<THREADS>;
+  if (mv.c >= width) return;
+  plane_t* at = reinterpret_cast<plane_t*>(to) + mv.row * stride + mv.c;
+#pragma unroll
+  for (int u = 0; u < M::TURNS; ++u) {
+    const int row = mv.row + u * M::STEP;
+    if (row >= n) break;
+    const plane_t* x = from + spot<C>(row, mv.c);
+    if (vec) {
+      *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (mv.c + i < width) at[i] = x[i];
+    }
+    at += M::STEP * stride;
+  }
+}
+// Whether something that this thread brought is not finite.
+template <int THREADS>
+__device__ __forceinline__ bool tile_odd(const plane_t* at, const Mover<THREADS>& mv) {
+  __nv_bfloat162 z = __floats2bfloat162_rn(0.0f, 0.0f);
+  const __nv_bfloat162 nothing = z;
+#pragma unroll
+  for (int u = 0; u < Mover<THREADS>::TURNS; ++u) {
+    const uint4 w = *reinterpret_cast<const uint4*>(at + spot<C>(mv.row + u * Mover<THREADS>::STEP, mv.c));
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), nothing, z);
+  }
+  const float sum = __low2float(z) + __high2float(z);
+  return sum != sum;
+}
+
+// The pieces that this thread brought, each row times factor weight[row], as three tiles of limbs.
+template <int THREADS>
+__device__ __forceinline__ void weigh(plane_t* to, const plane_t* from, const float* weight, float factor, const Mover<THREADS>& mv) {
+#pragma unroll
+  for (int u = 0; u < Mover<THREADS>::TURNS; ++u) {
+    const int row = mv.row + u * Mover<THREADS>::STEP, at = spot<C>(row, mv.c);
+    const float f = weight[row] * factor;
+    const uint4 w = *reinterpret_cast<const uint4*>(from + at);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    uint32_t r[4][3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split<3>(lower(x[i]) * f, upper(x[i]) * f, r[i]);
+#pragma unroll
+    for (int l = 0; l < 3; ++l) *reinterpret_cast<uint4*>(to + l * kTok + at) = make_uint4(r[0][l], r[1][l], r[2][l], r[3][l]);
+  }
+}
+
+// A part of a state in planes, N limbs.
+template <class S, int N>
+__device__ __forceinline__ void dump(const float (&m)[S::NM][2][4], plane_t* to, const Part<S>& part, int lane) {
+#pragma unroll
+  for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t w[N];
+        split<N>(m[j][h][2 * r], m[j][h][2 * r + 1], w);
+        const int at = spot<D>(part.row + (lane >> 2) + r * 8, part.col + j * 16 + h * 8 + (lane & 3) * 2);
+#pragma unroll
+        for (int l = 0; l < N; ++l) *reinterpret_cast<uint32_t*>(to + l * kState + at) = w[l];
+      }
+}
+
+// The part of a state that a warp has: 16 rows of its quarter of TMEM's lanes, and every column or half of them.
+template <class S>
+__device__ __forceinline__ Part<S> part_of(int warp) {
+  Part<S> part(0, D, D);
+  part.row = (warp & 3) * 32 + ((warp >> 2) & 1) * 16;
+  part.col = (warp >> 3) * S::NM * 16;
+  part.pairs = S::NM;
+  return part;
+}
+
+// m = keep m + the accumulators at `at`.
+template <class S>
+__device__ __forceinline__ void merge(float (&m)[S::NM][2][4], uint32_t at, float keep, const Part<S>& part) {
+#pragma unroll
+  for (int j = 0; j < S::NM; j += 2) {
+    float add[2][2][4];
+    fetch4(&add[0][0][0], at + (uint32_t(part.row) << 16) + part.col + j * 16);
+    fetched(add);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float& z = m[j + (e >> 3)][(e >> 2) & 1][e & 3];
+      const float y = add[e >> 3][(e >> 2) & 1][e & 3];
+      z = keep == 0.0f ? y : fmaf(keep, z, y);
+    }
+  }
+}
+// The same element by element, leaving out tokens of no weight.
+template <class S>
+__device__ __noinline__ void merge_slow(float* m, const plane_t* x, const plane_t* y, const float* weight, float factor, float keep, int n, int row, int col) {
+  float sum = 0.0f;
+  for (int j = 0; j < n; ++j)
+    if (weight[j] != 0.0f) sum = fmaf(weight[j] * factor * value_at<1, C>(x, 0, j, row), value_at<1, C>(y, 0, j, col), sum);
+  *m = keep == 0.0f ? sum : fmaf(keep, *m, sum);
+}
+template <class S>
+__device__ __forceinline__ void merge_masked(float (&m)[S::NM][2][4], const plane_t* x, const plane_t* y, const float* weight, float factor, float keep,
+                                             int n, const Part<S>& part, int lane) {
+#pragma unroll
+  for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float z = m[j][e >> 2][e & 3];
+      merge_slow<S>(&z, x, y, weight, factor, keep, n, part.row + (lane >> 2) + ((e >> 1) & 1) * 8,
+                    part.col + j * 16 + (e >> 2) * 8 + (lane & 3) * 2 + (e & 1));
+      m[j][e >> 2][e & 3] = z;
+    }
+}
+
+// What a block holds besides its tiles.
+struct Control {
+  uint64_t bar;
+  uint32_t tmem, pad;
+};
+template <int COLUMNS>
+__device__ __forceinline__ void begin(Control& c, int warp, int tid) {
+  if (tid == 0) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(delta::smem_at(&c.bar)) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(delta::smem_at(&c.tmem)), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+}
+template <int COLUMNS>
+__device__ __forceinline__ void end(uint32_t tmem, int warp) {
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLUMNS));
+}
+
+// The products issued since the last wait: whether they ended, the same answer in every thread.  Where they did not, another wait
+// lets them end before anything is given back.
+struct Products {
+  uint32_t bar, parity;
+  uint64_t patience;
+  __device__ __forceinline__ void issued(bool mine) {
+    if (mine) commit(bar);
+  }
+  __device__ __forceinline__ bool done() {
+    bool ok = ended(bar, parity, patience);
+    ok = __syncthreads_and(ok);
+    if (!ok) ended(bar, parity, kPatience);
+    parity ^= 1;
+    fence_after();
+    return ok;
+  }
+};
+
+template <bool FULL>
+using WideShape = Shape<bf16, D, C, 16, FULL>;     // main kernels
+template <bool FULL>
+using SegmentShape = Shape<bf16, D, C, 8, FULL>;   // segments
+
+// Not a number, where a block gave up.
+__device__ __forceinline__ float lost() { return __uint_as_float(0x7fffffffu); }
+
+constexpr int kForwardBytes = 1024 + 2 * (3 * kTok + 2 * kPair + 2 * kState + 3 * kTok) + int(sizeof(Gates<C>)) + int(sizeof(Control));
+constexpr int kSegmentBytes = 1024 + 2 * (2 * kTok + 3 * kTok) + int(sizeof(Gates<C>)) + int(sizeof(Control));
+
+template <class S>
+__global__ void __launch_bounds__(S::THREADS, 1)
+linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, const Segments sg, const uint64_t patience) {
+  extern __shared__ char smem[];
+  plane_t* q = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
+  plane_t *k = q + kTok, *v = k + kTok, *pr = v + kTok, *st = pr + 2 * kPair, *wk = st + 2 * kState;
+  Gates<C>& s = *reinterpret_cast<Gates<C>*>(wk + 3 * kTok);
+  Control& control = *reinterpret_cast<Control*>(&s + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rt = warp & 3, ct = warp >> 2;  // 16 tokens, and a quarter of a product's columns
+  const int dk = S::FULL ? D : int(p.key_dim), dv = S::FULL ? D : int(p.value_dim);
+  const At a = block_at(p, sg, 0, C);
+  if (a.b >= p.batch) return;
+  const Mover<S::THREADS> mv(tid);
+  const int64_t state_size = int64_t(dk) * dv;
+  const bf16 *gq = place<bf16>(p.q, a.b, a.kh), *gk = place<bf16>(p.k, a.b, a.kh), *gv = place<bf16>(p.v, a.b, a.h);
+  const float* gg = place<float>(p.g, a.b, a.h);
+  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
+  bf16* go = place<bf16>(p.out, a.b, a.h);
+  begin<512>(control, warp, tid);
+  const uint32_t tmem = control.tmem;
+  // columns of TMEM: S^T q's and P's part of the outputs, the update, the scores
+  const uint32_t t_state = tmem, t_pairs = tmem + 128, t_update = tmem + 256, t_scores = tmem + 384;
+  Products products{delta::smem_at(&control.bar), 0, patience};
+
+  const Part<S> part = part_of<S>(warp);
+  float m[S::NM][2][4];
+  const float* first = a.seg ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
+                             : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+  if (first) read_state<S>(m, first, part, dk, dv, lane);
+  else clear<S>(m);
+  bool ok = true;
+
+  for (int c = a.c0; c < a.c1; ++c) {
+    const int64_t t0 = int64_t(c) * C;
+    const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
+    const bool have = c > a.c0 || first, goes_on = c + 1 < a.c1 || (c + 1 == a.chunks && p.final_state);
+    __syncthreads();  // the last chunk's results have left
+    load_tile(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, mv);
+    load_tile(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, mv);
+    load_tile(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, mv);
+    if (warp == S::NW - 1) load_gates<C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    if (have) dump<S, 2>(m, st, part, lane);
+    if (p.saved && c > 0) write_state<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane);
+    copies_landed();
+    fence_shared();
+    fence_before();
+    __syncthreads();
+    if (tid == 0) {
+      fence_after();
+      const uint32_t aq = delta::smem_at(q), ak = delta::smem_at(k);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma(t_scores, along<C>(aq, kk), along<C>(ak, kk), kInstruction<64, 64, false, false>, kk > 0);
+    }
+    products.issued(tid == 0);
+    if (goes_on) weigh(wk, k, s.to_end, 1.0f, mv);
+    ok = products.done();
+    if (!ok) break;
+
+    {  // P, the masked pairs as zeros
+      float acc[1][2][4];
+      fetch2(&acc[0][0][0], t_scores + (uint32_t(rt * 32) << 16) + ct * 16);
+      fetched(acc);
+      const int i0 = rt * 16 + (lane >> 2);
+      const Token ti[2] = {s.token[i0], s.token[i0 + 8]};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = ct * 16 + h * 8 + (lane & 3) * 2;
+        const Token u0 = s.token[col], u1 = s.token[col + 1];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = i0 + r * 8;
+          const bool m0 = meets(ti[r], u0, i, col), m1 = meets(ti[r], u1, i, col + 1);
+          const float f0 = pair_decay(ti[r], u0, m0) * p.scale, f1 = pair_decay(ti[r], u1, m1) * p.scale;
+          uint32_t w[2];
+          split<2>(m0 ? acc[0][h][2 * r] * f0 : 0.0f, m1 ? acc[0][h][2 * r + 1] * f1 : 0.0f, w);
+          const int at = spot<C>(i, col);
+          *reinterpret_cast<uint32_t*>(pr + at) = w[0];
+          *reinterpret_cast<uint32_t*>(pr + kPair + at) = w[1];
+        }
+      }
+    }
+    fence_shared();
+    fence_before();
+    __syncthreads();
+    if (tid == 0) {
+      fence_after();
+      const uint32_t aq = delta::smem_at(q), av = delta::smem_at(v), ap = delta::smem_at(pr), as = delta::smem_at(st), aw = delta::smem_at(wk);
+#pragma unroll
+      for (int l = 1; l >= 0; --l)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma(t_pairs, along<C>(ap + l * kPair * 2, kk), across<C>(av, kk), kInstruction<64, 128, false, true>, l == 0 || kk > 0);
+      if (have) {
+#pragma unroll
+        for (int l = 1; l >= 0; --l)
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            mma(t_state, along<C>(aq, kk), across<D>(as + l * kState * 2, kk), kInstruction<64, 128, false, true>, l == 0 || kk > 0);
+      }
+      if (goes_on) {
+#pragma unroll
+        for (int l = 2; l >= 0; --l)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma(t_update, across<C>(aw + l * kTok * 2, kk), across<C>(av, kk), kInstruction<128, 128, true, true>, l < 2 || kk > 0);
+      }
+    }
+    products.issued(tid == 0);
+    ok = products.done();
+    if (!ok) break;
+
+    const int col = ct * 32;
+    float acc[2][2][4];
+    fetch4(&acc[0][0][0], t_pairs + (uint32_t(rt * 32) << 16) + col);
+    fetched(acc);
+    if (have) {
+      float more[2][2][4];
+      fetch4(&more[0][0][0], t_state + (uint32_t(rt * 32) << 16) + col);
+      fetched(more);
+      const float f0 = s.carried[rt * 16 + (lane >> 2)], f1 = s.carried[rt * 16 + (lane >> 2) + 8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = e & 2 ? f1 : f0;
+          float& y = acc[j][e >> 2][e & 3];
+          y = f == 0.0f ? y : fmaf(f * p.scale, more[j][e >> 2][e & 3], y);
+        }
+    }
+    const bool bad = __syncthreads_or(not_finite(acc));
+    if (bad) {
+#pragma unroll 1
+      for (int x = 0; x < 16; ++x) {
+        const int i = rt * 16 + (lane >> 2) + ((x >> 1) & 1) * 8, cc = col + (x >> 3) * 16 + ((x >> 2) & 1) * 8 + (lane & 3) * 2 + (x & 1);
+        if (i >= n || cc >= dv) continue;
+        float y = 0.0f;
+        if (have && s.carried[i] != 0.0f) {
+          for (int d = 0; d < dk; ++d) y = fmaf(value_at<1, C>(q, 0, i, d), value_at<2, D>(st, kState, d, cc), y);
+          y *= s.carried[i] * p.scale;
+        }
+        for (int j = 0; j <= i; ++j)
+          if (pair_decay(s.token[i], s.token[j], meets(s.token[i], s.token[j], i, j)) != 0.0f)
+            y = fmaf(value_at<2, C>(pr, kPair, i, j), value_at<1, C>(v, 0, j, cc), y);
+#pragma unroll
+        for (int z = 0; z < 16; ++z)
+          if (z == x) acc[z >> 3][(z >> 2) & 1][z & 3] = y;
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          *reinterpret_cast<uint32_t*>(q + spot<C>(rt * 16 + (lane >> 2) + r * 8, col + j * 16 + h * 8 + (lane & 3) * 2)) =
+              pack_round(acc[j][h][2 * r], acc[j][h][2 * r + 1]);
+    if (goes_on) {
+      if (bad) merge_masked<S>(m, k, v, s.to_end, 1.0f, s.keep, n, part, lane);
+      else merge<S>(m, t_update, s.keep, part);
+    }
+    fence_before();
+    __syncthreads();
+    store_tile(go + t0 * p.out.stride[1], p.out.stride[1], q, dv, sg.vec & kVecOut, n, mv);
+  }
+  if (!ok) {  // what this block would have written
+    for (int64_t t = int64_t(a.c0) * C + warp; t < min(int64_t(a.c1) * C, int64_t(p.tokens)); t += S::NW)
+      for (int x = lane; x < dv; x += 32) go[t * p.out.stride[1] + x] = __float2bfloat16_rn(lost());
+#pragma unroll
+    for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[j][e >> 2][e & 3] = lost();
+    if (p.saved)
+      for (int c = max(a.c0, 1); c < a.c1; ++c)
+        write_state<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane);
+  }
+  if (a.c1 == a.chunks && p.final_state) write_state<S>(m, p.final_state + int64_t(a.row) * state_size, part, dk, dv, lane);
+  end<512>(tmem, warp);
+}
+
+// What each segment adds to the state behind it, as linear_segment_kernel.
+template <class S>
+__global__ void __launch_bounds__(S::THREADS, 2)
+linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, const ZenoTensor tx, const ZenoTensor ty, const Segments sg, const bool reverse,
+                             const uint64_t patience) {
+  extern __shared__ char smem[];
+  plane_t* x = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
+  plane_t *y = x + kTok, *wx = y + kTok;
+  Gates<C>& s = *reinterpret_cast<Gates<C>*>(wx + 3 * kTok);
+  Control& control = *reinterpret_cast<Control*>(&s + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int dk = S::FULL ? D : int(p.key_dim), dv = S::FULL ? D : int(p.value_dim);
+  const At a = block_at(p, sg, reverse ? 1 : 0, C);
+  const Mover<S::THREADS> mv(tid);
+  const bf16 *gx = place<bf16>(tx, a.b, a.kh), *gy = place<bf16>(ty, a.b, a.h);
+  const float* gg = place<float>(p.g, a.b, a.h);
+  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
+  const bool vx = sg.vec & (reverse ? kVecQ : kVecK), vy = sg.vec & (reverse ? kVecOut : kVecV);
+  begin<128>(control, warp, tid);
+  const uint32_t tmem = control.tmem;
+  Products products{delta::smem_at(&control.bar), 0, patience};
+  const Part<S> part = part_of<S>(warp);
+  float m[S::NM][2][4];
+  clear<S>(m);
+  float kept = 1.0f;
+  bool ok = true;
+  for (int step = 0; step < a.c1 - a.c0; ++step) {
+    const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * C;
+    const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
+    __syncthreads();
+    load_tile(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, mv);
+    load_tile(y, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, mv);
+    if (warp == S::NW - 1) load_gates<C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    copies_landed();
+    const bool bad = __syncthreads_or(tile_odd(x, mv) || tile_odd(y, mv));
+    const float* weight = reverse ? s.carried : s.to_end;
+    const float factor = reverse ? p.scale : 1.0f, keep = step ? s.keep : 0.0f;
+    kept *= s.keep;
+    if (bad) {
+      merge_masked<S>(m, x, y, weight, factor, keep, n, part, lane);
+      continue;
+    }
+    weigh(wx, x, weight, factor, mv);
+    fence_shared();
+    fence_before();
+    __syncthreads();
+    if (tid == 0) {
+      fence_after();
+      const uint32_t aw = delta::smem_at(wx), ay = delta::smem_at(y);
+#pragma unroll
+      for (int l = 2; l >= 0; --l)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma(tmem, across<C>(aw + l * kTok * 2, kk), across<C>(ay, kk), kInstruction<128, 128, true, true>, l < 2 || kk > 0);
+    }
+    products.issued(tid == 0);
+    ok = products.done();
+    if (!ok) break;
+    merge<S>(m, tmem, keep, part);
+    fence_before();
+  }
+  if (!ok) {
+#pragma unroll
+    for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[j][e >> 2][e & 3] = lost();
+  }
+  const int64_t at = int64_t(a.row) * sg.count + a.seg;
+  write_state<S>(m, sg.state + at * dk * dv, part, dk, dv, lane);
+  if (tid == 0) sg.keep[at] = ok ? kept : lost();
+  end<128>(tmem, warp);
+}
+
+}  // namespace tensor
+}  // namespace linear
+}  // namespace zb

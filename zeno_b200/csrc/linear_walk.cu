@@ -91,7 +91,12 @@ __global__ void __launch_bounds__(1024) linear_decay_kernel(const double* from, 
   if (threadIdx.x == 0) to[blockIdx.x] = float(sum);
 }
 
+std::atomic<uint64_t> wait_limit{2000000000};  // nanoseconds that a block waits for its own products
+
 }  // namespace
+
+uint64_t linear_wait_limit(uint64_t nanoseconds) { return wait_limit.exchange(nanoseconds); }
+uint64_t linear_patience() { return wait_limit.load(); }
 
 cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t stream) {
   // at most a few hundred rows are cut into segments

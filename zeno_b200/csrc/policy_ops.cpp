@@ -191,6 +191,8 @@ int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream) 
   return zb::status(what, zb::launch_linear_step(*p, static_cast<cudaStream_t>(cuda_stream)));
 }
 
+uint64_t zeno_linear_attention_wait_limit(uint64_t nanoseconds) { return zb::linear_wait_limit(nanoseconds); }
+
 uint64_t zeno_linear_attention_saved_bytes(const ZenoLinearAttention* p) {
   return p && zb::shape_fault(*p).empty() ? zb::linear_saved_bytes(*p) : 0;
 }

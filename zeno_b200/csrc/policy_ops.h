@@ -70,6 +70,8 @@ struct LinearShared {  // gradients of a key head's rows from those of its value
 cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t stream);
 cudaError_t launch_linear_shared(const LinearShared& q, const LinearShared& k, uint32_t batch, uint32_t dtype, cudaStream_t stream);
 cudaError_t launch_linear_decay(const double* from, uint64_t count, uint32_t heads, float* to, cudaStream_t stream);
+uint64_t linear_wait_limit(uint64_t nanoseconds);  // sets it, returns the one before
+uint64_t linear_patience();
 uint64_t linear_saved_bytes(const ZenoLinearAttention& p);
 uint64_t linear_forward_workspace(const ZenoLinearAttention& p);
 uint64_t linear_backward_workspace(const ZenoLinearAttention& p);
