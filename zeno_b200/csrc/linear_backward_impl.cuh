@@ -42,6 +42,13 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
     }
     if (sizeof(T) == 2 && warp_a_head(p) && !d.d_final) {
       e = backward_by_warps(p, d, extra, vec, stream);
+    } else if constexpr (kTensor<S>) {
+      static std::atomic<uint64_t> devices{0};
+      auto kernel = tensor::linear_tensor_backward_kernel<S>;
+      e = allow_smem(kernel, tensor::kBackwardBytes, devices);
+      if (e != cudaSuccess) return e;
+      kernel<<<grid_of(p, c.count), S::THREADS, tensor::kBackwardBytes, stream>>>(p, d, sg, extra, linear_patience());
+      e = cudaGetLastError();
     } else {
       constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
       auto kernel = linear_backward_kernel<S, BLOCKS>;

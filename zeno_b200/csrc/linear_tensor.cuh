@@ -302,17 +302,19 @@ using SegmentShape = Shape<bf16, D, C, 8, FULL>;   // segments
 // Not a number, where a block gave up.
 __device__ __forceinline__ float lost() { return __uint_as_float(0x7fffffffu); }
 
-constexpr int kForwardBytes = 1024 + 2 * (3 * kTok + 2 * kPair + 2 * kState + 3 * kTok) + int(sizeof(Gates<C>)) + int(sizeof(Control));
-constexpr int kSegmentBytes = 1024 + 2 * (2 * kTok + 3 * kTok) + int(sizeof(Gates<C>)) + int(sizeof(Control));
+constexpr int kForwardBytes = 1024 + 2 * (5 * kTok + 2 * kPair + 2 * kState + 3 * kTok) + 2 * int(sizeof(Gates<C>)) + int(sizeof(Control));
+constexpr int kSegmentBytes = 1024 + 2 * (3 * kTok + 3 * kTok) + 2 * int(sizeof(Gates<C>)) + int(sizeof(Control));
 
+// The next chunk's rows and gates are fetched while a chunk's products run: Q and V into a second tile each, K, once it is not needed
+// any more, into its own.  The outputs leave by way of P's tiles.
 template <class S>
 __global__ void __launch_bounds__(S::THREADS, 1)
 linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, const Segments sg, const uint64_t patience) {
   extern __shared__ char smem[];
-  plane_t* q = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
-  plane_t *k = q + kTok, *v = k + kTok, *pr = v + kTok, *st = pr + 2 * kPair, *wk = st + 2 * kState;
-  Gates<C>& s = *reinterpret_cast<Gates<C>*>(wk + 3 * kTok);
-  Control& control = *reinterpret_cast<Control*>(&s + 1);
+  plane_t* const q0 = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
+  plane_t *const v0 = q0 + 2 * kTok, *const k = v0 + 2 * kTok, *const pr = k + kTok, *const st = pr + 2 * kPair, *const wk = st + 2 * kState;
+  Gates<C>* const gates = reinterpret_cast<Gates<C>*>(wk + 3 * kTok);
+  Control& control = *reinterpret_cast<Control*>(gates + 2);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = warp & 3, ct = warp >> 2;  // 16 tokens, and a quarter of a product's columns
   const int dk = S::FULL ? D : int(p.key_dim), dv = S::FULL ? D : int(p.value_dim);
@@ -324,6 +326,15 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   const float* gg = place<float>(p.g, a.b, a.h);
   const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
   bf16* go = place<bf16>(p.out, a.b, a.h);
+  auto tokens_of = [&](int c) { return int(min(int64_t(C), int64_t(p.tokens) - int64_t(c) * C)); };
+  auto fetch_k = [&](int c) { load_tile(k, gk + int64_t(c) * C * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, tokens_of(c), mv); };
+  auto fetch = [&](int c) {
+    const int n = tokens_of(c), turn = (c - a.c0) & 1;
+    load_tile(q0 + turn * kTok, gq + int64_t(c) * C * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, mv);
+    load_tile(v0 + turn * kTok, gv + int64_t(c) * C * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, mv);
+    if (warp == S::NW - 1) load_gates<C>(gates[turn], gg, p.g.stride[1], gr, p.reset.stride[1], int64_t(c) * C, n, lane);
+  };
+  if (a.c0 < a.c1) fetch_k(a.c0), fetch(a.c0);
   begin<512>(control, warp, tid);
   const uint32_t tmem = control.tmem;
   // columns of TMEM: S^T q's and P's part of the outputs, the update, the scores
@@ -340,19 +351,17 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
 
   for (int c = a.c0; c < a.c1; ++c) {
     const int64_t t0 = int64_t(c) * C;
-    const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
+    const int n = tokens_of(c), turn = (c - a.c0) & 1;
+    plane_t *const q = q0 + turn * kTok, *const v = v0 + turn * kTok;
+    const Gates<C>& s = gates[turn];
     const bool have = c > a.c0 || first, goes_on = c + 1 < a.c1 || (c + 1 == a.chunks && p.final_state);
-    __syncthreads();  // the last chunk's results have left
-    load_tile(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, mv);
-    load_tile(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, mv);
-    load_tile(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, mv);
-    if (warp == S::NW - 1) load_gates<C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     if (have) dump<S, 2>(m, st, part, lane);
     if (p.saved && c > 0) write_state<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane);
     copies_landed();
+    const bool odd = tile_odd(q, mv) || tile_odd(k, mv) || tile_odd(v, mv);
     fence_shared();
     fence_before();
-    __syncthreads();
+    const bool bad_rows = __syncthreads_or(odd);
     if (tid == 0) {
       fence_after();
       const uint32_t aq = delta::smem_at(q), ak = delta::smem_at(k);
@@ -360,6 +369,7 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
       for (int kk = 0; kk < 8; ++kk) mma(t_scores, along<C>(aq, kk), along<C>(ak, kk), kInstruction<64, 64, false, false>, kk > 0);
     }
     products.issued(tid == 0);
+    if (c + 1 < a.c1) fetch(c + 1);
     if (goes_on) weigh(wk, k, s.to_end, 1.0f, mv);
     ok = products.done();
     if (!ok) break;
@@ -414,6 +424,7 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
       }
     }
     products.issued(tid == 0);
+    if (c + 1 < a.c1 && !bad_rows) fetch_k(c + 1);
     ok = products.done();
     if (!ok) break;
 
@@ -435,8 +446,7 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
           y = f == 0.0f ? y : fmaf(f * p.scale, more[j][e >> 2][e & 3], y);
         }
     }
-    const bool bad = __syncthreads_or(not_finite(acc));
-    if (bad) {
+    if (__syncthreads_or(not_finite(acc))) {  // (products have overflowed, where the rows are finite)
 #pragma unroll 1
       for (int x = 0; x < 16; ++x) {
         const int i = rt * 16 + (lane >> 2) + ((x >> 1) & 1) * 8, cc = col + (x >> 3) * 16 + ((x >> 2) & 1) * 8 + (lane & 3) * 2 + (x & 1);
@@ -461,16 +471,18 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          *reinterpret_cast<uint32_t*>(q + spot<C>(rt * 16 + (lane >> 2) + r * 8, col + j * 16 + h * 8 + (lane & 3) * 2)) =
+          *reinterpret_cast<uint32_t*>(pr + spot<C>(rt * 16 + (lane >> 2) + r * 8, col + j * 16 + h * 8 + (lane & 3) * 2)) =
               pack_round(acc[j][h][2 * r], acc[j][h][2 * r + 1]);
     if (goes_on) {
-      if (bad) merge_masked<S>(m, k, v, s.to_end, 1.0f, s.keep, n, part, lane);
+      if (bad_rows) merge_masked<S>(m, k, v, s.to_end, 1.0f, s.keep, n, part, lane);
       else merge<S>(m, t_update, s.keep, part);
     }
     fence_before();
     __syncthreads();
-    store_tile(go + t0 * p.out.stride[1], p.out.stride[1], q, dv, sg.vec & kVecOut, n, mv);
+    if (bad_rows && c + 1 < a.c1) fetch_k(c + 1);
+    store_tile(go + t0 * p.out.stride[1], p.out.stride[1], pr, dv, sg.vec & kVecOut, n, mv);
   }
+  copies_landed();
   if (!ok) {  // what this block would have written
     for (int64_t t = int64_t(a.c0) * C + warp; t < min(int64_t(a.c1) * C, int64_t(p.tokens)); t += S::NW)
       for (int x = lane; x < dv; x += 32) go[t * p.out.stride[1] + x] = __float2bfloat16_rn(lost());
@@ -486,16 +498,17 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   end<512>(tmem, warp);
 }
 
-// What each segment adds to the state behind it, as linear_segment_kernel.
+// What each segment adds to the state behind it, as linear_segment_kernel.  The next chunk is fetched while a chunk's products run (X, whose limbs
+// they read, into its own tile).
 template <class S>
 __global__ void __launch_bounds__(S::THREADS, 2)
 linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, const ZenoTensor tx, const ZenoTensor ty, const Segments sg, const bool reverse,
                              const uint64_t patience) {
   extern __shared__ char smem[];
-  plane_t* x = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
-  plane_t *y = x + kTok, *wx = y + kTok;
-  Gates<C>& s = *reinterpret_cast<Gates<C>*>(wx + 3 * kTok);
-  Control& control = *reinterpret_cast<Control*>(&s + 1);
+  plane_t* const x = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
+  plane_t *const y0 = x + kTok, *const wx = y0 + 2 * kTok;
+  Gates<C>* const gates = reinterpret_cast<Gates<C>*>(wx + 3 * kTok);
+  Control& control = *reinterpret_cast<Control*>(gates + 2);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int dk = S::FULL ? D : int(p.key_dim), dv = S::FULL ? D : int(p.value_dim);
   const At a = block_at(p, sg, reverse ? 1 : 0, C);
@@ -504,6 +517,15 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   const float* gg = place<float>(p.g, a.b, a.h);
   const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
   const bool vx = sg.vec & (reverse ? kVecQ : kVecK), vy = sg.vec & (reverse ? kVecOut : kVecV);
+  const int steps = a.c1 - a.c0;
+  auto fetch = [&](int step) {
+    const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * C;
+    const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
+    load_tile(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, mv);
+    load_tile(y0 + (step & 1) * kTok, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, mv);
+    if (warp == S::NW - 1) load_gates<C>(gates[step & 1], gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+  };
+  fetch(0);
   begin<128>(control, warp, tid);
   const uint32_t tmem = control.tmem;
   Products products{delta::smem_at(&control.bar), 0, patience};
@@ -512,20 +534,20 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   clear<S>(m);
   float kept = 1.0f;
   bool ok = true;
-  for (int step = 0; step < a.c1 - a.c0; ++step) {
-    const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * C;
-    const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
-    __syncthreads();
-    load_tile(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, mv);
-    load_tile(y, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, mv);
-    if (warp == S::NW - 1) load_gates<C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+  for (int step = 0; step < steps; ++step) {
+    const Gates<C>& s = gates[step & 1];
+    const plane_t* y = y0 + (step & 1) * kTok;
+    const float* weight = reverse ? s.carried : s.to_end;
+    const float factor = reverse ? p.scale : 1.0f;
     copies_landed();
     const bool bad = __syncthreads_or(tile_odd(x, mv) || tile_odd(y, mv));
-    const float* weight = reverse ? s.carried : s.to_end;
-    const float factor = reverse ? p.scale : 1.0f, keep = step ? s.keep : 0.0f;
+    const float keep = step ? s.keep : 0.0f;
     kept *= s.keep;
     if (bad) {
-      merge_masked<S>(m, x, y, weight, factor, keep, n, part, lane);
+      const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * C;
+      merge_masked<S>(m, x, y, weight, factor, keep, int(min(int64_t(C), int64_t(p.tokens) - t0)), part, lane);
+      __syncthreads();
+      if (step + 1 < steps) fetch(step + 1);
       continue;
     }
     weigh(wx, x, weight, factor, mv);
@@ -542,11 +564,13 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
           mma(tmem, across<C>(aw + l * kTok * 2, kk), across<C>(ay, kk), kInstruction<128, 128, true, true>, l < 2 || kk > 0);
     }
     products.issued(tid == 0);
+    if (step + 1 < steps) fetch(step + 1);
     ok = products.done();
     if (!ok) break;
     merge<S>(m, tmem, keep, part);
     fence_before();
   }
+  copies_landed();
   if (!ok) {
 #pragma unroll
     for (int j = 0; j < S::NM; ++j)
@@ -557,6 +581,464 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   write_state<S>(m, sg.state + at * dk * dv, part, dk, dv, lane);
   if (tid == 0) sg.keep[at] = ok ? kept : lost();
   end<128>(tmem, warp);
+}
+
+// ---------------------------------------------------------------- gradients
+struct BackwardSums {
+  float x[4][C], y[4][C];  // x_i and y_j over each quarter of the columns
+  float pairs[4][C];       // sum over the rows of a tile i >= t of the A_ij in front of t in t's quarter
+  float row[4][C];         // sum of A_ij over each quarter
+  float state[16];         // <S, R> over each warp's part
+};
+constexpr int kBackwardBytes =
+    1024 + 2 * (4 * kTok + 4 * kPair + 3 * kState) + int(sizeof(Gates<C>)) + int(sizeof(BackwardSums)) + int(sizeof(Control));
+
+// acc = acc + f[i] scale more (what f is zero for is left out).  Returns the products of that with the lane's two rows of X over its columns.
+__device__ __forceinline__ float2 add_and_dot(float (&acc)[2][2][4], const float (&more)[2][2][4], const float* f, float scale, const plane_t* x, int rt,
+                                              int col, int lane) {
+  const int i0 = rt * 16 + (lane >> 2);
+  const float f0 = f[i0], f1 = f[i0 + 8], s0 = f0 * scale, s1 = f1 * scale;
+  float d0 = 0.0f, d1 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = col + j * 16 + h * 8 + (lane & 3) * 2;
+      const uint32_t w0 = *reinterpret_cast<const uint32_t*>(x + spot<C>(i0, at)), w1 = *reinterpret_cast<const uint32_t*>(x + spot<C>(i0 + 8, at));
+      float y[4];
+      y[0] = f0 == 0.0f ? 0.0f : more[j][h][0] * s0, y[1] = f0 == 0.0f ? 0.0f : more[j][h][1] * s0;
+      y[2] = f1 == 0.0f ? 0.0f : more[j][h][2] * s1, y[3] = f1 == 0.0f ? 0.0f : more[j][h][3] * s1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][h][e] += y[e];
+      d0 = fmaf(lower(w0), y[0], fmaf(upper(w0), y[1], d0)), d1 = fmaf(lower(w1), y[2], fmaf(upper(w1), y[3], d1));
+    }
+  return make_float2(f0 == 0.0f ? 0.0f : d0, f1 == 0.0f ? 0.0f : d1);
+}
+
+// One element of a gradient over the pairs that the mask leaves (ROWS: of a query's): pairs with y's column, after `sum` from the state.
+template <bool ROWS>
+__device__ __noinline__ float over_pairs(const Gates<C>& s, float sum, const plane_t* pairs, const plane_t* y, int at, int col, int n) {
+  for (int o = ROWS ? 0 : at; o < (ROWS ? at + 1 : n); ++o) {
+    const int i = ROWS ? at : o, j = ROWS ? o : at;
+    if (pair_decay(s.token[i], s.token[j], meets(s.token[i], s.token[j], i, j)) != 0.0f)
+      sum = fmaf(value_at<2, C>(pairs, kPair, i, j), value_at<1, C>(y, 0, o, col), sum);
+  }
+  return sum;
+}
+template <class F>
+__device__ __forceinline__ void again(float (&acc)[2][2][4], int rt, int col, int n, int width, int lane, F&& element) {
+#pragma unroll 1
+  for (int x = 0; x < 16; ++x) {
+    const int i = rt * 16 + (lane >> 2) + ((x >> 1) & 1) * 8, c = col + (x >> 3) * 16 + ((x >> 2) & 1) * 8 + (lane & 3) * 2 + (x & 1);
+    if (i >= n || c >= width) continue;
+    const float y = element(i, c);
+#pragma unroll
+    for (int z = 0; z < 16; ++z)
+      if (z == x) acc[z >> 3][(z >> 2) & 1][z & 3] = y;
+  }
+}
+__device__ __forceinline__ void stage_tile(plane_t* to, const float (&acc)[2][2][4], int rt, int col, int lane) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        *reinterpret_cast<uint32_t*>(to + spot<C>(rt * 16 + (lane >> 2) + r * 8, col + j * 16 + h * 8 + (lane & 3) * 2)) =
+            pack_round(acc[j][h][2 * r], acc[j][h][2 * r + 1]);
+}
+
+// As linear_backward_kernel.  Four rounds of products a chunk: the scores and S's part of dQ; all that P and D are in, while R's limbs take the
+// place of S's; R's part of dK and dV; the update of R, whose weighted queries take the place of its limbs.
+template <class S>
+__global__ void __launch_bounds__(S::THREADS, 1)
+linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __grid_constant__ ZenoLinearAttentionGrads d, const Segments sg,
+                              const BackwardOut extra, const uint64_t patience) {
+  extern __shared__ char smem[];
+  plane_t* const q = reinterpret_cast<plane_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) / 1024 * 1024);
+  plane_t *const k = q + kTok, *const v = k + kTok, *const o = v + kTok, *const pr = o + kTok, *const dp = pr + 2 * kPair, *const st = dp + 2 * kPair;
+  Gates<C>& s = *reinterpret_cast<Gates<C>*>(st + 3 * kState);
+  BackwardSums& sums = *reinterpret_cast<BackwardSums*>(&s + 1);
+  Control& control = *reinterpret_cast<Control*>(&sums + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rt = warp & 3, ct = warp >> 2, col = ct * 32;
+  const int dk = S::FULL ? D : int(p.key_dim), dv = S::FULL ? D : int(p.value_dim);
+  const At a = block_at(p, sg, 0, C);
+  if (a.b >= p.batch) return;
+  const Mover<S::THREADS> mv(tid);
+  const int64_t state_size = int64_t(dk) * dv;
+  const bool shared = extra.shared_q != nullptr;
+  const bf16 *gq = place<bf16>(p.q, a.b, a.kh), *gk = place<bf16>(p.k, a.b, a.kh), *gv = place<bf16>(p.v, a.b, a.h), *go = place<bf16>(d.d_out, a.b, a.h);
+  const float* gg = place<float>(p.g, a.b, a.h);
+  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
+  bf16 *wq = place<bf16>(d.d_q, a.b, a.kh), *wk = place<bf16>(d.d_k, a.b, a.kh), *wv = place<bf16>(d.d_v, a.b, a.h);
+  const int64_t shared_stride = int64_t(p.value_heads) * dk;
+  begin<512>(control, warp, tid);
+  const uint32_t tmem = control.tmem, quarter = uint32_t(rt * 32) << 16;
+  // regions of 128 columns: scores, then P's part of dV, then the update; S's part of dQ, then R's of dK; D's part of dQ, then R's of dV; D's of dK
+  const uint32_t t0_ = tmem, t1_ = tmem + 128, t2_ = tmem + 256, t3_ = tmem + 384;
+  Products products{delta::smem_at(&control.bar), 0, patience};
+  const uint32_t aq = delta::smem_at(q), ak = delta::smem_at(k), av = delta::smem_at(v), ao = delta::smem_at(o), ap = delta::smem_at(pr),
+                 ad = delta::smem_at(dp), as = delta::smem_at(st);
+
+  const Part<S> part = part_of<S>(warp);
+  float m[S::NM][2][4];
+  const bool last_segment = a.c1 == a.chunks;
+  const float* behind = !last_segment ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
+                                      : d.d_final ? d.d_final + int64_t(a.row) * state_size : nullptr;
+  if (behind) read_state<S>(m, behind, part, dk, dv, lane);
+  else clear<S>(m);
+  const bool each = d.d_g.data != nullptr;  // every token's decay has a gradient of its own
+  double decay_sum = 0.0;
+  bool ok = true;
+
+  for (int c = a.c1 - 1; c >= a.c0; --c) {
+    const int64_t t0 = int64_t(c) * C;
+    const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
+    const float* front = c > 0 ? p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size
+                               : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+    const bool have_r = c + 1 < a.c1 || behind, goes_on = c > a.c0 || (c == 0 && d.d_initial);
+    __syncthreads();  // the last chunk's results have left
+    load_tile(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, mv);
+    load_tile(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, mv);
+    load_tile(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, mv);
+    load_tile(o, go + t0 * d.d_out.stride[1], d.d_out.stride[1], dv, sg.vec & kVecOut, n, mv);
+    if (warp == S::NW - 1) load_gates<C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    float state_dot = 0.0f;  // <S, R> over this thread's elements
+    if (front) {
+      float x[S::NM][2][4];
+      read_state<S>(x, front, part, dk, dv, lane);
+      float dot = 0.0f;
+#pragma unroll
+      for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(x[j][e >> 2][e & 3], m[j][e >> 2][e & 3], dot);
+      dump<S, 3>(x, st, part, lane);
+      state_dot = have_r ? dot : 0.0f;
+      if (each) {
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(kAll, dot, x);
+        if (lane == 0) sums.state[warp] = dot;
+      }
+    }
+    copies_landed();
+    const bool odd = tile_odd(q, mv) || tile_odd(o, mv);
+    fence_shared();
+    fence_before();
+    const bool bad_rows = __syncthreads_or(odd);  // (of the update's)
+    if (tid == 0) {
+      fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma(t0_, along<C>(aq, kk), along<C>(ak, kk), kInstruction<64, 64, false, false>, kk > 0);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma(t0_ + 64, along<C>(ao, kk), along<C>(av, kk), kInstruction<64, 64, false, false>, kk > 0);
+      if (front) {
+#pragma unroll
+        for (int l = 2; l >= 0; --l)
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            mma(t1_, along<C>(ao, kk), along<D>(as + l * kState * 2, kk), kInstruction<64, 128, false, false>, l < 2 || kk > 0);
+      }
+    }
+    products.issued(tid == 0);
+    ok = products.done();
+    if (!ok) break;
+
+    // P, D, and what the pairs give the decays: this thread's part of their gradient, where all tokens of the head have one
+    float decays = each || s.keep == 0.0f ? 0.0f : state_dot * s.keep * float(n);
+    {
+      float sp[1][2][4], so[1][2][4];
+      fetch2(&sp[0][0][0], t0_ + quarter + ct * 16);
+      fetch2(&so[0][0][0], t0_ + quarter + 64 + ct * 16);
+      fetched(sp);
+      fetched(so);
+      const int i0 = rt * 16 + (lane >> 2);
+      const Token ti[2] = {s.token[i0], s.token[i0 + 8]};
+      float before[2] = {0.0f, 0.0f};  // of the quarter's columns so far, for each of the lane's two rows
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int cc = ct * 16 + h * 8 + (lane & 3) * 2;
+        const Token u0 = s.token[cc], u1 = s.token[cc + 1];
+        float pass[2][2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = i0 + r * 8, at = spot<C>(i, cc);
+          const bool m0 = meets(ti[r], u0, i, cc), m1 = meets(ti[r], u1, i, cc + 1);
+          const float f0 = pair_decay(ti[r], u0, m0) * p.scale, f1 = pair_decay(ti[r], u1, m1) * p.scale;
+          const float o0 = so[0][h][2 * r], o1 = so[0][h][2 * r + 1];
+          const float p0 = m0 ? sp[0][h][2 * r] * f0 : 0.0f, p1 = m1 ? sp[0][h][2 * r + 1] * f1 : 0.0f;
+          uint32_t w[2];
+          split<2>(p0, p1, w);
+          *reinterpret_cast<uint32_t*>(pr + at) = w[0], *reinterpret_cast<uint32_t*>(pr + kPair + at) = w[1];
+          split<2>(m0 ? o0 * f0 : 0.0f, m1 ? o1 * f1 : 0.0f, w);
+          *reinterpret_cast<uint32_t*>(dp + at) = w[0], *reinterpret_cast<uint32_t*>(dp + kPair + at) = w[1];
+          pass[r][0] = m0 ? p0 * o0 : 0.0f, pass[r][1] = m1 ? p1 * o1 : 0.0f;
+        }
+        if (!each) {  // a pair passes i - j tokens
+          const float far = float(i0 - cc);
+          decays = fmaf(pass[0][0], far, fmaf(pass[0][1], far - 1.0f, fmaf(pass[1][0], far + 8.0f, fmaf(pass[1][1], far + 7.0f, decays))));
+          continue;
+        }
+        float passes[2] = {0.0f, 0.0f};  // tokens cc and cc + 1, over the lane's rows
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = i0 + r * 8;
+          float sum = pass[r][0] + pass[r][1];
+          const float x1 = __shfl_up_sync(kAll, sum, 1, 4);
+          if ((lane & 3) >= 1) sum += x1;
+          const float x2 = __shfl_up_sync(kAll, sum, 2, 4);
+          if ((lane & 3) >= 2) sum += x2;
+          float left = __shfl_up_sync(kAll, sum, 1, 4);
+          left = (lane & 3) ? before[r] + left : before[r];
+          before[r] += __shfl_sync(kAll, sum, 3, 4);
+          if (i >= cc) passes[0] += left;
+          if (i >= cc + 1) passes[1] += left + pass[r][0];
+        }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          passes[0] += __shfl_xor_sync(kAll, passes[0], x);
+          passes[1] += __shfl_xor_sync(kAll, passes[1], x);
+        }
+        if (lane < 4) sums.pairs[rt][cc] = passes[0], sums.pairs[rt][cc + 1] = passes[1];
+      }
+      if (each && (lane & 3) == 0) sums.row[ct][i0] = before[0], sums.row[ct][i0 + 8] = before[1];
+    }
+    fence_shared();
+    fence_before();
+    __syncthreads();
+    if (tid == 0) {
+      fence_after();
+#pragma unroll
+      for (int l = 1; l >= 0; --l)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          mma(t2_, along<C>(ad + l * kPair * 2, kk), across<C>(ak, kk), kInstruction<64, 128, false, true>, l == 0 || kk > 0);
+          mma(t3_, across<C>(ad + l * kPair * 2, kk), across<C>(aq, kk), kInstruction<64, 128, true, true>, l == 0 || kk > 0);
+          mma(t0_, across<C>(ap + l * kPair * 2, kk), across<C>(ao, kk), kInstruction<64, 128, true, true>, l == 0 || kk > 0);
+        }
+    }
+    products.issued(tid == 0);
+    if (have_r) {  // (S's limbs have been read)
+      dump<S, 3>(m, st, part, lane);
+      fence_shared();
+    }
+    ok = products.done();
+    if (!ok) break;
+
+    float dq[2][2][4], dk_[2][2][4], dv_[2][2][4];
+    fetch4(&dq[0][0][0], t2_ + quarter + col);
+    fetch4(&dk_[0][0][0], t3_ + quarter + col);
+    fetch4(&dv_[0][0][0], t0_ + quarter + col);
+    if (front) {
+      float more[2][2][4];
+      fetch4(&more[0][0][0], t1_ + quarter + col);
+      fetched(more);
+      fetched(dq);
+      const float2 x = add_and_dot(dq, more, s.carried, p.scale, q, rt, col, lane);
+      const float i = float(rt * 16 + (lane >> 2));
+      if (each) keep_rows(sums.x[ct], x, rt, lane);
+      else decays = fmaf(x.x, i + 1.0f, fmaf(x.y, i + 9.0f, decays));  // the state in front passes every token up to this one
+    }
+    fetched(dq), fetched(dk_), fetched(dv_);
+    fence_before();
+    __syncthreads();
+    if (have_r) {
+      if (tid == 0) {
+        fence_after();
+#pragma unroll
+        for (int l = 2; l >= 0; --l)
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            mma(t1_, along<C>(av, kk), along<D>(as + l * kState * 2, kk), kInstruction<64, 128, false, false>, l < 2 || kk > 0);
+            if (l < 2) mma(t2_, along<C>(ak, kk), across<D>(as + l * kState * 2, kk), kInstruction<64, 128, false, true>, l == 0 || kk > 0);
+          }
+      }
+      products.issued(tid == 0);
+      ok = products.done();
+      if (!ok) break;
+      float more[2][2][4];
+      fetch4(&more[0][0][0], t1_ + quarter + col);
+      fetched(more);
+      const float2 y = add_and_dot(dk_, more, s.to_end, 1.0f, k, rt, col, lane);
+      const float rest = float(n - 1 - rt * 16 - (lane >> 2));
+      if (each) keep_rows(sums.y[ct], y, rt, lane);
+      else decays = fmaf(y.x, rest, fmaf(y.y, rest - 8.0f, decays));  // what begins here passes the tokens behind it
+      fetch4(&more[0][0][0], t2_ + quarter + col);
+      fetched(more);
+      const float e0 = s.to_end[rt * 16 + (lane >> 2)], e1 = s.to_end[rt * 16 + (lane >> 2) + 8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          float& z = dv_[j][x >> 2][x & 3];
+          const float e = x & 2 ? e1 : e0;
+          z = e == 0.0f ? z : fmaf(e, more[j][x >> 2][x & 3], z);
+        }
+    }
+    decay_sum += double(decays);
+    if (__syncthreads_or(not_finite(dq) || not_finite(dk_) || not_finite(dv_))) {
+      again(dq, rt, col, n, dk, lane, [&](int i, int cc) {
+        float y = 0.0f;
+        if (front && s.carried[i] != 0.0f) {
+          for (int e = 0; e < dv; ++e) y = fmaf(value_at<1, C>(o, 0, i, e), front[cc * dv + e], y);
+          y *= s.carried[i] * p.scale;
+        }
+        return over_pairs<true>(s, y, dp, k, i, cc, n);
+      });
+      again(dk_, rt, col, n, dk, lane, [&](int j, int cc) {
+        float y = 0.0f;
+        if (have_r && s.to_end[j] != 0.0f) {
+          for (int e = 0; e < dv; ++e) y = fmaf(value_at<1, C>(v, 0, j, e), value_at<3, D>(st, kState, cc, e), y);
+          y *= s.to_end[j];
+        }
+        return over_pairs<false>(s, y, dp, q, j, cc, n);
+      });
+      again(dv_, rt, col, n, dv, lane, [&](int j, int cc) {
+        float y = 0.0f;
+        if (have_r && s.to_end[j] != 0.0f) {
+          for (int e = 0; e < dk; ++e) y = fmaf(value_at<1, C>(k, 0, j, e), value_at<3, D>(st, kState, e, cc), y);
+          y *= s.to_end[j];
+        }
+        return over_pairs<false>(s, y, pr, o, j, cc, n);
+      });
+      __syncthreads();
+    }
+    if (goes_on && !bad_rows) {
+      weigh(st, q, s.carried, p.scale, mv);
+      fence_shared();
+      fence_before();
+      __syncthreads();
+      if (tid == 0) {
+        fence_after();
+#pragma unroll
+        for (int l = 2; l >= 0; --l)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma(t0_, across<C>(as + l * kTok * 2, kk), across<C>(ao, kk), kInstruction<128, 128, true, true>, l < 2 || kk > 0);
+      }
+      products.issued(tid == 0);
+    }
+    // results by way of tiles that are not needed any more (Q and dO still are)
+    if (shared) {
+      const int64_t at = (int64_t(a.b) * p.tokens + t0) * shared_stride + int64_t(a.h) * dk;
+      store_float(extra.shared_q + at, shared_stride, dq, rt * 16, col, n, dk, lane);
+      store_float(extra.shared_k + at, shared_stride, dk_, rt * 16, col, n, dk, lane);
+    } else {
+      stage_tile(k, dq, rt, col, lane);
+      stage_tile(v, dk_, rt, col, lane);
+    }
+    stage_tile(pr, dv_, rt, col, lane);
+    if (each && warp == S::NW - 1) {
+      // the decays: neighbouring tokens 2 lane and 2 lane + 1
+      float z = 0.0f;
+      if (front && have_r && s.keep != 0.0f) {
+        for (int w = 0; w < S::NW; ++w) z += sums.state[w];
+        z *= s.keep;
+      }
+      float dg[2], here[2] = {0.0f, 0.0f}, ahead[2] = {0.0f, 0.0f};  // what ends at this token; what begins at it
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = lane * 2 + u;
+        dg[u] = z;
+        if (t < n) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (front) here[u] += sums.x[x][t];
+            if (have_r) ahead[u] += sums.y[x][t];
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r * 16 + 15 >= t) dg[u] += sums.pairs[r][t];
+        }
+      }
+      // sums over the tokens in front, and from this one on: x_i, and pairs whose first token lies in an earlier quarter of the columns
+      float in_front = ahead[0] + ahead[1];
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const float y = __shfl_up_sync(kAll, in_front, x);
+        if (lane >= x) in_front += y;
+      }
+      in_front = __shfl_up_sync(kAll, in_front, 1);
+      if (lane == 0) in_front = 0.0f;
+      dg[0] += in_front, dg[1] += in_front + ahead[0];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float rest[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) rest[u] = g == 3 ? here[u] : lane * 2 + u < n ? sums.row[g][lane * 2 + u] : 0.0f;
+        float sum = rest[0] + rest[1];
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const float y = __shfl_down_sync(kAll, sum, x);
+          if (lane + x < 32) sum += y;
+        }
+        float from = __shfl_down_sync(kAll, sum, 1);
+        if (lane == 31) from = 0.0f;
+        if (g == 3 || lane * 2 >= (g + 1) * 16) {  // (both tokens of a lane are in one quarter)
+          dg[1] += from + rest[1];
+          dg[0] += from + rest[1] + rest[0];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = lane * 2 + u;
+        if (t < n) {
+          decay_sum += double(dg[u]);
+          place<float>(d.d_g, a.b, a.h)[(t0 + t) * d.d_g.stride[1]] = dg[u];
+        }
+      }
+    }
+    if (goes_on) {
+      if (bad_rows) {
+        merge_masked<S>(m, q, o, s.carried, p.scale, s.keep, n, part, lane);
+      } else {
+        ok = products.done();
+        if (!ok) break;
+        merge<S>(m, t0_, s.keep, part);
+      }
+    }
+    fence_before();
+    __syncthreads();
+    if (!shared) {
+      store_tile(wq + t0 * d.d_q.stride[1], d.d_q.stride[1], k, dk, sg.vec & kVecDq, n, mv);
+      store_tile(wk + t0 * d.d_k.stride[1], d.d_k.stride[1], v, dk, sg.vec & kVecDk, n, mv);
+    }
+    store_tile(wv + t0 * d.d_v.stride[1], d.d_v.stride[1], pr, dv, sg.vec & kVecDv, n, mv);
+  }
+  if (!ok) {  // what this block would have written
+    for (int64_t t = int64_t(a.c0) * C + warp; t < min(int64_t(a.c1) * C, int64_t(p.tokens)); t += S::NW) {
+      for (int x = lane; x < max(dk, dv); x += 32) {
+        if (x < dv) wv[t * d.d_v.stride[1] + x] = __float2bfloat16_rn(lost());
+        if (x >= dk) continue;
+        if (shared) {
+          const int64_t at = (int64_t(a.b) * p.tokens + t) * shared_stride + int64_t(a.h) * dk + x;
+          extra.shared_q[at] = extra.shared_k[at] = lost();
+        } else {
+          wq[t * d.d_q.stride[1] + x] = __float2bfloat16_rn(lost()), wk[t * d.d_k.stride[1] + x] = __float2bfloat16_rn(lost());
+        }
+      }
+      if (each && lane == 0) place<float>(d.d_g, a.b, a.h)[t * d.d_g.stride[1]] = lost();
+    }
+#pragma unroll
+    for (int j = 0; j < S::NM; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[j][e >> 2][e & 3] = lost();
+    decay_sum = double(lost());
+  }
+  if (a.c0 == 0 && d.d_initial) write_state<S>(m, d.d_initial + int64_t(a.row) * state_size, part, dk, dv, lane);
+  if (extra.decay) {
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) decay_sum += __shfl_xor_sync(kAll, decay_sum, x);
+    double* part_sum = reinterpret_cast<double*>(&s);  // (where the gates were)
+    __syncthreads();
+    if (lane == 0) part_sum[warp] = decay_sum;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < S::NW; ++w) decay_sum += part_sum[w];
+      extra.decay[(uint64_t(a.h) * p.batch + a.b) * sg.count + a.seg] = decay_sum;
+    }
+  }
+  end<512>(tmem, warp);
 }
 
 }  // namespace tensor
