@@ -135,11 +135,13 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
                                : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
     const bool have_r = c + 1 < a.c1 || behind;
     __syncthreads();  // the last chunk's results have left
+    GateIn<S::C> gates{};
+    if (warp == S::NW - 1) gates = fetch_gates<S::C>(gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     load_rows<S>(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, nt, mv);
     load_rows<S>(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, nt, mv);
     load_rows<S>(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, nt, mv);
     load_rows<S>(o, go + t0 * d.d_out.stride[1], d.d_out.stride[1], dv, sg.vec & kVecOut, n, nt, mv);
-    if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    if (warp == S::NW - 1) scan_gates<S::C>(s, gates, p.g.stride[1] == 0, n, lane);
     float state_dot = 0.0f;  // <S, R> over this thread's elements
     if (front) {
       float x[S::NM][2][4];

@@ -72,10 +72,12 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
     const int n = int(min(int64_t(S::C), int64_t(p.tokens) - t0)), nt = (n + 15) / 16;
     const bool have = c > a.c0 || first;
     __syncthreads();  // the last chunk's results have left
+    GateIn<S::C> gates{};
+    if (warp == S::NW - 1) gates = fetch_gates<S::C>(gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     load_rows<S>(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, nt, mv);
     load_rows<S>(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, nt, mv);
     load_rows<S>(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, nt, mv);
-    if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    if (warp == S::NW - 1) scan_gates<S::C>(s, gates, p.g.stride[1] == 0, n, lane);
     if (have) dump_state<S, S::PL>(m, st, part, lane);
     if (p.saved && c > 0) write_state<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane);
     copies_landed();
@@ -191,9 +193,11 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_segment_kernel(cons
     const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * S::C;
     const int n = int(min(int64_t(S::C), int64_t(p.tokens) - t0)), nt = (n + 15) / 16;
     __syncthreads();
+    GateIn<S::C> gates{};
+    if (warp == S::NW - 1) gates = fetch_gates<S::C>(gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     load_rows<S>(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, nt, mv);
     load_rows<S>(y, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, nt, mv);
-    if (warp == S::NW - 1) load_gates<S::C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    if (warp == S::NW - 1) scan_gates<S::C>(s, gates, p.g.stride[1] == 0, n, lane);
     copies_landed();
     const bool bad = __syncthreads_or(rows_odd<S>(x, dk, nt, mv) || rows_odd<S>(y, dv, nt, mv));
     const float* weight = reverse ? s.carried : s.to_end;

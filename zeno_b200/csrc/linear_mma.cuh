@@ -201,86 +201,121 @@ __device__ __forceinline__ float pair_decay(const Token& ti, const Token& tj, bo
   return meet ? ex2((ti.hi - tj.hi) + (ti.lo - tj.lo)) : 0.0f;
 }
 
-// One warp: the gates of n tokens, C / 32 neighbouring ones a lane.  Sums run from the last reset on, so that what one
-// episode's decays are, not finite included, stays in it.  One decay for all tokens (a stride of 0) needs no sum.
+// One warp: log decays and marks of n tokens, C / 32 neighbouring ones a lane.  Fetched before the rows, whose loads would be waited for first.
 template <int C>
-__device__ __forceinline__ void load_gates(Gates<C>& s, const float* g, int64_t g_stride, const uint8_t* reset, int64_t reset_stride, int64_t t0,
-                                           int n, int lane) {
+struct GateIn {
+  float x[C / 32];
+  uint8_t mark[C / 32];  // as in memory: looked at when the rows are under way
+};
+template <int C>
+__device__ __forceinline__ GateIn<C> fetch_gates(const float* g, int64_t g_stride, const uint8_t* reset, int64_t reset_stride, int64_t t0, int n, int lane) {
   constexpr int U = C / 32;
-  constexpr double kLog2e = 1.4426950408889634;
-  float x[U];
-  bool mark[U];
-  unsigned marks[U];
+  GateIn<C> in;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = lane * U + u;
-    x[u] = i < n ? g[(t0 + i) * g_stride] : 0.0f;
-    mark[u] = i < n && reset && reset[(t0 + i) * reset_stride];
+    in.x[u] = i < n ? g[(t0 + i) * g_stride] : 0.0f;
+    in.mark[u] = i < n && reset ? reset[(t0 + i) * reset_stride] : uint8_t(0);
   }
+  return in;
+}
+
+// One warp: their gates.  Sums run from the last reset on, so that what one episode's decays are, not finite included, stays in it.  They are
+// taken in 64-bit integers, in units of 2^-40 (exact, where a scan in double was a third of a chunk's time); a log decay of 2^22 and
+// more counts as not a number.  One decay for all tokens (`fixed`) needs no sum.
+template <int C>
+__device__ __forceinline__ void scan_gates(Gates<C>& s, GateIn<C> in, bool fixed, int n, int lane) {
+  constexpr int U = C / 32;
+  const float one = __shfl_sync(kAll, in.x[0], 0);
+  bool odd[U], mark[U];
+  unsigned marks[U], odds = 0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    mark[u] = mark[u] || expf(x[u]) == 0.0f;  // a decay to nothing is a reset: the sums behind it stay finite
-    if (mark[u]) x[u] = 0.0f;
+    // a decay to nothing is a reset: the sums behind it stay finite
+    mark[u] = in.mark[u] || ex2(in.x[u] * 1.4426950408889634f) == 0.0f;
+    if (mark[u]) in.x[u] = 0.0f;
+    odd[u] = !(fabsf(in.x[u]) < 4194304.0f);
     marks[u] = __ballot_sync(kAll, mark[u]);
+    odds |= __ballot_sync(kAll, odd[u]);
   }
-  double y[U], last;
-  int all = 0, episode = 0;
+  int all = 0, episode = 0, from = -1;  // from: the last mark in front of the lane's tokens
 #pragma unroll
-  for (int u = 0; u < U; ++u) all += __popc(marks[u]), episode += __popc(marks[u] & ((1u << lane) - 1));
-  if (g_stride == 0) {
-    int from = -1;  // the last mark in front of the lane's tokens, as a token; the sum counts from the one behind it
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned m = marks[u] & ((1u << lane) - 1);
-      if (m) from = max(from, (31 - __clz(m)) * U + u);
-    }
-    const double step = double(g[0]) * kLog2e;
+  for (int u = 0; u < U; ++u) {
+    const unsigned m = marks[u] & ((1u << lane) - 1);
+    all += __popc(marks[u]), episode += __popc(m);
+    if (m) from = max(from, (31 - __clz(m)) * U + u);
+  }
+  float hi[U], lo[U];  // of the sums' products with log2(e)
+  auto times_log2e = [](float p, float e, float unit, float& hi, float& lo) {
+    constexpr float kL = 1.44269502f, kRest = 1.92596303e-8f;  // log2(e) in two parts
+    hi = p * (kL * unit);
+    lo = fmaf(p, kL * unit, -hi) + (p * (kRest * unit) + e * (kL * unit));
+  };
+  if (fixed) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = lane * U + u;
       if (mark[u]) from = i;
       const int steps = min(i, n - 1) - from;
-      y[u] = steps > 0 ? steps * step : 0.0;
+      const float p = steps > 0 ? float(steps) * one : 0.0f, e = steps > 0 ? fmaf(float(steps), one, -p) : 0.0f;
+      times_log2e(p, e, 1.0f, hi[u], lo[u]);
     }
-    last = __shfl_sync(kAll, y[U - 1], 31);
   } else {
-    double sum[U];
-    bool any = false;
+    constexpr float kUnit = 1.0f / 1099511627776.0f;
+    long long sum[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      sum[u] = mark[u] ? 0.0 : double(x[u]) + (u ? sum[u - 1] : 0.0);
-      any |= mark[u];
-    }
-    double run = sum[U - 1];
-    bool cut = any;
+    for (int u = 0; u < U; ++u) sum[u] = (odd[u] ? 0 : __float2ll_rn(in.x[u] * 1099511627776.0f)) + (u ? sum[u - 1] : 0);
+    long long run = sum[U - 1];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const double z = __shfl_up_sync(kAll, run, d);
-      const bool c = __shfl_up_sync(kAll, int(cut), d);
-      if (lane >= d) {
-        if (!cut) run += z;
-        cut |= c;
-      }
+      const long long z = __shfl_up_sync(kAll, run, d);
+      if (lane >= d) run += z;
     }
-    last = __shfl_sync(kAll, run, 31) * kLog2e;
-    double before = __shfl_up_sync(kAll, run, 1);
-    if (lane == 0) before = 0.0;
-    any = false;
+    run -= sum[U - 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] += run;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      any |= mark[u];
-      y[u] = (any ? sum[u] : before + sum[u]) * kLog2e;
+      const int i = lane * U + u;
+      if (mark[u]) from = i;
+      long long y = sum[u];
+      if (all) {  // less the sum at the reset
+        long long at = 0;
+#pragma unroll
+        for (int w = 0; w < U; ++w) {
+          const long long z = __shfl_sync(kAll, sum[w], max(from, 0) / U);
+          if (from >= 0 && from % U == w) at = z;
+        }
+        y -= at;
+      }
+      const float p = __ll2float_rn(y);
+      times_log2e(p, __ll2float_rn(y - __float2ll_rn(p)), kUnit, hi[u], lo[u]);
+      if (odds) {
+        bool lost = false;
+#pragma unroll 1
+        for (int t = 0; t < C; ++t) {
+          bool z = false;
+#pragma unroll
+          for (int w = 0; w < U; ++w) {
+            const bool x = __shfl_sync(kAll, int(odd[w]), t / U);
+            if (t % U == w) z = x;
+          }
+          lost |= z && t > from && t <= i;
+        }
+        if (lost) hi[u] = __uint_as_float(0x7fffffffu);
+      }
     }
   }
+  const float last_hi = __shfl_sync(kAll, hi[U - 1], 31), last_lo = __shfl_sync(kAll, lo[U - 1], 31);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = lane * U + u;
     episode += mark[u];
-    s.token[i] = Token{float(y[u]), float(y[u] - float(y[u])), episode, 0};
-    s.carried[i] = i < n && episode == 0 ? ex2(float(y[u])) : 0.0f;
-    s.to_end[i] = i < n && episode == all ? ex2(float(last - y[u])) : 0.0f;
+    s.token[i] = Token{hi[u], lo[u], episode, 0};
+    s.carried[i] = i < n && episode == 0 ? ex2(hi[u] + lo[u]) : 0.0f;
+    s.to_end[i] = i < n && episode == all ? ex2((last_hi - hi[u]) + (last_lo - lo[u])) : 0.0f;
   }
-  if (lane == 0) s.keep = all == 0 ? ex2(float(last)) : 0.0f;
+  if (lane == 0) s.keep = all == 0 ? ex2(last_hi + last_lo) : 0.0f;
 }
 
 // ---------------------------------------------------------------- rows

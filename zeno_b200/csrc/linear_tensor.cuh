@@ -211,6 +211,39 @@ __device__ __forceinline__ Part<S> part_of(int warp) {
   return part;
 }
 
+// A state that is kept for the backward pass: as the threads hold it, whole vectors of a warp side by side, where it has the full width (and
+// then the same number of bytes), in rows otherwise.
+template <class S>
+__device__ __forceinline__ void write_saved(const float (&m)[S::NM][2][4], float* to, const Part<S>& part, int dk, int dv, int lane, int tid) {
+  if constexpr (S::FULL) {
+#pragma unroll
+    for (int i = 0; i < S::NM * 2; ++i)
+      reinterpret_cast<float4*>(to)[i * S::THREADS + tid] = make_float4(m[i >> 1][i & 1][0], m[i >> 1][i & 1][1], m[i >> 1][i & 1][2], m[i >> 1][i & 1][3]);
+  } else {
+    write_state<S>(m, to, part, dk, dv, lane);
+  }
+}
+template <class S>
+__device__ __forceinline__ void read_saved(float (&m)[S::NM][2][4], const float* from, const Part<S>& part, int dk, int dv, int lane, int tid) {
+  if constexpr (S::FULL) {
+#pragma unroll
+    for (int i = 0; i < S::NM * 2; ++i) {
+      const float4 x = reinterpret_cast<const float4*>(from)[i * S::THREADS + tid];
+      m[i >> 1][i & 1][0] = x.x, m[i >> 1][i & 1][1] = x.y, m[i >> 1][i & 1][2] = x.z, m[i >> 1][i & 1][3] = x.w;
+    }
+  } else {
+    read_state<S>(m, from, part, dk, dv, lane);
+  }
+}
+// One value of it.
+template <class S>
+__device__ __forceinline__ float saved_value(const float* from, bool saved, int row, int col, int dv) {
+  if (!S::FULL || !saved) return from[row * dv + col];
+  const int warp = (row >> 5) | ((row >> 4) & 1) << 2 | (col / (S::NM * 16)) << 3;
+  const int j = col % (S::NM * 16) / 16, h = (col >> 3) & 1, lane = (row & 7) * 4 + ((col & 7) >> 1);
+  return from[((j * 2 + h) * S::THREADS + warp * 32 + lane) * 4 + ((row >> 3) & 1) * 2 + (col & 1)];
+}
+
 // m = keep m + the accumulators at `at`.
 template <class S>
 __device__ __forceinline__ void merge(float (&m)[S::NM][2][4], uint32_t at, float keep, const Part<S>& part) {
@@ -330,9 +363,11 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   auto fetch_k = [&](int c) { load_tile(k, gk + int64_t(c) * C * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, tokens_of(c), mv); };
   auto fetch = [&](int c) {
     const int n = tokens_of(c), turn = (c - a.c0) & 1;
+    GateIn<C> in{};
+    if (warp == S::NW - 1) in = fetch_gates<C>(gg, p.g.stride[1], gr, p.reset.stride[1], int64_t(c) * C, n, lane);
     load_tile(q0 + turn * kTok, gq + int64_t(c) * C * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, mv);
     load_tile(v0 + turn * kTok, gv + int64_t(c) * C * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, mv);
-    if (warp == S::NW - 1) load_gates<C>(gates[turn], gg, p.g.stride[1], gr, p.reset.stride[1], int64_t(c) * C, n, lane);
+    if (warp == S::NW - 1) scan_gates<C>(gates[turn], in, p.g.stride[1] == 0, n, lane);
   };
   if (a.c0 < a.c1) fetch_k(a.c0), fetch(a.c0);
   begin<512>(control, warp, tid);
@@ -356,7 +391,7 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
     const Gates<C>& s = gates[turn];
     const bool have = c > a.c0 || first, goes_on = c + 1 < a.c1 || (c + 1 == a.chunks && p.final_state);
     if (have) dump<S, 2>(m, st, part, lane);
-    if (p.saved && c > 0) write_state<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane);
+    if (p.saved && c > 0) write_saved<S>(m, p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size, part, dk, dv, lane, tid);
     copies_landed();
     const bool odd = tile_odd(q, mv) || tile_odd(k, mv) || tile_odd(v, mv);
     fence_shared();
@@ -521,9 +556,11 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   auto fetch = [&](int step) {
     const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * C;
     const int n = int(min(int64_t(C), int64_t(p.tokens) - t0));
+    GateIn<C> in{};
+    if (warp == S::NW - 1) in = fetch_gates<C>(gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     load_tile(x, gx + t0 * tx.stride[1], tx.stride[1], dk, vx, n, mv);
     load_tile(y0 + (step & 1) * kTok, gy + t0 * ty.stride[1], ty.stride[1], dv, vy, n, mv);
-    if (warp == S::NW - 1) load_gates<C>(gates[step & 1], gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    if (warp == S::NW - 1) scan_gates<C>(gates[step & 1], in, p.g.stride[1] == 0, n, lane);
   };
   fetch(0);
   begin<128>(control, warp, tid);
@@ -648,6 +685,36 @@ __device__ __forceinline__ void stage_tile(plane_t* to, const float (&acc)[2][2]
             pack_round(acc[j][h][2 * r], acc[j][h][2 * r + 1]);
 }
 
+// 32-bit rows of 128 values in shared memory, their 16-byte pieces swapped within groups of 8 rows; to rows in memory.
+__device__ __forceinline__ int float_spot(int row, int col) { return row * D + (((col >> 2) ^ (row & 7)) << 2) + (col & 3); }
+__device__ __forceinline__ void stage_float(float* to, const float (&acc)[2][2][4], int rt, int col, int lane) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        *reinterpret_cast<float2*>(to + float_spot(rt * 16 + (lane >> 2) + r * 8, col + j * 16 + h * 8 + (lane & 3) * 2)) =
+            make_float2(acc[j][h][2 * r], acc[j][h][2 * r + 1]);
+}
+__device__ __forceinline__ void store_staged(float* to, int64_t stride, const float* from, int width, int n, int tid) {
+  const int c = (tid & 31) * 4;
+  if (c >= width) return;
+  const bool four = width % 4 == 0;  // (and then the workspace's rows are whole vectors)
+  for (int row = tid >> 5; row < n; row += 16) {
+    const float4 x = *reinterpret_cast<const float4*>(from + float_spot(row, c));
+    float* at = to + row * stride + c;
+    if (four) {
+      *reinterpret_cast<float4*>(at) = x;
+    } else {
+      at[0] = x.x;
+      if (c + 1 < width) at[1] = x.y;
+      if (c + 2 < width) at[2] = x.z;
+      if (c + 3 < width) at[3] = x.w;
+    }
+  }
+}
+
 // As linear_backward_kernel.  Four rounds of products a chunk: the scores and S's part of dQ; all that P and D are in, while R's limbs take the
 // place of S's; R's part of dK and dV; the update of R, whose weighted queries take the place of its limbs.
 template <class S>
@@ -681,6 +748,7 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
   const uint32_t aq = delta::smem_at(q), ak = delta::smem_at(k), av = delta::smem_at(v), ao = delta::smem_at(o), ap = delta::smem_at(pr),
                  ad = delta::smem_at(dp), as = delta::smem_at(st);
 
+  float *const sq = reinterpret_cast<float*>(k), *const sk = reinterpret_cast<float*>(st + 3 * kTok);
   const Part<S> part = part_of<S>(warp);
   float m[S::NM][2][4];
   const bool last_segment = a.c1 == a.chunks;
@@ -698,16 +766,19 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
     const float* front = c > 0 ? p.saved + (int64_t(a.row) * (a.chunks - 1) + c - 1) * state_size
                                : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
     const bool have_r = c + 1 < a.c1 || behind, goes_on = c > a.c0 || (c == 0 && d.d_initial);
+    GateIn<C> in{};
+    if (warp == S::NW - 1) in = fetch_gates<C>(gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
     __syncthreads();  // the last chunk's results have left
     load_tile(q, gq + t0 * p.q.stride[1], p.q.stride[1], dk, sg.vec & kVecQ, n, mv);
     load_tile(k, gk + t0 * p.k.stride[1], p.k.stride[1], dk, sg.vec & kVecK, n, mv);
     load_tile(v, gv + t0 * p.v.stride[1], p.v.stride[1], dv, sg.vec & kVecV, n, mv);
     load_tile(o, go + t0 * d.d_out.stride[1], d.d_out.stride[1], dv, sg.vec & kVecOut, n, mv);
-    if (warp == S::NW - 1) load_gates<C>(s, gg, p.g.stride[1], gr, p.reset.stride[1], t0, n, lane);
+    if (warp == S::NW - 1) scan_gates<C>(s, in, p.g.stride[1] == 0, n, lane);
     float state_dot = 0.0f;  // <S, R> over this thread's elements
     if (front) {
       float x[S::NM][2][4];
-      read_state<S>(x, front, part, dk, dv, lane);
+      if (c > 0) read_saved<S>(x, front, part, dk, dv, lane, tid);
+      else read_state<S>(x, front, part, dk, dv, lane);
       float dot = 0.0f;
 #pragma unroll
       for (int j = 0; j < S::NM; ++j)
@@ -818,6 +889,16 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
         }
     }
     products.issued(tid == 0);
+    if (c > a.c0) {  // the next chunk's rows, a line of 128 bytes a thread, and the state in front of it
+      const int row = tid >> 3, half = (tid & 1) * 64;
+      const int64_t t = t0 - C + row;
+      const int which = tid >> 1 & 3;
+      const bf16* at = which == 0 ? gq + t * p.q.stride[1] : which == 1 ? gk + t * p.k.stride[1] : which == 2 ? gv + t * p.v.stride[1]
+                                                                                                             : go + t * d.d_out.stride[1];
+      if (half < (which < 2 ? dk : dv)) delta::prefetch(at + half);
+      const float* next = c > 1 ? front - state_size : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+      if (next && tid * 32 < state_size) delta::prefetch(next + tid * 32);
+    }
     if (have_r) {  // (S's limbs have been read)
       dump<S, 3>(m, st, part, lane);
       fence_shared();
@@ -880,7 +961,7 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
       again(dq, rt, col, n, dk, lane, [&](int i, int cc) {
         float y = 0.0f;
         if (front && s.carried[i] != 0.0f) {
-          for (int e = 0; e < dv; ++e) y = fmaf(value_at<1, C>(o, 0, i, e), front[cc * dv + e], y);
+          for (int e = 0; e < dv; ++e) y = fmaf(value_at<1, C>(o, 0, i, e), saved_value<S>(front, c > 0, cc, e, dv), y);
           y *= s.carried[i] * p.scale;
         }
         return over_pairs<true>(s, y, dp, k, i, cc, n);
@@ -920,9 +1001,9 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
     }
     // results by way of tiles that are not needed any more (Q and dO still are)
     if (shared) {
-      const int64_t at = (int64_t(a.b) * p.tokens + t0) * shared_stride + int64_t(a.h) * dk;
-      store_float(extra.shared_q + at, shared_stride, dq, rt * 16, col, n, dk, lane);
-      store_float(extra.shared_k + at, shared_stride, dk_, rt * 16, col, n, dk, lane);
+      // (32-bit rows where K and V, and the rest of the limbs, were)
+      stage_float(sq, dq, rt, col, lane);
+      stage_float(sk, dk_, rt, col, lane);
     } else {
       stage_tile(k, dq, rt, col, lane);
       stage_tile(v, dk_, rt, col, lane);
@@ -999,7 +1080,11 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
     }
     fence_before();
     __syncthreads();
-    if (!shared) {
+    if (shared) {
+      const int64_t at = (int64_t(a.b) * p.tokens + t0) * shared_stride + int64_t(a.h) * dk;
+      store_staged(extra.shared_q + at, shared_stride, sq, dk, n, tid);
+      store_staged(extra.shared_k + at, shared_stride, sk, dk, n, tid);
+    } else {
       store_tile(wq + t0 * d.d_q.stride[1], d.d_q.stride[1], k, dk, sg.vec & kVecDq, n, mv);
       store_tile(wk + t0 * d.d_k.stride[1], d.d_k.stride[1], v, dk, sg.vec & kVecDk, n, mv);
     }

@@ -159,11 +159,12 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel
   plane_t *q = reinterpret_cast<plane_t*>(mine + sizeof(Gates<32>)), *k = q + S::PLANE, *v = k + S::PLANE;
   const int dk = FULL ? D : int(p.key_dim), dv = FULL ? D : int(p.value_dim), n = int(p.tokens), nt = (n + 15) / 16;
   const Mover<S> mv(lane);
+  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
   load_rows<S>(q, place<bf16>(p.q, a.b, a.kh), p.q.stride[1], dk, vec & kVecQ, n, nt, mv);
   load_rows<S>(k, place<bf16>(p.k, a.b, a.kh), p.k.stride[1], dk, vec & kVecK, n, nt, mv);
   load_rows<S>(v, place<bf16>(p.v, a.b, a.h), p.v.stride[1], dv, vec & kVecV, n, nt, mv);
-  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
-  load_gates<32>(s, place<float>(p.g, a.b, a.h), p.g.stride[1], gr, p.reset.stride[1], 0, n, lane);
+  const GateIn<32> gates = fetch_gates<32>(place<float>(p.g, a.b, a.h), p.g.stride[1], gr, p.reset.stride[1], 0, n, lane);
+  scan_gates<32>(s, gates, p.g.stride[1] == 0, n, lane);
   const int64_t state_size = int64_t(dk) * dv;
   const float* initial = p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
   float* final = p.final_state ? p.final_state + int64_t(a.row) * state_size : nullptr;
@@ -429,12 +430,13 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
   plane_t *q = reinterpret_cast<plane_t*>(mine + sizeof(WarpGates)), *k = q + S::PLANE, *v = k + S::PLANE, *o = v + S::PLANE;
   const int dk = FULL ? D : int(p.key_dim), dv = FULL ? D : int(p.value_dim), n = int(p.tokens), nt = (n + 15) / 16;
   const Mover<S> mv(lane);
+  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
   load_rows<S>(q, place<bf16>(p.q, a.b, a.kh), p.q.stride[1], dk, vec & kVecQ, n, nt, mv);
   load_rows<S>(k, place<bf16>(p.k, a.b, a.kh), p.k.stride[1], dk, vec & kVecK, n, nt, mv);
   load_rows<S>(v, place<bf16>(p.v, a.b, a.h), p.v.stride[1], dv, vec & kVecV, n, nt, mv);
   load_rows<S>(o, place<bf16>(d.d_out, a.b, a.h), d.d_out.stride[1], dv, vec & kVecOut, n, nt, mv);
-  const uint8_t* gr = p.reset.data ? static_cast<const uint8_t*>(p.reset.data) + int64_t(a.b) * p.reset.stride[0] : nullptr;
-  load_gates<32>(s, place<float>(p.g, a.b, a.h), p.g.stride[1], gr, p.reset.stride[1], 0, n, lane);
+  const GateIn<32> gates = fetch_gates<32>(place<float>(p.g, a.b, a.h), p.g.stride[1], gr, p.reset.stride[1], 0, n, lane);
+  scan_gates<32>(s, gates, p.g.stride[1] == 0, n, lane);
   const int64_t state_size = int64_t(dk) * dv;
   const float* initial = p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
   WarpResults to{place<bf16>(d.d_q, a.b, a.kh), place<bf16>(d.d_k, a.b, a.kh), place<bf16>(d.d_v, a.b, a.h), nullptr, nullptr, 0};
