@@ -9,7 +9,7 @@ struct BackwardLayout {  // bytes of a workspace's parts, in this order
   uint64_t cut, shared, decay;
 };
 inline BackwardLayout backward_layout(const ZenoLinearAttention& p) {
-  const Cut c = cut_of(p, fill_of(p));
+  const Cut c = cut_of(p);
   BackwardLayout l{c.total, 0, 0};
   if (p.value_heads != p.key_heads) l.shared = (uint64_t(p.batch) * p.tokens * p.value_heads * p.key_dim * 4 + 15) / 16 * 16;
   l.decay = uint64_t(p.batch) * p.value_heads * c.count * 8;
@@ -22,7 +22,7 @@ template <class T>
 cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream) {
   return with_shape<T>(p, [&](auto shape) {
     using S = decltype(shape);
-    const Cut c = cut_of(p, fill_of(p));
+    const Cut c = cut_of(p);
     const BackwardLayout l = backward_layout(p);
     char* at = static_cast<char*>(workspace);
     const uint32_t vec = vec_of(p, d.d_out) | vec_of(d.d_q, p.key_dim, p.dtype, kVecDq) | vec_of(d.d_k, p.key_dim, p.dtype, kVecDk) |

@@ -28,7 +28,7 @@ uint64_t linear_saved_bytes(const ZenoLinearAttention& p) {
   return chunks < 2 ? 0 : (chunks - 1) * p.batch * p.value_heads * p.key_dim * p.value_dim * 4;
 }
 
-uint64_t linear_forward_workspace(const ZenoLinearAttention& p) { return linear::cut_of(p, linear::fill_of(p)).total; }
+uint64_t linear_forward_workspace(const ZenoLinearAttention& p) { return linear::cut_of(p).total; }
 
 cudaError_t launch_linear_forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t stream) {
   if (linear::warp_a_head(p)) return linear::forward_by_warps(p, stream);

@@ -9,7 +9,7 @@ template <class T>
 cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t stream) {
   return with_shape<T>(p, [&](auto shape) {
     using S = decltype(shape);
-    const Cut c = cut_of(p, fill_of(p));
+    const Cut c = cut_of(p);
     Segments sg{c.count, c.chunks, vec_of(p, p.out), static_cast<float*>(workspace), nullptr};
     cudaError_t e;
     if (c.count > 1) {

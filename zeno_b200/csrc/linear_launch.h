@@ -21,26 +21,30 @@ struct Cut {
   uint32_t count, chunks;  // segments, and chunks of each
   uint64_t state, keep, total;  // bytes
 };
-// `fill`: blocks that fill the GPU.  Segments cost a second reading of two of the inputs and a walk over the states, so
-// a rollout is cut only where it at least doubles the blocks.
-inline Cut cut_of(const ZenoLinearAttention& p, uint32_t fill) {
+// How many segments: the least of the rounds of blocks that the main kernel takes, in chunks, and of what the segments cost besides: their sums,
+// the walk over them, the start of a block (as measured with 128 channels: 64 rollouts of 16 chunks are best in 2 segments, 322 us
+// with gradients against 346 in 4; 16 of 64 chunks in 8).
+inline Cut cut_of(const ZenoLinearAttention& p) {
   const uint32_t C = uint32_t(chunk_of(p)), chunks = (p.tokens + C - 1) / C;
   const uint64_t rows = uint64_t(p.batch) * p.value_heads;
   Cut c{1, chunks, 0, 0, 0};
-  if (rows == 0 || 2 * rows > fill || chunks < 2) return c;
-  const uint32_t want = uint32_t(fill / rows);
-  const uint32_t count = want < chunks ? want : chunks;
-  c.chunks = (chunks + count - 1) / count;
-  c.count = (chunks + c.chunks - 1) / c.chunks;
+  const uint64_t slots = kSms * (width_of(p) == 128 ? 1 : 2);
+  if (rows == 0 || rows >= slots || chunks < 2) return c;
+  float least = 0.0f;
+  for (uint32_t want = 1; want <= chunks && want <= 256; ++want) {
+    const uint32_t per = (chunks + want - 1) / want, count = (chunks + per - 1) / per;
+    if (count != want) continue;
+    float cost = float((rows * count + slots - 1) / slots) * (float(per) + 0.6f);
+    if (count > 1) cost += 0.45f * float(per) * float((rows * (count - 1) + slots - 1) / slots) + 0.005f * float(rows * count) + 0.4f;
+    if (count > 1 && cost >= least) continue;
+    least = cost;
+    c.count = count, c.chunks = per;
+  }
   if (c.count == 1) return c;
   c.state = (rows * c.count * p.key_dim * p.value_dim * 4 + 15) / 16 * 16;
   c.keep = (rows * c.count * 4 + 15) / 16 * 16;
   c.total = c.state + c.keep;
   return c;
-}
-inline uint32_t fill_of(const ZenoLinearAttention& p) {
-  const int w = width_of(p);
-  return kSms * (w == 128 ? 1 : 2);
 }
 
 inline uint32_t vec_of(const ZenoTensor& t, uint32_t width, uint32_t dtype, uint32_t flag) {
