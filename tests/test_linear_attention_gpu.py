@@ -210,9 +210,11 @@ def test_large_and_small_values(dtype):
 @pytest.mark.parametrize("name,value", [("q", "nan"), ("k", "nan"), ("k", "-inf"), ("v", "inf"), ("v", "nan"), ("g", "nan"), ("d_out", "nan"), ("d_out", "inf")])
 @pytest.mark.parametrize("B,T,resets,bad_at", [(2, 70, (20, 45), 30), (2, 70, (20, 32), 40), (2, 33, (32,), 32), (2, 900, (300, 500), 310), (2, 20, (7,), 3),
                                                (300, 20, (7,), 3), (300, 32, (5, 20), 20), (300, 32, (5, 20), 10)])
-@pytest.mark.parametrize("fixed", [False, True])
-def test_what_is_not_finite_stays_in_its_episode(B, T, resets, bad_at, fixed, name, value, dtype):
-    H, d = 2, 32
+@pytest.mark.parametrize("fixed,d", [(False, 32), (True, 32), (False, 128), (True, 100)])
+def test_what_is_not_finite_stays_in_its_episode(B, T, resets, bad_at, fixed, d, name, value, dtype):
+    H = 2
+    if d > 64 and (B > 2 or dtype == torch.float32):
+        return  # (the wide instances of bfloat16)
     x = inputs(B, T, H, H, d, d, dtype, reset=None, fixed=fixed)
     if fixed and name == "g":
         return  # (then it is in every episode)
@@ -253,11 +255,12 @@ def test_what_is_not_finite_stays_in_its_episode(B, T, resets, bad_at, fixed, na
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_a_dropped_state_may_hold_anything(dtype):
-    x = inputs(3, 40, 1, 1, 16, 16, dtype, reset=None)
-    x[4] = torch.zeros(3, 40, device=DEV, dtype=torch.uint8)
+@pytest.mark.parametrize("B,T,w", [(3, 40, 16), (600, 30, 48), (3, 200, 128)])
+def test_a_dropped_state_may_hold_anything(B, T, w, dtype):
+    x = inputs(B, T, 1, 1, w, w, dtype, reset=None)
+    x[4] = torch.zeros(B, T, device=DEV, dtype=torch.uint8)
     x[4][:, 0] = 1
-    d = torch.randn(3, 40, 1, 16, device=DEV).to(dtype)
+    d = torch.randn(B, T, 1, w, device=DEV).to(dtype)
     want = exact(x, d)
     x[5][:] = float("nan")
     for a, b in zip(gradients(zeno_b200.linear_attention, x, d), want):
@@ -343,8 +346,37 @@ def test_empty(dtype):
     assert zeno_b200.linear_attention_step(x[0][:, 0], x[1][:, 0], x[2][:, 0], x[3], x[5]).shape == (0, 2, 16)
 
 
+@pytest.mark.parametrize("d,T,B", [(128, 300, 2), (128, 64, 40), (100, 700, 1)])
+@pytest.mark.parametrize("fixed", [False, True])
+@pytest.mark.parametrize("Hk,H", [(2, 2), (1, 3)])
+def test_wide_heads(Hk, H, fixed, B, T, d):
+    """tcgen05: whole and padded widths, segments and none, shared heads, with and without what lies in front and behind."""
+    for initial, behind in ((True, True), (False, False), (True, False)):
+        x = inputs(B, T, Hk, H, d, d, torch.bfloat16, seed=T, fixed=fixed, reset=0.02, initial=initial)
+        check_all(x, torch.randn(B, T, H, d, device=DEV).bfloat16(), torch.randn(B, H, d, d, device=DEV) if behind else None)
+
+
+def test_products_that_are_not_waited_for_are_not_a_number():
+    """A block that gives up on its products writes NaN, in every result, and the next call is as before."""
+    from zeno_b200._ffi import _lib
+    x = inputs(2, 300, 1, 2, 128, 128, torch.bfloat16, fixed=True)
+    d = torch.randn(2, 300, 2, 128, device=DEV).bfloat16()
+    want = gradients(zeno_b200.linear_attention, x, d)
+    before = _lib.zeno_linear_attention_wait_limit(0)
+    try:
+        got = gradients(zeno_b200.linear_attention, x, d)
+        torch.cuda.synchronize()
+    finally:
+        assert _lib.zeno_linear_attention_wait_limit(before) == 0
+    assert before == 2000000000
+    for t in got:
+        assert torch.isnan(t).all()
+    for a, b in zip(gradients(zeno_b200.linear_attention, x, d), want):
+        assert torch.equal(a, b)
+
+
 def test_repeats_bit_for_bit():
-    for x in (inputs(9, 200, 1, 2, 64, 64, torch.bfloat16, fixed=True), inputs(1, 900, 1, 1, 64, 64, torch.float32)):
+    for x in (inputs(3, 300, 1, 2, 128, 128, torch.bfloat16, fixed=True), inputs(700, 30, 1, 2, 64, 64, torch.bfloat16), inputs(9, 200, 1, 2, 64, 64, torch.bfloat16, fixed=True), inputs(1, 900, 1, 1, 64, 64, torch.float32)):
         d = torch.randn(x[2].shape, device=DEV).to(x[2].dtype)
         first = gradients(zeno_b200.linear_attention, x, d)
         for _ in range(3):

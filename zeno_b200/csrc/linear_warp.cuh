@@ -25,6 +25,9 @@ struct WarpGates {
   float pass[32], x[32];  // what passes a token; x_i
 };
 
+// (out of line: it would hold registers that the rows' loads are waiting in)
+static __device__ __noinline__ void scan_gates_of(Gates<32>& s, GateIn<32> in, bool fixed, int n, int lane) { scan_gates<32>(s, in, fixed, n, lane); }
+
 struct WarpAt {
   uint32_t row, b, h, kh;
 };
@@ -164,9 +167,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) linear_warp_forward_kernel
   load_rows<S>(k, place<bf16>(p.k, a.b, a.kh), p.k.stride[1], dk, vec & kVecK, n, nt, mv);
   load_rows<S>(v, place<bf16>(p.v, a.b, a.h), p.v.stride[1], dv, vec & kVecV, n, nt, mv);
   const GateIn<32> gates = fetch_gates<32>(place<float>(p.g, a.b, a.h), p.g.stride[1], gr, p.reset.stride[1], 0, n, lane);
-  scan_gates<32>(s, gates, p.g.stride[1] == 0, n, lane);
+  scan_gates_of(s, gates, p.g.stride[1] == 0, n, lane);
   const int64_t state_size = int64_t(dk) * dv;
   const float* initial = p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+  if (initial)  // (to L2; it is read 16 channels at a time)
+    for (int x = lane * 32; x < state_size; x += 1024) delta::prefetch(initial + x);
   float* final = p.final_state ? p.final_state + int64_t(a.row) * state_size : nullptr;
   bf16* out = place<bf16>(p.out, a.b, a.h);
   copies_landed();
@@ -436,9 +441,11 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
   load_rows<S>(v, place<bf16>(p.v, a.b, a.h), p.v.stride[1], dv, vec & kVecV, n, nt, mv);
   load_rows<S>(o, place<bf16>(d.d_out, a.b, a.h), d.d_out.stride[1], dv, vec & kVecOut, n, nt, mv);
   const GateIn<32> gates = fetch_gates<32>(place<float>(p.g, a.b, a.h), p.g.stride[1], gr, p.reset.stride[1], 0, n, lane);
-  scan_gates<32>(s, gates, p.g.stride[1] == 0, n, lane);
+  scan_gates_of(s, gates, p.g.stride[1] == 0, n, lane);
   const int64_t state_size = int64_t(dk) * dv;
   const float* initial = p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+  if (initial)  // (to L2; it is read 16 channels at a time)
+    for (int x = lane * 32; x < state_size; x += 1024) delta::prefetch(initial + x);
   WarpResults to{place<bf16>(d.d_q, a.b, a.kh), place<bf16>(d.d_k, a.b, a.kh), place<bf16>(d.d_v, a.b, a.h), nullptr, nullptr, 0};
   if (extra.shared_q) {
     to.shared_stride = int64_t(p.value_heads) * dk;
