@@ -411,8 +411,8 @@ typedef struct {
 #define ZENO_LINEAR_FORWARD 0u
 #define ZENO_LINEAR_BACKWARD 1u
 uint64_t zeno_linear_attention_workspace_bytes(const ZenoLinearAttention* p, uint32_t pass);
-/* The state in front of every 64 tokens but the first (32 in 32-bit calls) of every environment and head: 0.27 GB for 4096
- * environments, 128 tokens and 4 heads of 64 x 64 in bfloat16. */
+/* The state in front of every 64 tokens but the first (32 in 32-bit calls and heads of up to 32 channels) of every
+ * environment and head: 0.27 GB for 4096 environments, 128 tokens and 4 heads of 64 x 64 in bfloat16. */
 uint64_t zeno_linear_attention_saved_bytes(const ZenoLinearAttention* p);
 int zeno_linear_attention_forward(const ZenoLinearAttention* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 int zeno_linear_attention_backward(const ZenoLinearAttention* p, const ZenoLinearAttentionGrads* d, void* workspace,

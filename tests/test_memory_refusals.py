@@ -100,8 +100,9 @@ def test_attention_workspaces():
     p.saved = ffi.cast("float*", AT)
     assert _lib.zeno_linear_attention_backward(p, d, ffi.cast("void*", AT), need - 1, ffi.NULL) == INVALID and "too small" in message()
     assert _lib.zeno_linear_attention_backward(p, d, ffi.NULL, need, ffi.NULL) == INVALID and "NULL" in message()
-    # the states in front of every 64 tokens but the first, of 32 in 32-bit calls
-    assert _lib.zeno_linear_attention_saved_bytes(attention(batch=3, tokens=130, value_heads=2, key_dim=7, dtype=1)) == 3 * 2 * 2 * 7 * 8 * 4
+    # the states in front of every 64 tokens but the first, of 32 in 32-bit calls and heads of up to 32 channels
+    assert _lib.zeno_linear_attention_saved_bytes(attention(batch=3, tokens=130, value_heads=2, key_dim=37, dtype=1)) == 3 * 2 * 2 * 37 * 8 * 4
+    assert _lib.zeno_linear_attention_saved_bytes(attention(batch=3, tokens=130, value_heads=2, key_dim=7, dtype=1)) == 3 * 2 * 4 * 7 * 8 * 4
     assert _lib.zeno_linear_attention_saved_bytes(attention(tokens=65)) == 2 * 8 * 8 * 4
     assert _lib.zeno_linear_attention_saved_bytes(attention(tokens=32)) == 0
     assert _lib.zeno_linear_attention_saved_bytes(attention(key_dim=0)) == 0

@@ -11,7 +11,7 @@ namespace linear {
 cudaError_t backward_by_warps(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, const BackwardOut& extra, uint32_t vec, cudaStream_t stream) {
   return with_warp_shape(p, [&](auto shape, auto full) {
     using S = decltype(shape);
-    constexpr int WARPS = 1, BLOCKS = 11;
+    constexpr int WARPS = 1, BLOCKS = S::D == 128 ? 6 : 11;  // as shared memory has room for
     constexpr int bytes = WARPS * (int(sizeof(WarpGates)) + 4 * 2 * S::PLANE);
     auto kernel = linear_warp_backward_kernel<S::D, decltype(full)::value, WARPS, BLOCKS>;
     static std::atomic<uint64_t> devices{0};

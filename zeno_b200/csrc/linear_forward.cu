@@ -11,7 +11,7 @@ namespace linear {
 cudaError_t forward_by_warps(const ZenoLinearAttention& p, cudaStream_t stream) {
   return with_warp_shape(p, [&](auto shape, auto full) {
     using S = decltype(shape);
-    constexpr int WARPS = 2, BLOCKS = 6;
+    constexpr int WARPS = S::D == 128 ? 1 : 2, BLOCKS = S::D == 128 ? 8 : 6;  // 12 warps an SM, 8 of wide heads: registers, shared memory
     constexpr int bytes = WARPS * (int(sizeof(Gates<32>)) + 3 * 2 * S::PLANE);
     auto kernel = linear_warp_forward_kernel<S::D, decltype(full)::value, WARPS, BLOCKS>;
     static std::atomic<uint64_t> devices{0};

@@ -6,16 +6,15 @@
 namespace zb {
 namespace linear {
 
-// Chunks of 64 tokens in bfloat16, so that what a chunk costs whatever its length (the state's limbs, its traffic in
-// training) comes half as often; rollouts of up to 32 tokens and 32-bit calls (three limbs of everything in shared
-// memory) take 32.
-inline int chunk_of(const ZenoLinearAttention& p) { return p.dtype == ZENO_DTYPE_BF16 && p.tokens > 32 ? 64 : 32; }
 inline int width_of(const ZenoLinearAttention& p) {
   const uint32_t w = p.key_dim > p.value_dim ? p.key_dim : p.value_dim;
   return w <= 32 ? 32 : w <= 64 ? 64 : 128;
 }
 
-constexpr int kWarpWidth = 64;
+// Chunks of 64 tokens in bfloat16 heads of more than 32 channels, so that what a chunk costs whatever its length (the state's limbs, its traffic in
+// training) comes half as often (64 x 512 tokens, 4 heads of 48 x 56, with gradients: 178 us against 232); rollouts of up to 32
+// tokens, heads of up to 32 channels (2048 x 128: 578 us against 644) and 32-bit calls (three limbs of everything in shared memory) take 32.
+inline int chunk_of(const ZenoLinearAttention& p) { return p.dtype == ZENO_DTYPE_BF16 && p.tokens > 32 && width_of(p) > 32 ? 64 : 32; }
 
 struct Cut {
   uint32_t count, chunks;  // segments, and chunks of each
@@ -66,7 +65,6 @@ cudaError_t with_shape_of(const ZenoLinearAttention& p, int w, F&& f) {
       if (w == 64) return f(Shape<T, 64, 32, 4, FULL>{});
       return f(Shape<T, 128, 32, 8, FULL>{});
     }
-    if (w == 32) return f(Shape<T, 32, 64, 4, FULL>{});
     if (w == 64) return f(Shape<T, 64, 64, 8, FULL>{});
     return f(Shape<T, 128, 64, 16, FULL>{});
   } else {
@@ -83,14 +81,15 @@ cudaError_t with_shape(const ZenoLinearAttention& p, F&& f) {
 
 // Short rollouts of many environments: a warp a head.  Few of them finish earlier with a block each.
 inline bool warp_a_head(const ZenoLinearAttention& p) {
-  return p.dtype == ZENO_DTYPE_BF16 && p.tokens >= 1 && p.tokens <= 32 && width_of(p) <= kWarpWidth && uint64_t(p.batch) * p.value_heads >= 4 * kSms;
+  return p.dtype == ZENO_DTYPE_BF16 && p.tokens >= 1 && p.tokens <= 32 && uint64_t(p.batch) * p.value_heads >= 4 * kSms;
 }
 template <class F>
 cudaError_t with_warp_shape(const ZenoLinearAttention& p, F&& f) {
   const int w = width_of(p);
   const bool full = full_width(p);
   if (w == 32) return full ? f(WarpShape<32>{}, std::true_type{}) : f(WarpShape<32>{}, std::false_type{});
-  return full ? f(WarpShape<64>{}, std::true_type{}) : f(WarpShape<64>{}, std::false_type{});
+  if (w == 64) return full ? f(WarpShape<64>{}, std::true_type{}) : f(WarpShape<64>{}, std::false_type{});
+  return full ? f(WarpShape<128>{}, std::true_type{}) : f(WarpShape<128>{}, std::false_type{});
 }
 
 template <class T>

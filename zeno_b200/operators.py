@@ -289,8 +289,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, reset: Optional
     Any strides are taken (a time-major buffer's transposed view needs no copy) as long as
     the last axis is contiguous.  The state is held in 32 bits.  Gradients flow to q, k, v, g and initial_state
     (once, and in reverse mode only); they are sums in a fixed order, so they repeat bit for bit.
-    For the gradients a call keeps the state in front of every 64 tokens but the first (32 in float32):
-    0.27 GB for 4096 x 128 tokens and 4 heads of 64 x 64 in bfloat16.
+    For the gradients a call keeps the state in front of every 64 tokens but the first (32 in float32, and of heads
+    of up to 32 channels): 0.27 GB for 4096 x 128 tokens and 4 heads of 64 x 64 in bfloat16.
     """
     return _torch.linear_attention(q, k, v, g, reset, initial_state, scale)
 
