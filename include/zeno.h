@@ -427,7 +427,7 @@ int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
 uint64_t zeno_linear_attention_wait_limit(uint64_t nanoseconds);
 
 /* Layer norm of rows of `width` values: out = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps), mean and
- * variance in 32 bits, the variance from the differences to the mean. */
+ * variance in 32 bits, the variance from the differences to the mean.  No output overlaps an input. */
 typedef struct {
   uint64_t rows[3];  /* the rows are [rows[0], rows[1], rows[2]] */
   uint32_t width;    /* at least 1 */

@@ -245,6 +245,15 @@ def test_forward_mode_derivatives_are_refused():
             zeno_b200.layer_norm(forward_ad.make_dual(x, torch.ones_like(x)))
 
 
+def test_second_derivatives_are_refused():
+    x, w, b, dy = inputs((4, 32), torch.float32, torch.float32)
+    w.requires_grad_(True)
+    once, = torch.autograd.grad(zeno_b200.layer_norm(x, w, b), w, dy, create_graph=True)
+    check(once, exact(x, w.detach(), b, dy)[2], 2)
+    with pytest.raises(RuntimeError, match="once"):
+        once.sum().backward()
+
+
 def test_refusals():
     x, w = torch.zeros(3, 8, device=DEV), torch.zeros(8, device=DEV)
     f = zeno_b200.layer_norm

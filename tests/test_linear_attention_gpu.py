@@ -375,6 +375,55 @@ def test_products_that_are_not_waited_for_are_not_a_number():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("B,T,w,dtype", [(1, 1500, 128, torch.bfloat16), (1, 1500, 32, torch.float32), (700, 20, 64, torch.bfloat16), (3, 50, 40, torch.float32)])
+def test_the_final_state_in_place_of_the_initial_one(B, T, w, dtype):
+    """At the C entry, which allows it: rollouts in segments, by warps and by blocks."""
+    from zeno_b200._ffi import _lib, ffi
+    x = inputs(B, T, 1, 1, w, w, dtype, fixed=True, reset=0.001)
+    out, final = zeno_b200.linear_attention(*x)
+
+    def tensor(t):
+        s = t.stride()
+        return dict(data=ffi.cast("void*", t.data_ptr()), stride=[s[0], s[1], s[2] if len(s) > 2 else 0])
+    p = ffi.new("ZenoLinearAttention*")
+    p.batch, p.tokens, p.key_heads, p.value_heads, p.key_dim, p.value_dim = B, T, 1, 1, w, w
+    p.dtype, p.scale = int(dtype == torch.bfloat16), w ** -0.5
+    p.q, p.k, p.v, p.reset = (tensor(x[i]) for i in (0, 1, 2, 4))
+    p.g = dict(data=ffi.cast("void*", x[3].data_ptr()), stride=[0, 0, 1])
+    got, state = torch.empty_like(out), x[5].clone()
+    p.out = tensor(got)
+    p.initial_state = p.final_state = ffi.cast("float*", state.data_ptr())
+    need = _lib.zeno_linear_attention_workspace_bytes(p, 0)
+    work = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+    stream = ffi.cast("void*", torch.cuda.current_stream().cuda_stream)
+    assert _lib.zeno_linear_attention_forward(p, ffi.cast("void*", work.data_ptr()), need, stream) == 0
+    assert torch.equal(got, out) and torch.equal(state, final)
+
+
+def test_second_derivatives_are_refused():
+    x = inputs(2, 5, 1, 1, 16, 16, torch.float32)
+    q = x[0].clone().requires_grad_(True)
+    out, _ = zeno_b200.linear_attention(q, *x[1:])
+    once, = torch.autograd.grad(out.sum(), q, create_graph=True)
+    check(once, exact([q.detach(), *x[1:]], torch.ones_like(out))[2])
+    with pytest.raises(RuntimeError, match="once"):
+        once.sum().backward()
+
+
+def test_growing_decays_of_any_size():
+    """exp(g) past what a float holds: what is infinite or not a number stays in its episode."""
+    x = inputs(2, 70, 1, 1, 16, 16, torch.float32, reset=None)
+    x[4] = torch.zeros(2, 70, device=DEV, dtype=torch.uint8)
+    x[4][:, 40] = 1
+    want = exact(x, torch.zeros(2, 70, 1, 16, device=DEV))[0]
+    for value in (100.0, 1e4, 1e9, float("inf")):
+        y = [t.clone() for t in x]
+        y[3][:, 20] = value
+        got = zeno_b200.linear_attention(*y)[0]
+        check(got[:, :20], want[:, :20]), check(got[:, 40:], want[:, 40:])
+        assert not torch.isfinite(got[:, 20:40]).any()
+
+
 def test_repeats_bit_for_bit():
     for x in (inputs(3, 300, 1, 2, 128, 128, torch.bfloat16, fixed=True), inputs(700, 30, 1, 2, 64, 64, torch.bfloat16), inputs(9, 200, 1, 2, 64, 64, torch.bfloat16, fixed=True), inputs(1, 900, 1, 1, 64, 64, torch.float32)):
         d = torch.randn(x[2].shape, device=DEV).to(x[2].dtype)

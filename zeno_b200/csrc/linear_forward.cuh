@@ -62,8 +62,10 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
 
   const Part<S> part(warp, dk, dv);
   float m[S::NM][2][4];
-  const float* first = a.seg ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
-                             : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+  // (of several segments the first one's is a copy too: the last one may be writing over the initial state by now)
+  const float* first = a.seg || (sg.count > 1 && p.initial_state) ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
+                       : p.initial_state                          ? p.initial_state + int64_t(a.row) * state_size
+                                                                  : nullptr;
   if (first) read_state<S>(m, first, part, dk, dv, lane);
   else clear<S>(m);
 

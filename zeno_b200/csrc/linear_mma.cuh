@@ -221,7 +221,7 @@ __device__ __forceinline__ GateIn<C> fetch_gates(const float* g, int64_t g_strid
 }
 
 // One warp: their gates.  Sums run from the last reset on, so that what one episode's decays are, not finite included, stays in it.  They are
-// taken in 64-bit integers, in units of 2^-40 (exact, where a scan in double was a third of a chunk's time); a log decay of 2^22 and
+// taken in 64-bit integers, in units of 2^-40 (exact, where a scan in double was a third of a chunk's time); a log decay of 2^16 and
 // more counts as not a number.  One decay for all tokens (`fixed`) needs no sum.
 template <int C>
 __device__ __forceinline__ void scan_gates(Gates<C>& s, GateIn<C> in, bool fixed, int n, int lane) {
@@ -234,7 +234,7 @@ __device__ __forceinline__ void scan_gates(Gates<C>& s, GateIn<C> in, bool fixed
     // a decay to nothing is a reset: the sums behind it stay finite
     mark[u] = in.mark[u] || ex2(in.x[u] * 1.4426950408889634f) == 0.0f;
     if (mark[u]) in.x[u] = 0.0f;
-    odd[u] = !(fabsf(in.x[u]) < 4194304.0f);
+    odd[u] = !(in.x[u] < 65536.0f);  // (the least that is no mark is -104)
     marks[u] = __ballot_sync(kAll, mark[u]);
     odds |= __ballot_sync(kAll, odd[u]);
   }

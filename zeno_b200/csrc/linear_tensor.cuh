@@ -378,8 +378,10 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
 
   const Part<S> part = part_of<S>(warp);
   float m[S::NM][2][4];
-  const float* first = a.seg ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
-                             : p.initial_state ? p.initial_state + int64_t(a.row) * state_size : nullptr;
+  // (of several segments the first one's is a copy too: the last one may be writing over the initial state by now)
+  const float* first = a.seg || (sg.count > 1 && p.initial_state) ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
+                       : p.initial_state                          ? p.initial_state + int64_t(a.row) * state_size
+                                                                  : nullptr;
   if (first) read_state<S>(m, first, part, dk, dv, lane);
   else clear<S>(m);
   bool ok = true;
