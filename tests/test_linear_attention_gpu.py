@@ -515,6 +515,16 @@ def test_offsets_that_pass_32_bits():
         assert torch.equal(zeno_b200.linear_attention(*x)[0], want[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_environments_than_one_axis_of_a_grid(dtype):
+    x = inputs(70001, 40, 1, 1, 8, 8, dtype)
+    part = [t[-5:] for t in x]
+    d = torch.randn(70001, 40, 1, 8, device=DEV).to(dtype)
+    got, want = gradients(zeno_b200.linear_attention, x, d), exact(part, d[-5:])
+    for name, a, b in zip(NAMES, got, want):
+        check(a[-5:], b, name)
+
+
 def test_forward_mode_derivatives_are_refused():
     from torch.autograd import forward_ad
     x = inputs(1, 4, 1, 1, 8, 8, torch.float32)

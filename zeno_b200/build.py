@@ -23,6 +23,7 @@ import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -75,11 +76,11 @@ def _runner(verbose: bool):
     return run
 
 
-def _compile_binding(run, cxx: str) -> Path:
-    """The object file of the PyTorch functions."""
+def _compile_binding(run, cxx: str) -> Optional[Path]:
+    """The object file of the PyTorch functions; None where there is no PyTorch (the library itself needs none)."""
     spec = importlib.util.find_spec("torch")
     if spec is None:
-        raise RuntimeError("build failed: the operators' functions need an installed PyTorch")
+        return None
     torch_dir = Path(spec.origin).parent
     obj = OBJ_DIR / (BINDING_SOURCE.name + ".o")
     includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", CUDA_HOME / "include",
@@ -88,7 +89,9 @@ def _compile_binding(run, cxx: str) -> Path:
     return obj
 
 
-def _link_binding(run, cxx: str, obj: Path) -> None:
+def _link_binding(run, cxx: str, obj: Optional[Path]) -> None:
+    if obj is None:
+        return
     torch_lib = Path(importlib.util.find_spec("torch").origin).parent / "lib"
     tmp = BINDING.with_suffix(".so.tmp")
     run([cxx, "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}", "-lzeno", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",

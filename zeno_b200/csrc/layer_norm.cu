@@ -328,6 +328,7 @@ __device__ __forceinline__ void norm_backward(const Norm& p) {
   const S at(p.width);
   const uint32_t own = S::BLOCK ? 0 : threadIdx.x / S::LANES;
   const float inverse = 1.0f / float(p.width);
+  early::let_next_start();
   Two dw[M], db[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) dw[m] = db[m] = two(0.0f, 0.0f);
@@ -489,10 +490,11 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* partial,
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t c = blockIdx.x * 32 + lane;
   W* to = blockIdx.y ? db : dw;
+  early::wait_for_previous();
   if (!to) return;
   float sum = 0.0f;
   if (c < width)
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t l = warp; l < lines; l += 32) sum += partial[(uint64_t(l) * 2 + blockIdx.y) * width + c];
   part[warp][lane] = sum;
   __syncthreads();
@@ -662,9 +664,8 @@ cudaError_t backward(const ZenoLayerNorm& p, const ZenoLayerNormGrads& d, void* 
     if (e != cudaSuccess) return e;
   }
   if (!d.d_weight && !d.d_bias) return cudaSuccess;
-  norm_reduce_kernel<W><<<dim3((p.width + 31) / 32, 2), 1024, 0, stream>>>(n.partial, blocks, p.width, static_cast<W*>(d.d_weight),
-                                                                          static_cast<W*>(d.d_bias));
-  return cudaGetLastError();
+  return launch_early(norm_reduce_kernel<W>, dim3((p.width + 31) / 32, 2), 1024, 0, stream, static_cast<const float*>(n.partial), uint32_t(blocks), p.width,
+                      static_cast<W*>(d.d_weight), static_cast<W*>(d.d_bias));
 }
 
 }  // namespace

@@ -122,6 +122,7 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
   const bool last_segment = a.c1 == a.chunks;
   const float* behind = !last_segment ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
                                       : d.d_final ? d.d_final + int64_t(a.row) * state_size : nullptr;
+  early::wait_for_previous();
   if (behind) read_state<S>(m, behind, part, dk, dv, lane);
   else clear<S>(m);
   const bool each = d.d_g.data != nullptr;  // every token's decay has a gradient of its own

@@ -47,8 +47,7 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
       auto kernel = tensor::linear_tensor_backward_kernel<S>;
       e = allow_smem(kernel, tensor::kBackwardBytes, devices);
       if (e != cudaSuccess) return e;
-      kernel<<<grid_of(p, c.count), S::THREADS, tensor::kBackwardBytes, stream>>>(p, d, sg, extra, linear_patience());
-      e = cudaGetLastError();
+      e = launch_main(kernel, grid_of(p, c.count), S::THREADS, tensor::kBackwardBytes, c.count > 1, stream, p, d, sg, extra, linear_patience());
     } else {
       constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
       auto kernel = linear_backward_kernel<S, BLOCKS>;
@@ -58,8 +57,7 @@ cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrad
       if (e != cudaSuccess) return e;
       static_assert(sizeof(T) == 4 || S::C * S::P <= 2 * S::PL * S::CPLANE, "dV is staged where P and D were");
       static_assert(BackwardSmem<S>::front + 2 * (4 * S::L * S::PLANE + 2 * S::PL * S::CPLANE + 3 * S::SPLANE) <= 232448, "shared memory of a block");
-      kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, d, sg, extra);
-      e = cudaGetLastError();
+      e = launch_main(kernel, grid_of(p, c.count), S::THREADS, bytes, c.count > 1, stream, p, d, sg, extra);
     }
     if (e != cudaSuccess) return e;
     if (l.shared) {

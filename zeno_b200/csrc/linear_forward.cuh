@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_forward_kernel(cons
   const float* first = a.seg || (sg.count > 1 && p.initial_state) ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
                        : p.initial_state                          ? p.initial_state + int64_t(a.row) * state_size
                                                                   : nullptr;
+  early::wait_for_previous();
   if (first) read_state<S>(m, first, part, dk, dv, lane);
   else clear<S>(m);
 
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_segment_kernel(cons
   float m[S::NM][2][4];
   clear<S>(m);
   float kept = 1.0f;
+  early::let_next_start();
   for (int step = 0; step < a.c1 - a.c0; ++step) {
     const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * S::C;
     const int n = int(min(int64_t(S::C), int64_t(p.tokens) - t0)), nt = (n + 15) / 16;

@@ -22,7 +22,7 @@ cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t 
       auto kernel = tensor::linear_tensor_forward_kernel<S>;
       e = allow_smem(kernel, tensor::kForwardBytes, devices);
       if (e != cudaSuccess) return e;
-      kernel<<<grid_of(p, c.count), S::THREADS, tensor::kForwardBytes, stream>>>(p, sg, linear_patience());
+      return launch_main(kernel, grid_of(p, c.count), S::THREADS, tensor::kForwardBytes, c.count > 1, stream, p, sg, linear_patience());
     } else {
       constexpr int BLOCKS = S::D == 128 ? 1 : 512 / S::THREADS;
       auto kernel = linear_forward_kernel<S, BLOCKS>;
@@ -30,9 +30,8 @@ cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t 
       const int bytes = ForwardSmem<S>::bytes(p.initial_state || c.count > 1 || p.tokens > uint32_t(S::C));
       e = allow_smem(kernel, ForwardSmem<S>::bytes(true), devices);
       if (e != cudaSuccess) return e;
-      kernel<<<grid_of(p, c.count), S::THREADS, bytes, stream>>>(p, sg);
+      return launch_main(kernel, grid_of(p, c.count), S::THREADS, bytes, c.count > 1, stream, p, sg);
     }
-    return cudaGetLastError();
   });
 }
 

@@ -97,6 +97,14 @@ cudaError_t forward(const ZenoLinearAttention& p, void* workspace, cudaStream_t 
 template <class T>
 cudaError_t backward(const ZenoLinearAttention& p, const ZenoLinearAttentionGrads& d, void* workspace, cudaStream_t stream);
 
+// A main kernel, which may start while a walk over segments is under way.
+template <class... Params, class... Args>
+cudaError_t launch_main(void (*kernel)(Params...), dim3 grid, int threads, int smem, bool after_walk, cudaStream_t stream, Args... args) {
+  if (after_walk) return launch_early(kernel, grid, threads, smem, stream, args...);
+  kernel<<<grid, threads, smem, stream>>>(args...);
+  return cudaGetLastError();
+}
+
 // What each segment adds, then the states in front of (behind) them.
 // Wide heads in chunks of 64: on tcgen05.
 template <class S>

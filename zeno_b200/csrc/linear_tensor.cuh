@@ -382,6 +382,7 @@ linear_tensor_forward_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   const float* first = a.seg || (sg.count > 1 && p.initial_state) ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
                        : p.initial_state                          ? p.initial_state + int64_t(a.row) * state_size
                                                                   : nullptr;
+  early::wait_for_previous();
   if (first) read_state<S>(m, first, part, dk, dv, lane);
   else clear<S>(m);
   bool ok = true;
@@ -572,6 +573,7 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
   float m[S::NM][2][4];
   clear<S>(m);
   float kept = 1.0f;
+  early::let_next_start();
   bool ok = true;
   for (int step = 0; step < steps; ++step) {
     const Gates<C>& s = gates[step & 1];
@@ -756,6 +758,7 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
   const bool last_segment = a.c1 == a.chunks;
   const float* behind = !last_segment ? sg.state + (int64_t(a.row) * sg.count + a.seg) * state_size
                                       : d.d_final ? d.d_final + int64_t(a.row) * state_size : nullptr;
+  early::wait_for_previous();
   if (behind) read_state<S>(m, behind, part, dk, dv, lane);
   else clear<S>(m);
   const bool each = d.d_g.data != nullptr;  // every token's decay has a gradient of its own

@@ -12,6 +12,8 @@ template <uint32_t kAhead>
 __global__ void __launch_bounds__(256) linear_walk_kernel(const LinearWalk w) {
   const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
   const uint64_t row = blockIdx.y;
+  early::wait_for_previous();
+  early::let_next_start();
   if (i >= w.size) return;
   float run = w.initial ? w.initial[row * w.size + i] : 0.0f;
   float* state = w.state + row * w.segments * w.size + i;
@@ -51,6 +53,8 @@ struct SharedPair {
 template <class T, int V>
 __global__ void __launch_bounds__(256) linear_shared_kernel(const SharedPair pair) {
   const LinearShared s = blockIdx.z ? pair.of[1] : pair.of[0];
+  early::wait_for_previous();
+  early::let_next_start();
   const uint32_t pieces = s.width / V, row = pieces * s.key_heads;
   for (uint32_t j = threadIdx.x; j < pair.turn * row; j += 256) {
     const uint32_t t = blockIdx.x * pair.turn + j / row, kh = j % row / pieces, c = j % pieces * V;
@@ -77,6 +81,7 @@ __global__ void __launch_bounds__(256) linear_shared_kernel(const SharedPair pai
 __global__ void __launch_bounds__(1024) linear_decay_kernel(const double* from, uint64_t count, float* to) {
   __shared__ double part[32];
   from += blockIdx.x * count;
+  early::wait_for_previous();
   double sum = 0.0;
 #pragma unroll 8
   for (uint64_t i = threadIdx.x; i < count; i += 1024) sum += from[i];
@@ -101,9 +106,7 @@ uint64_t linear_patience() { return wait_limit.load(); }
 cudaError_t launch_linear_walk(const LinearWalk& w, uint32_t rows, cudaStream_t stream) {
   // at most a few hundred rows are cut into segments
   const dim3 grid((w.size + 255) / 256, rows);
-  if (w.segments <= 2) linear_walk_kernel<2><<<grid, 256, 0, stream>>>(w);
-  else linear_walk_kernel<8><<<grid, 256, 0, stream>>>(w);
-  return cudaGetLastError();
+  return launch_early(w.segments <= 2 ? linear_walk_kernel<2> : linear_walk_kernel<8>, grid, 256, 0, stream, w);
 }
 
 cudaError_t launch_linear_shared(const LinearShared& q, const LinearShared& k, uint32_t batch, uint32_t dtype, cudaStream_t stream) {
@@ -112,19 +115,13 @@ cudaError_t launch_linear_shared(const LinearShared& q, const LinearShared& k, u
   const uint32_t row = q.key_heads * (four ? q.width / 4 : q.width), turn = row < 1024 ? 1024 / row : 1;
   const SharedPair pair{{q, k}, batch, turn};
   const dim3 grid((q.tokens + turn - 1) / turn, batch < 65535 ? batch : 65535, 2);
-  if (dtype == ZENO_DTYPE_BF16) {
-    if (four) linear_shared_kernel<__nv_bfloat16, 4><<<grid, 256, 0, stream>>>(pair);
-    else linear_shared_kernel<__nv_bfloat16, 1><<<grid, 256, 0, stream>>>(pair);
-  } else {
-    if (four) linear_shared_kernel<float, 4><<<grid, 256, 0, stream>>>(pair);
-    else linear_shared_kernel<float, 1><<<grid, 256, 0, stream>>>(pair);
-  }
-  return cudaGetLastError();
+  const auto kernel = dtype == ZENO_DTYPE_BF16 ? (four ? linear_shared_kernel<__nv_bfloat16, 4> : linear_shared_kernel<__nv_bfloat16, 1>)
+                                               : (four ? linear_shared_kernel<float, 4> : linear_shared_kernel<float, 1>);
+  return launch_early(kernel, grid, 256, 0, stream, pair);
 }
 
 cudaError_t launch_linear_decay(const double* from, uint64_t count, uint32_t heads, float* to, cudaStream_t stream) {
-  linear_decay_kernel<<<heads, 1024, 0, stream>>>(from, count, to);
-  return cudaGetLastError();
+  return launch_early(linear_decay_kernel, dim3(heads), 1024, 0, stream, from, count, to);
 }
 
 }  // namespace zb

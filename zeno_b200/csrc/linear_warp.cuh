@@ -427,6 +427,7 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
   constexpr int KT = S::KT;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  early::let_next_start();
   const WarpAt a = warp_at(p);
   if (a.row >= p.batch * p.value_heads) return;
   char* mine = smem + warp * (int(sizeof(WarpGates)) + 4 * 2 * S::PLANE);

@@ -29,6 +29,25 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& devices)
   return e;
 }
 
+// Launches a kernel whose blocks may start while the one in front of it in the stream still runs, where that one lets them
+// (let_next_start); each waits for its end (wait_for_previous) before it reads what it wrote, or writes anything.
+template <class... Params, class... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = size_t(smem), c.stream = stream;
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &a, c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+#ifdef __CUDACC__
+namespace early {
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+}  // namespace early
+#endif
+
 // A rollout in segments: what takes the state over a segment is M S + N.
 struct DeltaWalk {
   const float* m;      // [rows][segments][dk][dk]: M, in the forward walk M^T
