@@ -5,6 +5,9 @@
 // 512 values belongs to a part of a warp or a warp, a longer one to a block.  Backward, every thread keeps the
 // sums of its own columns over the rows it sees; a block's sums go to the workspace and a second kernel adds them in a
 // fixed order.  Sums are 32-bit (the last ones over blocks too), the variance is taken from the differences to the mean.
+//
+// 131072 rows of 256 bfloat16: 30 us forward, 40 us backward (20 and 31 us of bytes), 4 us for the sums over blocks; 524288 rows of 64: 26.5 us (20 us).
+// Those are bound by the issue of instructions (68 %).  2047 rows of 4099 floats, whose rows are not aligned: 25 and 36 us, value by value.
 #include <cuda_bf16.h>
 
 #include <algorithm>

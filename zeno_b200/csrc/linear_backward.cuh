@@ -7,6 +7,8 @@
 //   dg_t = sum_{i >= t > j} A_ij + sum_{i >= t} x_i + sum_{j < t} y_j + keep <S, R>
 // so no difference of long sums is taken.  A block walks over its chunks from the last one back, R in the warps'
 // accumulators; S comes from where the forward pass kept it.
+//
+// Bound as the forward pass is.  1024 x 64 tokens of 4 heads of 64 x 64: 32-bit 433 us (122 registers, 1.5 instructions a cycle and SM), bfloat16 at 2048 x 64 441 us.
 #pragma once
 #include "linear_forward.cuh"
 

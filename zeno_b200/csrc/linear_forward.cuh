@@ -4,6 +4,10 @@
 // One block takes one (environment, value head) and walks over its chunks, the state in the warps'
 // accumulators.  Few long rollouts are cut into segments: one kernel sums what each segment adds to the state, one walks
 // over the segments, and then every segment is a block of its own.
+//
+// What bounds it is neither bytes nor products: addresses, limbs and fragments are most of the instructions, and a chunk's steps wait
+// for one another (1.5 instructions a cycle and SM, two blocks of 8 warps).  1024 x 64 tokens of 4 heads of 64 x 64: 32-bit 230 us (six products
+// for one), bfloat16 at 2048 x 64 223 us.  Having the next chunk's rows on their way to L2 was worth 3 % and not kept.
 #pragma once
 #include "linear_mma.cuh"
 

@@ -221,8 +221,8 @@ __device__ __forceinline__ GateIn<C> fetch_gates(const float* g, int64_t g_strid
 }
 
 // One warp: their gates.  Sums run from the last reset on, so that what one episode's decays are, not finite included, stays in it.  They are
-// taken in 64-bit integers, in units of 2^-40 (exact, where a scan in double was a third of a chunk's time); a log decay of 2^16 and
-// more counts as not a number.  One decay for all tokens (`fixed`) needs no sum.
+// taken in 64-bit integers, in units of 2^-40: exact in any order, with additions that every SM has many of where those in double are few.  A
+// log decay of 2^16 and more counts as not a number.  One decay for all tokens (`fixed`) needs no sum.
 template <int C>
 __device__ __forceinline__ void scan_gates(Gates<C>& s, GateIn<C> in, bool fixed, int n, int lane) {
   constexpr int U = C / 32;
