@@ -263,3 +263,11 @@ def test_refusals():
             ((x,), {"eps": -1.0}, ValueError, "eps"), ((x,), {"eps": float("nan")}, ValueError, "eps"), ((x[:, :0],), {}, ValueError, "last axis"), ((x[0, 0],), {}, ValueError, "last axis")]:
         with pytest.raises(error, match=match):
             f(*args, **kw)
+
+
+def test_sizes_beyond_the_entries_are_refused():
+    """Before anything is allocated: such a width would not pass the entry's 32-bit field."""
+    x = torch.zeros(1, 1, device=DEV)
+    for shape in ((1, 2 ** 32 + 8), (1, 2 ** 30 + 1), (2 ** 31 + 1, 1), (2 ** 16, 2 ** 16, 1)):
+        with pytest.raises(ValueError, match="at most 2\\^31 rows"):
+            zeno_b200.layer_norm(x.expand(shape))

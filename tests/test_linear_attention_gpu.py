@@ -558,3 +558,16 @@ def test_refusals():
         step(*one, t(2, 4, 8, 16, dtype=torch.bfloat16))
     with pytest.raises(RuntimeError, match="no gradients"):
         step(*one, t(2, 4, 8, 16).requires_grad_(True))
+
+
+def test_sizes_beyond_the_entries_are_refused():
+    """Before anything is allocated: such sizes would not pass the entries' 32-bit fields."""
+    x, g = torch.zeros(1, 1, 1, 1, device=DEV), torch.zeros(1, device=DEV)
+    state = torch.zeros(1, 1, 1, 1, device=DEV)
+    for shape in ((2 ** 32 + 1, 1, 1, 1), (2 ** 27 + 1, 1, 1, 1), (1, 2 ** 32 + 1, 1, 1), (1, 2 ** 30 + 1, 1, 1), (1, 1, 2 ** 32 + 1, 1), (1, 1, 65536, 1)):
+        big = x.expand(shape)
+        with pytest.raises(ValueError, match="at most 65535 value heads"):
+            zeno_b200.linear_attention(big, big, big, g.expand(shape[2]))
+        if shape[1] == 1:
+            with pytest.raises(ValueError, match="at most 65535 value heads"):
+                zeno_b200.linear_attention_step(big[:, 0], big[:, 0], big[:, 0], g.expand(shape[2]), state.expand(shape[0], shape[2], 1, 1))

@@ -24,7 +24,8 @@ using Maybe = std::optional<Tensor>;
 
 namespace {
 
-constexpr int64_t kMaxDim = 128;
+constexpr int64_t kMaxDim = 128, kMaxHeads = 65535, kMaxStates = 1 << 27, kMaxTokens = 1 << 30;  // linear attention
+constexpr int64_t kMaxWidth = 1 << 30, kMaxRows = int64_t(1) << 31;                                 // layer norm
 
 std::string shape_of(at::IntArrayRef s) {
   std::string r = "(";
@@ -148,6 +149,9 @@ std::array<int64_t, 4> check_linear(const Tensor& q, const Tensor& k, const Tens
     bad_value("head widths must be 1 to " + std::to_string(kMaxDim) + ", got " + std::to_string(dk) + " and " + std::to_string(dv));
   if (key_heads < 1 || heads < 1 || heads % key_heads)
     bad_value("the " + std::to_string(heads) + " value heads must be a multiple of the " + std::to_string(key_heads) + " key heads");
+  // what the C entries take, before anything is allocated or cut to their types
+  if (heads > kMaxHeads || q.size(0) > kMaxStates / heads || (lead == 2 && q.size(1) > kMaxTokens))
+    bad_value("at most 65535 value heads, 2^27 states and 2^30 tokens, got q " + shape_of(q.sizes()) + " and " + std::to_string(heads) + " value heads");
   expect("k", k, q.sizes(), q.scalar_type(), q);
   const int64_t front[4] = {q.size(0), lead == 2 ? q.size(1) : heads, lead == 2 ? heads : dv, dv};
   expect("v", v, at::IntArrayRef(front, size_t(lead + 2)), q.scalar_type(), q);
@@ -340,6 +344,7 @@ Tensor layer_norm(const Tensor& x_, const Maybe& weight_, const Maybe& bias_, do
   if (!is_ours(x_.scalar_type())) bad_type("x must be float32 or bfloat16, got " + type_of(x_.scalar_type()));
   if (x_.dim() < 1 || x_.size(-1) < 1) bad_value("x needs a last axis to be normalised over, got shape " + shape_of(x_.sizes()));
   const int64_t width = x_.size(-1);
+  if (width > kMaxWidth || x_.numel() / width > kMaxRows) bad_value("at most 2^31 rows of 2^30 values, got shape " + shape_of(x_.sizes()));
   const std::pair<const char*, Tensor*> both[] = {{"weight", &weight}, {"bias", &bias}};
   for (const auto& [name, t] : both) {
     if (!t->defined()) continue;
