@@ -61,7 +61,7 @@ def test_gradients_of_every_parameter():
 
 
 def test_in_a_cuda_graph():
-    """A training step captured while an eager one of the same parameters is alive, replayed on another rollout."""
+    """A training step captured after an eager one of the same parameters, replayed on another rollout."""
     obs, begins = rollout(E=700, T=20, seed=2)
     policy = MemoryPolicy(29, 8, hidden=64, heads=2, width=32, memory="decay").cuda()
     parameters = list(policy.parameters())
