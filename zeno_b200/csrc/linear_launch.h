@@ -56,21 +56,23 @@ inline uint32_t vec_of(const ZenoLinearAttention& p, const ZenoTensor& out) {
          vec_of(out, p.value_dim, p.dtype, kVecOut);
 }
 
-// f(shape) of the call's instance, for one element type.
+// f(shape) of the call's instance, for one element type.  Heads of 128 channels are one block an SM: 16 warps for 32-bit calls (244 x 139 tokens, 2
+// heads of 40 x 128, with gradients: 464 us against 530 with 8; 2183 x 4, 128 x 64: 393 against 421) and where widths are not whole (bfloat16, 777 x 20, 4 heads
+// of 100 x 128, backward: 356 against 393); 8 for whole bfloat16 ones (1024 x 32, 4 of 128 x 128: 458 against 472).
 template <class T, bool FULL, class F>
 cudaError_t with_shape_of(const ZenoLinearAttention& p, int w, F&& f) {
   if constexpr (sizeof(T) == 2) {
     if (chunk_of(p) == 32) {
       if (w == 32) return f(Shape<T, 32, 32, 4, FULL>{});
       if (w == 64) return f(Shape<T, 64, 32, 4, FULL>{});
-      return f(Shape<T, 128, 32, 8, FULL>{});
+      return f(Shape<T, 128, 32, FULL ? 8 : 16, FULL>{});
     }
     if (w == 64) return f(Shape<T, 64, 64, 8, FULL>{});
     return f(Shape<T, 128, 64, 16, FULL>{});
   } else {
     if (w == 32) return f(Shape<T, 32, 32, 4, FULL>{});
     if (w == 64) return f(Shape<T, 64, 32, 8, FULL>{});
-    return f(Shape<T, 128, 32, 8, FULL>{});
+    return f(Shape<T, 128, 32, 16, FULL>{});
   }
 }
 inline bool full_width(const ZenoLinearAttention& p) { return int(p.key_dim) == width_of(p) && int(p.value_dim) == width_of(p); }
