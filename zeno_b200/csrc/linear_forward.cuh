@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(S::THREADS, BLOCKS) linear_segment_kernel(cons
     const bool bad = __syncthreads_or(rows_odd<S>(x, dk, nt, mv) || rows_odd<S>(y, dv, nt, mv));
     const float* weight = reverse ? s.carried : s.to_end;
     const float factor = reverse ? p.scale : 1.0f, keep = step ? s.keep : 0.0f;
-    kept *= s.keep;
+    kept = both_keep(kept, s.keep);
     if (bad) update_masked<S>(m, x, y, weight, factor, keep, n, part, dk, dv, lane);
     else update<S>(m, x, y, weight, factor, keep, nt, part, lane);
   }

@@ -201,6 +201,9 @@ __device__ __forceinline__ float pair_decay(const Token& ti, const Token& tj, bo
   return meet ? ex2((ti.hi - tj.hi) + (ti.lo - tj.lo)) : 0.0f;
 }
 
+// What is left of a state over two stretches: nothing where one of them drops it, whatever the other's decays are.
+__device__ __forceinline__ float both_keep(float a, float b) { return a == 0.0f || b == 0.0f ? 0.0f : a * b; }
+
 // One warp: log decays and marks of n tokens, C / 32 neighbouring ones a lane.  Fetched before the rows, whose loads would be waited for first.
 template <int C>
 struct GateIn {

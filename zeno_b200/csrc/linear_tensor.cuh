@@ -586,7 +586,7 @@ linear_tensor_segment_kernel(const __grid_constant__ ZenoLinearAttention p, cons
     copies_landed();
     const bool bad = __syncthreads_or(tile_odd(x, mv) || tile_odd(y, mv));
     const float keep = step ? s.keep : 0.0f;
-    kept *= s.keep;
+    kept = both_keep(kept, s.keep);
     if (bad) {
       const int64_t t0 = int64_t(reverse ? a.c1 - 1 - step : a.c0 + step) * C;
       merge_masked<S>(m, x, y, weight, factor, keep, int(min(int64_t(C), int64_t(p.tokens) - t0)), part, lane);
