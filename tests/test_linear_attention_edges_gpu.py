@@ -44,3 +44,60 @@ def test_a_reset_in_another_chunk_of_a_segment(dtype, d, segment, bad):
             continue
         check(a[1], b[1], name), check(a[0, :, 0], b[0, :, 0], name)
         check(a[0, outside, 1], b[0, outside, 1], name)
+
+
+def entry(t):
+    """A tensor as the C entries take it: [B, T, heads, ...], or [B, T]."""
+    from zeno_b200._ffi import ffi
+    s = t.stride()
+    return dict(data=ffi.cast("void*", t.data_ptr()), stride=[s[0], s[1], s[2] if len(s) > 2 else 0])
+
+
+@pytest.mark.parametrize("B,T,Hk,H,d,dtype,infinite", [
+    (300, 20, 2, 2, 64, torch.bfloat16, False), (300, 32, 1, 2, 40, torch.bfloat16, False), (300, 9, 2, 2, 128, torch.bfloat16, False),
+    (300, 20, 2, 2, 32, torch.bfloat16, True), (2, 300, 2, 2, 128, torch.bfloat16, False), (40, 64, 1, 2, 100, torch.bfloat16, False),
+    (3, 50, 1, 1, 40, torch.float32, False), (1, 900, 1, 2, 64, torch.bfloat16, False)])
+def test_both_gradients_of_the_decays(B, T, Hk, H, d, dtype, infinite):
+    """The C entry gives each token's gradient, their sum over batch and tokens, or both: by warps (`infinite`: element by element), on tcgen05, by blocks.
+    The sum is one in 64 bits of the 32-bit gradients, rounded once (2^-24)."""
+    from zeno_b200._ffi import _lib, ffi
+    x = inputs(B, T, Hk, H, d, d, dtype, reset=0.05)
+    if infinite:  # in every head, where it is masked from the gradients of the decays: a token that is its own episode
+        x[4][:, 4:6] = 1
+        x[0][:, 4, :, 3] = float("inf")
+    d_out = torch.randn(B, T, H, d, device=DEV).to(dtype)
+    p, grads = ffi.new("ZenoLinearAttention*"), ffi.new("ZenoLinearAttentionGrads*")
+    p.batch, p.tokens, p.key_heads, p.value_heads, p.key_dim, p.value_dim = B, T, Hk, H, d, d
+    p.dtype, p.scale = int(dtype == torch.bfloat16), d ** -0.5
+    out, (d_q, d_k, d_v, d_g) = torch.empty_like(x[2]), [torch.empty_like(t) for t in x[:4]]
+    d_decay = torch.full((H,), float("nan"), device=DEV)
+    p.q, p.k, p.v, p.g, p.reset, p.out = (entry(t) for t in (*x[:5], out))
+    p.initial_state = ffi.cast("float*", x[5].data_ptr())
+    saved = torch.empty(max(1, _lib.zeno_linear_attention_saved_bytes(p) // 4), device=DEV)
+    p.saved = ffi.cast("float*", saved.data_ptr())
+    need = max(_lib.zeno_linear_attention_workspace_bytes(p, i) for i in (0, 1))
+    work = torch.full((max(need // 4, 1),), float("nan"), device=DEV)
+    at, stream = ffi.cast("void*", work.data_ptr()), ffi.cast("void*", torch.cuda.current_stream().cuda_stream)
+    assert _lib.zeno_linear_attention_forward(p, at, need, stream) == 0
+    grads.d_out, grads.d_q, grads.d_k, grads.d_v, grads.d_g = (entry(t) for t in (d_out, d_q, d_k, d_v, d_g))
+    grads.d_decay = ffi.cast("float*", d_decay.data_ptr())
+    work.fill_(float("nan"))
+    assert _lib.zeno_linear_attention_backward(p, grads, at, need, stream) == 0
+    want = gradients(zeno_b200.linear_attention, x, d_out)
+    for a, b in zip((d_q, d_k, d_v, d_g), want[2:]):
+        assert torch.equal(a, b) or infinite
+    if infinite:
+        return check_sum(d_decay, d_g, finite=torch.isfinite(d_g).all())
+    check_sum(d_decay, d_g)
+    grads.d_g.data = ffi.NULL  # the sum alone
+    alone = torch.full((H,), float("nan"), device=DEV)
+    grads.d_decay = ffi.cast("float*", alone.data_ptr())
+    assert _lib.zeno_linear_attention_backward(p, grads, at, need, stream) == 0
+    # (there a pair's term is counted once, times the tokens it passes: other roundings, at most 3.6e-6 of the terms)
+    assert ((alone - d_decay).abs().double() <= 3.6e-6 * d_g.double().abs().sum((0, 1))).all()
+
+
+def check_sum(d_decay, d_g, finite=True):
+    assert finite
+    terms = d_g.double()
+    assert ((d_decay.double() - terms.sum((0, 1))).abs() <= 2.0 ** -24 * terms.sum((0, 1)).abs() + 2.0 ** -40 * terms.abs().sum((0, 1))).all()

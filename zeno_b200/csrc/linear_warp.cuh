@@ -331,14 +331,23 @@ struct WarpResults {
   int64_t shared_stride;
 };
 
-// dg of each token from what passes it and from the state in front.
-__device__ __forceinline__ void warp_decays(const ZenoLinearAttentionGrads& d, const WarpAt& a, float pass, float x, int n, int lane) {
+// dg of each token from what passes it and from the state in front; returns that of the lane's.
+__device__ __forceinline__ float warp_decays(const ZenoLinearAttentionGrads& d, const WarpAt& a, float pass, float x, int n, int lane) {
 #pragma unroll
   for (int y = 1; y < 32; y <<= 1) {
     const float z = __shfl_down_sync(kAll, x, y);
     if (lane + y < 32) x += z;
   }
-  if (lane < n) place<float>(d.d_g, a.b, a.h)[lane * d.d_g.stride[1]] = pass + x;
+  if (lane >= n) return 0.0f;
+  place<float>(d.d_g, a.b, a.h)[lane * d.d_g.stride[1]] = pass + x;
+  return pass + x;
+}
+// Their sum over the head, from the lanes' parts.
+__device__ __forceinline__ void sum_decays(const BackwardOut& extra, const WarpAt& a, uint32_t batch, double part, int lane) {
+  if (!extra.decay) return;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) part += __shfl_xor_sync(kAll, part, x);
+  if (lane == 0) extra.decay[uint64_t(a.h) * batch + a.b] = part;
 }
 
 template <class S>
@@ -417,8 +426,7 @@ __device__ __noinline__ double warp_backward_slow(const ZenoLinearAttention& p, 
         state[e * dv + c] = y;
       }
   }
-  if (d.d_g.data) warp_decays(d, a, passes, mine_x, n, lane);
-  return decays;
+  return d.d_g.data ? double(warp_decays(d, a, passes, mine_x, n, lane)) : decays;
 }
 
 // Without a gradient of the final state.
@@ -540,9 +548,7 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
     }
   }
   if (__any_sync(kAll, odd != odd)) {
-    double sum = warp_backward_slow<S>(p, d, a, to, s, q, k, v, o, initial, n, lane);
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(kAll, sum, x);
-    if (extra.decay && lane == 0) extra.decay[uint64_t(a.h) * p.batch + a.b] = sum;
+    sum_decays(extra, a, p.batch, warp_backward_slow<S>(p, d, a, to, s, q, k, v, o, initial, n, lane), lane);
     return;
   }
 
@@ -695,15 +701,12 @@ linear_warp_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const
 #pragma unroll
     for (int r = 0; r < 2; ++r) keep_rows(all.x, make_float2(x_rows[r][0], x_rows[r][1]), r, lane);
     __syncwarp();
-    warp_decays(d, a, all.pass[lane], lane < n ? all.x[lane] : 0.0f, n, lane);
-  } else if (extra.decay) {
+    sum_decays(extra, a, p.batch, double(warp_decays(d, a, all.pass[lane], lane < n ? all.x[lane] : 0.0f, n, lane)), lane);
+  } else {
 #pragma unroll
     for (int r = 0; r < 2; ++r)  // the state in front passes every token up to a row's own
       decays = fmaf(x_rows[r][0], float(r * 16 + g + 1), fmaf(x_rows[r][1], float(r * 16 + g + 9), decays));
-    double sum = double(decays);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(kAll, sum, x);
-    if (lane == 0) extra.decay[uint64_t(a.h) * p.batch + a.b] = sum;
+    sum_decays(extra, a, p.batch, double(decays), lane);
   }
   __syncwarp();
   if (!to.shared_q) {
