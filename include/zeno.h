@@ -427,7 +427,8 @@ int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
 uint64_t zeno_linear_attention_wait_limit(uint64_t nanoseconds);
 
 /* Layer norm of rows of `width` values: out = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps), mean and
- * variance in 32 bits, the variance from the differences to the mean.  No output overlaps an input. */
+ * variance in 32 bits, the variance from the differences to the mean.  Finite rows of any spread have a finite result (with eps = 0
+ * a row of no spread is 0 / 0): where squares leave a float's range the row is taken in other units.  No output overlaps an input. */
 typedef struct {
   uint64_t rows[3];  /* the rows are [rows[0], rows[1], rows[2]] */
   uint32_t width;    /* at least 1 */
@@ -438,7 +439,8 @@ typedef struct {
   const void* weight; /* [width], contiguous; NULL: 1 */
   const void* bias;   /* [width], contiguous; NULL: 0 */
   ZenoTensor out;
-  float* saved;       /* written by forward for backward: mean (in two parts) and rstd of every row, [3][rows]; NULL: no gradients wanted */
+  float* saved;       /* written by forward for backward: mean (in two parts) and rstd of every row, [3][rows] (rstd negative: all of x / 2^96);
+                         NULL: no gradients wanted */
 } ZenoLayerNorm;
 
 /* out and bias are not read.  d_x.data, d_weight and d_bias may be NULL: not wanted. */

@@ -6,11 +6,16 @@
 // sums of its own columns over the rows it sees; a block's sums go to the workspace and a second kernel adds them in a
 // fixed order.  Sums are 32-bit (the last ones over blocks too), the variance is taken from the differences to the mean.
 //
+// Rows whose squares leave a float's range are taken again in units that they fit in, once a thread's rows are through: rows of spreads past 1e19 (or
+// whose plain sum overflows) in units of 2^96, and differences below 2^-50, which count where eps is below 2^-100, times 2^96.  Powers of two round
+// nothing.  In the loops over the rows this costs a comparison of each (branches there cost 3 to 8 %, the registers of the other side included).
+//
 // 131072 rows of 256 bfloat16: 30 us forward, 40 us backward (20 and 31 us of bytes), 4 us for the sums over blocks; 524288 rows of 64: 26.5 us (20 us).
 // Those are bound by the issue of instructions (68 %).  2047 rows of 4099 floats, whose rows are not aligned: 25 and 36 us, value by value.
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "policy_ops.h"
 
@@ -30,7 +35,7 @@ struct Norm {
   const void *x, *weight, *bias, *dy;
   void *y, *dx;
   RowsAt at_x, at_y, at_dy, at_dx;
-  float* saved;    // [3][rows]: the mean as summed, what that sum's rounding left of it, rstd
+  float* saved;    // [3][rows]: the mean as summed, what that sum's rounding left of it, rstd; rstd negative: all three are of x in units of 2^96
   float* partial;  // [blocks][2][width]: sums of dy xhat and of dy
   uint32_t rows, rows1, rows2, width;
   float eps;
@@ -132,8 +137,24 @@ __device__ __forceinline__ void put(T* at, const float (&x)[V]) {
 // 1 / sqrt(x): the approximation and one Newton step
 __device__ __forceinline__ float inverse_sqrt(float x) {
   const float y = rsqrtf(x);
-  return x < INFINITY ? fmaf(0.5f * y, fmaf(-x * y, y, 1.0f), y) : y + (x - x);
+  return x < INFINITY ? fmaf(0.5f * y, fmaf(-x * y, y, 1.0f), y) : y;
 }
+
+constexpr float kUp = 79228162514264337593543950336.0f, kDown = 1.0f / kUp;  // 2^96
+// x where it is above 0 or not a number
+__device__ __forceinline__ float positive(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(0.0f));
+  return y;
+}
+// variance + eps, from the sums of the differences and of their squares and 1 / n; not a number where a difference is not finite.
+// rest: what the sum's rounding left of the mean
+__device__ __forceinline__ float spread(float2 sums, float inverse, float eps, float& rest) {
+  rest = sums.x * inverse;
+  return positive(fmaf(-rest, rest, sums.y * inverse)) + eps;
+}
+// Whether the squares kept 24 bits: above 2^-100.
+__device__ __forceinline__ bool in_range(float v) { return v > 7.888609e-31f && v < INFINITY; }
 
 // Sums over the LANES lanes of a row, or over a block.  A block's pass through `box` (taken in turns so that one barrier is enough).
 template <int LANES, bool BLOCK>
@@ -185,6 +206,8 @@ struct Shape {
   static constexpr bool BLOCK = BLOCK_;
   static constexpr int PER = BLOCK ? 1 : 256 / LANES;  // rows side by side in a block
   static constexpr bool AHEAD = N * V <= 8;
+  // blocks that an SM has registers for, where the compiler would take a few more than leave place for them (0: as it likes)
+  static constexpr int FORWARD_RESIDENT = V == 8 && N == 2 && !BLOCK ? 4 : 0, BACKWARD_RESIDENT = V == 8 && N == 1 ? 4 : 0;
   static constexpr int COLS = LANES * N * V;  // columns that there is room for (BLOCK: for each warp)
   int first;   // first column
   bool full;   // no column of this row (this warp) is past the width
@@ -196,10 +219,60 @@ struct Shape {
   __device__ __forceinline__ int column(int i) const { return first + i * LANES * V; }
 };
 
+// One row value by value, in ordinary units and, where its squares leave the range there, in others; such a row is written.  All lanes of a warp
+// come here, where a block has the row all of its threads.  columns(f): f of each column that is this thread's.
+template <int LANES, bool BLOCK, class T, class W, class F>
+__device__ __forceinline__ void norm_again(const Norm& p, uint32_t row, bool first_lane, float2 (*box)[32], F&& columns) {
+  int turn = 0;  // (the sums are even in number)
+  const bool here = row < p.rows;
+  const T* from = static_cast<const T*>(p.x) + (here ? offset(p.at_x, row, p) : 0);
+  const float inverse = 1.0f / float(p.width);
+  float unit = 1.0f, times = 1.0f, mean, rest, v;  // x times `unit`, its differences times `times`
+  auto difference = [&](uint32_t c) { return fmaf(float(from[c]), unit, -mean) * times; };
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    float sum = 0.0f;
+    if (here) columns([&](uint32_t c) { sum = fmaf(float(from[c]), unit, sum); });
+    mean = row_sum<LANES, BLOCK>(sum, box, turn) * inverse;
+    float2 sums = make_float2(0.0f, 0.0f);
+    if (here) columns([&](uint32_t c) {
+      const float d = difference(c);
+      sums.x += d, sums.y = fmaf(d, d, sums.y);
+    });
+    v = spread(row_sum<LANES, BLOCK>(sums, box, turn), inverse, p.eps * (unit * times) * (unit * times), rest);
+    if (pass == 0 && !in_range(v)) (v < INFINITY ? times : unit) = v < INFINITY ? kUp : kDown;
+  }
+  if (!here || unit * times == 1.0f) return;
+  const float rstd = inverse_sqrt(v);
+  T* to = static_cast<T*>(p.y) + offset(p.at_y, row, p);
+  columns([&](uint32_t c) {
+    float y[1] = {(difference(c) - rest) * rstd};
+    if (p.weight) y[0] *= float(static_cast<const W*>(p.weight)[c]);
+    if (p.bias) y[0] += float(static_cast<const W*>(p.bias)[c]);
+    put(to + c, y);
+  });
+  if (!p.saved || !first_lane) return;
+  p.saved[row] = mean, p.saved[uint64_t(p.rows) + row] = times == 1.0f ? rest : rest * kDown;
+  p.saved[2 * uint64_t(p.rows) + row] = unit == 1.0f ? fminf(rstd * times, 3.402823e38f) + (rstd - rstd) : -rstd;
+}
+// The rows of a thread.
+template <class S>
+__device__ __noinline__ void norm_forward_again(const Norm& p, float2 (*box)[32]) {
+  const S at(p.width);
+  for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER)
+    norm_again<S::LANES, S::BLOCK, typename S::T, typename S::W>(p, uint32_t(first) + (S::BLOCK ? 0 : threadIdx.x / S::LANES), at.first == 0, box, [&](auto&& f) {
+#pragma unroll 1
+      for (int i = 0; i < S::N * S::V; ++i) {
+        const uint32_t c = uint32_t(at.column(i / S::V)) + i % S::V;
+        if (c < p.width) f(c);
+      }
+    });
+}
+
 // Rows from blockIdx.x on in steps of the grid; the next one is on its way while one is worked on.  Where a lane has 16 values
 // there are more blocks instead (of 4099 values: 25 us against 28).
 template <class S>
-__global__ void __launch_bounds__(S::BLOCK ? 512 : 256) norm_forward_kernel(const __grid_constant__ Norm p) {
+__global__ void __launch_bounds__(S::BLOCK ? 512 : 256, S::FORWARD_RESIDENT) norm_forward_kernel(const __grid_constant__ Norm p) {
   using T = typename S::T;
   using W = typename S::W;
   constexpr int V = S::V, N = S::N, M = S::M;
@@ -232,6 +305,7 @@ __global__ void __launch_bounds__(S::BLOCK ? 512 : 256) norm_forward_kernel(cons
     for (int i = 0; i < N; ++i) fetch_affine(i);
   }
   const float inverse = 1.0f / float(p.width);
+  bool again = false;  // (where a block has the rows, the same in all of its threads)
   for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER) {
     const uint32_t row = uint32_t(first) + own;
     if (!AHEAD) fetch_row(row);
@@ -266,11 +340,10 @@ __global__ void __launch_bounds__(S::BLOCK ? 512 : 256) norm_forward_kernel(cons
 #pragma unroll
     for (int m = 1; m < M; ++m) s = s + y[m], q = fma2(y[m], y[m], q);
     const float2 c = apart(s), d = apart(q);
-    const float2 sums = row_sum<S::LANES, S::BLOCK>(make_float2(c.x + c.y, d.x + d.y), box, turn);
-    // what the sum's rounding left of the mean
-    const float rest = sums.x * inverse;
-    float rstd = inverse_sqrt(fmaxf(fmaf(-rest, rest, sums.y * inverse), 0.0f) + p.eps);
-    if (sums.y != sums.y) rstd = sums.y;
+    float rest;
+    const float v = spread(row_sum<S::LANES, S::BLOCK>(make_float2(c.x + c.y, d.x + d.y), box, turn), inverse, p.eps, rest);
+    const float rstd = inverse_sqrt(v);
+    again |= !in_range(v);
     if (row >= p.rows) continue;
     const float less = -rest * rstd;
     const Two f = two(rstd, rstd), r = two(less, less);
@@ -291,6 +364,7 @@ __global__ void __launch_bounds__(S::BLOCK ? 512 : 256) norm_forward_kernel(cons
     if (p.saved && (S::BLOCK ? threadIdx.x : threadIdx.x & (S::LANES - 1)) == 0)
       p.saved[row] = mean, p.saved[uint64_t(p.rows) + row] = rest, p.saved[2 * uint64_t(p.rows) + row] = rstd;
   }
+  if (S::BLOCK ? again : __any_sync(kAll, again)) norm_forward_again<S>(p, box);
 }
 
 // A row of x and dy, and what is known of it.
@@ -337,12 +411,10 @@ __device__ __forceinline__ void norm_backward(const Norm& p) {
   for (int m = 0; m < M; ++m) dw[m] = db[m] = two(0.0f, 0.0f);
   Fetched<S> next;
   if (AHEAD) next.fetch(p, at, blockIdx.x * S::PER + own);
-  for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER) {
-    const uint32_t row = uint32_t(first) + own;
-    if (!AHEAD) next.fetch(p, at, row);
-    Fetched<S> now = next;
-    const uint64_t ahead = first + uint64_t(gridDim.x) * S::PER;
-    if (AHEAD && ahead < p.rows) next.fetch(p, at, uint32_t(ahead) + own);
+  bool again = false;
+  // A row; its sums over dy xhat are zero where x is in other units (`large`: the rows that are, and those sums alone).
+  auto take = [&](auto large, const Fetched<S>& now, uint32_t row) {
+    constexpr bool LARGE = decltype(large)::value;
     Two x[M], g[M];
     {
       float a[N][V], b[N][V];
@@ -352,14 +424,18 @@ __device__ __forceinline__ void norm_backward(const Norm& p) {
 #pragma unroll
       for (int m = 0; m < M; ++m) x[m] = two(va[2 * m], va[2 * m + 1]), g[m] = two(vb[2 * m], vb[2 * m + 1]);
     }
-    const float less = -now.rest * now.rstd;
-    const Two minus = two(-now.mean, -now.mean), r = two(less, less), f = two(now.rstd, now.rstd);
+    const bool other = now.rstd < 0.0f;
+    const float rstd = LARGE ? -now.rstd : positive(now.rstd), less = -now.rest * rstd;
+    const Two minus = two(-now.mean, -now.mean), r = two(less, less), f = two(rstd, rstd);
 #pragma unroll
     for (int m = 0; m < M; ++m) {  // (what is not there has no gradient: it adds nothing)
+      if (LARGE) x[m] = other ? x[m] * two(kDown, kDown) : two(0.0f, 0.0f);
       x[m] = fma2(x[m] + minus, f, r);
-      dw[m] = fma2(g[m], x[m], dw[m]), db[m] = db[m] + g[m];
+      if (!LARGE) dw[m] = fma2(g[m], x[m], dw[m]), db[m] = db[m] + g[m];
+      else if (other) dw[m] = fma2(g[m], x[m], dw[m]);
     }
-    if (!p.dx) continue;
+    if (!LARGE) again |= other;
+    if (!p.dx) return;
     if (p.weight) {
       float w[N][V];
 #pragma unroll
@@ -377,18 +453,35 @@ __device__ __forceinline__ void norm_backward(const Norm& p) {
     for (int m = 1; m < M; ++m) s0 = s0 + g[m], s1 = fma2(g[m], x[m], s1);
     const float2 a = apart(s0), b = apart(s1);
     const float2 t = row_sum<S::LANES, S::BLOCK>(make_float2(a.x + a.y, b.x + b.y), box, turn);
-    if (row >= p.rows) continue;
+    if (row >= p.rows || (LARGE && !other)) return;
     const Two m0 = two(-t.x * inverse, -t.x * inverse), m1 = two(-t.y * inverse, -t.y * inverse);
     T* to = static_cast<T*>(p.dx) + offset(p.at_dx, row, p) + at.first;
     float z[N][V];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const float2 c = apart((g[m] + fma2(x[m], m1, m0)) * f);
+      Two y = (g[m] + fma2(x[m], m1, m0)) * f;
+      if (LARGE) y = y * two(kDown, kDown);
+      const float2 c = apart(y);
       (&z[0][0])[2 * m] = c.x, (&z[0][0])[2 * m + 1] = c.y;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (at.full || uint32_t(at.column(i)) < p.width) put(to + i * S::LANES * V, z[i]);
+  };
+  for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER) {
+    const uint32_t row = uint32_t(first) + own;
+    if (!AHEAD) next.fetch(p, at, row);
+    Fetched<S> now = next;
+    const uint64_t ahead = first + uint64_t(gridDim.x) * S::PER;
+    if (AHEAD && ahead < p.rows) next.fetch(p, at, uint32_t(ahead) + own);
+    take(std::false_type{}, now, row);
+  }
+  if (S::BLOCK ? again : __any_sync(kAll, again)) {
+#pragma unroll 1
+    for (uint64_t first = uint64_t(blockIdx.x) * S::PER; first < p.rows; first += uint64_t(gridDim.x) * S::PER) {
+      next.fetch(p, at, uint32_t(first) + own);
+      take(std::true_type{}, next, uint32_t(first) + own);
+    }
   }
   if (!p.partial) return;
   float* line = p.partial + uint64_t(blockIdx.x) * 2 * p.width;
@@ -415,7 +508,7 @@ __device__ __forceinline__ void norm_backward(const Norm& p) {
   }
 }
 template <class S>
-__global__ void __launch_bounds__(256) norm_backward_kernel(const __grid_constant__ Norm p) {
+__global__ void __launch_bounds__(256, S::BACKWARD_RESIDENT) norm_backward_kernel(const __grid_constant__ Norm p) {
   norm_backward<S>(p);
 }
 // (104 registers, so that rows of 4096 values are two to an SM)
@@ -426,10 +519,18 @@ __global__ void __maxnreg__(104) norm_backward_block_kernel(const __grid_constan
 
 // Rows too long for registers: one block a row, which is read three times forward (from L2 after the first).
 template <class T, class W>
+__device__ __noinline__ void norm_wide_forward_again(const Norm& p, float2 (*box)[32]) {
+  for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x)
+    norm_again<32, true, T, W>(p, row, threadIdx.x == 0, box, [&](auto&& f) {
+      for (uint32_t c = threadIdx.x; c < p.width; c += 1024) f(c);
+    });
+}
+template <class T, class W>
 __global__ void __launch_bounds__(1024) norm_wide_forward_kernel(const __grid_constant__ Norm p) {
   __shared__ float2 box[2][32];
   int turn = 0;
   const float inverse = 1.0f / float(p.width);
+  bool again = false;
   for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* from = static_cast<const T*>(p.x) + offset(p.at_x, row, p);
     T* to = static_cast<T*>(p.y) + offset(p.at_y, row, p);
@@ -441,10 +542,9 @@ __global__ void __launch_bounds__(1024) norm_wide_forward_kernel(const __grid_co
       const float d = float(from[c]) - mean;
       s.x += d, s.y = fmaf(d, d, s.y);
     }
-    s = row_sum<32, true>(s, box, turn);
-    const float rest = s.x * inverse;
-    float rstd = inverse_sqrt(fmaxf(fmaf(-rest, rest, s.y * inverse), 0.0f) + p.eps);
-    if (s.y != s.y) rstd = s.y;
+    float rest;
+    const float v = spread(row_sum<32, true>(s, box, turn), inverse, p.eps, rest), rstd = inverse_sqrt(v);
+    again |= !in_range(v);
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) {
       float y[1] = {(float(from[c]) - mean - rest) * rstd};
       if (p.weight) y[0] *= float(static_cast<const W*>(p.weight)[c]);
@@ -453,37 +553,57 @@ __global__ void __launch_bounds__(1024) norm_wide_forward_kernel(const __grid_co
     }
     if (p.saved && threadIdx.x == 0) p.saved[row] = mean, p.saved[uint64_t(p.rows) + row] = rest, p.saved[2 * uint64_t(p.rows) + row] = rstd;
   }
+  if (again) norm_wide_forward_again<T, W>(p, box);
 }
-template <class T, class W>
-__global__ void __launch_bounds__(1024) norm_wide_backward_kernel(const __grid_constant__ Norm p) {
-  __shared__ float2 box[2][32];
-  int turn = 0;
+// LARGE: the rows in other units (whose dy have been summed) alone; whether there are such.
+template <bool LARGE, class T, class W>
+__device__ __forceinline__ bool norm_wide_rows(const Norm& p, float2 (*box)[32], int& turn) {
   const float inverse = 1.0f / float(p.width);
   float* line = p.partial ? p.partial + uint64_t(blockIdx.x) * 2 * p.width : nullptr;
-  if (line)
-    for (uint32_t c = threadIdx.x; c < p.width; c += 1024) line[c] = 0.0f, line[p.width + c] = 0.0f;
+  bool again = false;
   for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* from = static_cast<const T*>(p.x) + offset(p.at_x, row, p);
     const T* grad = static_cast<const T*>(p.dy) + offset(p.at_dy, row, p);
-    const float mean = p.saved[row], rest = p.saved[uint64_t(p.rows) + row], rstd = p.saved[2 * uint64_t(p.rows) + row];
+    const float mean = p.saved[row], rest = p.saved[uint64_t(p.rows) + row], kept = p.saved[2 * uint64_t(p.rows) + row];
+    const float rstd = LARGE ? -kept : positive(kept);
+    again |= kept < 0.0f;
+    if (LARGE && !(kept < 0.0f)) continue;
+    auto hat_of = [&](uint32_t c) { return ((LARGE ? float(from[c]) * kDown : float(from[c])) - mean - rest) * rstd; };
     float2 s = make_float2(0.0f, 0.0f);
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) {  // a thread comes back to its own columns of the line
-      const float hat = (float(from[c]) - mean - rest) * rstd, dy = float(grad[c]);
+      const float hat = hat_of(c), dy = float(grad[c]);
       const float dh = p.weight ? dy * float(static_cast<const W*>(p.weight)[c]) : dy;
       s.x += dh, s.y = fmaf(dh, hat, s.y);
-      if (line) line[c] = fmaf(dy, hat, line[c]), line[p.width + c] += dy;
+      if (line) line[c] = fmaf(dy, hat, line[c]);
+      if (line && !LARGE) line[p.width + c] += dy;
     }
     if (!p.dx) continue;
     s = row_sum<32, true>(s, box, turn);
     const float m0 = s.x * inverse, m1 = s.y * inverse;
     T* to = static_cast<T*>(p.dx) + offset(p.at_dx, row, p);
     for (uint32_t c = threadIdx.x; c < p.width; c += 1024) {
-      const float hat = (float(from[c]) - mean - rest) * rstd, dy = float(grad[c]);
+      const float hat = hat_of(c), dy = float(grad[c]);
       const float dh = p.weight ? dy * float(static_cast<const W*>(p.weight)[c]) : dy;
-      const float y[1] = {(dh - fmaf(hat, m1, m0)) * rstd};
+      float y[1] = {(dh - fmaf(hat, m1, m0)) * rstd};
+      if (LARGE) y[0] *= kDown;
       put(to + c, y);
     }
   }
+  return again;
+}
+template <class T, class W>
+__device__ __noinline__ void norm_wide_backward_again(const Norm& p, float2 (*box)[32], int turn) {
+  norm_wide_rows<true, T, W>(p, box, turn);
+}
+template <class T, class W>
+__global__ void __launch_bounds__(1024) norm_wide_backward_kernel(const __grid_constant__ Norm p) {
+  __shared__ float2 box[2][32];
+  int turn = 0;
+  if (p.partial) {
+    float* line = p.partial + uint64_t(blockIdx.x) * 2 * p.width;
+    for (uint32_t c = threadIdx.x; c < p.width; c += 1024) line[c] = 0.0f, line[p.width + c] = 0.0f;
+  }
+  if (norm_wide_rows<false, T, W>(p, box, turn)) norm_wide_backward_again<T, W>(p, box, turn);
 }
 
 // dw and db from the blocks' sums: 32 columns a block, its warps over the lines.

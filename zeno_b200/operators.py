@@ -311,7 +311,8 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
     ``x`` [..., n] is float32 or bfloat16, of any strides (up to three leading axes need no copy while the last axis is
     contiguous; the result keeps a time-major order).  ``weight`` and ``bias`` [n] are float32 or of x's type, both of one
-    type; None: 1 and 0.  Mean, variance and all sums are held in 32 bits.  Gradients flow to x, weight and bias (once,
+    type; None: 1 and 0.  Mean, variance and all sums are held in 32 bits; a row whose squares leave their range is taken in other
+    units, so a finite row of any spread has a finite result (a row of no spread and ``eps`` 0 is 0 / 0).  Gradients flow to x, weight and bias (once,
     and in reverse mode only); they are sums in a fixed order, so they repeat bit for bit."""
     return _torch.layer_norm(x, weight, bias, eps)
 
