@@ -6,7 +6,8 @@ are the only fused operations); host model-building code is compiled with
 -ffp-contract=off for the same reason.
 
 The memory operators' PyTorch functions (zeno_b200/lib/zeno_torch.so, on libzeno.so) are compiled with g++ against the
-installed PyTorch.
+installed PyTorch, last, and again when another one is installed; without a PyTorch that has CUDA, or without Python's
+headers, they are left out.
 
 The library is also copied to <repo>/zig-out/lib/libzeno.so, where the reference's own
 Python package and ABI check look for it.  The sources compile in parallel.
@@ -31,6 +32,7 @@ INCLUDE = PKG.parent / "include"
 OUT_DIR = PKG / "lib"
 LIB = OUT_DIR / "libzeno.so"
 BINDING = OUT_DIR / "zeno_torch.so"
+BINDING_STAMP = OUT_DIR / "zeno_torch.txt"  # what the PyTorch functions were built against
 BINDING_SOURCE = CSRC / "torch_binding.cpp"
 # where the reference's own Python package (python/zeno/_ffi.py _find_library) and its
 # tests/check_abi_contract.py look for the library: <repo>/zig-out/lib/libzeno.so
@@ -76,40 +78,52 @@ def _runner(verbose: bool):
     return run
 
 
-def _compile_binding(run, cxx: str) -> Optional[Path]:
-    """The object file of the PyTorch functions; None where there is no PyTorch (the library itself needs none)."""
+def _torch_dir() -> Optional[Path]:
+    """The installed PyTorch, where the PyTorch functions can be built against it (the library itself needs none)."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
+    if spec is None or spec.origin is None:
         return None
     torch_dir = Path(spec.origin).parent
+    needed = (torch_dir / "lib" / "libtorch_cuda.so", Path(sysconfig.get_paths()["include"]) / "Python.h")
+    return torch_dir if all(f.exists() for f in needed) else None
+
+
+def _stamp(torch_dir: Path) -> str:
+    version = torch_dir / "version.py"
+    return "\n".join([str(torch_dir), sys.version, version.read_text() if version.exists() else ""])
+
+
+def _build_binding(run, cxx: str, force: bool) -> None:
+    torch_dir = _torch_dir()
+    if torch_dir is None:
+        return
+    stamp = _stamp(torch_dir)
+    if (not force and _newer(BINDING, [BINDING_SOURCE, INCLUDE / "zeno.h", Path(__file__)]) and BINDING_STAMP.exists()
+            and BINDING_STAMP.read_text() == stamp):
+        return
+    OBJ_DIR.mkdir(exist_ok=True)
     obj = OBJ_DIR / (BINDING_SOURCE.name + ".o")
     includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", CUDA_HOME / "include",
                 sysconfig.get_paths()["include"]]
     run([cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", *(f"-I{i}" for i in includes), "-c", str(BINDING_SOURCE), "-o", str(obj)])
-    return obj
-
-
-def _link_binding(run, cxx: str, obj: Optional[Path]) -> None:
-    if obj is None:
-        return
-    torch_lib = Path(importlib.util.find_spec("torch").origin).parent / "lib"
     tmp = BINDING.with_suffix(".so.tmp")
+    torch_lib = torch_dir / "lib"
     run([cxx, "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}", "-lzeno", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
          "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
     os.replace(tmp, BINDING)
+    BINDING_STAMP.write_text(stamp)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every CUDA/C++ source and link libzeno.so and the PyTorch functions; returns the library path."""
-    deps = [CSRC / s for s in CU_SOURCES + OP_SOURCES + CXX_SOURCES + HEADERS] + [INCLUDE / "zeno.h", Path(__file__)]
-    binding_deps = [BINDING_SOURCE, INCLUDE / "zeno.h", Path(__file__)]
-    cxx = shutil.which("g++") or "g++"
-    run = _runner(verbose)
-    if not force and _newer(LIB, deps):
-        if not _newer(BINDING, binding_deps):
-            OBJ_DIR.mkdir(exist_ok=True)
-            _link_binding(run, cxx, _compile_binding(run, cxx))
-        return LIB
+def _copy_for_reference() -> None:
+    if _newer(ZIG_OUT_LIB, [LIB]):
+        return
+    ZIG_OUT_LIB.parent.mkdir(parents=True, exist_ok=True)
+    tmp = ZIG_OUT_LIB.with_suffix(".so.tmp")
+    shutil.copyfile(LIB, tmp)
+    os.replace(tmp, ZIG_OUT_LIB)
+
+
+def _build_library(run, cxx: str) -> None:
     OBJ_DIR.mkdir(exist_ok=True)
     OUT_DIR.mkdir(exist_ok=True)
 
@@ -121,17 +135,23 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     objs = [cmd[-1] for cmd in jobs]
     jobs.sort(key=lambda cmd: "delta_" not in cmd[-3])  # the longest first
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as pool:
-        running = [pool.submit(run, cmd) for cmd in jobs]
-        binding = pool.submit(_compile_binding, run, cxx)
-        for f in running:
+        for f in [pool.submit(run, cmd) for cmd in jobs]:
             f.result()
     tmp = LIB.with_suffix(".so.tmp")
     run([NVCC, *ARCH, "-shared", "-o", str(tmp), *objs, "-Xlinker", "--no-undefined"])
     os.replace(tmp, LIB)
-    _link_binding(run, cxx, binding.result())
-    ZIG_OUT_LIB.parent.mkdir(parents=True, exist_ok=True)
-    shutil.copyfile(LIB, ZIG_OUT_LIB.with_suffix(".so.tmp"))
-    os.replace(ZIG_OUT_LIB.with_suffix(".so.tmp"), ZIG_OUT_LIB)
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every CUDA/C++ source and link libzeno.so and the PyTorch functions; returns the library path."""
+    deps = [CSRC / s for s in CU_SOURCES + OP_SOURCES + CXX_SOURCES + HEADERS] + [INCLUDE / "zeno.h", Path(__file__)]
+    cxx = shutil.which("g++") or "g++"
+    run = _runner(verbose)
+    if force or not _newer(LIB, deps):
+        _build_library(run, cxx)
+    _copy_for_reference()
+    # (the library and its copy are in place whatever becomes of these)
+    _build_binding(run, cxx, force)
     return LIB
 
 
