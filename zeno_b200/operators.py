@@ -12,6 +12,7 @@ there is no fallback.
 from __future__ import annotations
 
 import struct
+import threading
 from contextlib import nullcontext
 from importlib.machinery import ExtensionFileLoader
 from importlib.util import module_from_spec, spec_from_loader
@@ -25,18 +26,29 @@ from torch.autograd.graph import increment_version
 from ._ffi import _lib, ffi
 
 
+_binding_lock = threading.Lock()
+_torch = None
+
+
 def _binding():
-    """The compiled functions of the memory operators (csrc/torch_binding.cpp)."""
-    path = Path(__file__).resolve().parent / "lib" / "zeno_torch.so"
-    if not path.exists():
-        raise ImportError(f"{path} is missing: build it with `python -m zeno_b200.build`")
-    loader = ExtensionFileLoader("zeno_torch", str(path))
-    module = module_from_spec(spec_from_loader("zeno_torch", loader))
-    loader.exec_module(module)
-    return module
+    """The compiled functions of the memory operators (csrc/torch_binding.cpp), loaded at the first call of one: the others need
+    libzeno.so alone."""
+    global _torch
+    with _binding_lock:
+        if _torch is not None:
+            return _torch
+        path = Path(__file__).resolve().parent / "lib" / "zeno_torch.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build it with `python -m zeno_b200.build` (it needs a PyTorch with CUDA and Python's headers)")
+        try:
+            loader = ExtensionFileLoader("zeno_torch", str(path))
+            module = module_from_spec(spec_from_loader("zeno_torch", loader))
+            loader.exec_module(module)
+        except ImportError as e:
+            raise ImportError(f"{path} does not load with PyTorch {torch.__version__}: build it again with `python -m zeno_b200.build` ({e})") from e
+        _torch = module
+        return module
 
-
-_torch = _binding()
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _FLAGS = (torch.uint8, torch.bool)
@@ -292,7 +304,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, reset: Optional
     For the gradients a call keeps the state in front of every 64 tokens but the first (32 in float32, and of heads
     of up to 32 channels): 0.27 GB for 4096 x 128 tokens and 4 heads of 64 x 64 in bfloat16.
     """
-    return _torch.linear_attention(q, k, v, g, reset, initial_state, scale)
+    return (_torch or _binding()).linear_attention(q, k, v, g, reset, initial_state, scale)
 
 
 def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Tensor, reset: Optional[Tensor] = None,
@@ -303,7 +315,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, state: Ten
     world's ``dones`` buffer can be passed as it is).  ``state`` [B, H, dk, dv] float32,
     contiguous, is updated in place, and autograd knows: a rollout that was given the same
     tensor as its initial state and is yet to be differentiated needs a clone of it."""
-    return _torch.linear_attention_step(q, k, v, g, state, reset, scale)
+    return (_torch or _binding()).linear_attention_step(q, k, v, g, state, reset, scale)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, *, eps: float = 1e-5) -> Tensor:
@@ -314,7 +326,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     type; None: 1 and 0.  Mean, variance and all sums are held in 32 bits; a row whose squares leave their range is taken in other
     units, so a finite row of any spread has a finite result (a row of no spread and ``eps`` 0 is 0 / 0).  Gradients flow to x, weight and bias (once,
     and in reverse mode only); they are sums in a fixed order, so they repeat bit for bit."""
-    return _torch.layer_norm(x, weight, bias, eps)
+    return (_torch or _binding()).layer_norm(x, weight, bias, eps)
 
 
 def orthogonalize(update: Tensor, steps: int = 5) -> Tensor:
