@@ -102,3 +102,15 @@ def test_what_is_not_finite_stays_in_its_row(width, value):
         rows = [r for r in range(40) if r != 17]
         for a, c in zip(got[:2], want[:2]):
             assert torch.equal(a[rows], c[rows]) and torch.isnan(a[17]).all()
+
+
+def test_views_that_are_negative_by_a_flag():
+    """As the imaginary part of a conjugate is, which holds the opposite of its values."""
+    x, w, b, dy = inputs((9, 40), torch.float32, torch.float32)
+    want = gradients(zeno_b200.layer_norm, x, w, b, dy)
+    views = [torch._neg_view(-t) for t in (x, w, b, dy)]
+    assert all(t.is_neg() for t in views)
+    leaves = [t.requires_grad_(True) for t in views[:3]]
+    y = zeno_b200.layer_norm(*leaves)
+    for a, c in zip([y, *torch.autograd.grad(y, leaves, views[3])], want):
+        assert torch.equal(a, c)

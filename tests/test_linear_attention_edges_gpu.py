@@ -101,3 +101,29 @@ def check_sum(d_decay, d_g, finite=True):
     assert finite
     terms = d_g.double()
     assert ((d_decay.double() - terms.sum((0, 1))).abs() <= 2.0 ** -24 * terms.sum((0, 1)).abs() + 2.0 ** -40 * terms.abs().sum((0, 1))).all()
+
+
+def negative(t):
+    """t's values in a view that is negative by its flag, as the imaginary part of a conjugate is."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_views_that_are_negative_by_a_flag():
+    x = inputs(3, 40, 1, 2, 24, 20, torch.float32)
+    d_out, d_final = torch.randn(3, 40, 2, 20, device=DEV), torch.randn(3, 2, 24, 20, device=DEV)
+    want = gradients(zeno_b200.linear_attention, x, d_out, d_final)
+    y = [negative(t) if t.is_floating_point() else t for t in x]
+    leaves = [t.requires_grad_(True) if t.is_floating_point() else t for t in y]
+    out, final = zeno_b200.linear_attention(*leaves)
+    got = [out, final, *torch.autograd.grad([out, final], [t for t in leaves if t.requires_grad], [negative(d_out), negative(d_final)])]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        one = [t[:, 0] for t in x[:4]]
+        state, other = x[5].clone(), x[5].clone()
+        assert torch.equal(zeno_b200.linear_attention_step(*one, state), zeno_b200.linear_attention_step(*(negative(t) for t in one), other))
+        assert torch.equal(state, other)
+        with pytest.raises(ValueError, match="conjugated"):
+            zeno_b200.linear_attention_step(*one, negative(x[5]))

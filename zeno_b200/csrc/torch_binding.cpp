@@ -71,8 +71,13 @@ void expect(const char* name, const Tensor& t, at::IntArrayRef shape, at::Scalar
   expect_on(name, t, "q", q);
 }
 
-// t, or a copy of it where its last axis is not contiguous.
-Tensor rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// t, or a copy of it where it is negative by a flag alone (part of a conjugated complex tensor): its memory holds other values.
+Tensor held(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+// The same where its last axis is not contiguous.
+Tensor rows(const Tensor& t_) {
+  const Tensor t = held(t_);
+  return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
 
 // An empty tensor of t's shape, and of its order where that leaves the last axis contiguous.
 Tensor dense_like(const Tensor& t) {
@@ -205,7 +210,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     const at::AutoGradMode off(false);
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor d_out = grads[0].defined() ? rows(grads[0]) : at::zeros(v.sizes(), v.options());
-    const Tensor d_final = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor d_final = grads[1].defined() ? held(grads[1]).contiguous() : Tensor();
     ZenoLinearAttention p = linear_of(q, k, v, g, s[5], initial, d_out, ctx->saved_data["scale"].toDouble(), false);
     p.saved = floats(s[6]);
     const Tensor d_q = dense_like(q), d_k = dense_like(k), d_v = dense_like(v);
@@ -225,10 +230,11 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
   }
 };
 
-py::tuple linear_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g, const Maybe& reset_, const Maybe& initial_,
+py::tuple linear_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Maybe& reset_, const Maybe& initial_,
                            const std::optional<double>& scale_) {
   const Tensor reset = reset_.value_or(Tensor());
-  Tensor initial = initial_.value_or(Tensor());
+  Tensor initial = held(initial_.value_or(Tensor()));
+  const Tensor g = held(g_);
   const auto state = check_linear(q_, k_, v_, g, reset, 2);
   if (initial.defined()) {
     expect("initial_state", initial, state, at::kFloat, q_);
@@ -246,11 +252,12 @@ py::tuple linear_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_,
   return py::make_tuple(r.out, r.final);
 }
 
-Tensor linear_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g, const Tensor& state, const Maybe& reset_,
+Tensor linear_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& state, const Maybe& reset_,
                              const std::optional<double>& scale_) {
-  const Tensor reset = reset_.value_or(Tensor());
+  const Tensor reset = reset_.value_or(Tensor()), g = held(g_);
   expect("state", state, check_linear(q_, k_, v_, g, reset, 1), at::kFloat, q_);
   if (!state.is_contiguous()) bad_value("state must be contiguous: it is updated in place");
+  if (state.is_neg()) bad_value("state must hold its own values, not those of a conjugated tensor: it is updated in place");
   if (wants_gradient({&q_, &k_, &v_, &g, &state}))
     throw std::runtime_error("linear_attention_step has no gradients: call it under torch.no_grad(), and linear_attention to learn");
   refuse_tangents("linear_attention_step", {&q_, &k_, &v_, &g, &state});
@@ -353,7 +360,7 @@ Tensor layer_norm(const Tensor& x_, const Maybe& weight_, const Maybe& bias_, do
     if (t->scalar_type() != at::kFloat && t->scalar_type() != x_.scalar_type())
       bad_type(std::string(name) + " must be torch.float32 or " + type_of(x_.scalar_type()) + ", got " + type_of(t->scalar_type()));
     expect_on(name, *t, "x", x_);
-    if (!t->is_contiguous()) *t = t->contiguous();
+    *t = held(*t).contiguous();
   }
   if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type())
     bad_type("weight and bias must be of one type, got " + type_of(weight.scalar_type()) + " and " + type_of(bias.scalar_type()));
