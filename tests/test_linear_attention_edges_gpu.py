@@ -1,11 +1,12 @@
-"""Linear attention where its parts meet: chunks within a segment of a long rollout.
+"""Linear attention where its parts meet: chunks within a segment of a long rollout, short rollouts of wide heads, results that are
+asked for together, views.
 
 Tolerances and the plain implementation are those of test_linear_attention_gpu.py."""
 import pytest
 import torch
 
 import zeno_b200
-from test_linear_attention_gpu import NAMES, check, exact, gradients, inputs
+from test_linear_attention_gpu import NAMES, TOL, check, check_all, exact, gradients, inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -127,3 +128,51 @@ def test_views_that_are_negative_by_a_flag():
         assert torch.equal(state, other)
         with pytest.raises(ValueError, match="conjugated"):
             zeno_b200.linear_attention_step(*one, negative(x[5]))
+
+
+@pytest.mark.parametrize("T", [1, 7, 16, 17, 32])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (100, 128), (128, 7)])
+def test_short_rollouts_of_wide_heads(T, dk, dv):
+    """A warp a head of whole and of padded width past 64 channels, with and without what lies in front and behind, shared heads."""
+    for i, (B, Hk, H, fixed, reset, initial, behind) in enumerate([(600, 1, 1, True, None, False, False), (311, 2, 2, False, 0.1, True, False),
+                                                                   (200, 1, 3, True, 0.2, True, False), (300, 1, 2, False, None, False, True)]):
+        x = inputs(B, T, Hk, H, dk, dv, torch.bfloat16, seed=T + i, fixed=fixed, reset=reset, initial=initial)
+        check_all(x, torch.randn(B, T, H, dv, device=DEV).bfloat16(), torch.randn(B, H, dk, dv, device=DEV) if behind else None)
+
+
+BAD = [("q", "nan"), ("k", "-inf"), ("v", "inf"), ("v", "nan"), ("g", "nan"), ("d_out", "nan"), ("d_out", "inf")]
+
+
+@pytest.mark.parametrize("name,value,fixed", [(*b, f) for b in BAD for f in (False, True) if not (f and b[0] == "g")])
+@pytest.mark.parametrize("B,T,resets,at,d,dtype", [
+    (300, 20, (7,), 3, 128, torch.bfloat16), (300, 32, (5, 20), 20, 100, torch.bfloat16), (300, 32, (5, 20), 10, 128, torch.bfloat16),
+    (2, 70, (20, 45), 30, 128, torch.float32), (2, 900, (300, 500), 310, 100, torch.float32), (300, 20, (7,), 3, 128, torch.float32)])
+def test_what_is_not_finite_in_wide_heads(B, T, resets, at, d, dtype, name, value, fixed):
+    """By warps past 64 channels, and the wide instances of 32 bits: episodes on either side, the other head and the other environments are
+    what they are without it.  (One decay for all tokens has a gradient with every episode in it: the other head's is looked at.)"""
+    H = 2
+    x = inputs(B, T, H, H, d, d, dtype, reset=None, fixed=fixed)
+    x[4] = torch.zeros(B, T, device=DEV, dtype=torch.uint8)
+    for r in resets:
+        x[4][:, r] = 1
+    d_out = torch.randn(B, T, H, d, device=DEV).to(dtype)
+    want = exact(x, d_out)
+    y, z = [t.clone() for t in x], d_out.clone()
+    bad = z if name == "d_out" else y["qkvg".index(name)]
+    bad[(0, at, 1) if name == "g" else (0, at, 1, 5)] = float(value)
+    got = gradients(zeno_b200.linear_attention, y, z)
+    first, last = max([0, *(r for r in resets if r <= at)]), min([T, *(r for r in resets if r > at)])
+    outside = [t for t in range(T) if not first <= t < last]
+    for what, a, b in zip(NAMES, got, want):
+        if fixed and what == "d_g":
+            terms = exact([*x[:3], x[3].expand(B, T, H), *x[4:]], d_out)[5]
+            assert (a[0].double() - b[0].double()).abs() <= TOL * terms[..., 0].abs().sum()
+            continue
+        check(a[1:], b[1:], what), check(a[0, ..., 0, :, :] if what in ("state", "d_initial") else a[0, :, 0], b[0, ..., 0, :, :] if what in ("state", "d_initial") else b[0, :, 0], what)
+        if what in ("state", "d_initial"):
+            if not (last == T if what == "state" else first == 0):
+                check(a[0, 1], b[0, 1], what)
+            continue
+        check(a[0, outside, 1], b[0, outside, 1], what)
+    if name != "d_out":
+        assert not torch.isfinite(got[0][0, at, 1]).all() or (name == "g" and at in resets)
