@@ -404,7 +404,7 @@ typedef struct {
   const float* d_final; /* read, as final_state */
   ZenoTensor d_q, d_k, d_v;  /* written, as q, k, v */
   ZenoTensor d_g;       /* written, as g */
-  float* d_decay;       /* written, [value_heads]: the sum of g's gradients over batch and tokens */
+  float* d_decay;       /* written, [value_heads]: the sum of g's gradients over batch and tokens (with d_g or alone) */
   float* d_initial;     /* written, as initial_state */
 } ZenoLinearAttentionGrads;
 
@@ -417,8 +417,8 @@ uint64_t zeno_linear_attention_saved_bytes(const ZenoLinearAttention* p);
 int zeno_linear_attention_forward(const ZenoLinearAttention* p, void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 int zeno_linear_attention_backward(const ZenoLinearAttention* p, const ZenoLinearAttentionGrads* d, void* workspace,
                                    uint64_t workspace_bytes, void* cuda_stream);
-/* The recurrent form, for acting: tokens is usually 1 (0: the state is passed on), final_state usually
- * initial_state (updated in place).  Same results as forward up to rounding. */
+/* The recurrent form, for acting: tokens must be 1, final_state is usually initial_state (updated in place).
+ * Same results as forward up to rounding. */
 int zeno_linear_attention_step(const ZenoLinearAttention* p, void* cuda_stream);
 
 /* Chunks of wide heads wait for their own matrix instructions; one that waits longer than this gives up, and what

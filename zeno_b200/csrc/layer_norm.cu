@@ -10,8 +10,11 @@
 // whose plain sum overflows) in units of 2^96, and differences below 2^-50, which count where eps is below 2^-100, times 2^96.  Powers of two round
 // nothing.  In the loops over the rows this costs a comparison of each (branches there cost 3 to 8 %, the registers of the other side included).
 //
-// 131072 rows of 256 bfloat16: 30 us forward, 40 us backward (20 and 31 us of bytes), 4 us for the sums over blocks; 524288 rows of 64: 26.5 us (20 us).
-// Those are bound by the issue of instructions (68 %).  2047 rows of 4099 floats, whose rows are not aligned: 25 and 36 us, value by value.
+// 131072 rows of 256 bfloat16: 29 us forward, 40 us backward (20 and 31 us of bytes), 4 us for the sums over blocks; 524288 rows of 64: 26.5 us (20 us).
+// Nothing is full there: forward an SM issues in 65 % of its cycles, has 30 of 40 warps on average and is without work for 14 % of the time (start and
+// end of one round of blocks); a warp waits for its row's loads and for two sums across lanes, one behind the other.
+// 2047 rows of 4099 floats, whose rows are not aligned: 26 and 37 us, value by value.  2000 rows of 20000 floats, past what a block holds: 93 us
+// forward, 410 us with gradients (24 and 73 us of bytes), value by value from L2 and with the block's sums in memory.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -21,8 +21,9 @@ struct Cut {
   uint64_t state, keep, total;  // bytes
 };
 // How many segments: the least of the rounds of blocks that the main kernel takes, in chunks, and of what the segments cost besides: their sums,
-// the walk over them, the start of a block (as measured with 128 channels: 64 rollouts of 16 chunks are best in 2 segments, 322 us
-// with gradients against 346 in 4; 16 of 64 chunks in 8).
+// the walk over them, the start of a block.  The four weights are from bfloat16 heads of 128 channels (64 rollouts of 16 chunks are best in 2 segments, 322 us
+// with gradients against 346 in 4; 16 of 64 chunks in 8) and serve all widths and both types, forward and backward, though a chunk's cost differs
+// between them: only ratios to it count, and those of the others were not fitted.
 inline Cut cut_of(const ZenoLinearAttention& p) {
   const uint32_t C = uint32_t(chunk_of(p)), chunks = (p.tokens + C - 1) / C;
   const uint64_t rows = uint64_t(p.batch) * p.value_heads;

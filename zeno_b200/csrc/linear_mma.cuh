@@ -6,7 +6,7 @@
 // is left; three limbs are x exactly, and since a bfloat16 has the exponents of a float nothing is scaled and
 // nothing leaves the range.  What ends in a 32-bit result (the states, the decays' gradient, all of a 32-bit call)
 // takes three limbs, products of two such values the six terms above 2^-24.  What ends in a bfloat16 result (P in
-// out and dV, dP in dQ and dK of a bfloat16 call) takes two, the second one rounded: 2^-17 against the result's 2^-9.
+// out and dV, dP in dQ and dK of a bfloat16 call) takes two, the second one rounded: 2^-16 of the value against the result's 2^-8.
 // The instructions' sums truncate, so the state is not summed in them: each chunk's contribution is, and
 // is added to the state by an ordinary multiply-add.
 //

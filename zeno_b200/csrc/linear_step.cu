@@ -3,7 +3,9 @@
 // The time is the state's bytes, once in and once out.  A warp takes a slice of value channels of one (environment, head):
 // lane (r, c) has 4 neighbouring channels c of the rows r, r + RG, ...; the rows of a slice are whole 16-byte
 // vectors side by side, eight of them under way at once, and nothing but S^T q crosses lanes.
-// 16384 environments of 4 heads of 64 x 64, bfloat16: 336 us, 6.4 TB/s.  One environment: 3 us, the latency of two such turns of loads.
+// 16384 environments of 4 heads of 64 x 64, bfloat16: 336 us, 6.4 TB/s.  One environment: 3 us, the latency of
+// two loads one behind the other (k and q, then up to 64 rows of the state at once).  777 environments, 3 heads of 40 x 56 on one key head, 32-bit: 10.6 us (6.6 us of
+// bytes); four slices of 16 channels a state, of which the last is half empty, and each fetches its own k and q.
 #include <cuda_bf16.h>
 
 #include "policy_ops.h"

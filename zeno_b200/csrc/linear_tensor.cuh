@@ -7,8 +7,8 @@
 // and the warps do what is left: decays, limbs, the state's sum.  The accumulators come back in the same fragments as those of mma.sync, so that
 // the formulas are written as there.  Sums of a chunk are taken in TMEM, the state itself is summed in registers (the tensor cores truncate).
 //
-// 2 x 4096 tokens, 8 heads of 128 x 128: 27 us for the segments' sums and 61 us for the results (16 segments of 8 chunks for each head: a chain
-// that is walked twice); 8 x 1000 tokens backward: 150 us.  The tensor pipe is 16 % and 21 % busy; a chunk's loads, limbs and products wait for one another.
+// 2 x 4096 tokens, 8 heads of 128 x 128: 27 us for the segments' sums and 61 us for the results (8 segments of 8 chunks for each head, 128 blocks on 148 SMs:
+// a chain that is walked twice); 8 x 1000 tokens backward: 150 us.  The tensor pipe is 16 % and 21 % busy; a chunk's loads, limbs and products wait for one another.
 //
 // Waits end after a limit; a block whose products do not finish writes NaN.
 #pragma once
