@@ -381,7 +381,7 @@ int zeno_delta_rule_step(const ZenoDeltaRule* p, void* cuda_stream);
  *   S <- S + k v^T;  out = scale S^T q
  * Heads, resets, widths and strides as for the delta rule; q and k are taken as they are.  One log decay for
  * each head is a g whose first two strides are 0.  The state and all sums are 32-bit floats.  A product with a
- * 32-bit value keeps 24 bits of it where its result is 32-bit, 16 where it is a bfloat16. */
+ * 32-bit value keeps 24 bits of it where its result is 32-bit, 17 where it is a bfloat16. */
 typedef struct {
   uint32_t batch, tokens, key_heads, value_heads, key_dim, value_dim;
   uint32_t dtype; /* of q, k, v, out and their gradients: ZENO_DTYPE_* */

@@ -176,3 +176,63 @@ def test_what_is_not_finite_in_wide_heads(B, T, resets, at, d, dtype, name, valu
         check(a[0, outside, 1], b[0, outside, 1], what)
     if name != "d_out":
         assert not torch.isfinite(got[0][0, at, 1]).all() or (name == "g" and at in resets)
+
+
+def check_rounding(got, want, off):
+    """A bfloat16 result is the rounding of a value within `off` of the exact one (all of one sign); a 32-bit one is within `off`."""
+    if got.dtype == torch.float32:
+        worst = float(((got.double() - want).abs() / want.abs()).max())
+        assert worst <= off, worst
+        return
+    low, high = (want * (1 - off)).to(torch.bfloat16), (want * (1 + off)).to(torch.bfloat16)
+    missed = (got < low) | (got > high)
+    assert not missed.any(), float(missed.double().mean())
+
+
+SHAPES = [(700, 20, 64, torch.bfloat16), (700, 7, 128, torch.bfloat16), (500, 70, 64, torch.bfloat16), (500, 50, 32, torch.bfloat16), (40, 100, 128, torch.bfloat16),
+          (2, 400, 128, torch.bfloat16), (300, 40, 16, torch.float32), (1, 900, 16, torch.float32)]
+
+
+@pytest.mark.parametrize("B,T,d,dtype", SHAPES)
+def test_single_terms_to_their_limbs(B, T, d, dtype):
+    """Each token its own episode, every value positive: out = scale (q . k) v is one term, and so are the gradients.  In a bfloat16 call q . k loses at most
+    d / 16 truncations of 2^-23 and three roundings of 2^-24; then its limbs: of a value in [2^e, 2^(e+1)) the first, 8 bits, leaves at most 2^(e-8), of which the second,
+    8 bits below 2^(e-8), leaves 2^(e-17); their two products are truncated once: (1 + 8 / 64 + 1 / 42 + 1 / 64) 2^-17 for 128 channels, 1.2 * 2^-17.  In a 32-bit call
+    of 16 channels: one truncation, the rounding of the small terms' sum into it, of the scale and of the result, and twice the dropped products (2^-8 * 2^-17
+    twice): 2.75 * 2^-23."""
+    off = 1.2 * 2.0 ** -17 if dtype == torch.bfloat16 else 2.75 * 2.0 ** -23
+    x = inputs(B, T, 1, 1, d, d, dtype, initial=False)
+    x[:3] = [(t.float().abs() + 0.5).to(dtype) for t in x[:3]]
+    x[4][:] = 1
+    d_out = (torch.rand(B, T, 1, d, device=DEV) + 0.5).to(dtype)
+    for a, b in zip(gradients(zeno_b200.linear_attention, x, d_out), exact(x, d_out)):
+        if a.dim() == 4 and a.shape == x[0].shape:
+            check_rounding(a, b, off)
+
+
+@pytest.mark.parametrize("B,T,d,dtype", SHAPES)
+def test_states_to_their_limbs(B, T, d, dtype):
+    """Nothing but a positive state in front (keys of zero) or its gradient behind (no gradient of the outputs): out = scale c S^T q, dv = e R^T k.  As above, the limbs'
+    products in 2 * 8 truncations, and what a state loses on its way through the chunks and by their decays, 2^-22 each."""
+    off = 1.4 * 2.0 ** -17 + T / 32 * 2.0 ** -22 if dtype == torch.bfloat16 else (8 + T / 16) * 2.0 ** -23
+    x = inputs(B, T, 1, 1, d, d, dtype, reset=None, fixed=True)
+    x[3] = x[3] * 0.03
+    x[0], x[2], x[5] = ((t.float().abs() + 0.5).to(t.dtype) for t in (x[0], x[2], x[5]))
+    x[1] = torch.zeros_like(x[1])
+    zero = torch.zeros(B, T, 1, d, device=DEV, dtype=dtype)
+    check_rounding(zeno_b200.linear_attention(*x)[0], exact(x, zero)[0], off)
+    x[1], x[5] = x[0].clone(), None
+    behind = torch.rand(B, 1, d, d, device=DEV) + 0.5
+    got, want = gradients(zeno_b200.linear_attention, x, zero, behind), exact(x, zero, behind)
+    check_rounding(got[4], want[4], off)
+
+
+def test_states_next_to_the_largest_float():
+    """Their first limb would round to infinity."""
+    for B, T, d, dtype in SHAPES:
+        x = inputs(B, T, 1, 1, d, d, dtype, reset=None, fixed=True)
+        x[1], x[3] = torch.zeros_like(x[1]), torch.zeros_like(x[3])
+        x[0], x[5] = ((x[0].float().abs() + 0.5) * 2.0 ** -20).to(dtype), torch.full_like(x[5], 3.4e38)
+        got = zeno_b200.linear_attention(*x)
+        check_rounding(got[0], exact(x, torch.zeros_like(x[2]))[0], 1.4 * 2.0 ** -17 + T / 32 * 2.0 ** -22 if dtype == torch.bfloat16 else (8 + T / 16) * 2.0 ** -23)
+        assert torch.equal(got[1], x[5])

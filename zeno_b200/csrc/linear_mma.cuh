@@ -2,11 +2,11 @@
 // products on split operands, the gates of a chunk, and the state in the warps' accumulators.
 //
 // Precision.  The matrix instructions take bfloat16 operands and sum in 32 bits.  bfloat16 inputs enter as
-// they are.  A 32-bit value x enters as limbs of 8 bits each: hi = x cut to bfloat16, then the same of what
+// they are.  A 32-bit value x enters as limbs of 8 bits each: hi = x rounded to bfloat16, then the same of what
 // is left; three limbs are x exactly, and since a bfloat16 has the exponents of a float nothing is scaled and
-// nothing leaves the range.  What ends in a 32-bit result (the states, the decays' gradient, all of a 32-bit call)
-// takes three limbs, products of two such values the six terms above 2^-24.  What ends in a bfloat16 result (P in
-// out and dV, dP in dQ and dK of a bfloat16 call) takes two, the second one rounded: 2^-16 of the value against the result's 2^-8.
+// nothing leaves the range (what would round to infinity is the largest bfloat16 and the rest).  What ends in a 32-bit result (the states, the decays' gradient, all of a 32-bit call)
+// takes three limbs, products of two such values the six terms above 2^-25.  What ends in a bfloat16 result (P in
+// out and dV, dP in dQ and dK of a bfloat16 call) takes two: 2^-17 of the value against the result's 2^-8.
 // The instructions' sums truncate, so the state is not summed in them: each chunk's contribution is, and
 // is added to the state by an ordinary multiply-add.
 //
@@ -86,33 +86,34 @@ __device__ __forceinline__ uint32_t pack_round(float x, float y) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Two values as N packed limbs; three are exact, of two the second is rounded.
+// The same, of infinities and what would round to one the largest bfloat16 (the rest is the second limb's: an infinity, or what is left).
+__device__ __forceinline__ uint32_t pack_near(float x, float y) {
+  uint32_t w;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  return w;
+}
+__device__ __forceinline__ float lower(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float upper(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// Two values as N packed limbs, each the rounding of what is left; three are exact, two leave 2^-17 of the value.
 template <int N>
 __device__ __forceinline__ void split(float x, float y, uint32_t (&r)[N]) {
   if constexpr (N == 1) {
     r[0] = pack_round(x, y);
   } else {
-    r[0] = pack_cut(x, y);
-    x -= cut(x), y -= cut(y);
-    if constexpr (N == 2) {
-      r[1] = pack_round(x, y);
-    } else {
-      r[1] = pack_cut(x, y);
-      r[2] = pack_cut(x - cut(x), y - cut(y));
-    }
+    r[0] = pack_near(x, y);
+    x -= lower(r[0]), y -= upper(r[0]);
+    r[1] = pack_round(x, y);
+    if constexpr (N == 3) r[2] = pack_cut(x - lower(r[1]), y - upper(r[1]));  // (six bits are left)
   }
 }
-__device__ __forceinline__ float lower(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float upper(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// The value that N planes hold at `at`; the first alone where it is not finite.
+// The value that N planes hold at `at`; no further than a limb that is not finite.
 template <int N>
 __device__ __forceinline__ float value(const plane_t* at, int plane) {
   float x = __uint_as_float(uint32_t(at[0]) << 16);
-  if (fabsf(x) < INFINITY) {
 #pragma unroll
-    for (int l = 1; l < N; ++l) x += __uint_as_float(uint32_t(at[l * plane]) << 16);
-  }
+  for (int l = 1; l < N; ++l)
+    if (fabsf(x) < INFINITY) x += __uint_as_float(uint32_t(at[l * plane]) << 16);
   return x;
 }
 // Two neighbouring ones.
@@ -128,7 +129,7 @@ __device__ __forceinline__ float2 values(const plane_t* at, int plane) {
   return x;
 }
 
-// One 16-wide step: d += the products of the first limbs, low += the other terms above 2^-24 of the largest, smallest
+// One 16-wide step: d += the products of the first limbs, low += the other terms above 2^-25 of the largest, smallest
 // first.  The instructions' sums truncate at 2^-23 of what they hold, which is 2^-8 less for `low`.
 template <int LA, int LB, bool FIRST = false>
 __device__ __forceinline__ void mma_terms(float (&d)[2][4], float (&low)[2][4], const uint32_t (&a)[LA][4], const uint32_t (&b)[LB][4]) {

@@ -299,9 +299,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor, reset: Optional
     (None: zero).  ``scale`` defaults to dk ** -0.5.
 
     Any strides are taken (a time-major buffer's transposed view needs no copy) as long as
-    the last axis is contiguous.  The state and all sums are held in 32 bits.  Products with 32-bit values keep 24 bits of them where the result is 32-bit
-    (errors of 6e-8 to 2.9e-7 of a result's norm, where the same sums in plain 32-bit operations have 7e-8 to 2.3e-7), 16 where it is
-    bfloat16, which its rounding covers 256 times.  Gradients flow to q, k, v, g and initial_state
+    the last axis is contiguous.  The state and all sums are held in 32 bits.  Products with 32-bit values keep 24 bits of them where the result is 32-bit, 17
+    where it is bfloat16, which its rounding covers 512 times.  Gradients flow to q, k, v, g and initial_state
     (once, and in reverse mode only); they are sums in a fixed order, so they repeat bit for bit.
     For the gradients a call keeps the state in front of every 64 tokens but the first (32 in float32, and of heads
     of up to 32 channels): 0.27 GB for 4096 x 128 tokens and 4 heads of 64 x 64 in bfloat16.
