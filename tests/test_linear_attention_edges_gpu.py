@@ -236,3 +236,22 @@ def test_states_next_to_the_largest_float():
         got = zeno_b200.linear_attention(*x)
         check_rounding(got[0], exact(x, torch.zeros_like(x[2]))[0], 1.4 * 2.0 ** -17 + T / 32 * 2.0 ** -22 if dtype == torch.bfloat16 else (8 + T / 16) * 2.0 ** -23)
         assert torch.equal(got[1], x[5])
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "d_out"])
+@pytest.mark.parametrize("B,T,at,d,dtype", [(300, 20, 4, 64, torch.bfloat16), (300, 32, 31, 128, torch.bfloat16), (3, 60, 31, 32, torch.bfloat16), (3, 70, 9, 64, torch.bfloat16),
+                                            (3, 200, 63, 128, torch.bfloat16), (3, 200, 64, 100, torch.bfloat16), (3, 70, 31, 40, torch.float32), (1, 900, 95, 16, torch.float32)])
+def test_an_episode_of_one_token_has_no_part_in_the_decays(B, T, at, d, dtype, name):
+    """Whatever it holds: one decay for all tokens of a head has the gradient of the other episodes."""
+    x = inputs(B, T, 1, 2, d, d, dtype, fixed=True, reset=0.1)
+    x[4][:, at] = 1
+    if at + 1 < T:
+        x[4][:, at + 1] = 1
+    d_out = torch.randn(B, T, 2, d, device=DEV).to(dtype)
+    want = gradients(zeno_b200.linear_attention, x, d_out)[5]
+    y, z = [t.clone() for t in x], d_out.clone()
+    bad = z if name == "d_out" else y["qkv".index(name)]
+    bad[0, at, -1, 3] = float("inf")
+    got = gradients(zeno_b200.linear_attention, y, z)[5]
+    terms = exact([*x[:3], x[3].expand(B, T, 2), *x[4:]], d_out)[5]
+    assert ((got - want).abs() <= TOL * terms.abs().sum((0, 1))).all()

@@ -205,7 +205,8 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
             split<S::PL>(m0 ? o0 * f0 : 0.0f, m1 ? o1 * f1 : 0.0f, w);
 #pragma unroll
             for (int l = 0; l < S::PL; ++l) *reinterpret_cast<uint32_t*>(dp + l * S::CPLANE + i * S::CP + cc) = w[l];
-            pass[r][0] = m0 ? p0 * o0 : 0.0f, pass[r][1] = m1 ? p1 * o1 : 0.0f;
+            // (a token with itself passes none: where it is not finite that is not zero times it)
+            pass[r][0] = m0 && i != cc ? p0 * o0 : 0.0f, pass[r][1] = m1 && i != cc + 1 ? p1 * o1 : 0.0f;
           }
           if (!each) {  // a pair passes i - j tokens
             const float far = float(i0 - cc);
@@ -279,7 +280,7 @@ linear_backward_kernel(const __grid_constant__ ZenoLinearAttention p, const __gr
         const float2 y = scale_and_dot<S>(dk_, s.to_end, 1.0f, k, rt, ct, pk, lane);
         const float rest = float(n - 1 - rt * 16 - (lane >> 2));
         if (each) keep_rows(sums.y[ct], y, rt, lane);
-        else decays = fmaf(y.x, rest, fmaf(y.y, rest - 8.0f, decays));  // what begins here passes the tokens behind it
+        else decays += (rest == 0.0f ? 0.0f : y.x * rest) + (rest == 8.0f ? 0.0f : y.y * (rest - 8.0f));  // what begins here passes the tokens behind it
       }
       product<S::PL, S::L, true, true>(dk_, dp + rt * 16, S::CP, S::CPLANE, q + col, S::P, S::PLANE, rt, nt, pk, lane);
       bad = not_finite(dk_);

@@ -851,7 +851,8 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
           *reinterpret_cast<uint32_t*>(pr + at) = w[0], *reinterpret_cast<uint32_t*>(pr + kPair + at) = w[1];
           split<2>(m0 ? o0 * f0 : 0.0f, m1 ? o1 * f1 : 0.0f, w);
           *reinterpret_cast<uint32_t*>(dp + at) = w[0], *reinterpret_cast<uint32_t*>(dp + kPair + at) = w[1];
-          pass[r][0] = m0 ? p0 * o0 : 0.0f, pass[r][1] = m1 ? p1 * o1 : 0.0f;
+          // (a token with itself passes none: where it is not finite that is not zero times it)
+          pass[r][0] = m0 && i != cc ? p0 * o0 : 0.0f, pass[r][1] = m1 && i != cc + 1 ? p1 * o1 : 0.0f;
         }
         if (!each) {  // a pair passes i - j tokens
           const float far = float(i0 - cc);
@@ -951,7 +952,7 @@ linear_tensor_backward_kernel(const __grid_constant__ ZenoLinearAttention p, con
       const float2 y = add_and_dot(dk_, more, s.to_end, 1.0f, k, rt, col, lane);
       const float rest = float(n - 1 - rt * 16 - (lane >> 2));
       if (each) keep_rows(sums.y[ct], y, rt, lane);
-      else decays = fmaf(y.x, rest, fmaf(y.y, rest - 8.0f, decays));  // what begins here passes the tokens behind it
+      else decays += (rest == 0.0f ? 0.0f : y.x * rest) + (rest == 8.0f ? 0.0f : y.y * (rest - 8.0f));  // what begins here passes the tokens behind it
       fetch4(&more[0][0][0], t2_ + quarter + col);
       fetched(more);
       const float e0 = s.to_end[rt * 16 + (lane >> 2)], e1 = s.to_end[rt * 16 + (lane >> 2) + 8];

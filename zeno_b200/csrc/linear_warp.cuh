@@ -363,7 +363,7 @@ __device__ __noinline__ double warp_backward_slow(const ZenoLinearAttention& p, 
     const float raw = meet ? dot_rows<S>(o + i * S::P, v + lane * S::P, dv) : 0.0f;
     const float dp = meet ? raw * f : 0.0f;
     const float pass = meet ? dot_rows<S>(q + i * S::P, k + lane * S::P, dk) * f * raw : 0.0f;
-    decays += double(pass) * (i - lane);
+    if (lane < i) decays += double(pass) * (i - lane);
     float front = pass;
     for (int y = 1; y < 32; y <<= 1) {
       const float z = __shfl_up_sync(kAll, front, y);
